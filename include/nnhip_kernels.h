@@ -460,6 +460,84 @@ int nnhip_attn_query(const float* Q, const float* Kp, long kb, long kj, long kk,
                      long vd, const float* mask, long mask_bs, float* m, float* l, float* O, float* P, size_t batch,
                      size_t N, size_t K, size_t D, float alpha, void* workspace, void* stream);
 
+/* ── paged caches and beam search (no CUDA counterpart) ──────────────────
+ * Keys and values of a batch of sequences in pages of `page` rows, as the (seq, heads * dim) caches of
+ * incremental inference hold them: K and V have pages * page rows, `row` floats apart (>= heads * dim), head h
+ * of a row at h * dim. table (batch, width) holds page numbers: position p of sequence b is row
+ * table[b * width + p / page] * page + p % page. A position whose table entry is no page number (negative,
+ * NaN, >= pages) or that lies past width * page is absent: it is neither read nor written. Sequences may share
+ * pages. width * page and pages are at most 2^24 (index tensors hold integers as floats). */
+typedef struct nnhip_kv_pages
+{
+    float* K;
+    float* V;
+    const float* table;
+    size_t batch, width, pages, page, heads, dim, row;
+} nnhip_kv_pages;
+
+/* New tokens' keys and values into the pages, rotated on the way. Feature f of token n of x lies at
+ * x[n * x_t + f * x_f] (x_t = 1: the (features, tokens) outputs of the projections; x_f = 1: a token a row);
+ * k, v have heads * dim features, q and q_out q_heads * dim. Token n goes to position pos[n] of sequence
+ * seq[n] (seq NULL: of sequence n). With cos and sin (rope_rows, rope_dim / 2), row pos[n] turns the features
+ * j and j + rope_dim / 2 (j < rope_dim / 2) of each head of k and q as RotaryEmbedding does
+ * (compute_layer.hpp:884-984): x_j c - x_{j+r/2} s and x_{j+r/2} c + x_j s; the others, and v, are stored as
+ * they are. Without (cos and sin NULL, rope_dim 0) nothing is turned. q and q_out may both be NULL; q_out may
+ * be q itself with the same strides. A token whose sequence, position, page or, with a rotation, table row does not exist is padding:
+ * nothing of it is written. Two tokens of one call must not name the same row. dim <= 256. */
+int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f, const float* v, long v_t, long v_f,
+                    const float* q, long q_t, long q_f, float* q_out, long o_t, long o_f, size_t q_heads,
+                    size_t tokens, const float* seq, const float* pos, const float* cos, const float* sin,
+                    size_t rope_rows, size_t rope_dim, void* stream);
+
+/* One query per sequence and head against the sequence's pages (the batch form of nnhip_attn_query, and of
+ * AttentionBase::forward_step, compute_layer.hpp:1426-1511). For sequence b, head h (reading key head
+ * h / (q_heads / heads)), over the positions j < len[b] that are not absent:
+ *   s_j = alpha * (q_bh . k_j) - slopes[h] * (len[b] - 1 - j)     (no second term when slopes is NULL)
+ *   m = max_j s_j, l = sum_j exp(s_j - m), O = sum_j exp(s_j - m) v_j / l
+ * with m = lowest(), l = 0, O = 0 when there is no position or every s_j is -inf. q and O as the features of
+ * nnhip_kv_append's q; m, l (batch, q_heads) may be NULL. The batch is batch / group groups of `group`
+ * neighbouring sequences; shared (batch / group), when set, says how many first positions the group's
+ * sequences have in common: the tables of the group name the same rows there, and these are read once for all
+ * of them (through the table of the group's first sequence). A sequence shorter than that is read through its
+ * own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
+ * The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed); calls that may overlap in time
+ * need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
+ * bits every time. */
+size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t group);
+int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, const float* len,
+                     const float* shared, size_t group, const float* slopes, float alpha, float* O, long o_t,
+                     long o_f, float* m, float* l, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Beam search's selection. The logits of beam n (of groups * beams) lie in row n of a (groups * beams, vocab)
+ * matrix (beam_major) or in column n of a (vocab, groups * beams) matrix, the layout of the output head's
+ * logits; ld floats from a row to the next. Candidate (beam, token) of a group has the total
+ *   scores[beam] + (logit - log(sum over the vocabulary of exp(logit)))
+ * and a beam with done[beam] != 0 (done may be NULL) has ended: it offers `eos` with the total scores[beam]
+ * and every other token with -inf, and its logits are not read. A total that is NaN counts as -inf. The `take`
+ * best of each group's beams * vocab candidates go to out_score, out_beam, out_token (groups, take), best
+ * first; equal totals in the order of beam, then token. out_beam counts over all groups, so that it indexes
+ * the batch's tensors (nnhip_gather, nnhip_kv_reorder). Totals are formed and compared in 64 bits.
+ * take <= 256, take <= beams * vocab, beams <= 1024, vocab and groups * beams at most 2^24, beams * vocab below
+ * 2^31. Workspace: nnhip_beam_select_workspace_bytes; calls that may overlap in time need one each. */
+size_t nnhip_beam_select_workspace_bytes(size_t groups, size_t beams, size_t vocab, size_t take);
+int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const float* scores, const float* done,
+                      size_t groups, size_t beams, size_t vocab, size_t take, size_t eos, float* out_score,
+                      float* out_beam, float* out_token, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The caches after a selection: sequence b of the new batch (out_batch) continues sequence parent[b], which
+ * holds len[parent[b]] positions. `layers` caches (n_layers; K and V differ, table and sizes are those of the
+ * first) share the page tables. With n = len[parent[b]], i = n / page:
+ *   table_out[b][0 .. i) = table[parent[b]][0 .. i): full pages are shared, never copied;
+ *   table_out[b][i] = fresh[b], the page that b's next token goes to; its first n % page rows are copied from
+ *     the parent's page in every layer's K and V (unless it is that page itself);
+ *   table_out[b][i + 1 ..) = -1;  len_out[b] = n.
+ * With fresh NULL entry i is the parent's page when n % page != 0, else -1, and nothing is copied. A parent
+ * that is no sequence number gives a row of -1 and length 0; a fresh[b] that is no page number is stored as -1
+ * and nothing is copied. table_out (out_batch, width) must not overlap table. The pages of fresh must differ
+ * from each other and from every page that another sequence of the new batch continues or shares. */
+int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float* parent, const float* len,
+                     const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);
+
 /* ── column softmax / sparse cross-entropy (no CUDA counterpart) ─────────
  * cpu_engine.hpp:922-945 and :948-1006. Workspace from nnhip_col_softmax_workspace_bytes. */
 size_t nnhip_col_softmax_workspace_bytes(size_t C, size_t N);

@@ -1,0 +1,385 @@
+// k_beam.hip — beam search's selection: of each group's beams * vocab
+// continuations, with totals score + logit - log(sum exp(logits of the beam)),
+// the best `take`, equal totals in the order of their index beam * vocab + token.
+//
+// One pass over the logits leaves, for every segment of neighbouring tokens of
+// a beam, the largest logit and the sum of exp(logit - largest): the sums make
+// the beam's log-sum-exp, and the best `take` candidates lie in the best
+// `take` segments (a segment that ranks behind `take` others, by its largest
+// total and then its index, holds nothing that ranks before the best of each
+// of those). Only these segments are read again. Totals are formed in float64,
+// so that candidates of different beams compare as exactly as the sums allow.
+#include "common.hpp"
+#include "kv_pages.hpp"
+
+namespace nnhip
+{
+namespace
+{
+
+constexpr int kSegColumn = 64;    // tokens of a segment, (vocab, beams) logits
+constexpr int kSegRow = 256;      // tokens of a segment, (beams, vocab) logits
+constexpr int kMaxTake = 256;
+constexpr int kMaxBeams = 1024;
+constexpr int kList = 512;        // candidates that are ranked one against another
+constexpr int kBins = 1024;
+constexpr int kPickThreads = 1024;
+
+struct BeamArgs
+{
+    const float *logits, *scores, *done;
+    size_t ld;
+    unsigned groups, beams, vocab, take, eos, n_seg, seg;
+    int beam_major;
+    float2* part;   // per (beam of all groups, segment): largest logit, sum of exp(logit - largest)
+    float *out_score, *out_beam, *out_token;
+};
+
+// exp(x - m) of a logit and its segment's largest, m as 0 where that is -inf. The product with log2(e) is kept
+// in two parts: its rounding alone would be off by up to 2^-24 |x - m|.
+__device__ __forceinline__ float exp_below(float x, float m)
+{
+    constexpr float kHi = 1.44269502e+0f, kLo = 1.92596299e-8f, kLn2 = 6.93147182e-1f;   // log2(e) = kHi + kLo
+    const float d = x - m, y = d * kHi;
+    const float r = __builtin_fmaf(d, kHi, -y) + d * kLo;
+    const float e = __builtin_amdgcn_exp2f(y);
+    return e == 0.0f ? 0.0f : __builtin_fmaf(e, r * kLn2, e);   // r is NaN for d = -inf
+}
+
+// (vocab, beams) logits: a thread takes one segment of one beam, neighbouring threads neighbouring beams.
+__global__ __launch_bounds__(256) void k_beam_segments_column(BeamArgs a)
+{
+    const unsigned all = a.groups * a.beams;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)all * a.n_seg) return;
+    const unsigned seg = (unsigned)(i / all), n = (unsigned)(i % all);
+    if (a.done && a.done[n] != 0.0f) return;
+    const unsigned v0 = seg * kSegColumn, nv = min((unsigned)kSegColumn, a.vocab - v0);
+    const float* p = a.logits + (size_t)v0 * a.ld + n;
+    float x[kSegColumn], m = -__builtin_inff(), s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSegColumn; ++k) x[k] = k < (int)nv ? p[(size_t)k * a.ld] : -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < kSegColumn; ++k) m = fmax_std(m, x[k]);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int k = 0; k < kSegColumn; ++k) s += exp_below(x[k], base);
+    a.part[(size_t)n * a.n_seg + seg] = make_float2(m, s);
+}
+
+// (beams, vocab) logits: 16 lanes take one segment of one beam.
+__global__ __launch_bounds__(256) void k_beam_segments_row(BeamArgs a)
+{
+    constexpr int kPer = kSegRow / 16;
+    const unsigned n = blockIdx.y, lane = threadIdx.x & 15, seg = blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (a.done && a.done[n] != 0.0f) return;
+    if (seg >= a.n_seg) return;   // whole groups of 16 lanes
+    const unsigned v0 = seg * kSegRow;
+    const float* p = a.logits + (size_t)n * a.ld;
+    float x[kPer], m = -__builtin_inff(), s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+    {
+        const unsigned v = v0 + 16 * k + lane;
+        x[k] = v < a.vocab ? p[v] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) m = fmax_std(m, x[k]);
+    for (int o = 8; o > 0; o >>= 1) m = fmax_std(m, __shfl_xor(m, o, 16));
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s += exp_below(x[k], base);
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
+    if (lane == 0) a.part[(size_t)n * a.n_seg + seg] = make_float2(m, s);
+}
+
+typedef unsigned long long u64;
+
+// Totals as whole numbers of the same order; NaN as -inf, -0 as 0.
+__device__ __forceinline__ u64 key_of(double x)
+{
+    if (x != x) x = -__builtin_inf();
+    const u64 b = __builtin_bit_cast(u64, x + 0.0);
+    return (b >> 63) ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ double value_of(u64 k)
+{
+    return __builtin_bit_cast(double, (k >> 63) ? k & ~(1ull << 63) : ~k);
+}
+
+struct PickShared
+{
+    double lse[kMaxBeams];
+    u64 key[kList];
+    unsigned idx[kList];
+    unsigned hist[kBins];
+    unsigned wave[kPickThreads / 64];
+    u64 red[2][kPickThreads / 64];
+    unsigned count, bin, above;
+    unsigned order[kMaxTake];   // items of the list by rank
+};
+
+// The bin in which the running count, from bin 0 on (or from the last one down), reaches k: s.bin, and the
+// count before it, s.above.
+__device__ void find_bin(PickShared& s, unsigned k, bool down)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const unsigned own = s.hist[down ? kBins - 1 - t : t];
+    unsigned sum = own;
+    for (int o = 1; o < 64; o <<= 1)
+    {
+        const unsigned up = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 63) s.wave[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sum += s.wave[w];
+    if (sum >= k && sum - own < k)
+    {
+        s.bin = down ? kBins - 1 - t : t;
+        s.above = sum - own;
+    }
+    __syncthreads();
+}
+
+// Puts into the list at most kList of n items, the first k by (key descending, index ascending) among them; k
+// <= n, k <= kMaxTake. get(i) gives item i's key and index; indices differ. A histogram over the keys' range
+// narrows it to the bin that holds the k-th; where keys are equal, one over the indices follows.
+template <class Get> __device__ void pick(PickShared& s, unsigned n, unsigned k, Get get)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const u64 neg_inf = key_of(-__builtin_inf());
+    // Range of the keys above -inf, if those suffice.
+    u64 lo = ~0ull, hi = 0;
+    unsigned above_inf = 0;
+    for (unsigned i = t; i < n; i += kPickThreads)
+    {
+        u64 key;
+        unsigned idx;
+        get(i, key, idx);
+        hi = key > hi ? key : hi;
+        if (key > neg_inf)
+        {
+            lo = key < lo ? key : lo;
+            ++above_inf;
+        }
+    }
+    for (int o = 32; o > 0; o >>= 1)
+    {
+        const u64 l2 = __shfl_xor(lo, o, 64), h2 = __shfl_xor(hi, o, 64);
+        lo = l2 < lo ? l2 : lo;
+        hi = h2 > hi ? h2 : hi;
+        above_inf += __shfl_xor(above_inf, o, 64);
+    }
+    __syncthreads();
+    if (lane == 0)
+    {
+        s.red[0][wave] = lo;
+        s.red[1][wave] = hi;
+        s.wave[wave] = above_inf;
+    }
+    __syncthreads();
+    above_inf = 0;
+    for (int w = 0; w < kPickThreads / 64; ++w)
+    {
+        lo = s.red[0][w] < lo ? s.red[0][w] : lo;
+        hi = s.red[1][w] > hi ? s.red[1][w] : hi;
+        above_inf += s.wave[w];
+    }
+    if (above_inf < k) lo = neg_inf;
+    unsigned base = 0, ilo = 0, ihi = ~0u;   // base: items before the range
+    bool by_index = false;
+    for (;;)
+    {
+        u64 range = by_index ? (u64)(ihi - ilo) : hi - lo;
+        int shift = 0;
+        while ((range >> shift) >= (u64)kBins) ++shift;
+        __syncthreads();
+        s.hist[t] = 0;
+        __syncthreads();
+        for (unsigned i = t; i < n; i += kPickThreads)
+        {
+            u64 key;
+            unsigned idx;
+            get(i, key, idx);
+            if (key < lo || key > hi) continue;
+            if (!by_index) atomicAdd(&s.hist[(key - lo) >> shift], 1u);
+            else if (idx >= ilo && idx <= ihi) atomicAdd(&s.hist[(idx - ilo) >> shift], 1u);
+        }
+        __syncthreads();
+        find_bin(s, k - base, !by_index);
+        const unsigned bin = s.bin, here = s.hist[bin];
+        base += s.above;
+        if (by_index)
+        {
+            const unsigned l2 = ilo + (bin << shift);
+            const u64 h2 = (u64)l2 + ((1ull << shift) - 1);
+            ilo = l2;
+            ihi = h2 < ihi ? (unsigned)h2 : ihi;
+        }
+        else
+        {
+            const u64 l2 = lo + ((u64)bin << shift), h2 = l2 + ((1ull << shift) - 1);
+            lo = l2;
+            hi = h2 < hi && h2 >= l2 ? h2 : hi;
+        }
+        if (base + here <= kList) break;
+        if (!by_index && lo == hi)
+        {
+            by_index = true;
+            ilo = 0;
+            ihi = ~0u;
+        }
+    }
+    __syncthreads();
+    if (t == 0) s.count = 0;
+    __syncthreads();
+    for (unsigned i = t; i < n; i += kPickThreads)
+    {
+        u64 key;
+        unsigned idx;
+        get(i, key, idx);
+        if (key > hi || (key >= lo && (!by_index || idx <= ihi)))
+        {
+            const unsigned at = atomicAdd(&s.count, 1u);
+            s.key[at] = key;
+            s.idx[at] = idx;
+        }
+    }
+    __syncthreads();
+}
+
+// order[r] = the list's item of rank r, r < k (whatever order the items came in: indices differ).
+__device__ void rank_list(PickShared& s, unsigned k)
+{
+    const unsigned n = s.count;
+    for (unsigned i = threadIdx.x; i < n; i += kPickThreads)
+    {
+        const u64 key = s.key[i];
+        const unsigned idx = s.idx[i];
+        unsigned r = 0;
+        for (unsigned j = 0; j < n; ++j) r += s.key[j] > key || (s.key[j] == key && s.idx[j] < idx) ? 1u : 0u;
+        if (r < k) s.order[r] = i;
+    }
+    __syncthreads();
+}
+
+// One workgroup a group.
+__global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
+{
+    __shared__ PickShared s;
+    __shared__ unsigned seg_s[kMaxTake];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const unsigned b0 = blockIdx.x * a.beams;
+    for (unsigned w = wave; w < a.beams; w += kPickThreads / 64)
+    {
+        const unsigned n = b0 + w;
+        const float2* p = a.part + (size_t)n * a.n_seg;
+        double lse = 0.0;
+        if (!(a.done && a.done[n] != 0.0f))
+        {
+            float m = -__builtin_inff();
+            for (unsigned i = lane; i < a.n_seg; i += 64) m = fmax_std(m, p[i].x);
+            m = wave_max(m);
+            double sum = 0.0;
+            for (unsigned i = lane; i < a.n_seg; i += 64)
+            {
+                const float2 x = p[i];
+                sum += (double)x.y * exp((double)x.x - (double)m);
+            }
+            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            lse = (double)m + log(sum);
+        }
+        if (lane == 0) s.lse[w] = lse;
+    }
+    __syncthreads();
+    auto total = [&](unsigned w, bool ended, bool is_eos, float logit) {
+        const double sc = (double)a.scores[b0 + w];
+        return ended ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]);
+    };
+    // The best segments.
+    const unsigned n_all = a.beams * a.n_seg, k_seg = min(a.take, n_all);
+    pick(s, n_all, k_seg, [&](unsigned i, u64& key, unsigned& idx) {
+        const unsigned w = i / a.n_seg, g = i % a.n_seg, n = b0 + w;
+        const bool ended = a.done && a.done[n] != 0.0f;
+        key = key_of(total(w, ended, a.eos / a.seg == g, ended ? 0.0f : a.part[(size_t)n * a.n_seg + g].x));
+        idx = i;
+    });
+    rank_list(s, k_seg);
+    if (t < (int)k_seg) seg_s[t] = s.idx[s.order[t]];
+    __syncthreads();
+    // The best candidates of theirs.
+    pick(s, k_seg * a.seg, a.take, [&](unsigned i, u64& key, unsigned& idx) {
+        const unsigned g = seg_s[i / a.seg], w = g / a.n_seg, v = g % a.n_seg * a.seg + i % a.seg, n = b0 + w;
+        key = 0;   // behind every candidate
+        idx = w * a.vocab + v;
+        if (v >= a.vocab)
+        {
+            idx = a.beams * a.vocab + i;
+            return;
+        }
+        const bool ended = a.done && a.done[n] != 0.0f;
+        const float x = ended ? 0.0f : a.logits[a.beam_major ? (size_t)n * a.ld + v : (size_t)v * a.ld + n];
+        key = key_of(total(w, ended, v == a.eos, x));
+    });
+    rank_list(s, a.take);
+    if (t < (int)a.take)
+    {
+        const unsigned i = s.order[t], idx = s.idx[i];
+        const size_t o = (size_t)blockIdx.x * a.take + t;
+        a.out_score[o] = (float)value_of(s.key[i]);
+        a.out_beam[o] = (float)(b0 + idx / a.vocab);
+        a.out_token[o] = (float)(idx % a.vocab);
+    }
+}
+
+bool beam_sizes_ok(size_t groups, size_t beams, size_t vocab, size_t take)
+{
+    return groups > 0 && beams > 0 && beams <= kMaxBeams && vocab > 0 && vocab <= kMaxIndex &&
+           groups <= kMaxIndex && groups * beams <= kMaxIndex && beams * vocab < (size_t)0x80000000u - (1u << 20) &&
+           take > 0 && take <= kMaxTake && take <= beams * vocab;
+}
+
+} // namespace
+} // namespace nnhip
+
+using namespace nnhip;
+
+extern "C" size_t nnhip_beam_select_workspace_bytes(size_t groups, size_t beams, size_t vocab, size_t take)
+{
+    if (!beam_sizes_ok(groups, beams, vocab, take)) return 0;
+    return groups * beams * ((vocab + kSegColumn - 1) / kSegColumn) * sizeof(float2);
+}
+
+extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const float* scores,
+                                 const float* done, size_t groups, size_t beams, size_t vocab, size_t take, size_t eos,
+                                 float* out_score, float* out_beam, float* out_token, void* workspace,
+                                 size_t workspace_bytes, void* stream)
+{
+    if (groups == 0) return 0;
+    if (!beam_sizes_ok(groups, beams, vocab, take) || !logits || !scores || !out_score || !out_beam || !out_token ||
+        ld < (beam_major ? vocab : groups * beams) || (done && eos >= vocab) || !workspace ||
+        workspace_bytes < nnhip_beam_select_workspace_bytes(groups, beams, vocab, take) ||
+        reinterpret_cast<uintptr_t>(workspace) % sizeof(float2) != 0)
+        return -1;
+    const unsigned seg = beam_major ? kSegRow : kSegColumn;
+    const unsigned n_seg = static_cast<unsigned>((vocab + seg - 1) / seg), all = static_cast<unsigned>(groups * beams);
+    BeamArgs a{logits, scores, done, ld, static_cast<unsigned>(groups), static_cast<unsigned>(beams),
+               static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg,
+               beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
+    auto s = static_cast<hipStream_t>(stream);
+    if (beam_major)
+    {
+        if (all > 65535) return -1;
+        hipLaunchKernelGGL(k_beam_segments_row, dim3((n_seg + 15) / 16, all), dim3(256), 0, s, a);
+    }
+    else
+    {
+        const size_t blocks = ((size_t)all * n_seg + 255) / 256;
+        if (blocks > 0x7fffffffu) return -1;
+        hipLaunchKernelGGL(k_beam_segments_column, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+    }
+    if (int rc = launch_status()) return rc;
+    hipLaunchKernelGGL(k_beam_pick, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
+    return launch_status();
+}
