@@ -55,89 +55,159 @@ __device__ __forceinline__ int shared_of(const PagedArgs& a, unsigned b)
     return a.shared ? length_of(a.shared[b / a.group], (int)(a.c.width * a.c.page.d)) : 0;
 }
 
-template <int DP> struct Geometry
+// KS: groups of 16 key dims. Value columns of a lane: VW neighbouring ones of every 16 VW; columns past dim are
+// formed and dropped.
+template <int KS> struct Geometry
 {
-    // Value columns of a lane: VW neighbouring ones of every 16 VW.
-    static constexpr int VW = DP % 64 == 0 ? 4 : 2;
-    static constexpr int T = DP / (16 * VW);
-    static constexpr int KS = DP / 16;   // groups of 16 key dims
+    static constexpr int VW = KS % 4 == 0 || KS % 4 == 3 ? 4 : 2;
+    static constexpr int T = (KS + VW - 1) / VW;
+    static constexpr int DV = 16 * VW * T;
 };
 
-// The tile of 16 positions from p0 on, for the lane: its key dims and its value columns of 4 positions.
-template <int DP> struct Tile
+// How keys and values are loaded: whole groups of 16 dims in 16-byte pieces; 16-byte pieces whose last group is
+// cut (dim % 16 != 0); or one float at a time (rows that are not 16-byte aligned).
+enum { kWhole = 0, kCut = 1, kSingle = 2 };
+
+// 16 positions, for the lane: its dims of one key, its value columns of four positions.
+template <int KS> struct Tile
 {
-    using G = Geometry<DP>;
-    f32x4 k[G::KS];
+    using G = Geometry<KS>;
+    f32x4 k[KS];
     float v[4][G::T][G::VW];
-    bool there[4];   // of the lane's four positions
+    int row[4];   // of the values' positions, -1: none
 };
 
-template <int DP, bool VEC>
-__device__ __forceinline__ void load_tile(const PagedArgs& a, unsigned b, unsigned h, int p0, int end, int lane,
-                                          Tile<DP>& x)
+// Loads are issued whatever the positions are, from row 0 where there is none, so that no branch holds the next
+// tile's loads back behind this one's: the weights of such positions are 0, and their values are cleared before
+// use (0 times a NaN that lies there would be one).
+template <int KS, int MODE>
+__device__ __forceinline__ void load_tile(const PagedArgs& a, int row, unsigned h, int lane, Tile<KS>& x)
 {
-    using G = Geometry<DP>;
+    using G = Geometry<KS>;
     const int j = lane & 15, g = lane >> 4, dim = a.c.dim;
-    const long row = p0 + j < end ? a.c.row_of(b, p0 + j) : -1;
-    const float* kp = a.c.K + row * a.c.row + (long)h * dim;
+    const float* kp = a.c.K + (size_t)max(row, 0) * a.c.row + (size_t)h * dim;
 #pragma unroll
-    for (int i = 0; i < G::KS; ++i)
+    for (int i = 0; i < KS; ++i)
     {
         const int d = 16 * i + 4 * g;
-        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (row >= 0)
+        if constexpr (MODE == kWhole) x.k[i] = *reinterpret_cast<const f32x4*>(kp + d);
+        else if constexpr (MODE == kCut)
         {
-            if constexpr (VEC)
-            {
-                if (d < dim) z = *reinterpret_cast<const f32x4*>(kp + d);
-            }
-            else
-            {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < dim) z[e] = kp[d + e];
-            }
+            x.k[i] = *reinterpret_cast<const f32x4*>(kp + (d < dim ? d : 0));
         }
-        x.k[i] = z;
+        else
+        {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.k[i][e] = kp[d + e < dim ? d + e : 0];
+        }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
     {
-        const int lo = __shfl((int)row, 4 * g + r, 64), hi = __shfl((int)(row >> 32), 4 * g + r, 64);
-        const long vr = ((long)hi << 32) | (unsigned)lo;
-        x.there[r] = vr >= 0;
-        const float* vp = a.c.V + vr * a.c.row + (long)h * dim;
+        x.row[r] = __shfl(row, 4 * g + r, 64);
+        const float* vp = a.c.V + (size_t)max(x.row[r], 0) * a.c.row + (size_t)h * dim;
 #pragma unroll
         for (int t = 0; t < G::T; ++t)
         {
             const int d = 16 * G::VW * t + G::VW * j;
-#pragma unroll
-            for (int e = 0; e < G::VW; ++e) x.v[r][t][e] = 0.0f;
-            if (vr < 0) continue;
-            if constexpr (VEC)
+            if constexpr (MODE == kSingle)
             {
-                typedef float vec __attribute__((ext_vector_type(G::VW)));
-                if (d < dim)
-                {
-                    const vec z = *reinterpret_cast<const vec*>(vp + d);
 #pragma unroll
-                    for (int e = 0; e < G::VW; ++e) x.v[r][t][e] = z[e];
-                }
+                for (int e = 0; e < G::VW; ++e) x.v[r][t][e] = vp[d + e < dim ? d + e : 0];
             }
             else
             {
+                typedef float vec __attribute__((ext_vector_type(G::VW)));
+                const vec z = *reinterpret_cast<const vec*>(vp + (d < dim ? d : 0));
 #pragma unroll
-                for (int e = 0; e < G::VW; ++e)
-                    if (d + e < dim) x.v[r][t][e] = vp[d + e];
+                for (int e = 0; e < G::VW; ++e) x.v[r][t][e] = z[e];
             }
         }
     }
 }
 
-// rws of the 4 waves lie along the rows (16 rws rows a workgroup), the others take the range's positions in turn.
-template <int DP, bool VEC> __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a)
+// Dims past the last one are 0 in keys and queries.
+template <int KS, int MODE> __device__ __forceinline__ void cut(f32x4 (&x)[KS], int g, int dim)
 {
-    using G = Geometry<DP>;
+    if constexpr (MODE != kWhole)
+    {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = 16 * i + 4 * g + e < dim ? x[i][e] : 0.0f;
+    }
+}
+
+// What the running softmax of a lane's row holds.
+template <int KS> struct State
+{
+    using G = Geometry<KS>;
+    float m, l;   // l: of the lane's positions alone
+    f32x4 o[G::T][G::VW];
+};
+
+template <int KS, int MODE>
+__device__ __forceinline__ void use_tile(const PagedArgs& a, Tile<KS>& x, const f32x4 (&q)[KS], int p0, int g, int len,
+                                         bool counts, float slope, State<KS>& st)
+{
+    using G = Geometry<KS>;
+    cut<KS, MODE>(x.k, g, a.c.dim);
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[i][e], q[i][e], s, 0, 0, 0);
+    float top = kLowest;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+    {
+        float z = a.alpha * s[r];
+        if (a.slopes) z -= slope * (float)(len - 1 - (p0 + 4 * g + r));
+        s[r] = x.row[r] >= 0 && counts ? z : -__builtin_inff();
+        top = fmax_std(top, s[r]);
+    }
+    top = fmax_std(top, __shfl_xor(top, 16, 64));
+    top = fmax_std(top, __shfl_xor(top, 32, 64));
+    const float mn = fmax_std(st.m, top);
+    const float f = __builtin_amdgcn_exp2f((st.m - mn) * kLog2e);
+    const float mb = mn == kLowest ? 0.0f : mn * kLog2e;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+    {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], kLog2e, -mb));
+        sum += s[r];
+    }
+    st.l = st.l * f + sum;
+    st.m = mn;
+    const int least = min(min(x.row[0], x.row[1]), min(x.row[2], x.row[3]));
+    if (__builtin_amdgcn_ballot_w64(least < 0))
+    {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < G::T; ++t)
+#pragma unroll
+                for (int y = 0; y < G::VW; ++y) x.v[r][t][y] = x.row[r] < 0 ? 0.0f : x.v[r][t][y];
+    }
+#pragma unroll
+    for (int t = 0; t < G::T; ++t)
+#pragma unroll
+        for (int y = 0; y < G::VW; ++y) st.o[t][y] *= f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < G::T; ++t)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y)
+                st.o[t][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[r][t][y], s[r], st.o[t][y], 0, 0, 0);
+}
+
+// rws of the 4 waves lie along the rows (16 rws rows a workgroup), the others take the range's positions in turn.
+template <int KS, int MODE> __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a)
+{
+    using G = Geometry<KS>;
+    constexpr int DP = G::DV;
     __shared__ float o_s[4][kTile][DP + 4];
     __shared__ float ml_s[4][kTile][2];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -191,87 +261,62 @@ template <int DP, bool VEC> __global__ __launch_bounds__(256) void k_attn_paged(
     const bool counts = live && (!is_shared || len >= common);
     const float slope = a.slopes && live ? a.slopes[qh] : 0.0f;
     const int dim = a.c.dim;
-    float m = kLowest, l = 0.0f;
-    f32x4 o[G::T][G::VW];
-#pragma unroll
-    for (int x = 0; x < G::T; ++x)
-#pragma unroll
-        for (int y = 0; y < G::VW; ++y) o[x][y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
+    State<KS> st{kLowest, 0.0f, {}};
     if (begin < end)
     {
-        f32x4 q[G::KS];
+        f32x4 q[KS];
         const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;
 #pragma unroll
-        for (int x = 0; x < G::KS; ++x)
+        for (int x = 0; x < KS; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
             {
                 const int d = 16 * x + 4 * g + e;
-                q[x][e] = live && d < dim ? qp[(long)d * a.q_f] : 0.0f;
+                q[x][e] = qp[(long)(d < dim ? d : 0) * a.q_f];   // rows that are not live are formed and dropped
             }
-        Tile<DP> cur, next;
-        int p0 = begin + kw * kTile;
-        load_tile<DP, VEC>(a, b0, h, p0, end, lane, cur);
-        for (; p0 < end; p0 += step)
+        // The loads stay in one run: without this each would move into a branch of the selection below.
+#pragma unroll
+        for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[x]));
+        cut<KS, MODE>(q, g, dim);
+        // Table entries are loaded two tiles ahead of their use, keys and values one: the entries' loads are then
+        // older than the keys' and values' that are still on their way when the addresses are formed.
+        auto entry = [&](int p) { return a.c.entry_of(b0, p + j); };
+        auto row_at = [&](float e, int p) {
+            const int r = a.c.row_in(e, p + j);
+            return p + j < end ? r : -1;
+        };
+        const int p1 = begin + kw * kTile;
+        Tile<KS> x0, x1;
+        const float first = entry(p1);
+        float ahead = entry(p1 + step);
+        load_tile<KS, MODE>(a, row_at(first, p1), h, lane, x0);
+        for (int p = p1; p < end; p += 2 * step)
         {
-            load_tile<DP, VEC>(a, b0, h, p0 + step, end, lane, next);
-            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int x = 0; x < G::KS; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[x][e], q[x][e], s, 0, 0, 0);
-            float top = kLowest;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-            {
-                float z = a.alpha * s[r];
-                if (a.slopes) z -= slope * (float)(len - 1 - (p0 + 4 * g + r));
-                s[r] = cur.there[r] && counts ? z : -__builtin_inff();
-                top = fmax_std(top, s[r]);
-            }
-            top = fmax_std(top, __shfl_xor(top, 16, 64));
-            top = fmax_std(top, __shfl_xor(top, 32, 64));
-            const float mn = fmax_std(m, top);
-            const float f = __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-            const float mb = mn == kLowest ? 0.0f : mn * kLog2e;
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-            {
-                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], kLog2e, -mb));
-                sum += s[r];
-            }
-            l = l * f + sum;   // of the lane's positions
-            m = mn;
-#pragma unroll
-            for (int x = 0; x < G::T; ++x)
-#pragma unroll
-                for (int y = 0; y < G::VW; ++y)
-                {
-                    o[x][y] *= f;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        o[x][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.v[r][x][y], s[r], o[x][y], 0, 0, 0);
-                }
-            cur = next;
+            float further = entry(p + 2 * step);
+            load_tile<KS, MODE>(a, row_at(ahead, p + step), h, lane, x1);
+            __builtin_amdgcn_sched_barrier(0);
+            use_tile<KS, MODE>(a, x0, q, p, g, len, counts, slope, st);
+            ahead = entry(p + 3 * step);
+            load_tile<KS, MODE>(a, row_at(further, p + 2 * step), h, lane, x0);
+            __builtin_amdgcn_sched_barrier(0);
+            use_tile<KS, MODE>(a, x1, q, p + step, g, len, counts, slope, st);
         }
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
+        st.l += __shfl_xor(st.l, 16, 64);
+        st.l += __shfl_xor(st.l, 32, 64);
     }
 
     // The waves of the same rows are joined through LDS, in the order of their positions.
     if (g == 0)
     {
-        ml_s[wave][j][0] = m;
-        ml_s[wave][j][1] = l;
+        ml_s[wave][j][0] = st.m;
+        ml_s[wave][j][1] = st.l;
     }
 #pragma unroll
     for (int x = 0; x < G::T; ++x)
 #pragma unroll
         for (int y = 0; y < G::VW; ++y)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o_s[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = o[x][y][r];
+            for (int r = 0; r < 4; ++r) o_s[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = st.o[x][y][r];
     __syncthreads();
     const unsigned n_parts = a.n_shared + a.n_own, slot = is_shared ? c : a.n_shared + c;
     const bool direct = n_parts == 1;
@@ -312,27 +357,56 @@ template <int DP, bool VEC> __global__ __launch_bounds__(256) void k_attn_paged(
         }
 }
 
-// Joins the ranges of one row: blockIdx.x = sequence * q_heads + head.
-__global__ __launch_bounds__(128) void k_attn_paged_join(PagedArgs a)
+// Joins the ranges of one row in order: blockIdx.x = sequence * q_heads + head. The ranges' factors go to LDS,
+// then 2 or 4 groups of threads sum every 2nd or 4th range.
+__global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
 {
+    constexpr int kChunk = 256;
+    __shared__ float w_s[kChunk];
+    __shared__ float red[2][4];
+    __shared__ float o_s[256];
     const size_t at = blockIdx.x;
     const unsigned b = (unsigned)(at / a.q_heads), h = (unsigned)(at % a.q_heads), n = a.n_shared + a.n_own;
-    const int d = threadIdx.x, dim = a.c.dim;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, dim = a.c.dim;
+    const int cols = dim <= 64 ? 64 : 128, groups = 256 / cols, d = t % cols, g = t / cols;
     const float* ml = a.part_ml + 2 * at * n;
+    const float* po = a.part_o + at * n * dim + (d < dim ? d : 0);
     float m = kLowest, l = 0.0f, o = 0.0f;
-    for (unsigned i = 0; i < n; ++i)
+    for (unsigned i = t; i < n; i += 256)
         if (ml[2 * i + 1] != 0.0f) m = fmax_std(m, ml[2 * i]);
-    for (unsigned i = 0; i < n; ++i)
+    m = wave_max(m);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = fmax_std(fmax_std(red[0][0], red[0][1]), fmax_std(red[0][2], red[0][3]));
+    for (unsigned c = 0; c < n; c += kChunk)
     {
-        const float li = ml[2 * i + 1];
-        if (li == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f((ml[2 * i] - m) * kLog2e);
-        l += li * f;
-        if (d < dim) o += a.part_o[(at * n + i) * dim + d] * f;
+        float w = 0.0f;
+        if (c + t < n)
+        {
+            const float li = ml[2 * (c + t) + 1];
+            if (li != 0.0f) w = __builtin_amdgcn_exp2f((ml[2 * (c + t)] - m) * kLog2e);   // O is 0 where l is
+            l += li * w;
+        }
+        __syncthreads();
+        w_s[t] = w;
+        __syncthreads();
+        const int nc = min((int)(n - c), kChunk);
+#pragma unroll 8
+        for (int i = g; i < nc; i += groups) o += po[(size_t)(c + i) * dim] * w_s[i];
     }
-    if (d < dim) a.O[(long)b * a.o_t + ((long)h * dim + d) * a.o_f] = l == 0.0f ? 0.0f : o / l;
-    if (d == 0 && a.m) a.m[at] = m;
-    if (d == 0 && a.l) a.l[at] = l;
+    l = wave_sum(l);
+    if (lane == 0) red[1][wave] = l;
+    o_s[t] = o;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    if (t < dim)
+    {
+        o = 0.0f;
+        for (int i = 0; i < groups; ++i) o += o_s[i * cols + t];
+        a.O[(long)b * a.o_t + ((long)h * dim + t) * a.o_f] = l == 0.0f ? 0.0f : o / l;
+    }
+    if (t == 0 && a.m) a.m[at] = m;
+    if (t == 0 && a.l) a.l[at] = l;
 }
 
 struct PagedPlan
@@ -347,7 +421,7 @@ struct PagedPlan
 PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
 {
     PagedPlan p{};
-    const size_t per = q_heads / c.heads, most = c.width * c.page, target = 4 * (size_t)device_cus();
+    const size_t per = q_heads / c.heads, most = c.width * c.page, target = 2 * (size_t)device_cus();
     auto along_rows = [](size_t rows, int& rws, unsigned& blocks) {
         rws = rows > 32 ? 4 : rows > 16 ? 2 : 1;
         blocks = static_cast<unsigned>((rows + kTile * rws - 1) / (kTile * rws));
@@ -370,9 +444,9 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
     return p;
 }
 
-template <int DP, bool VEC> void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s)
+template <int KS, int MODE> void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s)
 {
-    hipLaunchKernelGGL((k_attn_paged<DP, VEC>), dim3(static_cast<unsigned>(p.shared_blocks + p.own_blocks)), dim3(256),
+    hipLaunchKernelGGL((k_attn_paged<KS, MODE>), dim3(static_cast<unsigned>(p.shared_blocks + p.own_blocks)), dim3(256),
                        0, s, a);
 }
 
@@ -420,15 +494,33 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     if (p.parts() > 1) a.part_o = ws + 2 * c->batch * q_heads * p.parts();
     const size_t d = c->dim;
     const bool vec = d % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V);
+    const int mode = !vec ? kSingle : d % 16 == 0 ? kWhole : kCut;
     auto s = static_cast<hipStream_t>(stream);
-    if (d <= 32) vec ? paged_launch<32, true>(a, p, s) : paged_launch<32, false>(a, p, s);
-    else if (d <= 64) vec ? paged_launch<64, true>(a, p, s) : paged_launch<64, false>(a, p, s);
-    else if (d <= 96) vec ? paged_launch<96, true>(a, p, s) : paged_launch<96, false>(a, p, s);
-    else vec ? paged_launch<128, true>(a, p, s) : paged_launch<128, false>(a, p, s);
+    // Whole groups have a kernel each; the others take the next even number of groups.
+    const int ks = static_cast<int>((d + 15) / 16);
+    switch (mode == kWhole ? ks : 8 * mode + (ks + 1) / 2)
+    {
+    case 1: paged_launch<1, kWhole>(a, p, s); break;
+    case 2: paged_launch<2, kWhole>(a, p, s); break;
+    case 3: paged_launch<3, kWhole>(a, p, s); break;
+    case 4: paged_launch<4, kWhole>(a, p, s); break;
+    case 5: paged_launch<5, kWhole>(a, p, s); break;
+    case 6: paged_launch<6, kWhole>(a, p, s); break;
+    case 7: paged_launch<7, kWhole>(a, p, s); break;
+    case 8: paged_launch<8, kWhole>(a, p, s); break;
+    case 9: paged_launch<2, kCut>(a, p, s); break;
+    case 10: paged_launch<4, kCut>(a, p, s); break;
+    case 11: paged_launch<6, kCut>(a, p, s); break;
+    case 12: paged_launch<8, kCut>(a, p, s); break;
+    case 17: paged_launch<2, kSingle>(a, p, s); break;
+    case 18: paged_launch<4, kSingle>(a, p, s); break;
+    case 19: paged_launch<6, kSingle>(a, p, s); break;
+    default: paged_launch<8, kSingle>(a, p, s); break;
+    }
     if (int rc = launch_status()) return rc;
     if (p.parts() > 1)
     {
-        hipLaunchKernelGGL(k_attn_paged_join, dim3(static_cast<unsigned>(c->batch * q_heads)), dim3(128), 0, s, a);
+        hipLaunchKernelGGL(k_attn_paged_join, dim3(static_cast<unsigned>(c->batch * q_heads)), dim3(256), 0, s, a);
         return launch_status();
     }
     return 0;

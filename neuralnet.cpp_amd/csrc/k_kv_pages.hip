@@ -33,7 +33,7 @@ struct AppendArgs
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
 {
     extern __shared__ float tile_s[];   // [token][dim + 1]
-    __shared__ long row_s[kAppendTokens];
+    __shared__ int row_s[kAppendTokens];
     __shared__ unsigned pos_s[kAppendTokens];
     const int t = threadIdx.x, dim = a.c.dim, ld = dim + 1;
     const unsigned n0 = blockIdx.x * a.tile, heads = a.c.heads;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
     {
         const unsigned n = n0 + t;
         size_t p = 0, b = n;
-        long row = -1;
+        int row = -1;
         const bool seq_ok = a.seq ? row_index(a.seq[n], a.c.batch, b) : n < a.c.batch;
         if (seq_ok && row_index(a.pos[n], kMaxIndex, p) && (!a.cos || p < a.rope_rows)) row = a.c.row_of(b, p);
         row_s[t] = row;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
     for (int i = t; i < count; i += 256)
     {
         const int n = by_token ? i / dim : i % nt, d = by_token ? i % dim : i / nt;
-        const long row = row_s[n];
+        const int row = row_s[n];
         if (row < 0) continue;
         float v = tile_s[n * ld + d];
         if (d < 2 * half)
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
         if (kind == 2)
             a.out[(long)(n0 + n) * a.o_t + ((long)h * dim + d) * a.o_f] = v;
         else
-            (kind == 0 ? a.c.K : a.c.V)[row * a.c.row + (long)h * dim + d] = v;
+            (kind == 0 ? a.c.K : a.c.V)[(long)row * a.c.row + (long)h * dim + d] = v;
     }
 }
 

@@ -37,15 +37,20 @@ struct Pages
     long row;
     FastDiv page;
 
-    // Row of position pos in the table's row b, or -1 where there is none.
-    __device__ __forceinline__ long row_of(unsigned b, unsigned pos) const
+    // The table's entry for position pos of sequence b (the last one past the table's end), and the row that it
+    // names, -1 where there is none. Neither branches: the kernels load entries ahead of their use, and a branch
+    // would make the wait for one a wait for every load behind it.
+    __device__ __forceinline__ float entry_of(unsigned b, unsigned pos) const
     {
-        const unsigned i = page.div(pos);
-        if (i >= width) return -1;
-        size_t p;
-        if (!row_index(table[(size_t)b * width + i], pages, p)) return -1;
-        return (long)p * page.d + (pos - i * page.d);
+        return table[(size_t)b * width + min(page.div(pos), width - 1)];
     }
+    __device__ __forceinline__ int row_in(float entry, unsigned pos) const
+    {
+        const unsigned i = page.div(pos), p = (unsigned)(int)entry;
+        const bool ok = i < width && entry > -1.0f && entry < (float)pages;   // pages <= 2^24 is exact
+        return ok ? (int)(p * page.d + (pos - i * page.d)) : -1;
+    }
+    __device__ __forceinline__ int row_of(unsigned b, unsigned pos) const { return row_in(entry_of(b, pos), pos); }
 };
 
 // A length held as a float: negative and NaN are 0, at most `most`.
@@ -60,7 +65,7 @@ inline bool pages_ok(const nnhip_kv_pages* c, size_t max_dim)
 {
     return c && c->K && c->V && c->table && c->batch > 0 && c->width > 0 && c->pages > 0 && c->page > 0 &&
            c->heads > 0 && c->dim > 0 && c->dim <= max_dim && c->batch <= kMaxIndex && c->pages <= kMaxIndex &&
-           c->page <= kMaxIndex && c->width <= kMaxIndex && c->width * c->page <= kMaxIndex &&
+           c->page <= kMaxIndex && c->pages * c->page < (size_t)0x80000000u && c->width <= kMaxIndex && c->width * c->page <= kMaxIndex &&
            c->heads <= kMaxIndex && c->row >= c->heads * c->dim && c->row <= ((size_t)1 << 32);
 }
 

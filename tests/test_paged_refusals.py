@@ -15,7 +15,7 @@ def pages(**kw):
 
 BAD_PAGES = [dict(K=None), dict(V=None), dict(table=None), dict(batch=0), dict(width=0), dict(pages=0), dict(page=0),
              dict(heads=0), dict(dim=0), dict(row=255), dict(pages=(1 << 24) + 1), dict(batch=(1 << 24) + 1),
-             dict(width=1 << 21, page=16), dict(width=1 << 63, page=2), dict(dim=257, row=4 * 257)]
+             dict(width=1 << 21, page=16), dict(pages=1 << 20, page=1 << 11), dict(width=1 << 63, page=2), dict(dim=257, row=4 * 257)]
 
 
 def append(c, **kw):
