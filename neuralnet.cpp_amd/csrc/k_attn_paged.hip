@@ -45,7 +45,7 @@ struct PagedArgs
     float *m, *l;
     float *part_ml, *part_o;   // per (row of the batch, range): m and l; O unnormalised
     unsigned q_heads, group, n_shared, n_own, shared_blocks, shared_row_blocks, own_row_blocks;
-    int shared_rws, own_rws;
+    int shared_row_waves, own_row_waves, own_wide;   // own_wide: own parts in RT row tiles a wave too
     float alpha;
 };
 
@@ -81,10 +81,9 @@ template <int KS> struct Tile
 // tile's loads back behind this one's: the weights of such positions are 0, and their values are cleared before
 // use (0 times a NaN that lies there would be one).
 template <int KS, int MODE>
-__device__ __forceinline__ void load_tile(const PagedArgs& a, int row, unsigned h, int lane, Tile<KS>& x)
+__device__ __forceinline__ void load_keys(const PagedArgs& a, int row, unsigned h, int lane, Tile<KS>& x)
 {
-    using G = Geometry<KS>;
-    const int j = lane & 15, g = lane >> 4, dim = a.c.dim;
+    const int g = lane >> 4, dim = a.c.dim;
     const float* kp = a.c.K + (size_t)max(row, 0) * a.c.row + (size_t)h * dim;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
@@ -101,6 +100,12 @@ __device__ __forceinline__ void load_tile(const PagedArgs& a, int row, unsigned 
             for (int e = 0; e < 4; ++e) x.k[i][e] = kp[d + e < dim ? d + e : 0];
         }
     }
+}
+template <int KS, int MODE>
+__device__ __forceinline__ void load_values(const PagedArgs& a, int row, unsigned h, int lane, Tile<KS>& x)
+{
+    using G = Geometry<KS>;
+    const int j = lane & 15, g = lane >> 4, dim = a.c.dim;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
     {
@@ -138,48 +143,39 @@ template <int KS, int MODE> __device__ __forceinline__ void cut(f32x4 (&x)[KS], 
     }
 }
 
-// What the running softmax of a lane's row holds.
-template <int KS> struct State
+// A lane's row of each of a wave's row tiles: its query dims, the sequence's length, the bias' slope, whether the
+// positions count for it; and the running softmax.
+template <int KS> struct Row
 {
     using G = Geometry<KS>;
+    f32x4 q[KS];
+    int len;
+    float slope;
+    bool counts;
     float m, l;   // l: of the lane's positions alone
     f32x4 o[G::T][G::VW];
 };
 
-template <int KS, int MODE>
-__device__ __forceinline__ void use_tile(const PagedArgs& a, Tile<KS>& x, const f32x4 (&q)[KS], int p0, int g, int len,
-                                         bool counts, float slope, State<KS>& st)
+template <int KS, int MODE, int RT>
+__device__ __forceinline__ void use_keys(const PagedArgs& a, Tile<KS>& x, const Row<KS> (&rows)[RT], int g, f32x4 (&s)[RT])
+{
+    cut<KS, MODE>(x.k, g, a.c.dim);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[k][e], rows[i].q[k][e], s[i], 0, 0, 0);
+}
+
+template <int KS, int RT>
+__device__ __forceinline__ void use_values(const PagedArgs& a, Tile<KS>& x, f32x4 (&s)[RT], Row<KS> (&rows)[RT], int p0,
+                                           int g)
 {
     using G = Geometry<KS>;
-    cut<KS, MODE>(x.k, g, a.c.dim);
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[i][e], q[i][e], s, 0, 0, 0);
-    float top = kLowest;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-    {
-        float z = a.alpha * s[r];
-        if (a.slopes) z -= slope * (float)(len - 1 - (p0 + 4 * g + r));
-        s[r] = x.row[r] >= 0 && counts ? z : -__builtin_inff();
-        top = fmax_std(top, s[r]);
-    }
-    top = fmax_std(top, __shfl_xor(top, 16, 64));
-    top = fmax_std(top, __shfl_xor(top, 32, 64));
-    const float mn = fmax_std(st.m, top);
-    const float f = __builtin_amdgcn_exp2f((st.m - mn) * kLog2e);
-    const float mb = mn == kLowest ? 0.0f : mn * kLog2e;
-    float sum = 0.0f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-    {
-        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], kLog2e, -mb));
-        sum += s[r];
-    }
-    st.l = st.l * f + sum;
-    st.m = mn;
     const int least = min(min(x.row[0], x.row[1]), min(x.row[2], x.row[3]));
     if (__builtin_amdgcn_ballot_w64(least < 0))
     {
@@ -191,80 +187,91 @@ __device__ __forceinline__ void use_tile(const PagedArgs& a, Tile<KS>& x, const 
                 for (int y = 0; y < G::VW; ++y) x.v[r][t][y] = x.row[r] < 0 ? 0.0f : x.v[r][t][y];
     }
 #pragma unroll
-    for (int t = 0; t < G::T; ++t)
+    for (int i = 0; i < RT; ++i)
+    {
+        Row<KS>& w = rows[i];
+        float top = kLowest;
 #pragma unroll
-        for (int y = 0; y < G::VW; ++y) st.o[t][y] *= f;
+        for (int r = 0; r < 4; ++r)
+        {
+            float z = a.alpha * s[i][r];
+            if (a.slopes) z -= w.slope * (float)(w.len - 1 - (p0 + 4 * g + r));
+            s[i][r] = x.row[r] >= 0 && w.counts ? z : -__builtin_inff();
+            top = fmax_std(top, s[i][r]);
+        }
+        top = fmax_std(top, __shfl_xor(top, 16, 64));
+        top = fmax_std(top, __shfl_xor(top, 32, 64));
+        const float mn = fmax_std(w.m, top);
+        const float f = __builtin_amdgcn_exp2f((w.m - mn) * kLog2e);
+        const float mb = mn == kLowest ? 0.0f : mn * kLog2e;
+        float sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
+        {
+            s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], kLog2e, -mb));
+            sum += s[i][r];
+        }
+        w.l = w.l * f + sum;
+        w.m = mn;
+        if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
+        {
 #pragma unroll
-        for (int t = 0; t < G::T; ++t)
+            for (int t = 0; t < G::T; ++t)
 #pragma unroll
-            for (int y = 0; y < G::VW; ++y)
-                st.o[t][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[r][t][y], s[r], st.o[t][y], 0, 0, 0);
+                for (int y = 0; y < G::VW; ++y) w.o[t][y] *= f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < G::T; ++t)
+#pragma unroll
+                for (int y = 0; y < G::VW; ++y)
+                    w.o[t][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[r][t][y], s[i][r], w.o[t][y], 0, 0, 0);
+    }
 }
 
-// rws of the 4 waves lie along the rows (16 rws rows a workgroup), the others take the range's positions in turn.
-template <int KS, int MODE> __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a)
+// A workgroup's rows and positions.
+struct Part
+{
+    unsigned b0, nb, h, rb, slot;   // sequences b0 .. b0 + nb - 1, key head, block of rows, range of all
+    int begin, end, common, row_waves;
+    bool is_shared;
+};
+template <int KS> struct PartShared
+{
+    float o[4][kTile][Geometry<KS>::DV + 4];
+    float ml[4][kTile][2];
+};
+
+// One range of positions. row_waves of the 4 waves lie along the rows, RT tiles each; the others take 16 positions
+// each in turn.
+template <int KS, int MODE, int RT>
+__device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartShared<KS>& sh)
 {
     using G = Geometry<KS>;
     constexpr int DP = G::DV;
-    __shared__ float o_s[4][kTile][DP + 4];
-    __shared__ float ml_s[4][kTile][2];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int j = lane & 15, g = lane >> 4;
-    const unsigned per = a.q_heads / a.c.heads;   // query heads of a key head
-
-    // Which range of which positions for which rows.
-    unsigned i = blockIdx.x;
-    const bool is_shared = i < a.shared_blocks;
-    const int rws = is_shared ? a.shared_rws : a.own_rws, kws = 4 / rws, rw = wave % rws, kw = wave / rws;
-    unsigned b0, nb, h, c, rb;   // sequences b0 .. b0 + nb - 1, key head, range, block of rows
-    if (is_shared)
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, j = lane & 15, g = lane >> 4, dim = a.c.dim;
+    const unsigned per = a.q_heads / a.c.heads, n_rows = part.nb * per;   // per: query heads of a key head
+    const int rws = part.row_waves, kws = 4 / rws, rw = wave % rws, kw = wave / rws, step = kws * kTile;
+    const int most = (int)(a.c.width * a.c.page.d), begin = part.begin, end = part.end;
+    Row<KS> rows[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
     {
-        rb = i % a.shared_row_blocks;
-        i /= a.shared_row_blocks;
-        c = i % a.n_shared;
-        i /= a.n_shared;
-        h = i % a.c.heads;
-        b0 = i / a.c.heads * a.group;
-        nb = a.group;
-    }
-    else
-    {
-        i -= a.shared_blocks;
-        rb = i % a.own_row_blocks;
-        i /= a.own_row_blocks;
-        c = i % a.n_own;
-        i /= a.n_own;
-        h = i % a.c.heads;
-        b0 = i / a.c.heads;
-        nb = 1;
-    }
-    const int most = (int)(a.c.width * a.c.page.d);
-    const int common = shared_of(a, b0);
-    int lo = 0, hi = common;
-    if (!is_shared)
-    {
-        hi = length_of(a.len[b0], most);
-        lo = hi >= common ? common : 0;
-    }
-    const int ranges = is_shared ? a.n_shared : a.n_own;
-    const int step = kws * kTile, steps = (hi - lo + step - 1) / step;
-    const int first = (int)((long)steps * c / ranges), last = (int)((long)steps * (c + 1) / ranges);
-    const int begin = lo + first * step, end = min(hi, lo + last * step);
-
-    // The lane's row.
-    const unsigned row = (rb * rws + rw) * kTile + j;
-    const bool live = row < nb * per;
-    const unsigned b = live ? b0 + row / per : b0, qh = h * per + (live ? row % per : 0);
-    const int len = live ? length_of(a.len[b], most) : 0;
-    const bool counts = live && (!is_shared || len >= common);
-    const float slope = a.slopes && live ? a.slopes[qh] : 0.0f;
-    const int dim = a.c.dim;
-    State<KS> st{kLowest, 0.0f, {}};
-    if (begin < end)
-    {
-        f32x4 q[KS];
+        Row<KS>& w = rows[i];
+        const unsigned row = ((part.rb * rws + rw) * RT + i) * kTile + j;
+        const bool live = row < n_rows;
+        const unsigned b = live ? part.b0 + row / per : part.b0, qh = part.h * per + (live ? row % per : 0);
+        w.len = live ? length_of(a.len[b], most) : 0;
+        w.counts = live && (!part.is_shared || w.len >= part.common);
+        w.slope = a.slopes && live ? a.slopes[qh] : 0.0f;
+        w.m = kLowest;
+        w.l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < G::T; ++x)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y) w.o[x][y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (begin >= end) continue;
         const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;
 #pragma unroll
         for (int x = 0; x < KS; ++x)
@@ -272,81 +279,122 @@ template <int KS, int MODE> __global__ __launch_bounds__(256) void k_attn_paged(
             for (int e = 0; e < 4; ++e)
             {
                 const int d = 16 * x + 4 * g + e;
-                q[x][e] = qp[(long)(d < dim ? d : 0) * a.q_f];   // rows that are not live are formed and dropped
+                w.q[x][e] = qp[(long)(d < dim ? d : 0) * a.q_f];   // rows that are not live are formed and dropped
             }
-        // The loads stay in one run: without this each would move into a branch of the selection below.
+    }
+    if (begin < end)
+    {
 #pragma unroll
-        for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[x]));
-        cut<KS, MODE>(q, g, dim);
+        for (int i = 0; i < RT; ++i)
+        {
+            // The loads stay in one run: without this each would move into a branch of the selection that follows.
+#pragma unroll
+            for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(rows[i].q[x]));
+            cut<KS, MODE>(rows[i].q, g, dim);
+        }
         // Table entries are loaded two tiles ahead of their use, keys and values one: the entries' loads are then
         // older than the keys' and values' that are still on their way when the addresses are formed.
-        auto entry = [&](int p) { return a.c.entry_of(b0, p + j); };
+        auto entry = [&](int p) { return a.c.entry_of(part.b0, p + j); };
         auto row_at = [&](float e, int p) {
             const int r = a.c.row_in(e, p + j);
             return p + j < end ? r : -1;
         };
         const int p1 = begin + kw * kTile;
-        Tile<KS> x0, x1;
         const float first = entry(p1);
         float ahead = entry(p1 + step);
-        load_tile<KS, MODE>(a, row_at(first, p1), h, lane, x0);
-        for (int p = p1; p < end; p += 2 * step)
+        f32x4 s[RT];
+        if constexpr (RT == 1)
         {
-            float further = entry(p + 2 * step);
-            load_tile<KS, MODE>(a, row_at(ahead, p + step), h, lane, x1);
-            __builtin_amdgcn_sched_barrier(0);
-            use_tile<KS, MODE>(a, x0, q, p, g, len, counts, slope, st);
-            ahead = entry(p + 3 * step);
-            load_tile<KS, MODE>(a, row_at(further, p + 2 * step), h, lane, x0);
-            __builtin_amdgcn_sched_barrier(0);
-            use_tile<KS, MODE>(a, x1, q, p + step, g, len, counts, slope, st);
+            Tile<KS> x[2];
+            const int r0 = row_at(first, p1);
+            load_keys<KS, MODE>(a, r0, part.h, lane, x[0]);
+            load_values<KS, MODE>(a, r0, part.h, lane, x[0]);
+            for (int p = p1; p < end; p += 2 * step)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                {
+                    const int at = p + half * step;
+                    const float further = entry(at + 2 * step);
+                    const int r = row_at(ahead, at + step);
+                    load_keys<KS, MODE>(a, r, part.h, lane, x[1 - half]);
+                    load_values<KS, MODE>(a, r, part.h, lane, x[1 - half]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    use_keys<KS, MODE, RT>(a, x[half], rows, g, s);
+                    use_values<KS, RT>(a, x[half], s, rows, at, g);
+                    ahead = further;
+                }
         }
-        st.l += __shfl_xor(st.l, 16, 64);
-        st.l += __shfl_xor(st.l, 32, 64);
+        else
+        {
+            // The registers hold one tile: its keys' loads follow the products of the keys before, its values' those
+            // of the values before. Each has the other products' time, some 2000 cycles, to arrive.
+            Tile<KS> x;
+            const int r0 = row_at(first, p1);
+            load_keys<KS, MODE>(a, r0, part.h, lane, x);
+            load_values<KS, MODE>(a, r0, part.h, lane, x);
+            for (int p = p1; p < end; p += step)
+            {
+                use_keys<KS, MODE, RT>(a, x, rows, g, s);
+                __builtin_amdgcn_sched_barrier(0);
+                const float further = entry(p + 2 * step);
+                const int r = row_at(ahead, p + step);
+                load_keys<KS, MODE>(a, r, part.h, lane, x);
+                __builtin_amdgcn_sched_barrier(0);
+                use_values<KS, RT>(a, x, s, rows, p, g);
+                __builtin_amdgcn_sched_barrier(0);
+                load_values<KS, MODE>(a, r, part.h, lane, x);
+                ahead = further;
+            }
+        }
     }
 
-    // The waves of the same rows are joined through LDS, in the order of their positions.
-    if (g == 0)
-    {
-        ml_s[wave][j][0] = st.m;
-        ml_s[wave][j][1] = st.l;
-    }
-#pragma unroll
-    for (int x = 0; x < G::T; ++x)
-#pragma unroll
-        for (int y = 0; y < G::VW; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o_s[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = st.o[x][y][r];
-    __syncthreads();
-    const unsigned n_parts = a.n_shared + a.n_own, slot = is_shared ? c : a.n_shared + c;
+    // The waves are joined through LDS, in the order of their positions, a row tile at a time.
+    const unsigned n_parts = a.n_shared + a.n_own;
     const bool direct = n_parts == 1;
-    for (int w = 0; w < rws; ++w)
-        for (int e = t; e < kTile * DP; e += 256)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        Row<KS>& w = rows[i];
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+        if (i) __syncthreads();
+        if (g == 0)
         {
-            const int jr = e / DP, d = e % DP;
-            const unsigned rr = (rb * rws + w) * kTile + jr;
-            if (rr >= nb * per || d >= dim) continue;
-            const unsigned bb = b0 + rr / per, hh = h * per + rr % per;
+            sh.ml[wave][j][0] = w.m;
+            sh.ml[wave][j][1] = w.l;
+        }
+#pragma unroll
+        for (int x = 0; x < G::T; ++x)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sh.o[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = w.o[x][y][r];
+        __syncthreads();
+        for (int e = t; e < rws * kTile * DP; e += 256)
+        {
+            const int d = e % DP, jr = e / DP % kTile, rv = e / (DP * kTile);   // rv: row wave
+            const unsigned row = ((part.rb * rws + rv) * RT + i) * kTile + jr;
+            if (row >= n_rows || d >= dim) continue;
+            const unsigned b = part.b0 + row / per, qh = part.h * per + row % per;
             float mm = kLowest, ll = 0.0f, oo = 0.0f;
-            for (int k = w; k < 4; k += rws) mm = fmax_std(mm, ml_s[k][jr][0]);
-            for (int k = w; k < 4; k += rws)
+            for (int k = rv; k < 4; k += rws) mm = fmax_std(mm, sh.ml[k][jr][0]);
+            for (int k = rv; k < 4; k += rws)
             {
-                const float lk = ml_s[k][jr][1];
-                if (lk == 0.0f) continue;
-                const float f = __builtin_amdgcn_exp2f((ml_s[k][jr][0] - mm) * kLog2e);
-                ll += lk * f;
-                oo += o_s[k][jr][d] * f;
+                const float lk = sh.ml[k][jr][1];
+                const float f = __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
+                ll += lk == 0.0f ? 0.0f : lk * f;
+                oo += lk == 0.0f ? 0.0f : sh.o[k][jr][d] * f;
             }
-            const size_t at = (size_t)bb * a.q_heads + hh;
+            const size_t at = (size_t)b * a.q_heads + qh;
             if (direct)
             {
-                a.O[(long)bb * a.o_t + ((long)hh * dim + d) * a.o_f] = ll == 0.0f ? 0.0f : oo / ll;
+                a.O[(long)b * a.o_t + ((long)qh * dim + d) * a.o_f] = ll == 0.0f ? 0.0f : oo / ll;
                 if (d == 0 && a.m) a.m[at] = mm;
                 if (d == 0 && a.l) a.l[at] = ll;
             }
             else
             {
-                const size_t p = at * n_parts + slot;
+                const size_t p = at * n_parts + part.slot;
                 a.part_o[p * dim + d] = oo;
                 if (d == 0)
                 {
@@ -355,6 +403,46 @@ template <int KS, int MODE> __global__ __launch_bounds__(256) void k_attn_paged(
                 }
             }
         }
+    }
+}
+
+// RT: row tiles of the shared parts, and of the own ones where a key head has more than 16 query heads.
+template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kSingle ? 1 : 2) void k_attn_paged(PagedArgs a)
+{
+    __shared__ PartShared<KS> sh;
+    Part part;
+    unsigned i = blockIdx.x, c;
+    part.is_shared = i < a.shared_blocks;
+    if (!part.is_shared) i -= a.shared_blocks;
+    const unsigned row_blocks = part.is_shared ? a.shared_row_blocks : a.own_row_blocks;
+    const unsigned ranges = part.is_shared ? a.n_shared : a.n_own;
+    // The blocks of rows that read the same keys and values run on one XCD (workgroups go to the 8 in turn), so
+    // that its L2 holds them once; the pieces are padded to a multiple of 8.
+    part.rb = i / 8 % row_blocks;
+    i = i / (8 * row_blocks) * 8 + i % 8;
+    c = i % ranges;
+    i /= ranges;
+    part.h = i % a.c.heads;
+    i /= a.c.heads;
+    part.nb = part.is_shared ? a.group : 1;
+    if (i >= a.c.batch / part.nb) return;
+    part.b0 = i * part.nb;
+    part.slot = part.is_shared ? c : a.n_shared + c;
+    part.row_waves = part.is_shared ? a.shared_row_waves : a.own_row_waves;
+    part.common = shared_of(a, part.b0);
+    int lo = 0, hi = part.common;
+    if (!part.is_shared)
+    {
+        hi = length_of(a.len[part.b0], (int)(a.c.width * a.c.page.d));
+        lo = hi >= part.common ? part.common : 0;
+    }
+    constexpr int kStep = 4 * kTile;
+    const int steps = (hi - lo + kStep - 1) / kStep;
+    const int first = (int)((long)steps * c / ranges), last = (int)((long)steps * (c + 1) / ranges);
+    part.begin = lo + first * kStep;
+    part.end = min(hi, lo + last * kStep);
+    if (RT == 1 || part.is_shared || a.own_wide) walk<KS, MODE, RT>(a, part, sh);
+    else walk<KS, MODE, 1>(a, part, sh);
 }
 
 // Joins the ranges of one row in order: blockIdx.x = sequence * q_heads + head. The ranges' factors go to LDS,
@@ -411,8 +499,8 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
 
 struct PagedPlan
 {
+    int row_tiles, shared_row_waves, own_row_waves, own_wide;
     unsigned n_shared, n_own, shared_row_blocks, own_row_blocks;
-    int shared_rws, own_rws;
     size_t shared_blocks, own_blocks;
     size_t parts() const { return (size_t)n_shared + n_own; }
 };
@@ -422,32 +510,38 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
 {
     PagedPlan p{};
     const size_t per = q_heads / c.heads, most = c.width * c.page, target = 2 * (size_t)device_cus();
-    auto along_rows = [](size_t rows, int& rws, unsigned& blocks) {
-        rws = rows > 32 ? 4 : rows > 16 ? 2 : 1;
-        blocks = static_cast<unsigned>((rows + kTile * rws - 1) / (kTile * rws));
+    const size_t rows = group > 1 ? group * per : per;   // that read the same positions
+    p.row_tiles = rows > kTile ? 2 : 1;
+    p.own_wide = per > kTile;
+    auto along_rows = [](size_t n, int tiles, int& waves) {
+        const size_t need = (n + kTile * tiles - 1) / (kTile * tiles);
+        waves = need > 2 ? 4 : need > 1 ? 2 : 1;
+        return static_cast<unsigned>((need + waves - 1) / waves);
     };
     auto ranges = [&](size_t others) {
         const size_t want = (target + others - 1) / others, most_ranges = (most + 63) / 64;
         return static_cast<unsigned>(want < most_ranges ? want : most_ranges);
     };
-    along_rows(per, p.own_rws, p.own_row_blocks);
-    const size_t own = c.batch * c.heads * p.own_row_blocks;
-    p.n_own = ranges(own);
-    p.own_blocks = own * p.n_own;
+    auto blocks = [](size_t pieces, unsigned row_blocks) { return (pieces + 7) / 8 * 8 * row_blocks; };
+    p.own_row_blocks = along_rows(per, p.own_wide ? 2 : 1, p.own_row_waves);
+    const size_t own = c.batch * c.heads;
+    p.n_own = ranges(own * p.own_row_blocks);
+    p.own_blocks = blocks(own * p.n_own, p.own_row_blocks);
     if (group > 1)
     {
-        along_rows(group * per, p.shared_rws, p.shared_row_blocks);
-        const size_t sh = c.batch / group * c.heads * p.shared_row_blocks;
-        p.n_shared = ranges(sh);
-        p.shared_blocks = sh * p.n_shared;
+        p.shared_row_blocks = along_rows(rows, p.row_tiles, p.shared_row_waves);
+        const size_t sh = c.batch / group * c.heads;
+        p.n_shared = ranges(sh * p.shared_row_blocks);
+        p.shared_blocks = blocks(sh * p.n_shared, p.shared_row_blocks);
     }
     return p;
 }
 
 template <int KS, int MODE> void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s)
 {
-    hipLaunchKernelGGL((k_attn_paged<KS, MODE>), dim3(static_cast<unsigned>(p.shared_blocks + p.own_blocks)), dim3(256),
-                       0, s, a);
+    const dim3 grid(static_cast<unsigned>(p.shared_blocks + p.own_blocks));
+    if (p.row_tiles == 1) hipLaunchKernelGGL((k_attn_paged<KS, MODE, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_paged<KS, MODE, 2>), grid, dim3(256), 0, s, a);
 }
 
 bool paged_ok(const nnhip_kv_pages* c, size_t q_heads, size_t group)
@@ -489,7 +583,8 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     auto* ws = static_cast<float*>(workspace);
     PagedArgs a{pages_of(*c), q, q_t, q_f, len, shared, slopes, O, o_t, o_f, m, l, ws, nullptr,
                 static_cast<unsigned>(q_heads), static_cast<unsigned>(group), p.n_shared, p.n_own,
-                static_cast<unsigned>(p.shared_blocks), p.shared_row_blocks, p.own_row_blocks, p.shared_rws, p.own_rws,
+                static_cast<unsigned>(p.shared_blocks), p.shared_row_blocks, p.own_row_blocks, p.shared_row_waves,
+                p.own_row_waves, p.own_wide,
                 alpha};
     if (p.parts() > 1) a.part_o = ws + 2 * c->batch * q_heads * p.parts();
     const size_t d = c->dim;
