@@ -331,7 +331,9 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
             Tile<KS> x;
             const int r0 = row_at(first, p1);
             load_keys<KS, MODE>(a, r0, part.h, lane, x);
+            __builtin_amdgcn_sched_barrier(0);
             load_values<KS, MODE>(a, r0, part.h, lane, x);
+            __builtin_amdgcn_sched_barrier(0);
             for (int p = p1; p < end; p += step)
             {
                 use_keys<KS, MODE, RT>(a, x, rows, g, s);
