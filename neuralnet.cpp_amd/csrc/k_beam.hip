@@ -17,12 +17,14 @@ namespace nnhip
 namespace
 {
 
-constexpr int kSegColumn = 64;    // tokens of a segment, (vocab, beams) logits
-constexpr int kSegRow = 256;      // tokens of a segment, (beams, vocab) logits
+constexpr unsigned kSegColumn = 64;   // tokens that a thread loads at once, (vocab, beams) logits
+constexpr unsigned kSegRow = 256;     // tokens that 16 lanes load at once, (beams, vocab) logits
+constexpr unsigned kSegMost = 4096;
+constexpr int kHeld = 16;             // items of a thread that the selection holds in registers
 constexpr int kMaxTake = 256;
 constexpr int kMaxBeams = 1024;
 constexpr int kList = 512;        // candidates that are ranked one against another
-constexpr int kBins = 1024;
+constexpr int kLog2Bins = 10, kBins = 1 << kLog2Bins;
 constexpr int kPickThreads = 1024;
 
 struct BeamArgs
@@ -30,6 +32,7 @@ struct BeamArgs
     const float *logits, *scores, *done;
     size_t ld;
     unsigned groups, beams, vocab, take, eos, n_seg, seg;
+    FastDiv by_seg, by_n_seg;
     int beam_major;
     float2* part;   // per (beam of all groups, segment): largest logit, sum of exp(logit - largest)
     float *out_score, *out_beam, *out_token;
@@ -46,6 +49,15 @@ __device__ __forceinline__ float exp_below(float x, float m)
     return e == 0.0f ? 0.0f : __builtin_fmaf(e, r * kLn2, e);   // r is NaN for d = -inf
 }
 
+// Takes a further part of a segment (largest m2, sum s2 of exp(logit - m2), m2 as 0 where it is -inf) in.
+__device__ __forceinline__ void take_in(float& m, float& s, float m2, float s2)
+{
+    const float mn = fmax_std(m, m2), base = mn == -__builtin_inff() ? 0.0f : mn;
+    // an all -inf part has the sum 0 (or NaN), whatever its factor is
+    s = s * exp_below(m, base) + s2 * exp_below(m2, base);
+    m = mn;
+}
+
 // (vocab, beams) logits: a thread takes one segment of one beam, neighbouring threads neighbouring beams.
 __global__ __launch_bounds__(256) void k_beam_segments_column(BeamArgs a)
 {
@@ -54,16 +66,27 @@ __global__ __launch_bounds__(256) void k_beam_segments_column(BeamArgs a)
     if (i >= (size_t)all * a.n_seg) return;
     const unsigned seg = (unsigned)(i / all), n = (unsigned)(i % all);
     if (a.done && a.done[n] != 0.0f) return;
-    const unsigned v0 = seg * kSegColumn, nv = min((unsigned)kSegColumn, a.vocab - v0);
-    const float* p = a.logits + (size_t)v0 * a.ld + n;
-    float x[kSegColumn], m = -__builtin_inff(), s = 0.0f;
+    float m = -__builtin_inff(), s = 0.0f;
+    const unsigned v1 = min((seg + 1) * a.seg, a.vocab);
+    for (unsigned v0 = seg * a.seg; v0 < v1; v0 += kSegColumn)
+    {
+        const unsigned nv = min(kSegColumn, v1 - v0);
+        const float* p = a.logits + (size_t)v0 * a.ld + n;
+        float x[kSegColumn], mc = -__builtin_inff(), sc = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kSegColumn; ++k) x[k] = k < (int)nv ? p[(size_t)k * a.ld] : -__builtin_inff();
+        for (unsigned k = 0; k < kSegColumn; ++k) x[k] = k < nv ? p[(size_t)k * a.ld] : -__builtin_inff();
 #pragma unroll
-    for (int k = 0; k < kSegColumn; ++k) m = fmax_std(m, x[k]);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
+        for (unsigned k = 0; k < kSegColumn; ++k) mc = fmax_std(mc, x[k]);
+        const float base = mc == -__builtin_inff() ? 0.0f : mc;
 #pragma unroll
-    for (int k = 0; k < kSegColumn; ++k) s += exp_below(x[k], base);
+        for (unsigned k = 0; k < kSegColumn; ++k) sc += exp_below(x[k], base);
+        if (v0 == seg * a.seg)
+        {
+            m = mc;
+            s = sc;
+        }
+        else take_in(m, s, mc, sc);
+    }
     a.part[(size_t)n * a.n_seg + seg] = make_float2(m, s);
 }
 
@@ -74,22 +97,32 @@ __global__ __launch_bounds__(256) void k_beam_segments_row(BeamArgs a)
     const unsigned n = blockIdx.y, lane = threadIdx.x & 15, seg = blockIdx.x * 16 + (threadIdx.x >> 4);
     if (a.done && a.done[n] != 0.0f) return;
     if (seg >= a.n_seg) return;   // whole groups of 16 lanes
-    const unsigned v0 = seg * kSegRow;
     const float* p = a.logits + (size_t)n * a.ld;
-    float x[kPer], m = -__builtin_inff(), s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k)
+    float m = -__builtin_inff(), s = 0.0f;
+    const unsigned v1 = min((seg + 1) * a.seg, a.vocab);
+    for (unsigned v0 = seg * a.seg; v0 < v1; v0 += kSegRow)
     {
-        const unsigned v = v0 + 16 * k + lane;
-        x[k] = v < a.vocab ? p[v] : -__builtin_inff();
+        float x[kPer], mc = -__builtin_inff(), sc = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+        {
+            const unsigned v = v0 + 16 * k + lane;
+            x[k] = v < v1 ? p[v] : -__builtin_inff();
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) mc = fmax_std(mc, x[k]);
+        for (int o = 8; o > 0; o >>= 1) mc = fmax_std(mc, __shfl_xor(mc, o, 16));
+        const float base = mc == -__builtin_inff() ? 0.0f : mc;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) sc += exp_below(x[k], base);
+        for (int o = 8; o > 0; o >>= 1) sc += __shfl_xor(sc, o, 16);
+        if (v0 == seg * a.seg)
+        {
+            m = mc;
+            s = sc;
+        }
+        else take_in(m, s, mc, sc);
     }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) m = fmax_std(m, x[k]);
-    for (int o = 8; o > 0; o >>= 1) m = fmax_std(m, __shfl_xor(m, o, 16));
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) s += exp_below(x[k], base);
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
     if (lane == 0) a.part[(size_t)n * a.n_seg + seg] = make_float2(m, s);
 }
 
@@ -110,6 +143,8 @@ __device__ __forceinline__ double value_of(u64 k)
 struct PickShared
 {
     double lse[kMaxBeams];
+    float score[kMaxBeams];
+    unsigned char ended[kMaxBeams];
     u64 key[kList];
     unsigned idx[kList];
     unsigned hist[kBins];
@@ -143,27 +178,40 @@ __device__ void find_bin(PickShared& s, unsigned k, bool down)
 }
 
 // Puts into the list at most kList of n items, the first k by (key descending, index ascending) among them; k
-// <= n, k <= kMaxTake. get(i) gives item i's key and index; indices differ. A histogram over the keys' range
-// narrows it to the bin that holds the k-th; where keys are equal, one over the indices follows.
-template <class Get> __device__ void pick(PickShared& s, unsigned n, unsigned k, Get get)
+// <= n, k <= kMaxTake. key(i) and index(i) give item i's; indices differ. A histogram over the keys' range
+// narrows it to the bin that holds the k-th; where keys are equal, one over the indices follows. With HELD the
+// keys stay in registers (n <= kHeld * kPickThreads), loaded all at once; else each pass forms them again.
+template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s, unsigned n, unsigned k, Key key, Index index)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const u64 neg_inf = key_of(-__builtin_inf());
+    u64 held[HELD ? kHeld : 1];
+    if constexpr (HELD)
+    {
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) held[r] = t + r * kPickThreads < n ? key(t + r * kPickThreads) : 0;
+    }
+    auto each = [&](auto&& f) {
+        if constexpr (HELD)
+        {
+#pragma unroll
+            for (int r = 0; r < kHeld; ++r)
+                if (t + r * kPickThreads < n) f(t + r * kPickThreads, held[r]);
+        }
+        else
+            for (unsigned i = t; i < n; i += kPickThreads) f(i, key(i));
+    };
     // Range of the keys above -inf, if those suffice.
     u64 lo = ~0ull, hi = 0;
     unsigned above_inf = 0;
-    for (unsigned i = t; i < n; i += kPickThreads)
-    {
-        u64 key;
-        unsigned idx;
-        get(i, key, idx);
-        hi = key > hi ? key : hi;
-        if (key > neg_inf)
+    each([&](unsigned, u64 x) {
+        hi = x > hi ? x : hi;
+        if (x > neg_inf)
         {
-            lo = key < lo ? key : lo;
+            lo = x < lo ? x : lo;
             ++above_inf;
         }
-    }
+    });
     for (int o = 32; o > 0; o >>= 1)
     {
         const u64 l2 = __shfl_xor(lo, o, 64), h2 = __shfl_xor(hi, o, 64);
@@ -178,8 +226,10 @@ template <class Get> __device__ void pick(PickShared& s, unsigned n, unsigned k,
         s.red[1][wave] = hi;
         s.wave[wave] = above_inf;
     }
+    s.hist[t] = 0;
     __syncthreads();
     above_inf = 0;
+#pragma unroll
     for (int w = 0; w < kPickThreads / 64; ++w)
     {
         lo = s.red[0][w] < lo ? s.red[0][w] : lo;
@@ -191,21 +241,17 @@ template <class Get> __device__ void pick(PickShared& s, unsigned n, unsigned k,
     bool by_index = false;
     for (;;)
     {
-        u64 range = by_index ? (u64)(ihi - ilo) : hi - lo;
-        int shift = 0;
-        while ((range >> shift) >= (u64)kBins) ++shift;
-        __syncthreads();
-        s.hist[t] = 0;
-        __syncthreads();
-        for (unsigned i = t; i < n; i += kPickThreads)
-        {
-            u64 key;
-            unsigned idx;
-            get(i, key, idx);
-            if (key < lo || key > hi) continue;
-            if (!by_index) atomicAdd(&s.hist[(key - lo) >> shift], 1u);
-            else if (idx >= ilo && idx <= ihi) atomicAdd(&s.hist[(idx - ilo) >> shift], 1u);
-        }
+        const u64 range = by_index ? (u64)(ihi - ilo) : hi - lo;
+        const int shift = max(0, 64 - __clzll(range) - kLog2Bins);   // range >> shift < kBins
+        each([&](unsigned i, u64 x) {
+            if (x < lo || x > hi) return;
+            if (!by_index) atomicAdd(&s.hist[(x - lo) >> shift], 1u);
+            else
+            {
+                const unsigned idx = index(i);
+                if (idx >= ilo && idx <= ihi) atomicAdd(&s.hist[(idx - ilo) >> shift], 1u);
+            }
+        });
         __syncthreads();
         find_bin(s, k - base, !by_index);
         const unsigned bin = s.bin, here = s.hist[bin];
@@ -230,22 +276,22 @@ template <class Get> __device__ void pick(PickShared& s, unsigned n, unsigned k,
             ilo = 0;
             ihi = ~0u;
         }
+        __syncthreads();
+        s.hist[t] = 0;
+        __syncthreads();
     }
-    __syncthreads();
     if (t == 0) s.count = 0;
     __syncthreads();
-    for (unsigned i = t; i < n; i += kPickThreads)
-    {
-        u64 key;
-        unsigned idx;
-        get(i, key, idx);
-        if (key > hi || (key >= lo && (!by_index || idx <= ihi)))
+    each([&](unsigned i, u64 x) {
+        if (x < lo) return;
+        const unsigned idx = index(i);
+        if (x > hi || !by_index || idx <= ihi)
         {
             const unsigned at = atomicAdd(&s.count, 1u);
-            s.key[at] = key;
+            s.key[at] = x;
             s.idx[at] = idx;
         }
-    }
+    });
     __syncthreads();
 }
 
@@ -265,7 +311,7 @@ __device__ void rank_list(PickShared& s, unsigned k)
 }
 
 // One workgroup a group.
-__global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
+template <bool HELD> __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
 {
     __shared__ PickShared s;
     __shared__ unsigned seg_s[kMaxTake];
@@ -275,53 +321,70 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
     {
         const unsigned n = b0 + w;
         const float2* p = a.part + (size_t)n * a.n_seg;
+        const bool ended = a.done && a.done[n] != 0.0f;
+        const float score = a.scores[n];
         double lse = 0.0;
-        if (!(a.done && a.done[n] != 0.0f))
+        if (!ended)
         {
             float m = -__builtin_inff();
+#pragma unroll 8
             for (unsigned i = lane; i < a.n_seg; i += 64) m = fmax_std(m, p[i].x);
             m = wave_max(m);
             double sum = 0.0;
+#pragma unroll 8
             for (unsigned i = lane; i < a.n_seg; i += 64)
             {
                 const float2 x = p[i];
-                sum += (double)x.y * exp((double)x.x - (double)m);
+                sum += (double)(x.y * exp_below(x.x, m));   // NaN where m is an infinity, and so is lse
             }
             for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
             lse = (double)m + log(sum);
         }
-        if (lane == 0) s.lse[w] = lse;
+        if (lane == 0)
+        {
+            s.lse[w] = lse;
+            s.score[w] = score;
+            s.ended[w] = ended;
+        }
     }
     __syncthreads();
-    auto total = [&](unsigned w, bool ended, bool is_eos, float logit) {
-        const double sc = (double)a.scores[b0 + w];
-        return ended ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]);
+    auto total = [&](unsigned w, bool is_eos, float logit) {
+        const double sc = (double)s.score[w];
+        return key_of(s.ended[w] ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]));
     };
     // The best segments.
     const unsigned n_all = a.beams * a.n_seg, k_seg = min(a.take, n_all);
-    pick(s, n_all, k_seg, [&](unsigned i, u64& key, unsigned& idx) {
-        const unsigned w = i / a.n_seg, g = i % a.n_seg, n = b0 + w;
-        const bool ended = a.done && a.done[n] != 0.0f;
-        key = key_of(total(w, ended, a.eos / a.seg == g, ended ? 0.0f : a.part[(size_t)n * a.n_seg + g].x));
-        idx = i;
-    });
+    pick<HELD>(
+        s, n_all, k_seg,
+        [&](unsigned i) {
+            const unsigned w = a.by_n_seg.div(i), g = i - w * a.n_seg;
+            const float x = a.part[(size_t)b0 * a.n_seg + i].x;   // of an ended beam: anything, not used
+            return total(w, a.by_seg.div(a.eos) == g, x);
+        },
+        [](unsigned i) { return i; });
     rank_list(s, k_seg);
     if (t < (int)k_seg) seg_s[t] = s.idx[s.order[t]];
     __syncthreads();
-    // The best candidates of theirs.
-    pick(s, k_seg * a.seg, a.take, [&](unsigned i, u64& key, unsigned& idx) {
-        const unsigned g = seg_s[i / a.seg], w = g / a.n_seg, v = g % a.n_seg * a.seg + i % a.seg, n = b0 + w;
-        key = 0;   // behind every candidate
-        idx = w * a.vocab + v;
-        if (v >= a.vocab)
-        {
-            idx = a.beams * a.vocab + i;
-            return;
-        }
-        const bool ended = a.done && a.done[n] != 0.0f;
-        const float x = ended ? 0.0f : a.logits[a.beam_major ? (size_t)n * a.ld + v : (size_t)v * a.ld + n];
-        key = key_of(total(w, ended, v == a.eos, x));
-    });
+    // The best candidates of theirs. Places past the vocabulary have key 0, behind every candidate's.
+    auto place = [&](unsigned i, unsigned& w, unsigned& v) {
+        const unsigned q = a.by_seg.div(i), g = seg_s[q];
+        w = a.by_n_seg.div(g);
+        v = (g - w * a.n_seg) * a.seg + (i - q * a.seg);
+    };
+    pick<HELD>(
+        s, k_seg * a.seg, a.take,
+        [&](unsigned i) {
+            unsigned w, v;
+            place(i, w, v);
+            const size_t n = b0 + w, at = min(v, a.vocab - 1);
+            const float x = a.logits[a.beam_major ? n * a.ld + at : at * a.ld + n];
+            return v < a.vocab ? total(w, v == a.eos, x) : 0;
+        },
+        [&](unsigned i) {
+            unsigned w, v;
+            place(i, w, v);
+            return v < a.vocab ? w * a.vocab + v : a.beams * a.vocab + i;
+        });
     rank_list(s, a.take);
     if (t < (int)a.take)
     {
@@ -331,6 +394,15 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         a.out_beam[o] = (float)(b0 + idx / a.vocab);
         a.out_token[o] = (float)(idx % a.vocab);
     }
+}
+
+// Tokens of a segment: as few as the loads take at once, unless the group then has more segments than the
+// selection holds in registers.
+unsigned segment_of(bool beam_major, size_t beams, size_t vocab)
+{
+    unsigned seg = beam_major ? kSegRow : kSegColumn;
+    while (seg < kSegMost && beams * ((vocab + seg - 1) / seg) > (size_t)kHeld * kPickThreads) seg *= 2;
+    return seg;
 }
 
 bool beam_sizes_ok(size_t groups, size_t beams, size_t vocab, size_t take)
@@ -362,11 +434,11 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
         workspace_bytes < nnhip_beam_select_workspace_bytes(groups, beams, vocab, take) ||
         reinterpret_cast<uintptr_t>(workspace) % sizeof(float2) != 0)
         return -1;
-    const unsigned seg = beam_major ? kSegRow : kSegColumn;
+    const unsigned seg = segment_of(beam_major != 0, beams, vocab);
     const unsigned n_seg = static_cast<unsigned>((vocab + seg - 1) / seg), all = static_cast<unsigned>(groups * beams);
     BeamArgs a{logits, scores, done, ld, static_cast<unsigned>(groups), static_cast<unsigned>(beams),
-               static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg,
-               beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
+               static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg, FastDiv(seg),
+               FastDiv(n_seg), beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
     auto s = static_cast<hipStream_t>(stream);
     if (beam_major)
     {
@@ -380,6 +452,8 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
         hipLaunchKernelGGL(k_beam_segments_column, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
     }
     if (int rc = launch_status()) return rc;
-    hipLaunchKernelGGL(k_beam_pick, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
+    const bool held = beams * n_seg <= (size_t)kHeld * kPickThreads && take * seg <= (size_t)kHeld * kPickThreads;
+    if (held) hipLaunchKernelGGL(k_beam_pick<true>, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
+    else hipLaunchKernelGGL(k_beam_pick<false>, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
     return launch_status();
 }
