@@ -20,7 +20,7 @@ namespace
 constexpr unsigned kSegColumn = 64;   // tokens that a thread loads at once, (vocab, beams) logits
 constexpr unsigned kSegRow = 256;     // tokens that 16 lanes load at once, (beams, vocab) logits
 constexpr unsigned kSegMost = 4096;
-constexpr int kHeld = 16;             // items of a thread that the selection holds in registers
+constexpr unsigned kStored = 8192;    // segments of a group whose bins the selection keeps in LDS
 constexpr int kMaxTake = 256;
 constexpr int kMaxBeams = 1024;
 constexpr int kList = 512;        // candidates that are ranked one against another
@@ -142,7 +142,7 @@ __device__ __forceinline__ double value_of(u64 k)
 
 struct PickShared
 {
-    double lse[kMaxBeams];
+    double lse[kMaxBeams], best[kMaxBeams];
     float score[kMaxBeams];
     unsigned char ended[kMaxBeams];
     u64 key[kList];
@@ -152,54 +152,64 @@ struct PickShared
     u64 red[2][kPickThreads / 64];
     unsigned count, bin, above;
     unsigned order[kMaxTake];   // items of the list by rank
+    unsigned seg[kMaxTake];
+    unsigned short bins[kStored];
 };
 
 // The bin in which the running count, from bin 0 on (or from the last one down), reaches k: s.bin, and the
-// count before it, s.above.
-__device__ void find_bin(PickShared& s, unsigned k, bool down)
+// count before it, s.above; s.bin = kBins where it never does. The first wave's work, 16 bins a lane.
+__device__ __forceinline__ void find_bin(PickShared& s, unsigned k, bool down)
 {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const unsigned own = s.hist[down ? kBins - 1 - t : t];
-    unsigned sum = own;
-    for (int o = 1; o < 64; o <<= 1)
+    constexpr int kEach = kBins / 64;
+    const int lane = threadIdx.x;
+    if (lane < 64)
     {
-        const unsigned up = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += up;
-    }
-    if (lane == 63) s.wave[wave] = sum;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) sum += s.wave[w];
-    if (sum >= k && sum - own < k)
-    {
-        s.bin = down ? kBins - 1 - t : t;
-        s.above = sum - own;
+        unsigned h[kEach], own = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            h[i] = s.hist[down ? kBins - 1 - (lane * kEach + i) : lane * kEach + i];
+            own += h[i];
+        }
+        unsigned sum = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const unsigned up = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 63 && sum < k) s.bin = kBins;
+        unsigned before = sum - own;
+        if (sum >= k && before < k)
+        {
+            unsigned at = 0, above = before;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+            {
+                if (before < k)
+                {
+                    at = i;
+                    above = before;
+                }
+                before += h[i];
+            }
+            s.bin = down ? kBins - 1 - (lane * kEach + at) : lane * kEach + at;
+            s.above = above;
+        }
     }
     __syncthreads();
 }
 
 // Puts into the list at most kList of n items, the first k by (key descending, index ascending) among them; k
 // <= n, k <= kMaxTake. key(i) and index(i) give item i's; indices differ. A histogram over the keys' range
-// narrows it to the bin that holds the k-th; where keys are equal, one over the indices follows. With HELD the
-// keys stay in registers (n <= kHeld * kPickThreads), loaded all at once; else each pass forms them again.
-template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s, unsigned n, unsigned k, Key key, Index index)
+// narrows it to the bin that holds the k-th; where keys are equal, one over the indices follows. This takes any
+// keys; the selection comes here where its quick way does not end in a short list.
+template <class Key, class Index> __device__ __noinline__ void pick(PickShared& s, unsigned n, unsigned k, Key key, Index index)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const u64 neg_inf = key_of(-__builtin_inf());
-    u64 held[HELD ? kHeld : 1];
-    if constexpr (HELD)
-    {
-#pragma unroll
-        for (int r = 0; r < kHeld; ++r) held[r] = t + r * kPickThreads < n ? key(t + r * kPickThreads) : 0;
-    }
     auto each = [&](auto&& f) {
-        if constexpr (HELD)
-        {
-#pragma unroll
-            for (int r = 0; r < kHeld; ++r)
-                if (t + r * kPickThreads < n) f(t + r * kPickThreads, held[r]);
-        }
-        else
-            for (unsigned i = t; i < n; i += kPickThreads) f(i, key(i));
+        for (unsigned i = t; i < n; i += kPickThreads) f(i, key(i));
     };
     // Range of the keys above -inf, if those suffice.
     u64 lo = ~0ull, hi = 0;
@@ -226,10 +236,8 @@ template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s,
         s.red[1][wave] = hi;
         s.wave[wave] = above_inf;
     }
-    s.hist[t] = 0;
     __syncthreads();
     above_inf = 0;
-#pragma unroll
     for (int w = 0; w < kPickThreads / 64; ++w)
     {
         lo = s.red[0][w] < lo ? s.red[0][w] : lo;
@@ -241,8 +249,11 @@ template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s,
     bool by_index = false;
     for (;;)
     {
+        __syncthreads();
+        s.hist[t] = 0;
+        __syncthreads();
         const u64 range = by_index ? (u64)(ihi - ilo) : hi - lo;
-        const int shift = max(0, 64 - __clzll(range) - kLog2Bins);   // range >> shift < kBins
+        const int shift = range ? max(0, 64 - __clzll((long long)range) - kLog2Bins) : 0;   // range >> shift < kBins
         each([&](unsigned i, u64 x) {
             if (x < lo || x > hi) return;
             if (!by_index) atomicAdd(&s.hist[(x - lo) >> shift], 1u);
@@ -276,9 +287,6 @@ template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s,
             ilo = 0;
             ihi = ~0u;
         }
-        __syncthreads();
-        s.hist[t] = 0;
-        __syncthreads();
     }
     if (t == 0) s.count = 0;
     __syncthreads();
@@ -295,98 +303,196 @@ template <bool HELD, class Key, class Index> __device__ void pick(PickShared& s,
     __syncthreads();
 }
 
-// order[r] = the list's item of rank r, r < k (whatever order the items came in: indices differ).
-__device__ void rank_list(PickShared& s, unsigned k)
+// order[r] = the list's item of rank r, r < k (whatever order the items came in: indices differ). 16 lanes an item.
+__device__ __forceinline__ void rank_list(PickShared& s, unsigned k)
 {
-    const unsigned n = s.count;
-    for (unsigned i = threadIdx.x; i < n; i += kPickThreads)
+    const unsigned n = s.count, part = threadIdx.x & 15;
+    for (unsigned i = threadIdx.x >> 4; i < n; i += kPickThreads / 16)
     {
         const u64 key = s.key[i];
         const unsigned idx = s.idx[i];
         unsigned r = 0;
-        for (unsigned j = 0; j < n; ++j) r += s.key[j] > key || (s.key[j] == key && s.idx[j] < idx) ? 1u : 0u;
-        if (r < k) s.order[r] = i;
+#pragma unroll 4
+        for (unsigned j = part; j < n; j += 16) r += s.key[j] > key || (s.key[j] == key && s.idx[j] < idx) ? 1u : 0u;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) r += __shfl_xor(r, o, 16);
+        if (part == 0 && r < k) s.order[r] = i;
     }
     __syncthreads();
 }
 
-// One workgroup a group.
-template <bool HELD> __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
+// One workgroup a group. The kernel runs once over little data, so its time is that of the loads it waits for one
+// after another and of fetching its own code: loads go four at a time, and loops stay loops.
+__global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
 {
     __shared__ PickShared s;
-    __shared__ unsigned seg_s[kMaxTake];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const unsigned b0 = blockIdx.x * a.beams;
+    const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const unsigned b0 = blockIdx.x * a.beams, n_all = a.beams * a.n_seg, k_seg = min(a.take, n_all);
+    const bool stored = n_all <= kStored;
+    s.hist[t] = 0;
+    if (t == 0) s.count = 0;
     for (unsigned w = wave; w < a.beams; w += kPickThreads / 64)
     {
         const unsigned n = b0 + w;
         const float2* p = a.part + (size_t)n * a.n_seg;
         const bool ended = a.done && a.done[n] != 0.0f;
         const float score = a.scores[n];
-        double lse = 0.0;
-        if (!ended)
+        auto four = [&](unsigned i, float2 (&x)[4]) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = p[min(i + 64 * r, a.n_seg - 1)];
+        };
+        float m = -__builtin_inff();
+        double sum = 0.0;
+#pragma unroll 1
+        for (unsigned i = lane; i < a.n_seg; i += 256)
         {
-            float m = -__builtin_inff();
-#pragma unroll 8
-            for (unsigned i = lane; i < a.n_seg; i += 64) m = fmax_std(m, p[i].x);
-            m = wave_max(m);
-            double sum = 0.0;
-#pragma unroll 8
-            for (unsigned i = lane; i < a.n_seg; i += 64)
-            {
-                const float2 x = p[i];
-                sum += (double)(x.y * exp_below(x.x, m));   // NaN where m is an infinity, and so is lse
-            }
-            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-            lse = (double)m + log(sum);
+            float2 x[4];
+            four(i, x);
+            m = fmax_std(m, fmax_std(fmax_std(x[0].x, x[1].x), fmax_std(x[2].x, x[3].x)));
         }
+        m = wave_max(m);
+#pragma unroll 1
+        for (unsigned i = lane; i < a.n_seg; i += 256)
+        {
+            float2 x[4];
+            four(i, x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+            {
+                const float e = x[r].y * exp_below(x[r].x, m);   // NaN where m is infinite, and so is the total
+                sum += i + 64 * r < a.n_seg ? (double)e : 0.0;
+            }
+        }
+#pragma unroll 1
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if (lane == 0)
         {
+            const double lse = (double)m + log(sum), best = ended ? (double)score : (double)score + ((double)m - lse);
             s.lse[w] = lse;
+            s.best[w] = best == best ? best : -__builtin_inf();
             s.score[w] = score;
-            s.ended[w] = ended;
+            s.ended[w] = ended;   // whose sums are anything, and not used
         }
     }
     __syncthreads();
+    // Totals, NaN as -inf.
     auto total = [&](unsigned w, bool is_eos, float logit) {
-        const double sc = (double)s.score[w];
-        return key_of(s.ended[w] ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]));
+        const double sc = (double)s.score[w], x = s.ended[w] ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]);
+        return x == x ? x : -__builtin_inf();
     };
-    // The best segments.
-    const unsigned n_all = a.beams * a.n_seg, k_seg = min(a.take, n_all);
-    pick<HELD>(
-        s, n_all, k_seg,
-        [&](unsigned i) {
-            const unsigned w = a.by_n_seg.div(i), g = i - w * a.n_seg;
-            const float x = a.part[(size_t)b0 * a.n_seg + i].x;   // of an ended beam: anything, not used
-            return total(w, a.by_seg.div(a.eos) == g, x);
-        },
-        [](unsigned i) { return i; });
-    rank_list(s, k_seg);
-    if (t < (int)k_seg) seg_s[t] = s.idx[s.order[t]];
+    const unsigned eos_seg = a.by_seg.div(a.eos);
+    auto largest = [&](unsigned i) { return a.part[(size_t)b0 * a.n_seg + i].x; };
+    auto of_segment = [&](unsigned i, float x) {
+        const unsigned w = a.by_n_seg.div(i);
+        return total(w, eos_seg == i - w * a.n_seg, x);
+    };
+
+    // The best segments. Bins of 1/32 over the 32 below the best total hold them, as a rule.
+    double hi = -__builtin_inf();
+#pragma unroll 1
+    for (unsigned w = lane; w < a.beams; w += 64) hi = s.best[w] > hi ? s.best[w] : hi;
+#pragma unroll 1
+    for (int o = 32; o > 0; o >>= 1)
+    {
+        const double h2 = __shfl_xor(hi, o, 64);
+        hi = h2 > hi ? h2 : hi;
+    }
+    auto bin_of = [&](double x) {
+        const double d = (hi - x) * 32.0;   // NaN where hi is infinite: no bin
+        return d >= 0.0 && d < (double)kBins ? (unsigned)(int)d : (unsigned)kBins;
+    };
+#pragma unroll 1
+    for (unsigned i = t; i < n_all; i += 4 * kPickThreads)
+    {
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = largest(min(i + r * kPickThreads, n_all - 1));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            const unsigned at = i + r * kPickThreads;
+            if (at >= n_all) continue;
+            const unsigned bin = bin_of(of_segment(at, x[r]));
+            if (bin < kBins) atomicAdd(&s.hist[bin], 1u);
+            if (stored) s.bins[at] = (unsigned short)bin;
+        }
+    }
     __syncthreads();
+    find_bin(s, k_seg, false);
+    if (s.bin < kBins && s.above + s.hist[s.bin] <= kList)
+    {
+        const unsigned last = s.bin;
+#pragma unroll 2
+        for (unsigned i = t; i < n_all; i += kPickThreads)
+        {
+            if ((stored ? s.bins[i] : bin_of(of_segment(i, largest(i)))) > last) continue;
+            const unsigned at = atomicAdd(&s.count, 1u);
+            s.key[at] = key_of(of_segment(i, largest(i)));
+            s.idx[at] = i;
+        }
+        __syncthreads();
+    }
+    else
+        pick(
+            s, n_all, k_seg, [&](unsigned i) { return key_of(of_segment(i, largest(i))); }, [](unsigned i) { return i; });
+    rank_list(s, k_seg);
+    if (t < k_seg) s.seg[t] = s.idx[s.order[t]];
+    // The k_seg segments' best are as many candidates from this total on.
+    const u64 least = n_all >= a.take ? s.key[s.order[k_seg - 1]] : 1;
+    __syncthreads();
+    if (t == 0) s.count = 0;
+    __syncthreads();
+
     // The best candidates of theirs. Places past the vocabulary have key 0, behind every candidate's.
     auto place = [&](unsigned i, unsigned& w, unsigned& v) {
-        const unsigned q = a.by_seg.div(i), g = seg_s[q];
+        const unsigned q = a.by_seg.div(i), g = s.seg[q];
         w = a.by_n_seg.div(g);
         v = (g - w * a.n_seg) * a.seg + (i - q * a.seg);
     };
-    pick<HELD>(
-        s, k_seg * a.seg, a.take,
-        [&](unsigned i) {
-            unsigned w, v;
-            place(i, w, v);
-            const size_t n = b0 + w, at = min(v, a.vocab - 1);
-            const float x = a.logits[a.beam_major ? n * a.ld + at : at * a.ld + n];
-            return v < a.vocab ? total(w, v == a.eos, x) : 0;
-        },
-        [&](unsigned i) {
-            unsigned w, v;
-            place(i, w, v);
-            return v < a.vocab ? w * a.vocab + v : a.beams * a.vocab + i;
-        });
+    auto logit = [&](unsigned w, unsigned v) {
+        const size_t n = b0 + w, at = min(v, a.vocab - 1);
+        return a.logits[a.beam_major ? n * a.ld + at : at * a.ld + n];
+    };
+    auto of_token = [&](unsigned w, unsigned v, float x) { return v < a.vocab ? key_of(total(w, v == a.eos, x)) : 0; };
+    const unsigned n_tok = k_seg * a.seg;
+#pragma unroll 1
+    for (unsigned i = t; i < n_tok; i += 4 * kPickThreads)
+    {
+        float x[4];
+        unsigned w[4], v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            place(min(i + r * kPickThreads, n_tok - 1), w[r], v[r]);
+            x[r] = logit(w[r], v[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            const u64 key = of_token(w[r], v[r], x[r]);
+            if (i + r * kPickThreads >= n_tok || key < least) continue;
+            const unsigned at = atomicAdd(&s.count, 1u);
+            if (at >= kList) continue;
+            s.key[at] = key;
+            s.idx[at] = w[r] * a.vocab + v[r];
+        }
+    }
+    __syncthreads();
+    if (s.count > kList)
+        pick(
+            s, n_tok, a.take,
+            [&](unsigned i) {
+                unsigned w, v;
+                place(i, w, v);
+                return of_token(w, v, logit(w, v));
+            },
+            [&](unsigned i) {
+                unsigned w, v;
+                place(i, w, v);
+                return v < a.vocab ? w * a.vocab + v : a.beams * a.vocab + i;
+            });
     rank_list(s, a.take);
-    if (t < (int)a.take)
+    if (t < a.take)
     {
         const unsigned i = s.order[t], idx = s.idx[i];
         const size_t o = (size_t)blockIdx.x * a.take + t;
@@ -397,11 +503,11 @@ template <bool HELD> __global__ __launch_bounds__(kPickThreads) void k_beam_pick
 }
 
 // Tokens of a segment: as few as the loads take at once, unless the group then has more segments than the
-// selection holds in registers.
+// selection keeps bins of.
 unsigned segment_of(bool beam_major, size_t beams, size_t vocab)
 {
     unsigned seg = beam_major ? kSegRow : kSegColumn;
-    while (seg < kSegMost && beams * ((vocab + seg - 1) / seg) > (size_t)kHeld * kPickThreads) seg *= 2;
+    while (seg < kSegMost && beams * ((vocab + seg - 1) / seg) > kStored) seg *= 2;
     return seg;
 }
 
@@ -452,8 +558,6 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
         hipLaunchKernelGGL(k_beam_segments_column, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
     }
     if (int rc = launch_status()) return rc;
-    const bool held = beams * n_seg <= (size_t)kHeld * kPickThreads && take * seg <= (size_t)kHeld * kPickThreads;
-    if (held) hipLaunchKernelGGL(k_beam_pick<true>, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
-    else hipLaunchKernelGGL(k_beam_pick<false>, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
+    hipLaunchKernelGGL(k_beam_pick, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
     return launch_status();
 }
