@@ -32,7 +32,8 @@ struct BeamArgs
     const float *logits, *scores, *done;
     size_t ld;
     unsigned groups, beams, vocab, take, eos, n_seg, seg;
-    FastDiv by_seg, by_n_seg;
+    unsigned log2_seg;
+    FastDiv by_n_seg;
     int beam_major;
     float2* part;   // per (beam of all groups, segment): largest logit, sum of exp(logit - largest)
     float *out_score, *out_beam, *out_token;
@@ -142,17 +143,17 @@ __device__ __forceinline__ double value_of(u64 k)
 
 struct PickShared
 {
-    double lse[kMaxBeams], best[kMaxBeams];
-    float score[kMaxBeams];
+    double lse[kMaxBeams], best[kMaxBeams], sum[kMaxBeams];   // sum, top: of a wave's segments of a beam
+    float score[kMaxBeams], top[kMaxBeams];
     unsigned char ended[kMaxBeams];
     u64 key[kList];
     unsigned idx[kList];
     unsigned hist[kBins];
     unsigned wave[kPickThreads / 64];
     u64 red[2][kPickThreads / 64];
-    unsigned count, bin, above;
+    unsigned count, bin, above, wide;
     unsigned order[kMaxTake];   // items of the list by rank
-    unsigned seg[kMaxTake];
+    unsigned seg_beam[kMaxTake], seg_token[kMaxTake];   // of the best segments: beam and first token
     unsigned short bins[kStored];
 };
 
@@ -322,73 +323,94 @@ __device__ __forceinline__ void rank_list(PickShared& s, unsigned k)
 }
 
 // One workgroup a group. The kernel runs once over little data, so its time is that of the loads it waits for one
-// after another and of fetching its own code: loads go four at a time, and loops stay loops.
+// after another, of its instructions (one CU's) and of fetching them: loads go several at a time, loops stay loops,
+// and most items are put aside by a float32 distance from the best total, before any 64-bit total is formed.
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
 {
+    constexpr unsigned kWaves = kPickThreads / 64;
     __shared__ PickShared s;
     const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const unsigned b0 = blockIdx.x * a.beams, n_all = a.beams * a.n_seg, k_seg = min(a.take, n_all);
     const bool stored = n_all <= kStored;
+    // A unit is a beam's segments, or where there are fewer beams than waves every 2^log2_slices-th 64 of them.
+    unsigned log2_slices = 0;
+    while ((a.beams << (log2_slices + 1)) <= kWaves) ++log2_slices;
+    const unsigned slices = 1u << log2_slices, units = a.beams << log2_slices, step = 64 << log2_slices;
+    const float2* part = a.part + (size_t)b0 * a.n_seg;
     s.hist[t] = 0;
-    if (t == 0) s.count = 0;
-    for (unsigned w = wave; w < a.beams; w += kPickThreads / 64)
+    if (t == 0) s.count = s.wide = 0;
+    static_assert(kMaxBeams <= kPickThreads);
+    float score = 0.0f, done = 0.0f;   // of beam t, on their way with the segments
+    if (t < a.beams)
     {
-        const unsigned n = b0 + w;
-        const float2* p = a.part + (size_t)n * a.n_seg;
-        const bool ended = a.done && a.done[n] != 0.0f;
-        const float score = a.scores[n];
-        auto four = [&](unsigned i, float2 (&x)[4]) {
+        score = a.scores[b0 + t];
+        if (a.done) done = a.done[b0 + t];
+    }
+    // f(first of 8 segments, each step apart, their values) over a unit's segments.
+    auto over_unit = [&](unsigned u, auto&& f) {
+        const unsigned w = u >> log2_slices;
+        const float2* p = part + (size_t)w * a.n_seg;
+#pragma unroll 1
+        for (unsigned i = (u - (w << log2_slices)) * 64 + lane; i < a.n_seg; i += 8 * step)
+        {
+            float2 x[8];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = p[min(i + 64 * r, a.n_seg - 1)];
-        };
+            for (int r = 0; r < 8; ++r) x[r] = p[min(i + step * r, a.n_seg - 1)];
+            f(w, i, x);
+        }
+    };
+#pragma unroll 1
+    for (unsigned u = wave; u < units; u += kWaves)
+    {
+        // Lanes past the last segment have none: -inf and 0.
         float m = -__builtin_inff();
         double sum = 0.0;
-#pragma unroll 1
-        for (unsigned i = lane; i < a.n_seg; i += 256)
-        {
-            float2 x[4];
-            four(i, x);
-            m = fmax_std(m, fmax_std(fmax_std(x[0].x, x[1].x), fmax_std(x[2].x, x[3].x)));
-        }
-        m = wave_max(m);
-#pragma unroll 1
-        for (unsigned i = lane; i < a.n_seg; i += 256)
-        {
-            float2 x[4];
-            four(i, x);
+        over_unit(u, [&](unsigned, unsigned i, const float2(&x)[8]) {
+            float mn = m;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 8; ++r) mn = fmax_std(mn, x[r].x);
+            const float base = mn == -__builtin_inff() ? 0.0f : mn;
+            if (m != mn) sum *= (double)exp_below(m, base);
+            m = mn;
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
             {
-                const float e = x[r].y * exp_below(x[r].x, m);   // NaN where m is infinite, and so is the total
-                sum += i + 64 * r < a.n_seg ? (double)e : 0.0;
+                const float e = x[r].y * exp_below(x[r].x, base);   // NaN where m is +inf, and so is the total
+                sum += i + step * r < a.n_seg ? (double)e : 0.0;
             }
-        }
+        });
+        const float top = wave_max(m);
+        sum *= (double)exp_below(m, top == -__builtin_inff() ? 0.0f : top);
 #pragma unroll 1
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if (lane == 0)
         {
-            const double lse = (double)m + log(sum), best = ended ? (double)score : (double)score + ((double)m - lse);
-            s.lse[w] = lse;
-            s.best[w] = best == best ? best : -__builtin_inf();
-            s.score[w] = score;
-            s.ended[w] = ended;   // whose sums are anything, and not used
+            s.top[u] = top;
+            s.sum[u] = sum;
         }
     }
     __syncthreads();
-    // Totals, NaN as -inf.
-    auto total = [&](unsigned w, bool is_eos, float logit) {
-        const double sc = (double)s.score[w], x = s.ended[w] ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]);
-        return x == x ? x : -__builtin_inf();
-    };
-    const unsigned eos_seg = a.by_seg.div(a.eos);
-    auto largest = [&](unsigned i) { return a.part[(size_t)b0 * a.n_seg + i].x; };
-    auto of_segment = [&](unsigned i, float x) {
-        const unsigned w = a.by_n_seg.div(i);
-        return total(w, eos_seg == i - w * a.n_seg, x);
-    };
-
-    // The best segments. Bins of 1/32 over the 32 below the best total hold them, as a rule.
-    double hi = -__builtin_inf();
+    const bool ended = done != 0.0f;   // whose segments' sums are anything, and not used
+    double lse = 0.0;
+    if (t < a.beams)
+    {
+        const unsigned w = t;
+        float m = -__builtin_inff();
+#pragma unroll 1
+        for (unsigned i = 0; i < slices; ++i) m = fmax_std(m, s.top[w * slices + i]);
+        double sum = 0.0;
+#pragma unroll 1
+        for (unsigned i = 0; i < slices; ++i)
+            sum += s.sum[w * slices + i] * (double)exp_below(s.top[w * slices + i], m == -__builtin_inff() ? 0.0f : m);
+        lse = (double)m + log(sum);
+        const double best = ended ? (double)score : (double)score + ((double)m - lse);
+        s.score[w] = score;
+        s.ended[w] = ended;
+        s.lse[w] = lse;
+        s.best[w] = best == best ? best : -__builtin_inf();
+    }
+    __syncthreads();
+    double hi = -__builtin_inf();   // the best total
 #pragma unroll 1
     for (unsigned w = lane; w < a.beams; w += 64) hi = s.best[w] > hi ? s.best[w] : hi;
 #pragma unroll 1
@@ -397,57 +419,87 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         const double h2 = __shfl_xor(hi, o, 64);
         hi = h2 > hi ? h2 : hi;
     }
-    auto bin_of = [&](double x) {
-        const double d = (hi - x) * 32.0;   // NaN where hi is infinite: no bin
-        return d >= 0.0 && d < (double)kBins ? (unsigned)(int)d : (unsigned)kBins;
+    // A candidate lies near[w] - logit below the best, to within half a bin of 1/32 while near[w] is at most 2^16.
+    float* near = s.top;
+    __syncthreads();
+    if (t < a.beams)
+    {
+        const float d = (float)(hi - (ended ? (double)score : (double)score - lse));
+        near[t] = d;
+        if (!(fabsf(d) <= 0x1p16f) && d != __builtin_inff()) s.wide = 1;
+    }
+    __syncthreads();
+    // Totals, NaN as -inf.
+    auto total = [&](unsigned w, bool is_eos, float logit) {
+        const double sc = (double)s.score[w], x = s.ended[w] ? (is_eos ? sc : -__builtin_inf()) : sc + ((double)logit - s.lse[w]);
+        return x == x ? x : -__builtin_inf();
+    };
+    const unsigned eos_seg = a.eos / a.seg;
+    auto of_segment = [&](unsigned i) {
+        const unsigned w = a.by_n_seg.div(i);
+        return key_of(total(w, eos_seg == i - w * a.n_seg, part[i].x));
+    };
+
+    // The best segments. Bins of 1/32 over the 32 below the best total hold them, as a rule; the bin behind the
+    // one where their count is reached is taken too, for the half bin that a distance may be off.
+    auto bin_of = [&](float distance) {
+        const float d = distance * 32.0f;
+        return d > -1.0f && d < (float)kBins ? (unsigned)(int)d : (unsigned)kBins;
     };
 #pragma unroll 1
-    for (unsigned i = t; i < n_all; i += 4 * kPickThreads)
+    for (unsigned u = wave; u < units; u += kWaves)
     {
-        float x[4];
+        const unsigned beam = u >> log2_slices;
+        const bool over = s.ended[beam];
+        const float dist = near[beam];
+        over_unit(u, [&](unsigned w, unsigned i, const float2(&x)[8]) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = largest(min(i + r * kPickThreads, n_all - 1));
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-        {
-            const unsigned at = i + r * kPickThreads;
-            if (at >= n_all) continue;
-            const unsigned bin = bin_of(of_segment(at, x[r]));
-            if (bin < kBins) atomicAdd(&s.hist[bin], 1u);
-            if (stored) s.bins[at] = (unsigned short)bin;
-        }
+            for (int r = 0; r < 8; ++r)
+            {
+                const unsigned g = i + step * r;
+                if (g >= a.n_seg) continue;
+                const unsigned bin = !over ? bin_of(dist - x[r].x) : g == eos_seg ? bin_of(dist) : (unsigned)kBins;
+                if (bin < kBins) atomicAdd(&s.hist[bin], 1u);
+                if (stored) s.bins[w * a.n_seg + g] = (unsigned short)bin;
+            }
+        });
     }
     __syncthreads();
     find_bin(s, k_seg, false);
-    if (s.bin < kBins && s.above + s.hist[s.bin] <= kList)
+    const unsigned last = min(s.bin + 1, (unsigned)kBins - 1);
+    if (stored && !s.wide && s.bin < kBins && s.above + s.hist[s.bin] + (last > s.bin ? s.hist[last] : 0) <= kList)
     {
-        const unsigned last = s.bin;
-#pragma unroll 2
+#pragma unroll 4
         for (unsigned i = t; i < n_all; i += kPickThreads)
         {
-            if ((stored ? s.bins[i] : bin_of(of_segment(i, largest(i)))) > last) continue;
+            if (s.bins[i] > last) continue;
             const unsigned at = atomicAdd(&s.count, 1u);
-            s.key[at] = key_of(of_segment(i, largest(i)));
+            s.key[at] = of_segment(i);
             s.idx[at] = i;
         }
         __syncthreads();
     }
     else
-        pick(
-            s, n_all, k_seg, [&](unsigned i) { return key_of(of_segment(i, largest(i))); }, [](unsigned i) { return i; });
+        pick(s, n_all, k_seg, of_segment, [](unsigned i) { return i; });
     rank_list(s, k_seg);
-    if (t < k_seg) s.seg[t] = s.idx[s.order[t]];
+    if (t < k_seg)
+    {
+        const unsigned g = s.idx[s.order[t]], w = a.by_n_seg.div(g);
+        s.seg_beam[t] = w;
+        s.seg_token[t] = (g - w * a.n_seg) * a.seg;
+    }
     // The k_seg segments' best are as many candidates from this total on.
     const u64 least = n_all >= a.take ? s.key[s.order[k_seg - 1]] : 1;
+    const float reach = (float)(hi - value_of(least));
     __syncthreads();
     if (t == 0) s.count = 0;
     __syncthreads();
 
     // The best candidates of theirs. Places past the vocabulary have key 0, behind every candidate's.
     auto place = [&](unsigned i, unsigned& w, unsigned& v) {
-        const unsigned q = a.by_seg.div(i), g = s.seg[q];
-        w = a.by_n_seg.div(g);
-        v = (g - w * a.n_seg) * a.seg + (i - q * a.seg);
+        const unsigned q = i >> a.log2_seg;
+        w = s.seg_beam[q];
+        v = s.seg_token[q] + (i & (a.seg - 1));
     };
     auto logit = [&](unsigned w, unsigned v) {
         const size_t n = b0 + w, at = min(v, a.vocab - 1);
@@ -466,15 +518,22 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
             place(min(i + r * kPickThreads, n_tok - 1), w[r], v[r]);
             x[r] = logit(w[r], v[r]);
         }
-#pragma unroll
+#pragma unroll 1
         for (int r = 0; r < 4; ++r)
         {
-            const u64 key = of_token(w[r], v[r], x[r]);
-            if (i + r * kPickThreads >= n_tok || key < least) continue;
+            const float xr = r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3];
+            const unsigned wr = r == 0 ? w[0] : r == 1 ? w[1] : r == 2 ? w[2] : w[3];
+            const unsigned vr = r == 0 ? v[0] : r == 1 ? v[1] : r == 2 ? v[2] : v[3];
+            if (i + r * kPickThreads >= n_tok) break;
+            // The distances are off by less than 2^-20 of their terms.
+            const float d = near[wr];
+            if (!s.ended[wr] && d - xr > reach + 0x1p-20f * (fabsf(d) + fabsf(xr) + fabsf(reach))) continue;
+            const u64 key = of_token(wr, vr, xr);
+            if (key < least) continue;
             const unsigned at = atomicAdd(&s.count, 1u);
             if (at >= kList) continue;
             s.key[at] = key;
-            s.idx[at] = w[r] * a.vocab + v[r];
+            s.idx[at] = wr * a.vocab + vr;
         }
     }
     __syncthreads();
@@ -543,8 +602,8 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
     const unsigned seg = segment_of(beam_major != 0, beams, vocab);
     const unsigned n_seg = static_cast<unsigned>((vocab + seg - 1) / seg), all = static_cast<unsigned>(groups * beams);
     BeamArgs a{logits, scores, done, ld, static_cast<unsigned>(groups), static_cast<unsigned>(beams),
-               static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg, FastDiv(seg),
-               FastDiv(n_seg), beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
+               static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg,
+               static_cast<unsigned>(__builtin_ctz(seg)), FastDiv(n_seg), beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
     auto s = static_cast<hipStream_t>(stream);
     if (beam_major)
     {
