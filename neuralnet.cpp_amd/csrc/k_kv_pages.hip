@@ -10,6 +10,8 @@ namespace
 constexpr int kAppendTokens = 32;   // tokens of a tile
 constexpr int kAppendDim = 256;     // widest head
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 struct HeadsView
 {
     const float* p;
@@ -23,50 +25,89 @@ struct AppendArgs
     float* out;
     long o_t, o_f;
     const float *seq, *pos, *cos, *sin;
-    unsigned tokens, tile, rope_rows;
-    int half;   // rope_dim / 2
+    unsigned tokens, rope_rows, head_slots;   // head_slots: k heads, v heads, q heads
+    int half;                                 // rope_dim / 2
+    unsigned pieces;                          // rows of 4 values that a thread takes two of, of a head
+    FastDiv by_pieces, by_slots;
 };
 
-// One tile of tokens of one head: k heads, then v heads, then q heads along blockIdx.y. The tile is read in the
-// order of its own layout into LDS and written in the order of the destination's, so either layout of either
-// side gives whole lines.
+// Where token n goes: its row, or -1 for padding, and its position.
+__device__ __forceinline__ int append_row(const AppendArgs& a, unsigned n, unsigned& pos)
+{
+    size_t p = 0, b = n;
+    const bool seq_ok = a.seq ? row_index(a.seq[n], a.c.batch, b) : n < a.c.batch;
+    const bool ok = row_index(a.pos[n], kMaxIndex, p) && seq_ok && (!a.cos || p < a.rope_rows);
+    pos = (unsigned)p;
+    return ok ? a.c.row_of((unsigned)b, pos) : -1;
+}
+
+// Tokens a row each on every side, 16-byte aligned: a thread takes 4 neighbouring values of a head and the 4 that
+// they turn with (j and j + rope_dim / 2), or two neighbouring fours of what is not turned. Both are on their way
+// before the position is known.
+__global__ __launch_bounds__(256) void k_kv_append_rows(AppendArgs a)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const unsigned at = a.by_pieces.div((unsigned)i), piece = (unsigned)i - at * a.pieces;   // at: token and head slot
+    const unsigned n = a.by_slots.div(at), slot = at - n * a.head_slots, heads = a.c.heads;
+    if (n >= a.tokens) return;
+    const int kind = slot < heads ? 0 : slot < 2 * heads ? 1 : 2, dim = a.c.dim;
+    const unsigned h = kind == 0 ? slot : kind == 1 ? slot - heads : slot - 2 * heads;
+    const int half = kind == 1 ? 0 : a.half, turned = half / 4;
+    const bool turn = (int)piece < turned;
+    const int d0 = turn ? 4 * piece : 2 * half + 8 * (piece - turned), d1 = turn ? d0 + half : d0 + 4;
+    if (d0 >= dim) return;
+    const HeadsView& x = kind == 0 ? a.k : kind == 1 ? a.v : a.q;
+    const float* xp = x.p + (long)n * x.t + (long)h * dim;
+    f32x4 x0 = *reinterpret_cast<const f32x4*>(xp + d0), x1 = x0;
+    if (d1 < dim) x1 = *reinterpret_cast<const f32x4*>(xp + d1);
+    unsigned pos;
+    const int row = append_row(a, n, pos);
+    if (row < 0) return;
+    if (turn)
+    {
+        const f32x4 co = *reinterpret_cast<const f32x4*>(a.cos + (size_t)pos * half + d0);
+        const f32x4 si = *reinterpret_cast<const f32x4*>(a.sin + (size_t)pos * half + d0);
+        const f32x4 y0 = x0 * co - x1 * si;
+        x1 = x1 * co + x0 * si;
+        x0 = y0;
+    }
+    float* o = kind == 2 ? a.out + (long)n * a.o_t : (kind == 0 ? a.c.K : a.c.V) + (long)row * a.c.row;
+    o += (long)h * dim;
+    *reinterpret_cast<f32x4*>(o + d0) = x0;
+    if (d1 < dim) *reinterpret_cast<f32x4*>(o + d1) = x1;
+}
+
+// Any layout: one tile of tokens of one head slot (blockIdx.y). The tile is read in the order of its own layout
+// into LDS and written in the order of the destination's, so either layout of either side gives whole lines:
+// 64 lanes along a token's features, or 32 along the tokens.
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
 {
     extern __shared__ float tile_s[];   // [token][dim + 1]
     __shared__ int row_s[kAppendTokens];
     __shared__ unsigned pos_s[kAppendTokens];
     const int t = threadIdx.x, dim = a.c.dim, ld = dim + 1;
-    const unsigned n0 = blockIdx.x * a.tile, heads = a.c.heads;
-    const int nt = min(a.tile, a.tokens - n0);
+    const unsigned n0 = blockIdx.x * kAppendTokens, heads = a.c.heads;
+    const int nt = min((unsigned)kAppendTokens, a.tokens - n0);
     const unsigned y = blockIdx.y;
     const int kind = y < heads ? 0 : y < 2 * heads ? 1 : 2;
     const unsigned h = kind == 0 ? y : kind == 1 ? y - heads : y - 2 * heads;
-    const HeadsView x = kind == 0 ? a.k : kind == 1 ? a.v : a.q;
+    const HeadsView& x = kind == 0 ? a.k : kind == 1 ? a.v : a.q;
     const float* xp = x.p + (long)n0 * x.t + (long)h * dim * x.f;
-    if (t < nt)
-    {
-        const unsigned n = n0 + t;
-        size_t p = 0, b = n;
-        int row = -1;
-        const bool seq_ok = a.seq ? row_index(a.seq[n], a.c.batch, b) : n < a.c.batch;
-        if (seq_ok && row_index(a.pos[n], kMaxIndex, p) && (!a.cos || p < a.rope_rows)) row = a.c.row_of(b, p);
-        row_s[t] = row;
-        pos_s[t] = (unsigned)p;
-    }
-    const int count = nt * dim;
-    for (int i = t; i < count; i += 256)
-    {
-        const int n = x.f == 1 ? i / dim : i % nt, d = x.f == 1 ? i % dim : i / nt;
-        tile_s[n * ld + d] = xp[(long)n * x.t + (long)d * x.f];
-    }
+    // Every (token, feature) of the tile, f(n, d).
+    auto over = [&](bool along_features, auto&& f) {
+        if (along_features)
+            for (int n = t >> 6; n < nt; n += 4)
+                for (int d = t & 63; d < dim; d += 64) f(n, d);
+        else if ((t & (kAppendTokens - 1)) < nt)
+            for (int d = t / kAppendTokens; d < dim; d += 256 / kAppendTokens) f(t & (kAppendTokens - 1), d);
+    };
+    over(x.f == 1, [&](int n, int d) { tile_s[n * ld + d] = xp[(long)n * x.t + (long)d * x.f]; });
+    if (t < nt) row_s[t] = append_row(a, n0 + t, pos_s[t]);
     __syncthreads();
     const int half = kind == 1 ? 0 : a.half;
-    const bool by_token = kind != 2 || a.o_f == 1;
-    for (int i = t; i < count; i += 256)
-    {
-        const int n = by_token ? i / dim : i % nt, d = by_token ? i % dim : i / nt;
+    over(kind != 2 || a.o_f == 1, [&](int n, int d) {
         const int row = row_s[n];
-        if (row < 0) continue;
+        if (row < 0) return;
         float v = tile_s[n * ld + d];
         if (d < 2 * half)
         {
@@ -79,7 +120,7 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
             a.out[(long)(n0 + n) * a.o_t + ((long)h * dim + d) * a.o_f] = v;
         else
             (kind == 0 ? a.c.K : a.c.V)[(long)row * a.c.row + (long)h * dim + d] = v;
-    }
+    });
 }
 
 constexpr int kReorderLayers = 32;   // caches of a launch
@@ -91,6 +132,7 @@ struct ReorderArgs
     const float *parent, *len, *fresh;
     float *table_out, *len_out;
     unsigned out_batch, table_blocks, copy_rows, n_mem;   // copy_rows: row groups of a page
+    int vec;                                              // rows are copied 4 floats at a time
     float* mem[2 * kReorderLayers];
 };
 
@@ -144,6 +186,20 @@ __global__ __launch_bounds__(256) void k_kv_reorder(ReorderArgs a)
     const unsigned rows = min(r.tail - r0, (unsigned)kReorderRows), len = a.c.heads * a.c.dim;
     const float* s = m + ((long)src * a.c.page.d + r0) * a.c.row;
     float* d = m + ((long)dst * a.c.page.d + r0) * a.c.row;
+    if (a.vec)
+    {
+        for (unsigned j = t; j < len / 4; j += 256)
+        {
+            f32x4 x[kReorderRows];
+#pragma unroll
+            for (unsigned k = 0; k < kReorderRows; ++k)
+                x[k] = *reinterpret_cast<const f32x4*>(s + (long)min(k, rows - 1) * a.c.row + 4 * j);
+#pragma unroll
+            for (unsigned k = 0; k < kReorderRows; ++k)
+                if (k < rows) *reinterpret_cast<f32x4*>(d + (long)k * a.c.row + 4 * j) = x[k];
+        }
+        return;
+    }
     for (unsigned k = 0; k < rows; ++k)
         for (unsigned j = t; j < len; j += 256) d[(long)k * a.c.row + j] = s[(long)k * a.c.row + j];
 }
@@ -173,12 +229,38 @@ extern "C" int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t
         return -1;
     const size_t y = 2 * c->heads + (q ? q_heads : 0);
     if (y > 65535) return -1;
-    AppendArgs a{pages_of(*c), {k, k_t, k_f}, {v, v_t, v_f}, {q, q_t, q_f}, q_out, o_t, o_f, seq, pos, cos, sin,
-                 static_cast<unsigned>(tokens), kAppendTokens, static_cast<unsigned>(rope_rows),
-                 static_cast<int>(rope_dim / 2)};
-    const dim3 grid(static_cast<unsigned>((tokens + a.tile - 1) / a.tile), static_cast<unsigned>(y));
-    hipLaunchKernelGGL(k_kv_append, grid, dim3(256), a.tile * (c->dim + 1) * sizeof(float),
-                       static_cast<hipStream_t>(stream), a);
+    AppendArgs a{};
+    a.c = pages_of(*c);
+    a.k = {k, k_t, k_f};
+    a.v = {v, v_t, v_f};
+    a.q = {q, q_t, q_f};
+    a.out = q_out;
+    a.o_t = o_t;
+    a.o_f = o_f;
+    a.seq = seq;
+    a.pos = pos;
+    a.cos = cos;
+    a.sin = sin;
+    a.tokens = static_cast<unsigned>(tokens);
+    a.rope_rows = static_cast<unsigned>(rope_rows);
+    a.head_slots = static_cast<unsigned>(y);
+    a.half = static_cast<int>(rope_dim / 2);
+    auto rows_of_4 = [](const float* p, long t, long f) { return !p || (f == 1 && t % 4 == 0 && aligned16(p)); };
+    const size_t turned = rope_dim / 8, rest = c->dim - rope_dim, all_v = (c->dim + 7) / 8;
+    a.pieces = static_cast<unsigned>(turned + (rest + 7) / 8 > all_v ? turned + (rest + 7) / 8 : all_v);
+    const size_t threads = tokens * y * a.pieces;
+    auto s = static_cast<hipStream_t>(stream);
+    if (c->dim % 4 == 0 && rope_dim % 8 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V) &&
+        rows_of_4(k, k_t, k_f) && rows_of_4(v, v_t, v_f) && rows_of_4(q, q_t, q_f) && rows_of_4(q_out, o_t, o_f) &&
+        (!cos || (aligned16(cos) && aligned16(sin))) && threads + 256 < 0x80000000u)
+    {
+        a.by_pieces = FastDiv(a.pieces);
+        a.by_slots = FastDiv(a.head_slots);
+        hipLaunchKernelGGL(k_kv_append_rows, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
+        return launch_status();
+    }
+    const dim3 grid(static_cast<unsigned>((tokens + kAppendTokens - 1) / kAppendTokens), static_cast<unsigned>(y));
+    hipLaunchKernelGGL(k_kv_append, grid, dim3(256), kAppendTokens * (c->dim + 1) * sizeof(float), s, a);
     return launch_status();
 }
 
@@ -218,6 +300,8 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
             a.mem[2 * i + 1] = layers[at + i].V;
         }
         a.n_mem = static_cast<unsigned>(2 * n);
+        a.vec = c.heads * c.dim % 4 == 0 && c.row % 4 == 0;
+        for (size_t i = 0; i < 2 * n; ++i) a.vec = a.vec && aligned16(a.mem[i]);
         const size_t tables = at == 0 ? (out_batch * c.width + 255) / 256 : 0;
         const size_t blocks = tables + (size_t)a.copy_rows * a.n_mem * out_batch;
         if (blocks == 0) break;
