@@ -26,7 +26,7 @@ struct AppendArgs
     long o_t, o_f;
     const float *seq, *pos, *cos, *sin;
     unsigned tokens, rope_rows, head_slots;   // head_slots: k heads, v heads, q heads
-    int half;                                 // rope_dim / 2
+    int half, log2_lanes;                     // rope_dim / 2; lanes along a tile's tokens
     unsigned pieces;                          // rows of 4 values that a thread takes two of, of a head
     FastDiv by_pieces, by_slots;
 };
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void k_kv_append_rows(AppendArgs a)
 
 // Any layout: one tile of tokens of one head slot (blockIdx.y). The tile is read in the order of its own layout
 // into LDS and written in the order of the destination's, so either layout of either side gives whole lines:
-// 64 lanes along a token's features, or 32 along the tokens.
+// 64 lanes along a token's features, or as many along the tokens as there are, 32 at most.
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
 {
     extern __shared__ float tile_s[];   // [token][dim + 1]
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a)
         if (along_features)
             for (int n = t >> 6; n < nt; n += 4)
                 for (int d = t & 63; d < dim; d += 64) f(n, d);
-        else if ((t & (kAppendTokens - 1)) < nt)
-            for (int d = t / kAppendTokens; d < dim; d += 256 / kAppendTokens) f(t & (kAppendTokens - 1), d);
+        else if (const int n = t & ((1 << a.log2_lanes) - 1); n < nt)
+            for (int d = t >> a.log2_lanes; d < dim; d += 256 >> a.log2_lanes) f(n, d);
     };
     over(x.f == 1, [&](int n, int d) { tile_s[n * ld + d] = xp[(long)n * x.t + (long)d * x.f]; });
     if (t < nt) row_s[t] = append_row(a, n0 + t, pos_s[t]);
@@ -131,7 +131,7 @@ struct ReorderArgs
     Pages c;
     const float *parent, *len, *fresh;
     float *table_out, *len_out;
-    unsigned out_batch, table_blocks, copy_rows, n_mem;   // copy_rows: row groups of a page
+    unsigned out_batch, table_blocks, splits, n_mem;   // splits: workgroups that a page's rows are cut into
     int vec;                                              // rows are copied 4 floats at a time
     float* mem[2 * kReorderLayers];
 };
@@ -171,23 +171,32 @@ __global__ __launch_bounds__(256) void k_kv_reorder(ReorderArgs a)
         a.table_out[i] = v;
         return;
     }
-    // Rows [r0, r0 + kReorderRows) of the page in progress of new sequence b, in one cache.
+    // The page in progress of new sequence b, in one cache: kReorderRows rows at a time, in turn with the others
+    // of the page's workgroups.
     unsigned i = blockIdx.x - a.table_blocks;
-    const unsigned r0 = (i % a.copy_rows) * kReorderRows;
-    i /= a.copy_rows;
+    const unsigned split = i % a.splits;
+    i /= a.splits;
     const unsigned mi = i % a.n_mem, b = i / a.n_mem;
+    const float fresh = a.fresh[b];
     const Continued r = continued(a, b);
-    if (!r.ok || r0 >= r.tail || r.full >= a.c.width) return;
+    if (!r.ok || r.full >= a.c.width) return;
     size_t dst, src;
-    if (!row_index(a.fresh[b], a.c.pages, dst) || !row_index(a.c.table[r.parent * a.c.width + r.full], a.c.pages, src) ||
+    if (!row_index(fresh, a.c.pages, dst) || !row_index(a.c.table[r.parent * a.c.width + r.full], a.c.pages, src) ||
         src == dst)
         return;
     float* m = a.mem[mi];
-    const unsigned rows = min(r.tail - r0, (unsigned)kReorderRows), len = a.c.heads * a.c.dim;
-    const float* s = m + ((long)src * a.c.page.d + r0) * a.c.row;
-    float* d = m + ((long)dst * a.c.page.d + r0) * a.c.row;
-    if (a.vec)
+    const unsigned len = a.c.heads * a.c.dim;
+    for (unsigned r0 = split * kReorderRows; r0 < r.tail; r0 += a.splits * kReorderRows)
     {
+        const unsigned rows = min(r.tail - r0, (unsigned)kReorderRows);
+        const float* s = m + ((long)src * a.c.page.d + r0) * a.c.row;
+        float* d = m + ((long)dst * a.c.page.d + r0) * a.c.row;
+        if (!a.vec)
+        {
+            for (unsigned k = 0; k < rows; ++k)
+                for (unsigned j = t; j < len; j += 256) d[(long)k * a.c.row + j] = s[(long)k * a.c.row + j];
+            continue;
+        }
         for (unsigned j = t; j < len / 4; j += 256)
         {
             f32x4 x[kReorderRows];
@@ -198,10 +207,7 @@ __global__ __launch_bounds__(256) void k_kv_reorder(ReorderArgs a)
             for (unsigned k = 0; k < kReorderRows; ++k)
                 if (k < rows) *reinterpret_cast<f32x4*>(d + (long)k * a.c.row + 4 * j) = x[k];
         }
-        return;
     }
-    for (unsigned k = 0; k < rows; ++k)
-        for (unsigned j = t; j < len; j += 256) d[(long)k * a.c.row + j] = s[(long)k * a.c.row + j];
 }
 
 bool overlap(const float* a, size_t na, const float* b, size_t nb)
@@ -259,6 +265,8 @@ extern "C" int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t
         hipLaunchKernelGGL(k_kv_append_rows, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a);
         return launch_status();
     }
+    while (a.log2_lanes < 5 && ((size_t)1 << a.log2_lanes) < tokens) ++a.log2_lanes;
+    static_assert(kAppendTokens == 1 << 5);
     const dim3 grid(static_cast<unsigned>((tokens + kAppendTokens - 1) / kAppendTokens), static_cast<unsigned>(y));
     hipLaunchKernelGGL(k_kv_append, grid, dim3(256), kAppendTokens * (c->dim + 1) * sizeof(float), s, a);
     return launch_status();
@@ -290,7 +298,6 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
     a.len_out = len_out;
     a.out_batch = static_cast<unsigned>(out_batch);
     const bool copy = fresh && c.page > 1;
-    a.copy_rows = copy ? static_cast<unsigned>((c.page - 1 + kReorderRows - 1) / kReorderRows) : 0;
     for (size_t at = 0; at < n_layers; at += kReorderLayers)
     {
         const size_t n = n_layers - at < kReorderLayers ? n_layers - at : kReorderLayers;
@@ -303,7 +310,12 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
         a.vec = c.heads * c.dim % 4 == 0 && c.row % 4 == 0;
         for (size_t i = 0; i < 2 * n; ++i) a.vec = a.vec && aligned16(a.mem[i]);
         const size_t tables = at == 0 ? (out_batch * c.width + 255) / 256 : 0;
-        const size_t blocks = tables + (size_t)a.copy_rows * a.n_mem * out_batch;
+        // Some 4 workgroups a CU: the lengths are on the device, and one that finds nothing to copy still waits for
+        // the parent, its length and its page, one after another.
+        const size_t pages = copy ? a.n_mem * out_batch : 0, most = (c.page - 1 + kReorderRows - 1) / kReorderRows;
+        const size_t want = pages ? 4 * (size_t)device_cus() / pages : 0;
+        a.splits = static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
+        const size_t blocks = tables + a.splits * pages;
         if (blocks == 0) break;
         if (blocks > 0x7fffffffu) return -1;
         a.table_blocks = static_cast<unsigned>(tables);
