@@ -66,7 +66,18 @@ enum nnhip_op {
     NNHIP_OP_UNARY = 27,           /* in A; args op         out C              :357-358 */
     NNHIP_OP_BINARY = 28,          /* in A,B; args op       out C              :361-362 */
     NNHIP_OP_BINARY_SCALAR = 29,   /* in A; args op,s,scalar_first  out C      :366-367 */
-    NNHIP_OP_SELECT_SCALAR_COND = 30 /* in A,then; args cmp,scalar_b,scalar_else  out C  :376-378 */
+    NNHIP_OP_SELECT_SCALAR_COND = 30, /* in A,then; args cmp,scalar_b,scalar_else  out C  :376-378 */
+    /* Paged caches and beam search (no reference counterpart; nnhip_kernels.h says what they compute). K and V
+     * (pages*page, heads*dim), table (batch, width); k, v, q (features, tokens); pos, seq, len, shared, parent,
+     * fresh as many floats as there are tokens or sequences; a flag says whether an optional input follows. */
+    NNHIP_OP_KV_APPEND = 31,   /* in K,V,table,k,v,pos[,q][,cos,sin][,seq]; args page,heads,has_q,has_rope,has_seq
+                                * out [q turned] (K, V in place) */
+    NNHIP_OP_ATTN_PAGED = 32,  /* in K,V,table,q,len[,shared][,slopes]; args page,heads,group,alpha,has_shared,
+                                * has_slopes  out O */
+    NNHIP_OP_BEAM_SELECT = 33, /* in logits (vocab, groups*beams),scores[,done]; args groups,take,eos
+                                * out totals,beams,tokens (groups, take) */
+    NNHIP_OP_KV_REORDER = 34   /* in table,parent,len[,fresh],K0,V0,K1,V1,..; args page,heads,layers,has_fresh
+                                * out table,len (K, V in place) */
 };
 
 const char* nnhip_last_error(void);
@@ -191,6 +202,16 @@ int nnhip_gpt_train_step_ex(nnhip_gpt* g, size_t accum_steps, float max_norm, in
  * reference seeds its generator from std::random_device; the seed argument makes runs repeatable. */
 int nnhip_gpt_forward_step(nnhip_gpt* g, uint64_t token, size_t pos, size_t cur_len, float* logits_out);
 int nnhip_gpt_reset_cache(nnhip_gpt* g);
+/* Beam search over the session's model (no reference counterpart): the `beams` continuations of the prompt (at
+ * most seq_len tokens) with the largest sums of log probabilities, each extended from the `beams` best of the
+ * token before. A continuation ends at eos (an id past the vocabulary: none does), after max_new tokens or
+ * where the context is full (seq_len - n_prompt + 1 tokens). Best first: out (beams * max_new places, beam i's
+ * tokens from i * max_new on, eos not among them), out_len (beams), out_scores (beams: the sums, eos's
+ * among them). 1 to 256 beams, at most the vocabulary's size; heads at most 128 wide. The session's own caches
+ * (_forward_step) are left as they are. It uses the layers that the backward pass reads their inputs from: a
+ * backward pass after it is refused until the next forward pass. */
+int nnhip_gpt_beam_search(nnhip_gpt* g, const uint64_t* prompt, size_t n_prompt, size_t beams, size_t max_new,
+                          uint64_t eos, uint64_t* out, size_t* out_len, float* out_scores);
 int nnhip_gpt_generate(nnhip_gpt* g, const uint64_t* prompt, size_t n_prompt, size_t max_new, float temperature,
                        uint64_t eos, size_t min_new, uint64_t seed, uint64_t* out, size_t out_cap, size_t* n_out);
 

@@ -16,6 +16,7 @@
 
 #include "nn/expr_dsl.hpp"
 #include "nn/layer_exprs.hpp"
+#include "nn/paged_checks.hpp"
 #include "nnhip_kernels.h"
 
 namespace nn
@@ -2189,6 +2190,106 @@ Result<void> HipEngine::scatter_add_rows(Tensor& dst, const Tensor& indices, con
     NN_TRY(ws, scratch_(nnhip_scatter_add_workspace_bytes(n)));
     return kernel_(nnhip_scatter_add(W(dst), D(indices), D(grad), dst.rows(), dst.cols(), n, ws->data(), stream_),
                    "scatter_add_rows");
+}
+
+// ── paged caches and beam search (no reference counterpart) ─────────────────
+namespace
+{
+nnhip_kv_pages pages_of(const KvPages& c, std::size_t dim)
+{
+    return nnhip_kv_pages{W(c.K), W(c.V), D(c.table), c.table.rows(), c.table.cols(), c.K.rows() / c.page, c.page,
+                          c.heads, dim, c.K.cols()};
+}
+} // namespace
+
+Result<Tensor> HipEngine::kv_append(KvPages& c, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                                    const Tensor* seq, const Tensor* cos, const Tensor* sin)
+{
+    NN_TRY(s, paged::check_append(c, k, v, q, pos, seq, cos, sin));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.table, &k, &v, q, &pos, seq, cos, sin}, "kv_append"));
+    NN_CHECK(settle_write_(c.K));
+    NN_CHECK(settle_write_(c.V));
+    const std::size_t n = k.cols();
+    const long t = 1, f = static_cast<long>(n);
+    Tensor out;
+    if (q)
+    {
+        NN_TRY(o, alloc_(q->rows(), n));
+        // The tokens that are padding are not written.
+        if (q->size()) NN_CHECK(kernel_(nnhip_copy(D(*q), W(o), q->size(), stream_), "kv_append"));
+        out = o;
+    }
+    const nnhip_kv_pages p = pages_of(c, s.dim);
+    NN_CHECK(kernel_(nnhip_kv_append(&p, D(k), t, f, D(v), t, f, q ? D(*q) : nullptr, t, f, q ? W(out) : nullptr, t, f,
+                                     s.q_heads, n, seq ? D(*seq) : nullptr, D(pos), cos ? D(*cos) : nullptr,
+                                     sin ? D(*sin) : nullptr, cos ? cos->rows() : 0, 2 * s.half, stream_),
+                     "kv_append"));
+    return out;
+}
+
+Result<Tensor> HipEngine::attn_paged(const KvPages& c, const Tensor& q, const Tensor& len, const Tensor* shared,
+                                     std::size_t group, const Tensor* slopes, Scalar alpha)
+{
+    NN_TRY(dim, paged::check_attn(c, q, len, shared, group, slopes));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.table, &q, &len, shared, slopes}, "attn_paged"));
+    const std::size_t n = q.cols(), heads = q.rows() / dim;
+    NN_TRY(out, alloc_(q.rows(), n));
+    const nnhip_kv_pages p = pages_of(c, dim);
+    const std::size_t need = nnhip_attn_paged_workspace_bytes(&p, heads, group);
+    NN_TRY(ws, scratch_(need));
+    NN_CHECK(kernel_(nnhip_attn_paged(&p, D(q), 1, static_cast<long>(n), heads, D(len), shared ? D(*shared) : nullptr,
+                                      group, slopes ? D(*slopes) : nullptr, alpha, W(out), 1, static_cast<long>(n),
+                                      nullptr, nullptr, ws->data(), need, stream_),
+                     "attn_paged"));
+    return out;
+}
+
+Result<Tensor> HipEngine::beam_select(const Tensor& logits, const Tensor& scores, const Tensor* done, std::size_t groups,
+                                      std::size_t take, std::size_t eos, Tensor& beams_out, Tensor& tokens_out)
+{
+    NN_TRY(beams, paged::check_select(logits, scores, done, groups, take, eos));
+    NN_CHECK(need_gpu_({&logits, &scores, done}, "beam_select"));
+    NN_TRY(out, alloc_(groups, take));
+    NN_TRY(ob, alloc_(groups, take));
+    NN_TRY(ot, alloc_(groups, take));
+    const std::size_t need = nnhip_beam_select_workspace_bytes(groups, beams, logits.rows(), take);
+    NN_TRY(ws, scratch_(need));
+    NN_CHECK(kernel_(nnhip_beam_select(D(logits), logits.cols(), 0, D(scores), done ? D(*done) : nullptr, groups, beams,
+                                       logits.rows(), take, eos, W(out), W(ob), W(ot), ws->data(), need, stream_),
+                     "beam_select"));
+    beams_out = ob;
+    tokens_out = ot;
+    return out;
+}
+
+Result<Tensor> HipEngine::kv_reorder(std::span<KvPages> layers, const Tensor& parent, const Tensor& len,
+                                     const Tensor* fresh, Tensor& len_out)
+{
+    NN_CHECK(paged::check_reorder(layers, parent, len, fresh));
+    NN_CHECK(need_gpu_({&layers[0].table, &parent, &len, fresh}, "kv_reorder"));
+    const std::size_t dim = paged::dim_of(layers[0]), n = parent.size();
+    std::vector<nnhip_kv_pages> p;
+    for (KvPages& c : layers)
+    {
+        NN_CHECK(need_gpu_({&c.K, &c.V}, "kv_reorder"));
+        if (fresh && c.page > 1)
+        {
+            NN_CHECK(settle_write_(c.K));
+            NN_CHECK(settle_write_(c.V));
+        }
+    }
+    for (KvPages& c : layers)
+    {
+        p.push_back(pages_of(c, dim));
+        p.back().table = D(layers[0].table);
+    }
+    NN_TRY(out, alloc_(n, layers[0].table.cols()));
+    NN_TRY(lens, alloc_(n, 1));
+    NN_CHECK(kernel_(nnhip_kv_reorder(p.data(), p.size(), D(parent), D(len), fresh ? D(*fresh) : nullptr, n, W(out),
+                                      W(lens), stream_),
+                     "kv_reorder"));
+    len_out = lens;
+    return out;
 }
 
 // ── layout (cpu_engine.hpp:226-287) ─────────────────────────────────────────

@@ -33,6 +33,14 @@ enum class BinaryOp : std::uint32_t { Add = 0, Sub = 1, Mul = 2, Div = 3, Max = 
 enum class CompareOp : std::uint32_t { Lt = 0, Le = 1, Gt = 2, Ge = 3, Eq = 4, Ne = 5 };
 enum class ReduceOp : std::uint32_t { Sum = 0, Max = 1, Min = 2 };
 
+// Keys and values of a batch of sequences in pages (nnhip_kv_pages, nnhip_kernels.h): K and V (pages * page,
+// heads * dim), table (batch, width) of page numbers. No reference counterpart.
+struct KvPages
+{
+    Tensor K, V, table;
+    std::size_t page = 1, heads = 1;
+};
+
 class ComputeEngine
 {
 public:
@@ -147,6 +155,44 @@ public:
         (void)rows;
         (void)cols;
         return fail("eval_expr_reduce: not supported by this engine");
+    }
+
+    // Paged caches and beam search (no reference counterpart; nnhip_kernels.h has the definitions). Activations are
+    // (features, tokens): k, v (heads * dim, N), q (q_heads * dim, N); index tensors hold integers as floats.
+    // Stores the tokens' keys and values at pos (N) of the sequences seq (N; null: token n of sequence n), k and q
+    // turned by rows pos of cos and sin (rows, rope_dim / 2) when these are set; gives q so turned (empty without q).
+    [[nodiscard]] virtual Result<Tensor> kv_append(KvPages& cache, const Tensor& k, const Tensor& v, const Tensor* q,
+                                                   const Tensor& pos, const Tensor* seq, const Tensor* cos,
+                                                   const Tensor* sin)
+    {
+        (void)cache, (void)k, (void)v, (void)q, (void)pos, (void)seq, (void)cos, (void)sin;
+        return fail("kv_append: not supported by this engine");
+    }
+    // Attention of one query per sequence over its first len (batch) positions; shared (batch / group), when set,
+    // counts the positions that each group's sequences have in common. O (q_heads * dim, batch).
+    [[nodiscard]] virtual Result<Tensor> attn_paged(const KvPages& cache, const Tensor& q, const Tensor& len,
+                                                    const Tensor* shared, std::size_t group, const Tensor* slopes,
+                                                    Scalar alpha)
+    {
+        (void)cache, (void)q, (void)len, (void)shared, (void)group, (void)slopes, (void)alpha;
+        return fail("attn_paged: not supported by this engine");
+    }
+    // The best `take` continuations of each group's beams: logits (vocab, groups * beams), scores and done (size
+    // groups * beams; done may be null). Totals (groups, take), and the beams and tokens.
+    [[nodiscard]] virtual Result<Tensor> beam_select(const Tensor& logits, const Tensor& scores, const Tensor* done,
+                                                     std::size_t groups, std::size_t take, std::size_t eos,
+                                                     Tensor& beams_out, Tensor& tokens_out)
+    {
+        (void)logits, (void)scores, (void)done, (void)groups, (void)take, (void)eos, (void)beams_out, (void)tokens_out;
+        return fail("beam_select: not supported by this engine");
+    }
+    // The page tables of the sequences that continue parent (their tail pages copied into the pages fresh, which may
+    // be null); layers share the table. New table, and its lengths in len_out.
+    [[nodiscard]] virtual Result<Tensor> kv_reorder(std::span<KvPages> layers, const Tensor& parent, const Tensor& len,
+                                                    const Tensor* fresh, Tensor& len_out)
+    {
+        (void)layers, (void)parent, (void)len, (void)fresh, (void)len_out;
+        return fail("kv_reorder: not supported by this engine");
     }
 
     // Queues everything t's values depend on, as a read through the engine

@@ -410,6 +410,25 @@ public:
         return rotate_(engine, q, ct, st, backward);
     }
 
+    // Positions 0 .. rows - 1 as kv_append takes them: cos and sin (rows, d_k / 2).
+    Result<void> table(ComputeEngine& engine, std::size_t rows, Tensor& cos, Tensor& sin) const
+    {
+        if (d_k_ == 0 || d_k_ % 2 != 0) return fail("RotaryEmbedding::table: d_k must be positive and even");
+        const std::size_t half = d_k_ / 2;
+        Matrix c(rows, half), s(rows, half), cc(d_k_, 1), sc(d_k_, 1);
+        for (std::size_t p = 0; p < rows; ++p)
+        {
+            fill_column_(cc, sc, p, 0);
+            std::copy_n(cc.data(), half, c.data() + p * half);
+            std::copy_n(sc.data(), half, s.data() + p * half);
+        }
+        NN_TRY(ct, engine.from_matrix(c));
+        NN_TRY(st, engine.from_matrix(s));
+        cos = ct;
+        sin = st;
+        return {};
+    }
+
 private:
     void fill_column_(Matrix& c, Matrix& sn, std::size_t pos, std::size_t col) const
     {
@@ -435,6 +454,14 @@ private:
 
     std::size_t d_k_ = 0, seq_cached_ = 0;
     Tensor cos_, sin_;
+};
+
+// One step of a batch of sequences over paged caches: each sequence's position and length after it, the positions
+// that its group shares (or none), and what the position encoding needs (RoPE's tables, ALiBi's slopes).
+struct PagedStep
+{
+    Tensor pos, len, shared, cos, sin, slopes;
+    std::size_t group = 1;
 };
 
 // ── multi-head attention core (reference compute_layer.hpp:1016-1412) ─────
@@ -645,6 +672,22 @@ public:
         return w_o_.forward(engine, attn_out);
     }
 
+    // One token each of a batch of sequences over a paged cache (no reference counterpart): x (d_model, batch),
+    // token b at position step.pos[b] of sequence b, attending over step.len[b] positions.
+    Result<Tensor> forward_paged(ComputeEngine& engine, const Tensor& x, KvPages& cache, const PagedStep& step)
+    {
+        NN_TRY(q0, w_q_.forward(engine, x));
+        NN_TRY(k, w_k_.forward(engine, x));
+        NN_TRY(v, w_v_.forward(engine, x));
+        NN_TRY(turned, engine.kv_append(cache, k, v, use_rope_ ? &q0 : nullptr, step.pos, nullptr,
+                                        use_rope_ ? &step.cos : nullptr, use_rope_ ? &step.sin : nullptr));
+        NN_TRY(o, engine.attn_paged(cache, use_rope_ ? turned : q0, step.len, step.shared.valid() ? &step.shared : nullptr,
+                                    step.group, step.slopes.valid() ? &step.slopes : nullptr, scale_));
+        return w_o_.forward(engine, o);
+    }
+    [[nodiscard]] std::size_t heads() const { return num_heads_; }
+    [[nodiscard]] const RotaryEmbedding* rope() const { return use_rope_ ? &rope_ : nullptr; }
+
 protected:
     struct TwoPassMask
     {
@@ -778,6 +821,7 @@ protected:
     }
 
 public:
+    [[nodiscard]] const std::vector<Scalar>& slopes() const { return slopes_; }
     // Layers of one model (same engine, same head count) share one cache.
     void share_step_bias(std::shared_ptr<StepBiasCache> c) { step_bias_ = std::move(c); }
 
@@ -933,7 +977,19 @@ public:
         return engine.elementwise_binary(BinaryOp::Add, r2, f);
     }
 
+    // One token each of a batch of sequences, x (d_model, batch), over the layer's paged cache.
+    Result<Tensor> forward_paged(ComputeEngine& engine, const Tensor& x, KvPages& cache, const PagedStep& step)
+    {
+        NN_TRY(n1, norm1_->forward(engine, x));
+        NN_TRY(a, attn_.forward_paged(engine, n1, cache, step));
+        NN_TRY(r2, engine.elementwise_binary(BinaryOp::Add, x, a));
+        NN_TRY(n2, norm2_->forward(engine, r2));
+        NN_TRY(f, ff_.forward(engine, n2));
+        return engine.elementwise_binary(BinaryOp::Add, r2, f);
+    }
+
     void share_step_bias(std::shared_ptr<StepBiasCache> c) { attn_.share_step_bias(std::move(c)); }
+    [[nodiscard]] const CausalSelfAttention& attention() const { return attn_; }
 
 private:
     CausalSelfAttention attn_;
@@ -951,6 +1007,8 @@ public:
     virtual Result<Tensor> apply(ComputeEngine& engine, const Tensor& emb_T, std::size_t batch, std::size_t seq) = 0;
     // One position at inference (reference :2467-2468): x (d_model, 1).
     virtual Result<Tensor> apply_step(ComputeEngine& engine, const Tensor& x, std::size_t pos) = 0;
+    // Positions of a batch: x (d_model, batch), pos (batch) on the device.
+    virtual Result<Tensor> apply_positions(ComputeEngine& engine, const Tensor& x, const Tensor& pos) = 0;
     virtual Result<void> backward(ComputeEngine& engine, const Tensor& grad_T) = 0;
     virtual std::vector<TensorRef> parameters() { return {}; }
     virtual std::vector<TensorRef> param_gradients() { return {}; }
@@ -996,6 +1054,12 @@ public:
         NN_TRY(gT, engine.transpose(g));
         return engine.elementwise_binary(BinaryOp::Add, x, gT);
     }
+    Result<Tensor> apply_positions(ComputeEngine& engine, const Tensor& x, const Tensor& pos) override
+    {
+        NN_TRY(g, engine.gather_rows(table_, pos));
+        NN_TRY(gT, engine.transpose(g));
+        return engine.elementwise_binary(BinaryOp::Add, x, gT);
+    }
     Result<void> backward(ComputeEngine& engine, const Tensor& grad_T) override
     {
         if (!learnable_)
@@ -1024,6 +1088,7 @@ class NoPositionEncoder final : public PositionEncoder
 public:
     Result<Tensor> apply(ComputeEngine&, const Tensor& emb_T, std::size_t, std::size_t) override { return emb_T; }
     Result<Tensor> apply_step(ComputeEngine&, const Tensor& x, std::size_t) override { return x; }
+    Result<Tensor> apply_positions(ComputeEngine&, const Tensor& x, const Tensor&) override { return x; }
     Result<void> backward(ComputeEngine&, const Tensor&) override { return {}; }
 };
 
@@ -1278,7 +1343,181 @@ public:
         return generated;
     }
 
+    // What a beam search found: the sequences, best first, without the prompt and eos, and their totals.
+    struct Beams
+    {
+        std::vector<std::vector<std::size_t>> tokens;
+        std::vector<Scalar> scores;
+    };
+
+    // Beam search (no reference counterpart): the `beams` continuations of the prompt with the largest sum of log
+    // probabilities among those that extend, token by token, the `beams` best so far. A continuation ends at eos (an
+    // id past the vocabulary: none does), after max_new tokens or where the context is full, and keeps its total.
+    //
+    // The prompt's keys and values are stored once, in rows that every beam's table names; a beam adds a row of its
+    // own per token (pages of one row), so that following another beam is a copy of its table's row, never of keys
+    // and values. The prompt is taken kPromptChunk tokens at a time: a batch in which token i is a sequence of its
+    // own that shares what was stored before the chunk.
+    Result<Beams> beam_search(ComputeEngine& engine, const std::vector<std::size_t>& prompt, std::size_t beams,
+                              std::size_t max_new, std::size_t eos)
+    {
+        constexpr std::size_t kPromptChunk = 64;
+        const std::size_t P = prompt.size();
+        if (P == 0) return fail("GPTModel beam_search: empty prompt");
+        if (P > seq_len_) return fail("GPTModel beam_search: the prompt is longer than the context");
+        if (beams == 0 || beams > 256) return fail("GPTModel beam_search: 1 to 256 beams");
+        if (beams > vocab_) return fail("GPTModel beam_search: more beams than tokens to begin with");
+        const std::size_t steps = std::min(max_new, seq_len_ - P + 1);   // the last token is not fed
+        Beams out{std::vector<std::vector<std::size_t>>(beams), std::vector<Scalar>(beams, Scalar{0})};
+        if (steps == 0) return out;
+        const std::size_t rows = P + beams * (steps - 1);
+        if (rows >= (std::size_t{1} << 24)) return fail("GPTModel beam_search: too many cache rows");
+
+        std::vector<KvPages> caches(blocks_.size());
+        for (KvPages& c : caches)
+        {
+            c.K = engine.create_tensor(rows, d_model_);
+            c.V = engine.create_tensor(rows, d_model_);
+            c.heads = blocks_[0]->attention().heads();
+            NN_CHECK(engine.zero(c.K));
+            NN_CHECK(engine.zero(c.V));
+        }
+        auto set_table = [&](const Tensor& t) {
+            for (KvPages& c : caches) c.table = t;
+        };
+        PagedStep step;
+        const CausalSelfAttention& attn = blocks_[0]->attention();
+        if (attn.rope()) NN_CHECK(attn.rope()->table(engine, std::min(seq_len_, P + steps), step.cos, step.sin));
+        if (!attn.slopes().empty())
+        {
+            Matrix m(attn.slopes().size(), 1);
+            std::copy(attn.slopes().begin(), attn.slopes().end(), m.data());
+            NN_TRY(t, engine.from_matrix(m));
+            step.slopes = t;
+        }
+        auto column = [&](std::size_t n, auto&& f) {
+            Matrix m(n, 1);
+            for (std::size_t i = 0; i < n; ++i) m.set_value_unchecked(i, 0, static_cast<Scalar>(f(i)));
+            return engine.from_matrix(m);
+        };
+
+        // The prompt: the hidden state of its last token.
+        Tensor last;
+        for (std::size_t at = 0; at < P; at += kPromptChunk)
+        {
+            const std::size_t n = std::min(kPromptChunk, P - at);
+            NN_TRY(ids, column(n, [&](std::size_t i) { return prompt[at + i]; }));
+            NN_TRY(pos, column(n, [&](std::size_t i) { return at + i; }));
+            NN_TRY(len, column(n, [&](std::size_t i) { return at + i + 1; }));
+            NN_TRY(shared, column(1, [&](std::size_t) { return at; }));
+            Matrix table(n, P);
+            for (std::size_t i = 0; i < n * P; ++i) table.data()[i] = static_cast<Scalar>(i % P);
+            NN_TRY(tt, engine.from_matrix(table));
+            set_table(tt);
+            step.pos = pos;
+            step.len = len;
+            step.shared = shared;
+            step.group = n;
+            NN_TRY(x, paged_hidden_(engine, ids, caches, step));
+            last = x;
+        }
+        NN_TRY(lt, engine.transpose(last));   // (n, d_model)
+        NN_TRY(lr, engine.slice_rows(lt, lt.rows() - 1, 1));
+        NN_TRY(lx, engine.transpose(lr));
+        NN_TRY(logits0, paged_logits_(engine, lx));
+
+        // The beams, fed one token at a time. found[t]: each beam's parent and token of step t.
+        const bool ends = eos < vocab_;
+        std::vector<std::vector<std::size_t>> parents, toks;
+        std::vector<char> ended(beams, 0);
+        NN_TRY(zero, engine.from_matrix(Matrix(1, 1, Scalar{0})));
+        Tensor b, k, len;
+        NN_TRY(s0, engine.beam_select(logits0, zero, nullptr, 1, beams, 0, b, k));
+        Tensor scores = s0;
+        for (std::size_t t = 0;; ++t)
+        {
+            NN_TRY(bm, engine.to_matrix(b));
+            NN_TRY(km, engine.to_matrix(k));
+            std::vector<std::size_t> pt(beams), kt(beams);
+            std::vector<char> now(beams);
+            bool live = false;
+            for (std::size_t i = 0; i < beams; ++i)
+            {
+                pt[i] = static_cast<std::size_t>(bm.data()[i]);
+                kt[i] = static_cast<std::size_t>(km.data()[i]);
+                now[i] = ends && kt[i] == eos;   // an ended beam goes on with eos
+                live = live || !now[i];
+            }
+            ended = now;
+            parents.push_back(std::move(pt));
+            toks.push_back(std::move(kt));
+            if (!live || t + 1 == steps) break;
+
+            NN_TRY(fresh, column(beams, [&](std::size_t i) { return P + t * beams + i; }));
+            if (t == 0)
+            {
+                Matrix table(beams, P + steps - 1, Scalar{-1});
+                for (std::size_t i = 0; i < beams; ++i)
+                    for (std::size_t j = 0; j <= P; ++j)
+                        table.set_value_unchecked(i, j, static_cast<Scalar>(j < P ? j : P + i));
+                NN_TRY(tt, engine.from_matrix(table));
+                set_table(tt);
+                NN_TRY(shared, column(1, [&](std::size_t) { return P; }));
+                step.shared = shared;
+                step.group = beams;
+            }
+            else
+            {
+                NN_TRY(tt, engine.kv_reorder(caches, b, step.len, &fresh, len));
+                set_table(tt);
+            }
+            NN_TRY(pos, column(beams, [&](std::size_t) { return P + t; }));
+            NN_TRY(lens, column(beams, [&](std::size_t) { return P + t + 1; }));
+            step.pos = pos;
+            step.len = lens;
+            NN_TRY(x, paged_hidden_(engine, k, caches, step));
+            NN_TRY(logits, paged_logits_(engine, x));
+            NN_TRY(done, column(beams, [&](std::size_t i) { return ended[i] ? 1 : 0; }));
+            NN_TRY(s, engine.beam_select(logits, scores, ends ? &done : nullptr, 1, beams, ends ? eos : 0, b, k));
+            scores = s;
+        }
+        NN_TRY(sm, engine.to_matrix(scores));
+        for (std::size_t i = 0; i < beams; ++i)
+        {
+            out.scores[i] = sm.data()[i];
+            std::vector<std::size_t>& seq = out.tokens[i];
+            for (std::size_t t = toks.size(), at = i; t-- > 0;)
+            {
+                if (!(ends && toks[t][at] == eos)) seq.push_back(toks[t][at]);
+                at = parents[t][at];
+            }
+            std::reverse(seq.begin(), seq.end());
+        }
+        return out;
+    }
+
 private:
+    // Tokens ids (batch) of a step through the blocks: hidden states (d_model, batch).
+    Result<Tensor> paged_hidden_(ComputeEngine& engine, const Tensor& ids, std::vector<KvPages>& caches,
+                                 const PagedStep& step)
+    {
+        NN_TRY(emb, engine.gather_rows(token_emb_, ids));
+        NN_TRY(x0, engine.transpose(emb));
+        NN_TRY(xp, pos_->apply_positions(engine, x0, step.pos));
+        Tensor x = xp;
+        for (std::size_t i = 0; i < blocks_.size(); ++i)
+        {
+            NN_TRY(y, blocks_[i]->forward_paged(engine, x, caches[i], step));
+            x = y;
+        }
+        return x;
+    }
+    Result<Tensor> paged_logits_(ComputeEngine& engine, const Tensor& x)
+    {
+        NN_TRY(ln, ln_f_->forward(engine, x));
+        return lm_head_.forward(engine, ln);
+    }
+
     std::size_t vocab_, d_model_, seq_len_;
     Tensor token_emb_, grad_token_emb_, tokens_;
     std::unique_ptr<PositionEncoder> pos_;

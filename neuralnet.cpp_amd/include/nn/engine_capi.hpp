@@ -200,6 +200,54 @@ inline int engine_op(EngineHandle* e, int op, void* const* in, std::size_t n_in,
         auto r = E.elementwise_select_scalar_cond(static_cast<CompareOp>(sz(0)), in_t(0), sc(1), in_t(1), sc(2));
         return put(0, r);
     }
+    case 31:   // args page, heads, with q, with cos and sin, with seq: K, V, table, k, v, pos[, q][, cos, sin][, seq]
+    {
+        if (!need(6, 0, 5)) return 1;
+        const bool q = flag(2), rope = flag(3), seq = flag(4);
+        if (!need(6 + (q ? 1 : 0) + (rope ? 2 : 0) + (seq ? 1 : 0), q ? 1 : 0, 5)) return 1;
+        KvPages c{in_t(0), in_t(1), in_t(2), sz(0), sz(1)};
+        std::size_t i = 6;
+        const Tensor *tq = q ? &in_t(i++) : nullptr, *cos = rope ? &in_t(i++) : nullptr, *sin = rope ? &in_t(i++) : nullptr;
+        auto r = E.kv_append(c, in_t(3), in_t(4), tq, in_t(5), seq ? &in_t(i) : nullptr, cos, sin);
+        if (!r) return set_error(r.error().message);
+        if (q) out[0] = new_tensor(*r);
+        return 0;
+    }
+    case 32:   // args page, heads, group, alpha, with shared, with slopes: K, V, table, q, len[, shared][, slopes]
+    {
+        if (!need(5, 1, 6)) return 1;
+        const bool shared = flag(4), slopes = flag(5);
+        if (!need(5 + (shared ? 1 : 0) + (slopes ? 1 : 0), 1, 6)) return 1;
+        const KvPages c{in_t(0), in_t(1), in_t(2), sz(0), sz(1)};
+        auto r = E.attn_paged(c, in_t(3), in_t(4), shared ? &in_t(5) : nullptr, sz(2),
+                              slopes ? &in_t(shared ? 6 : 5) : nullptr, sc(3));
+        return put(0, r);
+    }
+    case 33:   // args groups, take, eos: logits, scores[, done]
+    {
+        if (!need(2, 3, 3)) return 1;
+        Tensor b, k;
+        auto r = E.beam_select(in_t(0), in_t(1), opt_mask(2), sz(0), sz(1), sz(2), b, k);
+        if (put(0, r)) return 1;
+        out[1] = new_tensor(b);
+        out[2] = new_tensor(k);
+        return 0;
+    }
+    case 34:   // args page, heads, layers, with fresh: table, parent, len[, fresh], then K, V of each layer
+    {
+        if (!need(3, 2, 4)) return 1;
+        const bool fresh = flag(3);
+        const std::size_t layers = sz(2), first = fresh ? 4 : 3;
+        if (layers > n_in || !need(first + 2 * layers, 2, 4)) return 1;
+        std::vector<KvPages> c;
+        for (std::size_t i = 0; i < layers; ++i)
+            c.push_back(KvPages{in_t(first + 2 * i), in_t(first + 2 * i + 1), in_t(0), sz(0), sz(1)});
+        Tensor len;
+        auto r = E.kv_reorder(c, in_t(1), in_t(2), fresh ? &in_t(3) : nullptr, len);
+        if (put(0, r)) return 1;
+        out[1] = new_tensor(len);
+        return 0;
+    }
     default:
         return set_error("engine_op: unknown op " + std::to_string(op));
     }
@@ -262,6 +310,7 @@ struct GptSession
     std::size_t vocab = 0, seq = 0, batch = 0, num_valid = 0;
     Tensor tokens, labels, mask, logits;
     bool has_batch = false, has_mask = false;
+    bool searched = false;   // a beam search took the layers' inputs since the last forward pass
     GptConfigC cfg{};
 };
 
@@ -383,6 +432,7 @@ inline int gpt_forward_total(GptSession* g, Tensor& total)
     auto lg = g->model.forward(g->tokens);
     if (!lg) return set_error(lg.error().message);
     g->logits = *lg;
+    g->searched = false;
     auto t = g->ce.forward_sparse_total(*g->eng, g->logits, g->labels, g->has_mask ? &g->mask : nullptr, g->vocab,
                                         g->num_valid);
     if (!t) return set_error(t.error().message);
@@ -412,6 +462,7 @@ inline int gpt_forward_loss(GptSession* g, float* loss)
 // backward, so the accumulated gradients are the mean over the micro-batches.
 inline int gpt_backward_queued(GptSession* g, float grad_scale)
 {
+    if (g->searched) return set_error("gpt: a beam search ran since the forward pass; run the forward pass again");
     auto gr = g->ce.backward();
     if (!gr) return set_error(gr.error().message);
     if (grad_scale != 1.0f)
@@ -599,6 +650,40 @@ inline int gpt_generate(GptSession* g, const std::uint64_t* prompt, std::size_t 
     if (n_out) *n_out = toks->size();
     for (std::size_t i = 0; i < toks->size() && i < out_cap && out; ++i) out[i] = (*toks)[i];
     return 0;
+}
+
+// GPTModel::beam_search: the beams' tokens one after another (beams * max_new places), lengths and totals.
+inline int gpt_beam_search(GptSession* g, const std::uint64_t* prompt, std::size_t n_prompt, std::size_t beams,
+                           std::size_t max_new, std::uint64_t eos, std::uint64_t* out, std::size_t* out_len,
+                           float* out_scores)
+try
+{
+    GPTModel* m = g ? gpt_model(g) : nullptr;
+    if (!m) return set_error("gpt_beam_search: the session holds no GPT model");
+    if (!prompt || n_prompt == 0) return set_error("gpt_beam_search: empty prompt");
+    if (!out || !out_len || !out_scores) return set_error("gpt_beam_search: null output");
+    std::vector<std::size_t> pr(n_prompt);
+    for (std::size_t i = 0; i < n_prompt; ++i)
+    {
+        if (prompt[i] >= m->vocab_size()) return set_error("gpt_beam_search: prompt token out of range");
+        pr[i] = static_cast<std::size_t>(prompt[i]);
+    }
+    g->searched = true;
+    if (auto r = g->eng->begin_batch(); !r) return set_error(r.error().message);
+    auto b = m->beam_search(*g->eng, pr, beams, max_new, static_cast<std::size_t>(eos));
+    if (!b) return set_error(b.error().message);
+    if (auto r = g->eng->end_batch(); !r) return set_error(r.error().message);
+    for (std::size_t i = 0; i < beams; ++i)
+    {
+        out_len[i] = b->tokens[i].size();
+        out_scores[i] = b->scores[i];
+        std::copy(b->tokens[i].begin(), b->tokens[i].end(), out + i * max_new);
+    }
+    return 0;
+}
+catch (const std::exception& e)
+{
+    return set_error(std::string("gpt_beam_search: ") + e.what());
 }
 
 inline int gpt_step(GptSession* g)
@@ -893,6 +978,13 @@ inline int layer_program(const char* name, std::uint32_t param, std::uint8_t* in
         return nn::capi::gpt_forward_step(static_cast<nn::capi::GptSession*>(g), token, pos, cur_len, logits);     \
     }                                                                                                               \
     int NN_CAPI_CAT(P, gpt_reset_cache)(void* g) { return nn::capi::gpt_reset_cache(static_cast<nn::capi::GptSession*>(g)); } \
+    int NN_CAPI_CAT(P, gpt_beam_search)(void* g, const uint64_t* prompt, size_t n_prompt, size_t beams,            \
+                                        size_t max_new, uint64_t eos, uint64_t* out, size_t* out_len,              \
+                                        float* out_scores)                                                         \
+    {                                                                                                               \
+        return nn::capi::gpt_beam_search(static_cast<nn::capi::GptSession*>(g), prompt, n_prompt, beams, max_new,  \
+                                         eos, out, out_len, out_scores);                                            \
+    }                                                                                                               \
     int NN_CAPI_CAT(P, gpt_generate)(void* g, const uint64_t* prompt, size_t n_prompt, size_t max_new,             \
                                      float temperature, uint64_t eos, size_t min_new, uint64_t seed, uint64_t* out,  \
                                      size_t out_cap, size_t* n_out)                                                 \

@@ -84,6 +84,14 @@ public:
     Result<void> scatter_add_rows(Tensor& dst, const Tensor& indices, const Tensor& grad) override;
     Result<Tensor> rearrange_3d(const Tensor& x, std::size_t M, std::size_t B, std::size_t N, bool inverse) override;
     Result<Tensor> transpose(const Tensor& A) override;
+    Result<Tensor> kv_append(KvPages& cache, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                             const Tensor* seq, const Tensor* cos, const Tensor* sin) override;
+    Result<Tensor> attn_paged(const KvPages& cache, const Tensor& q, const Tensor& len, const Tensor* shared,
+                              std::size_t group, const Tensor* slopes, Scalar alpha) override;
+    Result<Tensor> beam_select(const Tensor& logits, const Tensor& scores, const Tensor* done, std::size_t groups,
+                               std::size_t take, std::size_t eos, Tensor& beams_out, Tensor& tokens_out) override;
+    Result<Tensor> kv_reorder(std::span<KvPages> layers, const Tensor& parent, const Tensor& len, const Tensor* fresh,
+                              Tensor& len_out) override;
 
     Result<Tensor> matmul(const Tensor& A, const Tensor& B, bool transA, bool transB) override;
     Result<Tensor> batched_matmul(const Tensor& A, const Tensor& B, std::size_t batch, bool transA, bool transB,

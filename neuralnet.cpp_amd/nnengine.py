@@ -30,7 +30,7 @@ OP = dict(CLONE=1, SLICE_ROWS=2, INSERT_ROWS=3, GATHER_ROWS=4, SCATTER_ADD_ROWS=
           BMM_BWD_KV=14, COL_SOFTMAX_DENOM=15, COL_SOFTMAX_SPARSE=16, ADD_INPLACE=17, SCALE_INPLACE=18,
           AXPY_INPLACE=19, ZERO=20, ROW_REDUCE_SUM=21, COL_REDUCE_SUM=22, ROW_REDUCE_MAX=23,
           COL_REDUCE_MAX=24, BROADCAST_ROW=25, BROADCAST_COL=26, UNARY=27, BINARY=28, BINARY_SCALAR=29,
-          SELECT_SCALAR_COND=30)
+          SELECT_SCALAR_COND=30, KV_APPEND=31, ATTN_PAGED=32, BEAM_SELECT=33, KV_REORDER=34)
 
 # Enum values of compute_engine.hpp:43-82.
 UNARY = dict(Neg=0, Exp=1, Log=2, Sqrt=3, Rsqrt=4, Abs=5, Tanh=6)
@@ -127,6 +127,7 @@ def _bind(lib: ctypes.CDLL, prefix: str):
         "gpt_reset_cache": (i32, [vp]),
         "gpt_generate": (i32, [vp, u64p, sz, sz, ctypes.c_float, ctypes.c_uint64, sz, ctypes.c_uint64, u64p, sz,
                                ctypes.POINTER(ctypes.c_size_t)]),
+        "gpt_beam_search": (i32, [vp, u64p, sz, sz, sz, ctypes.c_uint64, u64p, ctypes.POINTER(sz), fp]),
         "build_attention_mask": (i32, [sz, sz, sz, i32, fp, ctypes.POINTER(ctypes.c_uint64), sz, fp]),
     }
     fns = {}
@@ -341,6 +342,31 @@ class Engine:
 
     def eval_expr_reduce(self, spec, inputs, rows, cols):
         return self.eval_expr(spec, inputs, rows, cols, vector_out=True)
+
+    # -- paged caches and beam search (no reference counterpart; nnhip_engine.h) --------
+    def kv_append(self, K, V, table, k, v, pos, page=1, heads=1, q=None, cos=None, sin=None, seq=None):
+        """Stores the tokens' keys and values in the pages (K and V in place), k and q turned by rows pos of cos and
+        sin; returns q so turned, or None without q."""
+        if (cos is None) != (sin is None):
+            raise EngineError("kv_append: cos and sin go together")
+        ins = [K, V, table, k, v, pos] + [t for t in (q, cos, sin, seq) if t is not None]
+        out = self._op("KV_APPEND", ins, 0 if q is None else 1, [page, heads, q is not None, cos is not None, seq is not None])
+        return out[0] if out else None
+
+    def attn_paged(self, K, V, table, q, lens, alpha, page=1, heads=1, shared=None, group=1, slopes=None):
+        """Attention of one query per sequence over its first lens positions; shared counts the positions that each
+        group of `group` sequences has in common."""
+        ins = [K, V, table, q, lens] + [t for t in (shared, slopes) if t is not None]
+        return self._op("ATTN_PAGED", ins, 1, [page, heads, group, alpha, shared is not None, slopes is not None])[0]
+
+    def beam_select(self, logits, scores, take, done=None, groups=1, eos=0):
+        """Returns (totals, beams, tokens), (groups, take) each, of logits (vocab, groups * beams)."""
+        return tuple(self._op("BEAM_SELECT", [logits, scores] + ([done] if done is not None else []), 3, [groups, take, eos]))
+
+    def kv_reorder(self, caches, table, parent, lens, fresh=None, page=1, heads=1):
+        """caches: (K, V) of each layer. Returns (table, lens) of the sequences that continue parent."""
+        ins = [table, parent, lens] + ([fresh] if fresh is not None else []) + [t for kv in caches for t in kv]
+        return tuple(self._op("KV_REORDER", ins, 2, [page, heads, len(caches), fresh is not None]))
 
     # -- pure host helpers ------------------------------------------------------
     def build_attention_mask(self, batch, seq, heads, use_alibi, slopes=(), doc_ids=()):
@@ -575,6 +601,17 @@ class GptSession:
                                                  float(temperature), int(eos), int(min_new), int(seed),
                                                  out.ctypes.data_as(u64p), out.size, ctypes.byref(n)))
         return out[:n.value].astype(np.int64).tolist()
+
+    def beam_search(self, prompt, beams: int, max_new: int, eos: int = 2 ** 64 - 1):
+        """The `beams` best continuations of the prompt: a list of (token ids, sum of log probabilities), best first."""
+        pr = np.ascontiguousarray(np.asarray(prompt, dtype=np.uint64))
+        out = np.zeros(max(1, beams * max_new), dtype=np.uint64)
+        n = (ctypes.c_size_t * max(1, beams))()
+        scores = np.zeros(max(1, beams), dtype=np.float32)
+        u64p = ctypes.POINTER(ctypes.c_uint64)
+        self._eng._check(self._f["gpt_beam_search"](self._g, pr.ctypes.data_as(u64p), pr.size, int(beams), int(max_new),
+                                                    int(eos), out.ctypes.data_as(u64p), n, _fptr(scores)))
+        return [(out[i * max_new:i * max_new + n[i]].astype(np.int64).tolist(), float(scores[i])) for i in range(beams)]
 
     def backward_scaled(self, grad_scale: float) -> None:
         """Backward of one accumulated micro-batch: loss gradient scaled by grad_scale first."""

@@ -20,6 +20,7 @@
 
 #include "cpu_algebra.hpp"
 #include "nn/compute_engine.hpp"
+#include "nn/paged_checks.hpp"
 
 namespace nn::oracle
 {
@@ -72,6 +73,26 @@ class CpuEngine final : public ComputeEngine
 {
     static constexpr float kNegInf = -std::numeric_limits<float>::infinity();
 
+    static std::size_t length_(float f, std::size_t most)
+    {
+        if (!(f >= 1.0f)) return 0;
+        return f >= static_cast<float>(most) ? most : static_cast<std::size_t>(f);
+    }
+    // Row of position pos of the table's row b; false where there is none.
+    static bool page_row_(const KvPages& c, std::size_t b, std::size_t pos, std::size_t& row)
+    {
+        const std::size_t i = pos / c.page;
+        std::size_t p;
+        if (i >= c.table.cols() || !row_index(P(c.table)[b * c.table.cols() + i], c.K.rows() / c.page, p)) return false;
+        row = p * c.page + pos % c.page;
+        return true;
+    }
+    static bool on_cpu_(std::initializer_list<const Tensor*> ts)
+    {
+        for (const Tensor* t : ts)
+            if (t && !t->is_cpu()) return false;
+        return true;
+    }
     static const float* P(const Tensor& t) { return t.cpu_matrix().data(); }
     static float* W(Tensor& t) { return t.cpu_matrix().data(); }
     static Result<void> need_cpu(std::initializer_list<const Tensor*> ts)
@@ -179,6 +200,164 @@ public:
             for (std::size_t c = 0; c < D; ++c) d[r * D + c] += g[i * D + c];
         }
         return {};
+    }
+
+    // Paged caches and beam search (no reference counterpart): plain loops, sums in float64.
+    Result<Tensor> kv_append(KvPages& c, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                             const Tensor* seq, const Tensor* cos, const Tensor* sin) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.table, &k, &v, q, &pos, seq, cos, sin})) return fail("kv_append: tensors are not CPU");
+        NN_TRY(s, paged::check_append(c, k, v, q, pos, seq, cos, sin));
+        const std::size_t N = k.cols(), d = s.dim, h = s.half;
+        Tensor out;
+        if (q) out = Tensor::from_matrix(Matrix(q->cpu_matrix()));
+        for (std::size_t n = 0; n < N; ++n)
+        {
+            std::size_t b = n, p, row;
+            if (seq ? !row_index(P(*seq)[n], c.table.rows(), b) : n >= c.table.rows()) continue;
+            if (!row_index(P(pos)[n], paged::kMaxIndex, p) || (cos && p >= cos->rows()) || !page_row_(c, b, p, row)) continue;
+            // f(head, feature): x turned by the position's angles, to y(index)
+            auto turned = [&](const Tensor& x, std::size_t heads, auto&& put) {
+                for (std::size_t e = 0; e < heads; ++e)
+                    for (std::size_t j = 0; j < d; ++j)
+                    {
+                        const float a = P(x)[(e * d + j) * N + n];
+                        float y = a;
+                        if (j < 2 * h)
+                        {
+                            const std::size_t i = j < h ? j : j - h;
+                            const float o = P(x)[(e * d + (j < h ? j + h : i)) * N + n];
+                            const float co = P(*cos)[p * h + i], si = P(*sin)[p * h + i];
+                            y = j < h ? a * co - o * si : a * co + o * si;
+                        }
+                        put(e * d + j, y);
+                    }
+            };
+            turned(k, c.heads, [&](std::size_t f, float y) { W(c.K)[row * c.K.cols() + f] = y; });
+            for (std::size_t f = 0; f < v.rows(); ++f) W(c.V)[row * c.V.cols() + f] = P(v)[f * N + n];
+            if (q) turned(*q, s.q_heads, [&](std::size_t f, float y) { W(out)[f * N + n] = y; });
+        }
+        return out;
+    }
+    Result<Tensor> attn_paged(const KvPages& c, const Tensor& q, const Tensor& len, const Tensor* shared, std::size_t group,
+                              const Tensor* slopes, Scalar alpha) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.table, &q, &len, shared, slopes})) return fail("attn_paged: tensors are not CPU");
+        NN_TRY(d, paged::check_attn(c, q, len, shared, group, slopes));
+        const std::size_t B = q.cols(), H = q.rows() / d, per = H / c.heads, most = c.table.cols() * c.page;
+        Matrix out(q.rows(), B);
+        std::vector<std::size_t> rows, at;
+        std::vector<double> s, o(d);
+        for (std::size_t b = 0; b < B; ++b)
+        {
+            const std::size_t n = length_(P(len)[b], most);
+            const std::size_t common = shared ? length_(P(*shared)[b / group], most) : 0;
+            rows.clear();
+            at.clear();
+            for (std::size_t j = 0; j < n; ++j)
+            {
+                std::size_t r;
+                if (!page_row_(c, n >= common && j < common ? b / group * group : b, j, r)) continue;
+                rows.push_back(r);
+                at.push_back(j);
+            }
+            for (std::size_t h = 0; h < H; ++h)
+            {
+                s.assign(rows.size(), 0.0);
+                double m = -std::numeric_limits<double>::infinity(), l = 0.0;
+                for (std::size_t i = 0; i < rows.size(); ++i)
+                {
+                    double dot = 0.0;
+                    for (std::size_t e = 0; e < d; ++e)
+                        dot += static_cast<double>(P(q)[(h * d + e) * B + b]) * P(c.K)[rows[i] * c.K.cols() + h / per * d + e];
+                    s[i] = alpha * dot - (slopes ? static_cast<double>(P(*slopes)[h]) * static_cast<double>(n - 1 - at[i]) : 0.0);
+                    m = std::max(m, s[i]);
+                }
+                std::fill(o.begin(), o.end(), 0.0);
+                if (m != -std::numeric_limits<double>::infinity())
+                    for (std::size_t i = 0; i < rows.size(); ++i)
+                    {
+                        const double w = std::exp(s[i] - m);
+                        l += w;
+                        for (std::size_t e = 0; e < d; ++e) o[e] += w * P(c.V)[rows[i] * c.V.cols() + h / per * d + e];
+                    }
+                for (std::size_t e = 0; e < d; ++e) out.data()[(h * d + e) * B + b] = l == 0.0 ? 0.0f : static_cast<float>(o[e] / l);
+            }
+        }
+        return Tensor::from_matrix(std::move(out));
+    }
+    Result<Tensor> beam_select(const Tensor& logits, const Tensor& scores, const Tensor* done, std::size_t groups,
+                               std::size_t take, std::size_t eos, Tensor& beams_out, Tensor& tokens_out) override
+    {
+        if (!on_cpu_({&logits, &scores, done})) return fail("beam_select: tensors are not CPU");
+        NN_TRY(beams, paged::check_select(logits, scores, done, groups, take, eos));
+        const std::size_t V = logits.rows(), N = logits.cols();
+        const double none = -std::numeric_limits<double>::infinity();
+        Matrix os(groups, take), ob(groups, take), ot(groups, take);
+        std::vector<std::pair<double, std::size_t>> all(beams * V);
+        for (std::size_t g = 0; g < groups; ++g)
+        {
+            for (std::size_t w = 0; w < beams; ++w)
+            {
+                const std::size_t n = g * beams + w;
+                const bool ended = done && P(*done)[n] != 0.0f;
+                double m = none, sum = 0.0;
+                for (std::size_t v = 0; v < V; ++v) m = std::max(m, static_cast<double>(P(logits)[v * N + n]));
+                for (std::size_t v = 0; v < V; ++v) sum += std::exp(static_cast<double>(P(logits)[v * N + n]) - m);
+                const double lse = m + std::log(sum), score = P(scores)[n];
+                for (std::size_t v = 0; v < V; ++v)
+                {
+                    double x = ended ? (v == eos ? score : none) : score + (static_cast<double>(P(logits)[v * N + n]) - lse);
+                    if (x != x) x = none;
+                    all[w * V + v] = {x, w * V + v};
+                }
+            }
+            std::partial_sort(all.begin(), all.begin() + static_cast<std::ptrdiff_t>(take), all.end(),
+                              [](const auto& a, const auto& b) { return a.first > b.first || (a.first == b.first && a.second < b.second); });
+            for (std::size_t i = 0; i < take; ++i)
+            {
+                os.data()[g * take + i] = static_cast<float>(all[i].first);
+                ob.data()[g * take + i] = static_cast<float>(g * beams + all[i].second / V);
+                ot.data()[g * take + i] = static_cast<float>(all[i].second % V);
+            }
+        }
+        beams_out = Tensor::from_matrix(std::move(ob));
+        tokens_out = Tensor::from_matrix(std::move(ot));
+        return Tensor::from_matrix(std::move(os));
+    }
+    Result<Tensor> kv_reorder(std::span<KvPages> layers, const Tensor& parent, const Tensor& len, const Tensor* fresh,
+                              Tensor& len_out) override
+    {
+        NN_CHECK(paged::check_reorder(layers, parent, len, fresh));
+        for (const KvPages& x : layers)
+            if (!on_cpu_({&x.K, &x.V, &x.table, &parent, &len, fresh})) return fail("kv_reorder: tensors are not CPU");
+        const KvPages& c = layers[0];
+        const std::size_t n = parent.size(), width = c.table.cols(), pages = c.K.rows() / c.page;
+        Matrix out(n, width, -1.0f), lens(n, 1, 0.0f);
+        for (std::size_t b = 0; b < n; ++b)
+        {
+            std::size_t p, f, src;
+            if (!row_index(P(parent)[b], c.table.rows(), p)) continue;
+            const float* row = P(c.table) + p * width;
+            const std::size_t have = length_(P(len)[p], width * c.page), full = have / c.page, tail = have % c.page;
+            lens.data()[b] = static_cast<float>(have);
+            std::copy_n(row, full, out.data() + b * width);
+            if (full >= width) continue;
+            float& next = out.data()[b * width + full];
+            if (!fresh)
+            {
+                if (tail) next = row[full];
+                continue;
+            }
+            if (!row_index(P(*fresh)[b], pages, f)) continue;
+            next = static_cast<float>(f);
+            if (!row_index(row[full], pages, src) || src == f) continue;
+            for (KvPages& x : layers)
+                for (Tensor* t : {&x.K, &x.V})
+                    std::memcpy(W(*t) + f * c.page * t->cols(), P(*t) + src * c.page * t->cols(), tail * t->cols() * sizeof(float));
+        }
+        len_out = Tensor::from_matrix(std::move(lens));
+        return Tensor::from_matrix(std::move(out));
     }
 
     // reference :226-279
