@@ -501,7 +501,7 @@ int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f,
  * sequences have in common: the tables of the group name the same rows there, and these are read once for all
  * of them (through the table of the group's first sequence). A sequence shorter than that is read through its
  * own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
- * The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed); calls that may overlap in time
+ * The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte aligned; calls that may overlap in time
  * need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
  * bits every time. */
 size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t group);

@@ -44,7 +44,9 @@ struct PagedArgs
     long o_t, o_f;
     float *m, *l;
     float *part_ml, *part_o;   // per (row of the batch, range): m and l; O unnormalised
-    unsigned q_heads, group, n_shared, n_own, shared_blocks, shared_row_blocks, own_row_blocks;
+    unsigned q_heads, group, n_shared, n_own, shared_blocks;
+    // per: query heads of a key head; of the shared and the own parts: 8 row blocks, ranges
+    FastDiv by_per, by_heads, by_shared_rows, by_own_rows, by_n_shared, by_n_own;
     int shared_row_waves, own_row_waves, own_wide;   // own_wide: own parts in RT row tiles a wave too
     float alpha;
 };
@@ -251,7 +253,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
     using G = Geometry<KS>;
     constexpr int DP = G::DV;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, j = lane & 15, g = lane >> 4, dim = a.c.dim;
-    const unsigned per = a.q_heads / a.c.heads, n_rows = part.nb * per;   // per: query heads of a key head
+    const unsigned per = a.by_per.d, n_rows = part.nb * per;
     const int rws = part.row_waves, kws = 4 / rws, rw = wave % rws, kw = wave / rws, step = kws * kTile;
     const int most = (int)(a.c.width * a.c.page.d), begin = part.begin, end = part.end;
     Row<KS> rows[RT];
@@ -261,7 +263,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
         Row<KS>& w = rows[i];
         const unsigned row = ((part.rb * rws + rw) * RT + i) * kTile + j;
         const bool live = row < n_rows;
-        const unsigned b = live ? part.b0 + row / per : part.b0, qh = part.h * per + (live ? row % per : 0);
+        const unsigned bq = live ? a.by_per.div(row) : 0, b = part.b0 + bq, qh = part.h * per + (live ? row - bq * per : 0);
         w.len = live ? length_of(a.len[b], most) : 0;
         w.counts = live && (!part.is_shared || w.len >= part.common);
         w.slope = a.slopes && live ? a.slopes[qh] : 0.0f;
@@ -314,6 +316,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
                 for (int half = 0; half < 2; ++half)
                 {
                     const int at = p + half * step;
+                    if (half && at >= end) break;
                     const float further = entry(at + 2 * step);
                     const int r = row_at(ahead, at + step);
                     load_keys<KS, MODE>(a, r, part.h, lane, x[1 - half]);
@@ -372,36 +375,57 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sh.o[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = w.o[x][y][r];
         __syncthreads();
-        for (int e = t; e < rws * kTile * DP; e += 256)
+        // 16 threads a row, 4 neighbouring values at a time.
+        const int jr = t >> 4;
+        for (int rv = 0; rv < rws; ++rv)   // row waves
         {
-            const int d = e % DP, jr = e / DP % kTile, rv = e / (DP * kTile);   // rv: row wave
             const unsigned row = ((part.rb * rws + rv) * RT + i) * kTile + jr;
-            if (row >= n_rows || d >= dim) continue;
-            const unsigned b = part.b0 + row / per, qh = part.h * per + row % per;
-            float mm = kLowest, ll = 0.0f, oo = 0.0f;
-            for (int k = rv; k < 4; k += rws) mm = fmax_std(mm, sh.ml[k][jr][0]);
-            for (int k = rv; k < 4; k += rws)
+            if (row >= n_rows) break;
+            const unsigned bq = a.by_per.div(row), b = part.b0 + bq, qh = part.h * per + (row - bq * per);
+            float mm = kLowest, ll = 0.0f, f[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k % rws == rv) mm = fmax_std(mm, sh.ml[k][jr][0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
             {
                 const float lk = sh.ml[k][jr][1];
-                const float f = __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
-                ll += lk == 0.0f ? 0.0f : lk * f;
-                oo += lk == 0.0f ? 0.0f : sh.o[k][jr][d] * f;
+                f[k] = k % rws != rv || lk == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
+                ll += f[k] == 0.0f ? 0.0f : lk * f[k];
             }
-            const size_t at = (size_t)b * a.q_heads + qh;
-            if (direct)
+            const size_t at = (size_t)b * a.q_heads + qh, p = at * n_parts + part.slot;
+            const float inv = !direct ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+            for (int x = 0; x < (DP + 63) / 64; ++x)
             {
-                a.O[(long)b * a.o_t + ((long)qh * dim + d) * a.o_f] = ll == 0.0f ? 0.0f : oo / ll;
-                if (d == 0 && a.m) a.m[at] = mm;
-                if (d == 0 && a.l) a.l[at] = ll;
+                const int d = 64 * x + 4 * (t & 15);
+                if (d >= dim) continue;
+                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (f[k] != 0.0f) o += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
+                o *= inv;
+                if (!direct && MODE != kSingle) *reinterpret_cast<f32x4*>(a.part_o + p * dim + d) = o;
+                else
+                {
+                    float* to = direct ? a.O + (long)b * a.o_t + (long)qh * dim * a.o_f : a.part_o + p * dim;
+                    const long step_f = direct ? a.o_f : 1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < dim) to[(d + e) * step_f] = o[e];
+                }
             }
-            else
+            if ((t & 15) == 0)
             {
-                const size_t p = at * n_parts + part.slot;
-                a.part_o[p * dim + d] = oo;
-                if (d == 0)
+                if (!direct)
                 {
                     a.part_ml[2 * p] = mm;
                     a.part_ml[2 * p + 1] = ll;
+                }
+                else
+                {
+                    if (a.m) a.m[at] = mm;
+                    if (a.l) a.l[at] = ll;
                 }
             }
         }
@@ -416,18 +440,20 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     unsigned i = blockIdx.x, c;
     part.is_shared = i < a.shared_blocks;
     if (!part.is_shared) i -= a.shared_blocks;
-    const unsigned row_blocks = part.is_shared ? a.shared_row_blocks : a.own_row_blocks;
-    const unsigned ranges = part.is_shared ? a.n_shared : a.n_own;
+    const FastDiv by_rows = part.is_shared ? a.by_shared_rows : a.by_own_rows;
+    const FastDiv by_ranges = part.is_shared ? a.by_n_shared : a.by_n_own;
+    const unsigned ranges = by_ranges.d;
     // The blocks of rows that read the same keys and values run on one XCD (workgroups go to the 8 in turn), so
     // that its L2 holds them once; the pieces are padded to a multiple of 8.
-    part.rb = i / 8 % row_blocks;
-    i = i / (8 * row_blocks) * 8 + i % 8;
-    c = i % ranges;
-    i /= ranges;
-    part.h = i % a.c.heads;
-    i /= a.c.heads;
+    const unsigned eight = by_rows.div(i);
+    part.rb = (i - eight * by_rows.d) / 8;
+    i = eight * 8 + i % 8;
+    unsigned next = by_ranges.div(i);
+    c = i - next * ranges;
+    i = a.by_heads.div(next);
+    part.h = next - i * a.c.heads;
     part.nb = part.is_shared ? a.group : 1;
-    if (i >= a.c.batch / part.nb) return;
+    if (i * part.nb >= a.c.batch) return;
     part.b0 = i * part.nb;
     part.slot = part.is_shared ? c : a.n_shared + c;
     part.row_waves = part.is_shared ? a.shared_row_waves : a.own_row_waves;
@@ -443,6 +469,21 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     const int first = (int)((long)steps * c / ranges), last = (int)((long)steps * (c + 1) / ranges);
     part.begin = lo + first * kStep;
     part.end = min(hi, lo + last * kStep);
+    if (part.begin >= part.end && a.n_shared + a.n_own > 1)
+    {
+        // Nothing here: the join leaves out ranges of l = 0, whatever their O is.
+        const unsigned rows_here = kTile * part.row_waves * (part.is_shared || a.own_wide ? RT : 1);
+        const unsigned n_rows = part.nb * a.by_per.d, row = part.rb * rows_here + threadIdx.x;
+        if (threadIdx.x < rows_here && row < n_rows)
+        {
+            const unsigned q = a.by_per.div(row);
+            const size_t at = (size_t)(part.b0 + q) * a.q_heads + part.h * a.by_per.d + (row - q * a.by_per.d);
+            const size_t p = at * (a.n_shared + a.n_own) + part.slot;
+            a.part_ml[2 * p] = kLowest;
+            a.part_ml[2 * p + 1] = 0.0f;
+        }
+        return;
+    }
     if (RT == 1 || part.is_shared || a.own_wide) walk<KS, MODE, RT>(a, part, sh);
     else walk<KS, MODE, 1>(a, part, sh);
 }
@@ -474,7 +515,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
         if (c + t < n)
         {
             const float li = ml[2 * (c + t) + 1];
-            if (li != 0.0f) w = __builtin_amdgcn_exp2f((ml[2 * (c + t)] - m) * kLog2e);   // O is 0 where l is
+            if (li != 0.0f) w = __builtin_amdgcn_exp2f((ml[2 * (c + t)] - m) * kLog2e);
             l += li * w;
         }
         __syncthreads();
@@ -482,7 +523,11 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
         __syncthreads();
         const int nc = min((int)(n - c), kChunk);
 #pragma unroll 8
-        for (int i = g; i < nc; i += groups) o += po[(size_t)(c + i) * dim] * w_s[i];
+        for (int i = g; i < nc; i += groups)
+        {
+            const float x = po[(size_t)(c + i) * dim], f = w_s[i];
+            o += f == 0.0f ? 0.0f : x * f;   // where l is 0, O is anything
+        }
     }
     l = wave_sum(l);
     if (lane == 0) red[1][wave] = l;
@@ -546,6 +591,12 @@ template <int KS, int MODE> void paged_launch(const PagedArgs& a, const PagedPla
     else hipLaunchKernelGGL((k_attn_paged<KS, MODE, 2>), grid, dim3(256), 0, s, a);
 }
 
+// m and l of every row and range, in whole 16 bytes.
+size_t ml_floats(const nnhip_kv_pages& c, size_t q_heads, const PagedPlan& p)
+{
+    return (2 * c.batch * q_heads * p.parts() + 3) / 4 * 4;
+}
+
 bool paged_ok(const nnhip_kv_pages* c, size_t q_heads, size_t group)
 {
     return pages_ok(c, kPagedMaxDim) && q_heads > 0 && q_heads % c->heads == 0 && q_heads <= kMaxIndex && group > 0 &&
@@ -561,7 +612,7 @@ extern "C" size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size
 {
     if (!paged_ok(c, q_heads, group)) return 0;
     const PagedPlan p = paged_plan(*c, q_heads, group);
-    return p.parts() == 1 ? 0 : c->batch * q_heads * p.parts() * (2 + c->dim) * sizeof(float);
+    return p.parts() == 1 ? 0 : (ml_floats(*c, q_heads, p) + c->batch * q_heads * p.parts() * c->dim) * sizeof(float);
 }
 
 extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads,
@@ -573,7 +624,7 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
         c->batch * q_heads > 0x7fffffffu)
         return -1;
     const size_t need = nnhip_attn_paged_workspace_bytes(c, q_heads, group);
-    if (need > 0 && (!workspace || workspace_bytes < need)) return -1;
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
     PagedPlan p = paged_plan(*c, q_heads, group);
     if (group == 1) shared = nullptr;   // a group of one has all positions to itself
     if (!shared)
@@ -583,12 +634,36 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     }
     if (p.shared_blocks + p.own_blocks > 0x7fffffffu) return -1;
     auto* ws = static_cast<float*>(workspace);
-    PagedArgs a{pages_of(*c), q, q_t, q_f, len, shared, slopes, O, o_t, o_f, m, l, ws, nullptr,
-                static_cast<unsigned>(q_heads), static_cast<unsigned>(group), p.n_shared, p.n_own,
-                static_cast<unsigned>(p.shared_blocks), p.shared_row_blocks, p.own_row_blocks, p.shared_row_waves,
-                p.own_row_waves, p.own_wide,
-                alpha};
-    if (p.parts() > 1) a.part_o = ws + 2 * c->batch * q_heads * p.parts();
+    PagedArgs a{};
+    a.c = pages_of(*c);
+    a.q = q;
+    a.q_t = q_t;
+    a.q_f = q_f;
+    a.len = len;
+    a.shared = shared;
+    a.slopes = slopes;
+    a.O = O;
+    a.o_t = o_t;
+    a.o_f = o_f;
+    a.m = m;
+    a.l = l;
+    a.part_ml = ws;
+    a.q_heads = static_cast<unsigned>(q_heads);
+    a.group = static_cast<unsigned>(group);
+    a.n_shared = p.n_shared;
+    a.n_own = p.n_own;
+    a.shared_blocks = static_cast<unsigned>(p.shared_blocks);
+    a.by_per = FastDiv(static_cast<unsigned>(q_heads / c->heads));
+    a.by_heads = FastDiv(a.c.heads);
+    a.by_shared_rows = FastDiv(8 * (shared ? p.shared_row_blocks : 1));
+    a.by_own_rows = FastDiv(8 * p.own_row_blocks);
+    a.by_n_shared = FastDiv(shared ? p.n_shared : 1);
+    a.by_n_own = FastDiv(p.n_own);
+    a.shared_row_waves = p.shared_row_waves;
+    a.own_row_waves = p.own_row_waves;
+    a.own_wide = p.own_wide;
+    a.alpha = alpha;
+    if (p.parts() > 1) a.part_o = ws + ml_floats(*c, q_heads, p);
     const size_t d = c->dim;
     const bool vec = d % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V);
     const int mode = !vec ? kSingle : d % 16 == 0 ? kWhole : kCut;

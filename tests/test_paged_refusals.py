@@ -60,7 +60,7 @@ def test_attend_pages(bad):
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(len=None), dict(O=None), dict(q_heads=0), dict(q_heads=6), dict(group=0),
                                  dict(group=3), dict(group=8), dict(st=(-1, 1)), dict(st=(1, -1)), dict(ws=None),
-                                 dict(nbytes=0)])
+                                 dict(ws=P + 8), dict(nbytes=0)])
 def test_attend_arguments(bad):
     need = library().nnhip_attn_paged_workspace_bytes(pages(), 4, 2)
     assert need > 0
