@@ -383,6 +383,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
             if (row >= n_rows) break;
             const unsigned bq = a.by_per.div(row), b = part.b0 + bq, qh = part.h * per + (row - bq * per);
             float mm = kLowest, ll = 0.0f, f[4];
+            bool any[4];   // waves that had positions: a NaN among these stays one, whatever its factor is
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 if (k % rws == rv) mm = fmax_std(mm, sh.ml[k][jr][0]);
@@ -390,8 +391,9 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
             for (int k = 0; k < 4; ++k)
             {
                 const float lk = sh.ml[k][jr][1];
-                f[k] = k % rws != rv || lk == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
-                ll += f[k] == 0.0f ? 0.0f : lk * f[k];
+                any[k] = k % rws == rv && lk != 0.0f;
+                f[k] = __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
+                ll += any[k] ? lk * f[k] : 0.0f;
             }
             const size_t at = (size_t)b * a.q_heads + qh, p = at * n_parts + part.slot;
             const float inv = !direct ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -403,7 +405,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
                 f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (f[k] != 0.0f) o += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
+                    if (any[k]) o += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
                 o *= inv;
                 if (!direct && MODE != kSingle) *reinterpret_cast<f32x4*>(a.part_o + p * dim + d) = o;
                 else

@@ -301,6 +301,20 @@ def test_attend_scores_of_minus_infinity():
         assert np.all(np.isnan(O[0, 2:])) and not np.isnan(O[1]).any()
 
 
+@pytest.mark.parametrize("at,n", [(0, 1), (0, 300), (16, 17), (70, 71), (299, 300), (150, 300)])
+@pytest.mark.parametrize("shared", [None, 288])
+def test_attend_one_nan(at, n, shared):
+    """One NaN key, alone in its tile, its wave or its range or not, makes the sequences that see it NaN, and no other."""
+    rng = np.random.default_rng(at + n)
+    K, V = (rng.normal(size=(304, 1, 64)).astype(np.float32) for _ in range(2))
+    K[at] = np.nan
+    q = rng.normal(size=(2, 2, 64)).astype(np.float32)
+    table = np.arange(19, dtype=np.float32)[None, :].repeat(2, 0)
+    c = dict(pages=19, page=16, heads=1, dim=64)
+    O, m, l = run_attend(c, q, K, V, table, [n, at], None if shared is None else [shared], 2, None, 1.0)
+    assert np.isnan(O[0]).all() and np.isnan(l[0]).all() and not np.isnan(O[1]).any()
+
+
 def test_attend_large_scores():
     """Scores around 1e4 in both directions: exact weights of 0 and 1, no overflow."""
     rng = np.random.default_rng(8)
