@@ -558,7 +558,7 @@ struct PagedPlan
 PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
 {
     PagedPlan p{};
-    const size_t per = q_heads / c.heads, most = c.width * c.page, target = 2 * (size_t)device_cus();
+    const size_t per = q_heads / c.heads, most = c.width * c.page, cus = device_cus();
     const size_t rows = group > 1 ? group * per : per;   // that read the same positions
     p.row_tiles = rows > kTile ? 2 : 1;
     p.own_wide = per > kTile;
@@ -567,20 +567,23 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
         waves = need > 2 ? 4 : need > 1 ? 2 : 1;
         return static_cast<unsigned>((need + waves - 1) / waves);
     };
-    auto ranges = [&](size_t others) {
-        const size_t want = (target + others - 1) / others, most_ranges = (most + 63) / 64;
+    // Workgroups a CU: the streams of unshared sequences run best with 6 (attend of 24 sequences of 2500 to 5000:
+    // 120 us with 2, 109 with 4, 103 with 6, 108 with 8); ranges of shared positions cost a partial result of every
+    // row, so 2; beside them the sequences' own parts are short.
+    auto ranges = [&](size_t others, size_t per_cu) {
+        const size_t want = (per_cu * cus + others - 1) / others, most_ranges = (most + 63) / 64;
         return static_cast<unsigned>(want < most_ranges ? want : most_ranges);
     };
     auto blocks = [](size_t pieces, unsigned row_blocks) { return (pieces + 7) / 8 * 8 * row_blocks; };
     p.own_row_blocks = along_rows(per, p.own_wide ? 2 : 1, p.own_row_waves);
     const size_t own = c.batch * c.heads;
-    p.n_own = ranges(own * p.own_row_blocks);
+    p.n_own = ranges(own * p.own_row_blocks, group > 1 ? 1 : 6);
     p.own_blocks = blocks(own * p.n_own, p.own_row_blocks);
     if (group > 1)
     {
         p.shared_row_blocks = along_rows(rows, p.row_tiles, p.shared_row_waves);
         const size_t sh = c.batch / group * c.heads;
-        p.n_shared = ranges(sh * p.shared_row_blocks);
+        p.n_shared = ranges(sh * p.shared_row_blocks, 2);
         p.shared_blocks = blocks(sh * p.n_shared, p.shared_row_blocks);
     }
     return p;
