@@ -22,6 +22,7 @@
 // or exchange between lanes, and the row's factor exp(m_old - m_new) is the
 // lane's own.
 #include "kv_pages.hpp"
+#include "split_bf16.hpp"
 
 namespace nnhip
 {
@@ -205,12 +206,13 @@ __device__ __forceinline__ void use_values(const PagedArgs& a, Tile<KS>& x, f32x
         top = fmax_std(top, __shfl_xor(top, 32, 64));
         const float mn = fmax_std(w.m, top);
         const float f = __builtin_amdgcn_exp2f((w.m - mn) * kLog2e);
-        const float mb = mn == kLowest ? 0.0f : mn * kLog2e;
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
         {
-            s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], kLog2e, -mb));
+            // The difference first: of scores times log2(e) it would be off by their size, and past 2^30 exp2 of that
+            // overflows.
+            s[i][r] = __builtin_amdgcn_exp2f((s[i][r] - mn) * kLog2e);
             sum += s[i][r];
         }
         w.l = w.l * f + sum;
@@ -245,13 +247,94 @@ template <int KS> struct PartShared
     float ml[4][kTile][2];
 };
 
+// The waves' results for 16 rows of each row wave (rows first + rv * apart on) are joined through LDS, in the order
+// of their positions, and written: 16 threads a row, 4 neighbouring values at a time.
+template <int KS, int MODE>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, const Part& part, PartShared<KS>& sh, float m, float l,
+                                           const f32x4 (&o)[Geometry<KS>::T][Geometry<KS>::VW], unsigned first, int rws,
+                                           unsigned apart, unsigned n_rows)
+{
+    using G = Geometry<KS>;
+    constexpr int DP = G::DV;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, j = lane & 15, g = lane >> 4, dim = a.c.dim;
+    const unsigned per = a.by_per.d, n_parts = a.n_shared + a.n_own;
+    const bool direct = n_parts == 1;
+    __syncthreads();
+    if (g == 0)
+    {
+        sh.ml[wave][j][0] = m;
+        sh.ml[wave][j][1] = l;
+    }
+#pragma unroll
+    for (int x = 0; x < G::T; ++x)
+#pragma unroll
+        for (int y = 0; y < G::VW; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sh.o[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = o[x][y][r];
+    __syncthreads();
+    const int jr = t >> 4;
+    for (int rv = 0; rv < rws; ++rv)   // row waves
+    {
+        const unsigned row = first + rv * apart + jr;
+        if (row >= n_rows) break;
+        const unsigned bq = a.by_per.div(row), b = part.b0 + bq, qh = part.h * per + (row - bq * per);
+        float mm = kLowest, ll = 0.0f, f[4];
+        bool any[4];   // waves that had positions: a NaN among these stays one, whatever its factor is
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k % rws == rv) mm = fmax_std(mm, sh.ml[k][jr][0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const float lk = sh.ml[k][jr][1];
+            any[k] = k % rws == rv && lk != 0.0f;
+            f[k] = __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
+            ll += any[k] ? lk * f[k] : 0.0f;
+        }
+        const size_t at = (size_t)b * a.q_heads + qh, p = at * n_parts + part.slot;
+        const float inv = !direct ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+        for (int x = 0; x < (DP + 63) / 64; ++x)
+        {
+            const int d = 64 * x + 4 * (t & 15);
+            if (d >= dim) continue;
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (any[k]) o += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
+            o *= inv;
+            if (!direct && MODE != kSingle) *reinterpret_cast<f32x4*>(a.part_o + p * dim + d) = o;
+            else
+            {
+                float* to = direct ? a.O + (long)b * a.o_t + (long)qh * dim * a.o_f : a.part_o + p * dim;
+                const long step_f = direct ? a.o_f : 1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < dim) to[(d + e) * step_f] = o[e];
+            }
+        }
+        if ((t & 15) == 0)
+        {
+            if (!direct)
+            {
+                a.part_ml[2 * p] = mm;
+                a.part_ml[2 * p + 1] = ll;
+            }
+            else
+            {
+                if (a.m) a.m[at] = mm;
+                if (a.l) a.l[at] = ll;
+            }
+        }
+    }
+}
+
 // One range of positions. row_waves of the 4 waves lie along the rows, RT tiles each; the others take 16 positions
 // each in turn.
 template <int KS, int MODE, int RT>
 __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartShared<KS>& sh)
 {
     using G = Geometry<KS>;
-    constexpr int DP = G::DV;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, j = lane & 15, g = lane >> 4, dim = a.c.dim;
     const unsigned per = a.by_per.d, n_rows = part.nb * per;
     const int rws = part.row_waves, kws = 4 / rws, rw = wave % rws, kw = wave / rws, step = kws * kTile;
@@ -353,91 +436,291 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
         }
     }
 
-    // The waves are joined through LDS, in the order of their positions, a row tile at a time.
-    const unsigned n_parts = a.n_shared + a.n_own;
-    const bool direct = n_parts == 1;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
     {
         Row<KS>& w = rows[i];
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
-        if (i) __syncthreads();
-        if (g == 0)
-        {
-            sh.ml[wave][j][0] = w.m;
-            sh.ml[wave][j][1] = w.l;
-        }
-#pragma unroll
-        for (int x = 0; x < G::T; ++x)
-#pragma unroll
-            for (int y = 0; y < G::VW; ++y)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sh.o[wave][j][16 * G::VW * x + G::VW * (4 * g + r) + y] = w.o[x][y][r];
-        __syncthreads();
-        // 16 threads a row, 4 neighbouring values at a time.
-        const int jr = t >> 4;
-        for (int rv = 0; rv < rws; ++rv)   // row waves
-        {
-            const unsigned row = ((part.rb * rws + rv) * RT + i) * kTile + jr;
-            if (row >= n_rows) break;
-            const unsigned bq = a.by_per.div(row), b = part.b0 + bq, qh = part.h * per + (row - bq * per);
-            float mm = kLowest, ll = 0.0f, f[4];
-            bool any[4];   // waves that had positions: a NaN among these stays one, whatever its factor is
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k % rws == rv) mm = fmax_std(mm, sh.ml[k][jr][0]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-            {
-                const float lk = sh.ml[k][jr][1];
-                any[k] = k % rws == rv && lk != 0.0f;
-                f[k] = __builtin_amdgcn_exp2f((sh.ml[k][jr][0] - mm) * kLog2e);
-                ll += any[k] ? lk * f[k] : 0.0f;
-            }
-            const size_t at = (size_t)b * a.q_heads + qh, p = at * n_parts + part.slot;
-            const float inv = !direct ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll
-            for (int x = 0; x < (DP + 63) / 64; ++x)
-            {
-                const int d = 64 * x + 4 * (t & 15);
-                if (d >= dim) continue;
-                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (any[k]) o += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
-                o *= inv;
-                if (!direct && MODE != kSingle) *reinterpret_cast<f32x4*>(a.part_o + p * dim + d) = o;
-                else
-                {
-                    float* to = direct ? a.O + (long)b * a.o_t + (long)qh * dim * a.o_f : a.part_o + p * dim;
-                    const long step_f = direct ? a.o_f : 1;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < dim) to[(d + e) * step_f] = o[e];
-                }
-            }
-            if ((t & 15) == 0)
-            {
-                if (!direct)
-                {
-                    a.part_ml[2 * p] = mm;
-                    a.part_ml[2 * p + 1] = ll;
-                }
-                else
-                {
-                    if (a.m) a.m[at] = mm;
-                    if (a.l) a.l[at] = ll;
-                }
-            }
-        }
+        join_waves<KS, MODE>(a, part, sh, w.m, w.l, w.o, (part.rb * rws * RT + i) * kTile, rws, RT * kTile, n_rows);
     }
 }
 
-// RT: row tiles of the shared parts, and of the own ones where a key head has more than 16 query heads.
-template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kSingle ? 1 : 2) void k_attn_paged(PagedArgs a)
+// ── many rows: the products from bf16 parts ─────────────────────────────────
+// Where more than 32 rows read the same positions the float32 matrix cores bound the walk above. This one forms
+// both products from three bf16 parts of each operand (split_bf16.hpp), six products of 16 x 16 x 32 for each: a
+// wave takes 32 positions for 64 rows, so that splitting keys and values, some 9 instructions a pair, is shared by 4
+// row tiles. The queries' parts lie in LDS, laid out by lane. Positions and weights are ordered alike on both sides
+// of the second product: its k index 8 (l / 16) + e stands for position 16 (e / 4) + 4 (l / 16) + e % 4, which are
+// the ones that the lane's scores belong to.
+//
+// Values that the parts do not hold (inputs of 2^104 and above, sums of 2^80 and above, infinities, NaN) give scores
+// or sums that are not finite; the range is then walked again in float32.
+constexpr int kSplitRows = 4;   // row tiles of a wave
+
+template <int KS> struct SplitTile
 {
-    __shared__ PartShared<KS> sh;
+    using G = Geometry<KS>;
+    f32x4 k[2][KS];
+    float v[2][4][G::T][G::VW];
+    int row[2][4];   // of the values' positions, -1: none
+};
+template <int KS> struct SplitRow
+{
+    using G = Geometry<KS>;
+    int len;
+    float slope;
+    bool counts;
+    float m, l;   // l: of the lane's positions alone, times kSplitScale
+    f32x4 o[G::T][G::VW];
+};
+
+__device__ __forceinline__ f32x4 mfma16(const bf16x8& x, const bf16x8& y, const f32x4& c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+}
+// Which parts (0 large, 2 small) the six products take, the small products first.
+constexpr int kPartA[6] = {0, 2, 1, 0, 1, 0}, kPartB[6] = {2, 0, 1, 1, 0, 0};
+
+// Whether every result is finite; false leaves the partial results for the walk that follows.
+template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a, const Part& part, bf16x8* qparts, PartShared<KS>& sh)
+{
+    using G = Geometry<KS>;
+    constexpr int RT = kSplitRows, steps = KS / 2;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, j = lane & 15, g = lane >> 4, dim = a.c.dim;
+    const unsigned per = a.by_per.d, n_rows = part.nb * per;
+    const int most = (int)(a.c.width * a.c.page.d), begin = part.begin, end = part.end, step = 4 * 2 * kTile;
+    const SplitUnits units;
+    SplitRow<KS> rows[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        SplitRow<KS>& w = rows[i];
+        const unsigned row = (part.rb * RT + i) * kTile + j;
+        const bool live = row < n_rows;
+        const unsigned bq = live ? a.by_per.div(row) : 0, b = part.b0 + bq, qh = part.h * per + (live ? row - bq * per : 0);
+        w.len = live ? length_of(a.len[b], most) : 0;
+        w.counts = live && w.len >= part.common;
+        w.slope = a.slopes && live ? a.slopes[qh] : 0.0f;
+        w.m = kLowest;
+        w.l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < G::T; ++x)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y) w.o[x][y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i != wave) continue;   // a wave splits the queries of one row tile
+        const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;
+#pragma unroll
+        for (int x = 0; x < steps; ++x)
+        {
+            floatx8 z;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = qp[(long)(32 * x + 8 * g + e) * a.q_f];
+            bf16x8 h, m, l;
+            split3(units, z, h, m, l);
+            qparts[((i * 3 + 0) * steps + x) * 64 + lane] = h;
+            qparts[((i * 3 + 1) * steps + x) * 64 + lane] = m;
+            qparts[((i * 3 + 2) * steps + x) * 64 + lane] = l;
+        }
+    }
+    __syncthreads();
+
+    auto entry = [&](int p) { return a.c.entry_of(part.b0, p + j); };
+    auto row_at = [&](float e, int p) {
+        const int r = a.c.row_in(e, p + j);
+        return p + j < end ? r : -1;
+    };
+    SplitTile<KS> x;
+    auto load_k = [&](int (&r)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+        {
+            const float* kp = a.c.K + (size_t)max(r[u], 0) * a.c.row + (size_t)part.h * dim;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) x.k[u][i] = *reinterpret_cast<const f32x4*>(kp + 32 * (i / 2) + 8 * g + 4 * (i % 2));
+        }
+    };
+    auto load_v = [&](int (&r)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                x.row[u][e] = __shfl(r[u], 4 * g + e, 64);
+                const float* vp = a.c.V + (size_t)max(x.row[u][e], 0) * a.c.row + (size_t)part.h * dim;
+#pragma unroll
+                for (int i = 0; i < G::T; ++i)
+                {
+                    typedef float vec __attribute__((ext_vector_type(G::VW)));
+                    const int d = 16 * G::VW * i + G::VW * j;
+                    const vec z = *reinterpret_cast<const vec*>(vp + (d < dim ? d : 0));
+#pragma unroll
+                    for (int y = 0; y < G::VW; ++y) x.v[u][e][i][y] = z[y];
+                }
+            }
+    };
+    const int p1 = begin + wave * 2 * kTile;
+    float first[2] = {entry(p1), entry(p1 + kTile)}, ahead[2] = {entry(p1 + step), entry(p1 + step + kTile)};
+    int r[2] = {row_at(first[0], p1), row_at(first[1], p1 + kTile)};
+    load_k(r);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(r);
+    __builtin_amdgcn_sched_barrier(0);
+    // -inf among the scores, which a sum too large for the parts may be too, shows in the smallest; NaN and +inf make
+    // the row's l one that is not finite.
+    float low = 0.0f;
+    const float alpha = a.alpha * kSplitUnscale;
+    for (int p = p1; p < end; p += step)
+    {
+        f32x4 s[2][RT];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) s[u][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < steps; ++k)
+        {
+            bf16x8 kp[2][3], qp[RT][3];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int c = 0; c < 3; ++c) qp[i][c] = qparts[((i * 3 + c) * steps + k) * 64 + lane];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+            {
+                const f32x4 lo = x.k[u][2 * k], hi = x.k[u][2 * k + 1];
+                split3(units, floatx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, kp[u][0], kp[u][1], kp[u][2]);
+            }
+#pragma unroll
+            for (int c = 0; c < 6; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) s[u][i] = mfma16(kp[u][kPartA[c]], qp[i][kPartB[c]], s[u][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const float further[2] = {entry(p + 2 * step), entry(p + 2 * step + kTile)};
+        r[0] = row_at(ahead[0], p + step);
+        r[1] = row_at(ahead[1], p + step + kTile);
+        load_k(r);
+        __builtin_amdgcn_sched_barrier(0);
+
+        int least = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) least = min(least, x.row[u][e]);
+        if (__builtin_amdgcn_ballot_w64(least < 0))
+        {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < G::T; ++i)
+#pragma unroll
+                        for (int y = 0; y < G::VW; ++y) x.v[u][e][i][y] = x.row[u][e] < 0 ? 0.0f : x.v[u][e][i][y];
+        }
+        bf16x8 pp[RT][3];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+        {
+            SplitRow<KS>& w = rows[i];
+            float top = kLowest;
+            floatx8 z;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const int u = e / 4, q = e % 4;
+                float y = alpha * s[u][i][q];
+                if (a.slopes) y -= w.slope * (float)(w.len - 1 - (p + kTile * u + 4 * g + q));
+                low = fminf(low, y);
+                z[e] = x.row[u][q] >= 0 && w.counts ? y : -__builtin_inff();
+                top = fmax_std(top, z[e]);
+            }
+            top = fmax_std(top, __shfl_xor(top, 16, 64));
+            top = fmax_std(top, __shfl_xor(top, 32, 64));
+            const float mn = fmax_std(w.m, top);
+            const float f = __builtin_amdgcn_exp2f((w.m - mn) * kLog2e);
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] - mn, kLog2e, 24.0f));   // times kSplitScale
+                sum += z[e];
+            }
+            w.l = w.l * f + sum;
+            w.m = mn;
+            split3_scaled(units, z, pp[i][0], pp[i][1], pp[i][2]);
+            if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
+            {
+#pragma unroll
+                for (int b = 0; b < G::T; ++b)
+#pragma unroll
+                    for (int y = 0; y < G::VW; ++y) w.o[b][y] *= f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < G::T; ++b)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y)
+            {
+                bf16x8 vp[3];
+                floatx8 z;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = x.v[e / 4][e % 4][b][y];
+                split3(units, z, vp[0], vp[1], vp[2]);
+#pragma unroll
+                for (int c = 0; c < 6; ++c)
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) rows[i].o[b][y] = mfma16(vp[kPartA[c]], pp[i][kPartB[c]], rows[i].o[b][y]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(r);
+        __builtin_amdgcn_sched_barrier(0);
+        ahead[0] = further[0];
+        ahead[1] = further[1];
+    }
+
+    // The waves are joined as in walk, once all results are known to be finite.
+    bool bad = !(low >= -kMaxF);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        SplitRow<KS>& w = rows[i];
+        w.l *= 1.0f / kSplitScale;
+        float size = 0.0f;
+#pragma unroll
+        for (int b = 0; b < G::T; ++b)
+#pragma unroll
+            for (int y = 0; y < G::VW; ++y)
+            {
+                w.o[b][y] *= kSplitUnscale;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) size += fabsf(w.o[b][y][e]) * 0x1p-12f;   // NaN or infinite if one is
+            }
+        bad |= w.counts && !(size + w.l <= kMaxF);
+    }
+    if (__syncthreads_or(bad)) return false;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        SplitRow<KS>& w = rows[i];
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+        join_waves<KS, kWhole>(a, part, sh, w.m, w.l, w.o, (part.rb * RT + i) * kTile, 1, 0, n_rows);
+    }
+    return true;
+}
+
+// RT: a wave's row tiles of the shared parts (kSplitRows: in bf16 parts), and 2 of the own ones where a key head has
+// more than 16 query heads.
+template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kSingle || RT == kSplitRows ? 1 : 2) void k_attn_paged(PagedArgs a)
+{
+    constexpr size_t kQueries = RT == kSplitRows ? (size_t)kSplitRows * 3 * (KS / 2) * 64 * sizeof(bf16x8) : 0;
+    constexpr size_t kShared = sizeof(PartShared<KS>) > kQueries ? sizeof(PartShared<KS>) : kQueries;
+    __shared__ __attribute__((aligned(16))) char lds[kShared];
+    PartShared<KS>& sh = *reinterpret_cast<PartShared<KS>*>(lds);
     Part part;
     unsigned i = blockIdx.x, c;
     part.is_shared = i < a.shared_blocks;
@@ -474,7 +757,7 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     if (part.begin >= part.end && a.n_shared + a.n_own > 1)
     {
         // Nothing here: the join leaves out ranges of l = 0, whatever their O is.
-        const unsigned rows_here = kTile * part.row_waves * (part.is_shared || a.own_wide ? RT : 1);
+        const unsigned tiles = part.is_shared ? RT : a.own_wide ? 2 : 1, rows_here = kTile * part.row_waves * tiles;
         const unsigned n_rows = part.nb * a.by_per.d, row = part.rb * rows_here + threadIdx.x;
         if (threadIdx.x < rows_here && row < n_rows)
         {
@@ -486,8 +769,15 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
         }
         return;
     }
-    if (RT == 1 || part.is_shared || a.own_wide) walk<KS, MODE, RT>(a, part, sh);
-    else walk<KS, MODE, 1>(a, part, sh);
+    if constexpr (RT == kSplitRows)
+        if (part.is_shared)
+        {
+            if (walk_split<KS>(a, part, reinterpret_cast<bf16x8*>(lds), sh)) return;
+            part.row_waves = 2;   // the same rows
+        }
+    constexpr bool kAll = RT == kSplitRows;   // shared parts alone: the own ones have a launch of their own
+    if (kAll || (RT == 2 && (part.is_shared || a.own_wide))) walk<KS, MODE, 2>(a, part, sh);
+    else if constexpr (!kAll) walk<KS, MODE, 1>(a, part, sh);
 }
 
 // Joins the ranges of one row in order: blockIdx.x = sequence * q_heads + head. The ranges' factors go to LDS,
@@ -555,12 +845,16 @@ struct PagedPlan
 };
 
 // How a call is cut, from its sizes alone: the lengths are on the device.
-PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
+PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group, int mode, bool alpha_ok = true)
 {
     PagedPlan p{};
     const size_t per = q_heads / c.heads, most = c.width * c.page, cus = device_cus();
     const size_t rows = group > 1 ? group * per : per;   // that read the same positions
-    p.row_tiles = rows > kTile ? 2 : 1;
+    // More than 32 rows: bf16 parts. In float32 and so, 128 wide heads: 24 rows over 16000 positions 75 us and 87, 32
+    // rows 77 and 84, 36 rows (of 4 key heads) 52 and 47, 128 rows 77 and 61, 64 rows over 65000 positions 208 and
+    // 165; 64 wide: 32 rows 42 and 54, 36 rows 33 and 32, 128 rows 47 and 41.
+    const bool split = group > 1 && rows > 32 && mode == kWhole && c.dim % 32 == 0 && alpha_ok;
+    p.row_tiles = split ? kSplitRows : rows > kTile ? 2 : 1;
     p.own_wide = per > kTile;
     auto along_rows = [](size_t n, int tiles, int& waves) {
         const size_t need = (n + kTile * tiles - 1) / (kTile * tiles);
@@ -568,8 +862,9 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
         return static_cast<unsigned>((need + waves - 1) / waves);
     };
     // Workgroups a CU: the streams of unshared sequences run best with 6 (attend of 24 sequences of 2500 to 5000:
-    // 120 us with 2, 109 with 4, 103 with 6, 108 with 8); ranges of shared positions cost a partial result of every
-    // row, so 2; beside them the sequences' own parts are short.
+    // 120 us with 2, 109 with 4, 103 with 6, 108 with 8). Ranges of shared positions cost a partial result of every
+    // row, and a workgroup in bf16 parts has a CU to itself: 2 and 1. Beside shared positions the sequences' own are
+    // few: 1, and 2 in the launch of their own that they have beside bf16 parts.
     auto ranges = [&](size_t others, size_t per_cu) {
         const size_t want = (per_cu * cus + others - 1) / others, most_ranges = (most + 63) / 64;
         return static_cast<unsigned>(want < most_ranges ? want : most_ranges);
@@ -577,13 +872,14 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
     auto blocks = [](size_t pieces, unsigned row_blocks) { return (pieces + 7) / 8 * 8 * row_blocks; };
     p.own_row_blocks = along_rows(per, p.own_wide ? 2 : 1, p.own_row_waves);
     const size_t own = c.batch * c.heads;
-    p.n_own = ranges(own * p.own_row_blocks, group > 1 ? 1 : 6);
+    p.n_own = ranges(own * p.own_row_blocks, group == 1 ? 6 : split ? 2 : 1);
     p.own_blocks = blocks(own * p.n_own, p.own_row_blocks);
     if (group > 1)
     {
         p.shared_row_blocks = along_rows(rows, p.row_tiles, p.shared_row_waves);
+        if (split) p.shared_row_waves = 1, p.shared_row_blocks = static_cast<unsigned>((rows + kTile * kSplitRows - 1) / (kTile * kSplitRows));
         const size_t sh = c.batch / group * c.heads;
-        p.n_shared = ranges(sh * p.shared_row_blocks, 2);
+        p.n_shared = ranges(sh * p.shared_row_blocks, split ? 1 : 2);
         p.shared_blocks = blocks(sh * p.n_shared, p.shared_row_blocks);
     }
     return p;
@@ -591,15 +887,38 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group)
 
 template <int KS, int MODE> void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s)
 {
-    const dim3 grid(static_cast<unsigned>(p.shared_blocks + p.own_blocks));
-    if (p.row_tiles == 1) hipLaunchKernelGGL((k_attn_paged<KS, MODE, 1>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_paged<KS, MODE, 2>), grid, dim3(256), 0, s, a);
+    auto go = [&](auto kernel, PagedArgs args, size_t shared_blocks, size_t own_blocks) {
+        args.shared_blocks = static_cast<unsigned>(shared_blocks);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(shared_blocks + own_blocks)), dim3(256), 0, s, args);
+    };
+    if constexpr (MODE == kWhole && KS % 2 == 0)
+        if (p.row_tiles == kSplitRows)
+        {
+            // In one launch the own parts would run at the one wave a SIMD that the bf16 parts' registers leave.
+            go(k_attn_paged<KS, MODE, kSplitRows>, a, p.shared_blocks, 0);
+            if (p.own_wide) go(k_attn_paged<KS, MODE, 2>, a, 0, p.own_blocks);
+            else go(k_attn_paged<KS, MODE, 1>, a, 0, p.own_blocks);
+            return;
+        }
+    if (p.row_tiles == 1) go(k_attn_paged<KS, MODE, 1>, a, p.shared_blocks, p.own_blocks);
+    else go(k_attn_paged<KS, MODE, 2>, a, p.shared_blocks, p.own_blocks);
 }
 
 // m and l of every row and range, in whole 16 bytes.
 size_t ml_floats(const nnhip_kv_pages& c, size_t q_heads, const PagedPlan& p)
 {
     return (2 * c.batch * q_heads * p.parts() + 3) / 4 * 4;
+}
+
+int paged_mode(const nnhip_kv_pages& c)
+{
+    const bool vec = c.dim % 4 == 0 && c.row % 4 == 0 && aligned16(c.K) && aligned16(c.V);
+    return !vec ? kSingle : c.dim % 16 == 0 ? kWhole : kCut;
+}
+
+size_t paged_workspace(const nnhip_kv_pages& c, size_t q_heads, const PagedPlan& p)
+{
+    return p.parts() == 1 ? 0 : (ml_floats(c, q_heads, p) + c.batch * q_heads * p.parts() * c.dim) * sizeof(float);
 }
 
 bool paged_ok(const nnhip_kv_pages* c, size_t q_heads, size_t group)
@@ -616,8 +935,15 @@ using namespace nnhip;
 extern "C" size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t group)
 {
     if (!paged_ok(c, q_heads, group)) return 0;
-    const PagedPlan p = paged_plan(*c, q_heads, group);
-    return p.parts() == 1 ? 0 : (ml_floats(*c, q_heads, p) + c->batch * q_heads * p.parts() * c->dim) * sizeof(float);
+    // Enough for either way of the products, and without sharing.
+    size_t most = 0;
+    for (const int mode : {static_cast<int>(kWhole), static_cast<int>(kSingle)})
+        for (const size_t g : {group, (size_t)1})
+        {
+            const size_t n = paged_workspace(*c, q_heads, paged_plan(*c, q_heads, g, mode));
+            most = n > most ? n : most;
+        }
+    return most;
 }
 
 extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads,
@@ -628,15 +954,11 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     if (!paged_ok(c, q_heads, group) || !q || !len || !O || q_t < 0 || q_f < 0 || o_t < 0 || o_f < 0 ||
         c->batch * q_heads > 0x7fffffffu)
         return -1;
-    const size_t need = nnhip_attn_paged_workspace_bytes(c, q_heads, group);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
-    PagedPlan p = paged_plan(*c, q_heads, group);
     if (group == 1) shared = nullptr;   // a group of one has all positions to itself
-    if (!shared)
-    {
-        p.n_shared = 0;
-        p.shared_blocks = 0;
-    }
+    const int mode = paged_mode(*c);
+    const PagedPlan p = paged_plan(*c, q_heads, shared ? group : 1, mode, __builtin_fabsf(alpha) >= 0x1p-64f);
+    const size_t need = paged_workspace(*c, q_heads, p);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
     if (p.shared_blocks + p.own_blocks > 0x7fffffffu) return -1;
     auto* ws = static_cast<float*>(workspace);
     PagedArgs a{};
@@ -670,8 +992,6 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     a.alpha = alpha;
     if (p.parts() > 1) a.part_o = ws + ml_floats(*c, q_heads, p);
     const size_t d = c->dim;
-    const bool vec = d % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V);
-    const int mode = !vec ? kSingle : d % 16 == 0 ? kWhole : kCut;
     auto s = static_cast<hipStream_t>(stream);
     // Whole groups have a kernel each; the others take the next even number of groups.
     const int ks = static_cast<int>((d + 15) / 16);

@@ -254,6 +254,95 @@ def test_attend(groups, beams, q_heads, heads, dim, page, prefix, own, share, sl
     assert np.all(np.abs(l - wl) <= wl * (4 * s_tol + 2 * max(lens) * U))
 
 
+# Many rows to a position (more than 32): the products are formed from bf16 parts, and again in float32 where these
+# do not hold the values.
+def many_rows(rng, beams, per, dim, prefix, own, page=16):
+    lens = [prefix + int(rng.integers(1, own + 1)) for _ in range(beams)]
+    lens[0] = prefix + own
+    table, pages = batch_of(rng, 1, beams, page, [prefix], lens, True)
+    K, V = (rng.normal(size=(pages * page, 1, dim)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(beams, per, dim)).astype(np.float32)
+    return dict(pages=pages, page=page, heads=1, dim=dim), q, K, V, table, lens, [prefix // page * page]
+
+
+def check_many(c, q, K, V, table, lens, shared, alpha, slopes=None):
+    beams = q.shape[0]
+    O, m, l = run_attend(c, q, K, V, table, lens, shared, beams, slopes, alpha)
+    wO, wm, wl, tol = ph.attend(q, K, V, table, c["page"], c["pages"], 1, lens, alpha, slopes)
+    assert np.array_equal(np.isfinite(O), np.isfinite(wO))
+    ok = np.isfinite(wO)
+    assert np.all(np.abs(O[ok] - wO[ok]) <= tol[ok])
+    return O
+
+
+@pytest.mark.parametrize("beams,per,dim,prefix,own", [(9, 4, 32, 130, 20), (33, 1, 64, 400, 9), (40, 3, 96, 700, 5),
+                                                     (16, 4, 128, 1500, 40), (70, 2, 128, 333, 3), (40, 1, 80, 200, 7),
+                                                     (20, 2, 48, 300, 4), (3, 20, 128, 200, 50), (2, 17, 64, 129, 2)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_attend_many_rows(beams, per, dim, prefix, own, slopes):
+    rng = np.random.default_rng(beams * 100 + dim)
+    c, q, K, V, table, lens, shared = many_rows(rng, beams, per, dim, prefix, own)
+    poison(K, V, table, lens, c["page"], c["pages"])
+    lens[1] = shared[0] - 3            # one reads its own table, one nothing
+    if beams > 2:
+        lens[2] = 0
+    sl = (2.0 ** -np.arange(3, per + 3)).astype(np.float32) if slopes else None
+    check_many(c, q, K, V, table, lens, shared, 1 / math.sqrt(dim), sl)
+
+
+@pytest.mark.parametrize("what", ["keys 2^104", "keys 2^127", "queries 2^110", "values 2^104", "values 2^126", "scores 2^90",
+                                  "scores -2^90", "tiny", "tiny values", "alpha 2^-70", "key -inf", "key inf", "key nan",
+                                  "value inf", "value nan", "query nan", "wide values"])
+def test_attend_many_rows_range(what):
+    rng = np.random.default_rng(len(what))
+    c, q, K, V, table, lens, shared = many_rows(rng, 12, 4, 64, 300, 6)
+    alpha = 0.125
+    at = ph.row_of(table, 0, 77, c["page"], c["pages"])
+    if what.startswith("keys"):        # one dim of the keys, which the queries weigh as little
+        e = int(what.split("^")[1])
+        K[:, 0, 5] *= np.float32(2.0 ** (e - 2))
+        q[:, :, 5] *= np.float32(2.0 ** -(e - 1))
+    elif what == "queries 2^110":
+        q[:, :, 5] *= np.float32(2.0 ** 110)
+        K[:, 0, 5] *= np.float32(2.0 ** -111)
+    elif what.startswith("values 2"):
+        V *= np.float32(2.0 ** (int(what.split("^")[1]) - 3))
+    elif what == "scores 2^90":
+        q *= np.float32(2.0 ** 45)
+        K *= np.float32(2.0 ** 45)
+    elif what == "scores -2^90":       # every score far below any sum that the parts hold
+        q, K = -np.abs(q) * np.float32(2.0 ** 45), np.abs(K) * np.float32(2.0 ** 45)
+    elif what == "tiny":
+        q *= np.float32(2.0 ** -60)
+        K *= np.float32(2.0 ** -66)
+        alpha = 2.0 ** 123
+    elif what == "tiny values":
+        V *= np.float32(2.0 ** -120)
+    elif what == "alpha 2^-70":
+        q *= np.float32(2.0 ** 34)
+        K *= np.float32(2.0 ** 34)
+        alpha = 2.0 ** -70
+    elif what == "key -inf":
+        K[at, 0, 3] = -np.inf
+        q[:, :, 3] = np.abs(q[:, :, 3]) + 0.5
+    elif what == "key inf":
+        K[at, 0, 3] = np.inf
+        q[:, :, 3] = np.abs(q[:, :, 3]) + 0.5
+    elif what == "key nan":
+        K[at, 0, 3] = np.nan
+    elif what == "value inf":
+        V[at, 0, 3] = np.inf
+    elif what == "value nan":
+        V[at, 0, 3] = np.nan
+    elif what == "query nan":
+        q[4, 2, 1] = np.nan
+    elif what == "wide values":
+        V *= (2.0 ** rng.integers(-60, 60, V.shape)).astype(np.float32)
+    O = check_many(c, q, K, V, table, lens, shared, alpha)
+    if what == "query nan":
+        assert np.isnan(O[4, 2]).all() and np.isfinite(np.delete(O.reshape(48, 64), 18, 0)).all()
+
+
 def test_attend_lengths_and_pages():
     """Lengths of zero, one, below the shared prefix, NaN, negative and beyond the table; pages that do not exist in
     the prefix, in a sequence's own part and at its end; infinities in rows that another sequence reads."""
