@@ -20,10 +20,12 @@ namespace
 constexpr unsigned kSegColumn = 64;   // tokens that a thread loads at once, (vocab, beams) logits
 constexpr unsigned kSegRow = 256;     // tokens that 16 lanes load at once, (beams, vocab) logits
 constexpr unsigned kSegMost = 4096;
+constexpr unsigned kSegments = 32768; // segments of a group that the selection looks at, unless they grew to kSegMost
 constexpr unsigned kStored = 8192;    // segments of a group whose bins the selection keeps in LDS
 constexpr int kMaxTake = 256;
 constexpr int kMaxBeams = 1024;
 constexpr int kList = 512;        // candidates that are ranked one against another
+constexpr unsigned kFew = 128;    // segments of a group that are ranked at once
 constexpr int kLog2Bins = 10, kBins = 1 << kLog2Bins;
 constexpr int kPickThreads = 1024;
 
@@ -446,41 +448,62 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         const float d = distance * 32.0f;
         return d > -1.0f && d < (float)kBins ? (unsigned)(int)d : (unsigned)kBins;
     };
+    // f(segment, bin) over all.
+    auto over_bins = [&](auto&& f) {
 #pragma unroll 1
-    for (unsigned u = wave; u < units; u += kWaves)
-    {
-        const unsigned beam = u >> log2_slices;
-        const bool over = s.ended[beam];
-        const float dist = near[beam];
-        over_unit(u, [&](unsigned w, unsigned i, const float2(&x)[8]) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-            {
-                const unsigned g = i + step * r;
-                if (g >= a.n_seg) continue;
-                const unsigned bin = !over ? bin_of(dist - x[r].x) : g == eos_seg ? bin_of(dist) : (unsigned)kBins;
-                if (bin < kBins) atomicAdd(&s.hist[bin], 1u);
-                if (stored) s.bins[w * a.n_seg + g] = (unsigned short)bin;
-            }
-        });
-    }
-    __syncthreads();
-    find_bin(s, k_seg, false);
-    const unsigned last = min(s.bin + 1, (unsigned)kBins - 1);
-    if (stored && !s.wide && s.bin < kBins && s.above + s.hist[s.bin] + (last > s.bin ? s.hist[last] : 0) <= kList)
-    {
-#pragma unroll 4
-        for (unsigned i = t; i < n_all; i += kPickThreads)
+        for (unsigned u = wave; u < units; u += kWaves)
         {
-            if (s.bins[i] > last) continue;
-            const unsigned at = atomicAdd(&s.count, 1u);
-            s.key[at] = of_segment(i);
-            s.idx[at] = i;
+            const unsigned beam = u >> log2_slices;
+            const bool over = s.ended[beam];
+            const float dist = near[beam];
+            over_unit(u, [&](unsigned w, unsigned i, const float2(&x)[8]) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                {
+                    const unsigned g = i + step * r;
+                    if (g < a.n_seg)
+                        f(w * a.n_seg + g, !over ? bin_of(dist - x[r].x) : g == eos_seg ? bin_of(dist) : (unsigned)kBins);
+                }
+            });
         }
+    };
+    auto list_segment = [&](unsigned i) {
+        const unsigned at = atomicAdd(&s.count, 1u);
+        s.key[at] = of_segment(i);
+        s.idx[at] = i;
+    };
+    bool listed = n_all <= kFew;
+    if (listed)
+    {
+        for (unsigned i = t; i < n_all; i += kPickThreads) list_segment(i);
         __syncthreads();
     }
     else
-        pick(s, n_all, k_seg, of_segment, [](unsigned i) { return i; });
+    {
+        over_bins([&](unsigned i, unsigned bin) {
+            if (bin < kBins) atomicAdd(&s.hist[bin], 1u);
+            if (stored) s.bins[i] = (unsigned short)bin;
+        });
+        __syncthreads();
+        find_bin(s, k_seg, false);
+        const unsigned last = min(s.bin + 1, (unsigned)kBins - 1);
+        listed = !s.wide && s.bin < kBins && s.above + s.hist[s.bin] + (last > s.bin ? s.hist[last] : 0) <= kList;
+        if (listed)
+        {
+            if (stored)
+            {
+#pragma unroll 4
+                for (unsigned i = t; i < n_all; i += kPickThreads)
+                    if (s.bins[i] <= last) list_segment(i);
+            }
+            else
+                over_bins([&](unsigned i, unsigned bin) {
+                    if (bin <= last) list_segment(i);
+                });
+            __syncthreads();
+        }
+    }
+    if (!listed) pick(s, n_all, k_seg, of_segment, [](unsigned i) { return i; });
     rank_list(s, k_seg);
     if (t < k_seg)
     {
@@ -488,8 +511,10 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         s.seg_beam[t] = w;
         s.seg_token[t] = (g - w * a.n_seg) * a.seg;
     }
-    // The k_seg segments' best are as many candidates from this total on.
-    const u64 least = n_all >= a.take ? s.key[s.order[k_seg - 1]] : 1;
+    // The k_seg segments' best are as many candidates from this total on. Those of -inf are left out, unless the
+    // others do not suffice.
+    const u64 above = key_of(-__builtin_inf()) + 1, kth = s.key[s.order[k_seg - 1]];
+    const u64 least = n_all >= a.take && kth > above ? kth : above;
     const float reach = (float)(hi - value_of(least));
     __syncthreads();
     if (t == 0) s.count = 0;
@@ -537,7 +562,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         }
     }
     __syncthreads();
-    if (s.count > kList)
+    if (s.count > kList || s.count < a.take)
         pick(
             s, n_tok, a.take,
             [&](unsigned i) {
@@ -561,12 +586,12 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
     }
 }
 
-// Tokens of a segment: as few as the loads take at once, unless the group then has more segments than the
-// selection keeps bins of.
+// Tokens of a segment: as few as the loads take at once, unless the group's segments then take the selection, which
+// is one workgroup a group, longer than reading the best ones again.
 unsigned segment_of(bool beam_major, size_t beams, size_t vocab)
 {
     unsigned seg = beam_major ? kSegRow : kSegColumn;
-    while (seg < kSegMost && beams * ((vocab + seg - 1) / seg) > kStored) seg *= 2;
+    while (seg < kSegMost && beams * ((vocab + seg - 1) / seg) > kSegments) seg *= 2;
     return seg;
 }
 
@@ -599,6 +624,11 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
         workspace_bytes < nnhip_beam_select_workspace_bytes(groups, beams, vocab, take) ||
         reinterpret_cast<uintptr_t>(workspace) % sizeof(float2) != 0)
         return -1;
+    if (groups * beams == 1 && !beam_major && ld == 1)   // one column without gaps is a row
+    {
+        beam_major = 1;
+        ld = vocab;
+    }
     const unsigned seg = segment_of(beam_major != 0, beams, vocab);
     const unsigned n_seg = static_cast<unsigned>((vocab + seg - 1) / seg), all = static_cast<unsigned>(groups * beams);
     BeamArgs a{logits, scores, done, ld, static_cast<unsigned>(groups), static_cast<unsigned>(beams),
