@@ -97,9 +97,9 @@ __global__ __launch_bounds__(256) void k_beam_segments_column(BeamArgs a)
 __global__ __launch_bounds__(256) void k_beam_segments_row(BeamArgs a)
 {
     constexpr int kPer = kSegRow / 16;
-    const unsigned n = blockIdx.y, lane = threadIdx.x & 15, seg = blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (a.done && a.done[n] != 0.0f) return;
-    if (seg >= a.n_seg) return;   // whole groups of 16 lanes
+    const unsigned lane = threadIdx.x & 15, i = blockIdx.x * 16 + (threadIdx.x >> 4), n = a.by_n_seg.div(i);
+    if (n >= a.groups * a.beams || (a.done && a.done[n] != 0.0f)) return;   // whole groups of 16 lanes
+    const unsigned seg = i - n * a.n_seg;
     const float* p = a.logits + (size_t)n * a.ld;
     float m = -__builtin_inff(), s = 0.0f;
     const unsigned v1 = min((seg + 1) * a.seg, a.vocab);
@@ -635,17 +635,12 @@ extern "C" int nnhip_beam_select(const float* logits, size_t ld, int beam_major,
                static_cast<unsigned>(vocab), static_cast<unsigned>(take), static_cast<unsigned>(done ? eos : 0), n_seg, seg,
                static_cast<unsigned>(__builtin_ctz(seg)), FastDiv(n_seg), beam_major, static_cast<float2*>(workspace), out_score, out_beam, out_token};
     auto s = static_cast<hipStream_t>(stream);
+    const size_t segments = (size_t)all * n_seg;
+    if (segments + 16 > 0x7fffffffu) return -1;
     if (beam_major)
-    {
-        if (all > 65535) return -1;
-        hipLaunchKernelGGL(k_beam_segments_row, dim3((n_seg + 15) / 16, all), dim3(256), 0, s, a);
-    }
+        hipLaunchKernelGGL(k_beam_segments_row, dim3(static_cast<unsigned>((segments + 15) / 16)), dim3(256), 0, s, a);
     else
-    {
-        const size_t blocks = ((size_t)all * n_seg + 255) / 256;
-        if (blocks > 0x7fffffffu) return -1;
-        hipLaunchKernelGGL(k_beam_segments_column, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
-    }
+        hipLaunchKernelGGL(k_beam_segments_column, dim3(static_cast<unsigned>((segments + 255) / 256)), dim3(256), 0, s, a);
     if (int rc = launch_status()) return rc;
     hipLaunchKernelGGL(k_beam_pick, dim3(all / a.beams), dim3(kPickThreads), 0, s, a);
     return launch_status();

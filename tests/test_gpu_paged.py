@@ -519,6 +519,33 @@ def test_select(groups, beams, vocab, take, beam_major, ended, ld_more):
 
 
 @pytest.mark.parametrize("beam_major", [False, True])
+def test_select_many_groups(beam_major):
+    """More beams than a launch has rows along its second axis."""
+    g, w, v, take = 35001, 2, 37, 3
+    rng = np.random.default_rng(5)
+    logits = rng.normal(0, 3, (g, w, v)).astype(np.float32)
+    scores = rng.uniform(-30, 0, (g, w)).astype(np.float32)
+    check_select(run_select(logits, scores, None, take, 0, beam_major), ph.select(logits, scores, None, take, 0))
+
+
+def test_select_scores_in_place():
+    """out_score may be scores where as many are taken as there are beams."""
+    g, w, v = 3, 7, 900
+    rng = np.random.default_rng(6)
+    logits = rng.normal(0, 3, (g, w, v)).astype(np.float32)
+    scores = rng.uniform(-30, 0, (g, w)).astype(np.float32)
+    want = run_select(logits, scores, None, w, 0, True)
+    lib = ph.library()
+    tl, ts = dev(logits.reshape(g * w, v)), dev(scores)
+    need = lib.nnhip_beam_select_workspace_bytes(g, w, v, w)
+    ws = torch.empty(need // 4, device="cuda")
+    ob, ot = (torch.zeros(g, w).cuda() for _ in range(2))
+    assert lib.nnhip_beam_select(ptr(tl), v, 1, ptr(ts), None, g, w, v, w, 0, ptr(ts), ptr(ob), ptr(ot), ptr(ws), need,
+                                 stream()) == 0
+    assert np.array_equal(np.stack([x.cpu().numpy() for x in (ts, ob, ot)]), want)
+
+
+@pytest.mark.parametrize("beam_major", [False, True])
 def test_select_ties(beam_major):
     """Equal totals in the order of beam, then token: all logits equal; two values; equal beams; no live beam."""
     g, w, v, take = 2, 6, 3001, 24
