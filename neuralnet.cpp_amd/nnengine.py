@@ -604,6 +604,8 @@ class GptSession:
 
     def beam_search(self, prompt, beams: int, max_new: int, eos: int = 2 ** 64 - 1):
         """The `beams` best continuations of the prompt: a list of (token ids, sum of log probabilities), best first."""
+        if beams < 1 or max_new < 0:
+            raise EngineError("beam_search: 1 to 256 beams, max_new not negative")
         pr = np.ascontiguousarray(np.asarray(prompt, dtype=np.uint64))
         out = np.zeros(max(1, beams * max_new), dtype=np.uint64)
         n = (ctypes.c_size_t * max(1, beams))()
