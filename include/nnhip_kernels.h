@@ -484,7 +484,7 @@ typedef struct nnhip_kv_pages
  * (compute_layer.hpp:884-984): x_j c - x_{j+r/2} s and x_{j+r/2} c + x_j s; the others, and v, are stored as
  * they are. Without (cos and sin NULL, rope_dim 0) nothing is turned. q and q_out may both be NULL; q_out may
  * be q itself with the same strides. A token whose sequence, position, page or, with a rotation, table row does not exist is padding:
- * nothing of it is written. Two tokens of one call must not name the same row. dim <= 256. */
+ * nothing of it is written. Two tokens of one call must not name the same row, and K must not be V. dim <= 256. */
 int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f, const float* v, long v_t, long v_f,
                     const float* q, long q_t, long q_f, float* q_out, long o_t, long o_f, size_t q_heads,
                     size_t tokens, const float* seq, const float* pos, const float* cos, const float* sin,
@@ -501,8 +501,8 @@ int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f,
  * sequences have in common: the tables of the group name the same rows there, and these are read once for all
  * of them (through the table of the group's first sequence). A sequence shorter than that is read through its
  * own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
- * The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte aligned; calls that may overlap in time
- * need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
+ * O, m and l overlap no input. The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte
+ * aligned; calls that may overlap in time need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
  * bits every time. */
 size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t group);
 int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, const float* len,
@@ -514,12 +514,13 @@ int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f
  * logits; ld floats from a row to the next. Candidate (beam, token) of a group has the total
  *   scores[beam] + (logit - log(sum over the vocabulary of exp(logit)))
  * and a beam with done[beam] != 0 (done may be NULL) has ended: it offers `eos` with the total scores[beam]
- * and every other token with -inf, and its logits are not read. A total that is NaN counts as -inf. The `take`
+ * and every other token with -inf, whatever its logits are. A total that is NaN counts as -inf. The `take`
  * best of each group's beams * vocab candidates go to out_score, out_beam, out_token (groups, take), best
  * first; equal totals in the order of beam, then token. out_beam counts over all groups, so that it indexes
  * the batch's tensors (nnhip_gather, nnhip_kv_reorder). Totals are formed and compared in 64 bits.
  * take <= 256, take <= beams * vocab, beams <= 1024, vocab and groups * beams at most 2^24, beams * vocab below
- * 2^31. Workspace: nnhip_beam_select_workspace_bytes; calls that may overlap in time need one each. */
+ * 2^31 - 2^20. out_score may be scores itself where take == beams; else the outputs overlap no input. Workspace:
+ * nnhip_beam_select_workspace_bytes; calls that may overlap in time need one each. */
 size_t nnhip_beam_select_workspace_bytes(size_t groups, size_t beams, size_t vocab, size_t take);
 int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const float* scores, const float* done,
                       size_t groups, size_t beams, size_t vocab, size_t take, size_t eos, float* out_score,
@@ -534,7 +535,7 @@ int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const floa
  *   table_out[b][i + 1 ..) = -1;  len_out[b] = n.
  * With fresh NULL entry i is the parent's page when n % page != 0, else -1, and nothing is copied. A parent
  * that is no sequence number gives a row of -1 and length 0; a fresh[b] that is no page number is stored as -1
- * and nothing is copied. table_out (out_batch, width) must not overlap table. The pages of fresh must differ
+ * and nothing is copied. table_out (out_batch, width) and len_out overlap no input (-1). The pages of fresh must differ
  * from each other and from every page that another sequence of the new batch continues or shares. */
 int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float* parent, const float* len,
                      const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);

@@ -2209,6 +2209,7 @@ Result<Tensor> HipEngine::kv_append(KvPages& c, const Tensor& k, const Tensor& v
     NN_CHECK(need_gpu_({&c.K, &c.V, &c.table, &k, &v, q, &pos, seq, cos, sin}, "kv_append"));
     NN_CHECK(settle_write_(c.K));
     NN_CHECK(settle_write_(c.V));
+    if (W(c.K) == W(c.V)) return fail("kv_append: K and V are one tensor");
     const std::size_t n = k.cols();
     const long t = 1, f = static_cast<long>(n);
     Tensor out;

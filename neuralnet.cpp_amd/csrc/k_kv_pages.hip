@@ -228,7 +228,7 @@ extern "C" int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t
 {
     if (!pages_ok(c, kAppendDim)) return -1;
     if (tokens == 0) return 0;
-    if (!k || !v || !pos || (q == nullptr) != (q_out == nullptr) || tokens > kMaxIndex || k_t < 0 || k_f < 0 ||
+    if (c->K == c->V || !k || !v || !pos || (q == nullptr) != (q_out == nullptr) || tokens > kMaxIndex || k_t < 0 || k_f < 0 ||
         v_t < 0 || v_f < 0 || q_t < 0 || q_f < 0 || o_t < 0 || o_f < 0 || (q && (q_heads == 0 || q_heads > kMaxIndex)) ||
         (cos == nullptr) != (sin == nullptr) || rope_dim % 2 != 0 || rope_dim > c->dim ||
         (cos ? rope_rows == 0 || rope_rows > kMaxIndex || rope_dim == 0 : rope_dim != 0))
@@ -287,7 +287,9 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
     const nnhip_kv_pages& c = layers[0];
     if (out_batch == 0) return 0;
     if (!parent || !len || !table_out || !len_out || out_batch > kMaxIndex ||
-        overlap(c.table, c.batch * c.width, table_out, out_batch * c.width))
+        overlap(c.table, c.batch * c.width, table_out, out_batch * c.width) || overlap(len, c.batch, len_out, out_batch) ||
+        overlap(parent, out_batch, table_out, out_batch * c.width) || overlap(parent, out_batch, len_out, out_batch) ||
+        (fresh && (overlap(fresh, out_batch, table_out, out_batch * c.width) || overlap(fresh, out_batch, len_out, out_batch))))
         return -1;
     ReorderArgs a{};
     a.c = pages_of(c);

@@ -208,6 +208,7 @@ public:
     {
         if (!on_cpu_({&c.K, &c.V, &c.table, &k, &v, q, &pos, seq, cos, sin})) return fail("kv_append: tensors are not CPU");
         NN_TRY(s, paged::check_append(c, k, v, q, pos, seq, cos, sin));
+        if (&c.K.cpu_matrix() == &c.V.cpu_matrix()) return fail("kv_append: K and V are one tensor");
         const std::size_t N = k.cols(), d = s.dim, h = s.half;
         Tensor out;
         if (q) out = Tensor::from_matrix(Matrix(q->cpu_matrix()));

@@ -88,7 +88,8 @@ def test_session_refusals(cpu):
     cfg = dict(SMALL, pos_enc="learned")
     g = cpu.gpt(**cfg)
     for args, msg in [(([], 2, 3), "empty prompt"), (([23], 2, 3), "out of range"), (([1] * 15, 2, 3), "longer than"),
-                      (([1], 0, 3), "beams"), (([1], 257, 3), "beams"), (([1], 24, 3), "more beams")]:
+                      (([1], 0, 3), "beams"), (([1], 257, 3), "beams"), (([1], 24, 3), "more beams"),
+                      (([1], 2, -1), "max_new"), (([1], -1, 3), "beams")]:
         with pytest.raises(nnengine.EngineError, match=msg):
             g.beam_search(*args)
     assert g.beam_search([1, 2], 3, 0) == [([], 0.0)] * 3
@@ -169,6 +170,7 @@ def refusals(e):
         e.zero(t)
     return [
         (lambda: e.kv_append(K, V, table, x, x, col, 3, 2), "cache shapes"),
+        (lambda: e.kv_append(K, K, table, x, x, col, 2, 2), "one tensor"),
         (lambda: e.kv_append(K, V, table, x, x, col, 2, 4), "cache shapes"),
         (lambda: e.kv_append(K, V, table, x, x, col, 0, 2), "cache shapes"),
         (lambda: e.kv_append(K, V, table, x, T(6, 2), col, 2, 2), "k, v"),

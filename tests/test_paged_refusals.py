@@ -8,7 +8,7 @@ P = 4096   # a pointer's stand-in, aligned
 
 
 def pages(**kw):
-    d = dict(K=P, V=P, table=P, batch=4, width=8, pages=16, page=16, heads=4, dim=64, row=256)
+    d = dict(K=P, V=1 << 24, table=P, batch=4, width=8, pages=16, page=16, heads=4, dim=64, row=256)
     d.update(kw)
     return Pages(**d)
 
@@ -37,6 +37,10 @@ def test_append_pages(bad):
                                  dict(tokens=(1 << 24) + 1), dict(q_heads=70000), dict(rows=(1 << 24) + 1)])
 def test_append_arguments(bad):
     assert append(pages(), **bad) == -1
+
+
+def test_append_keys_over_values():
+    assert append(pages(V=P)) == -1
 
 
 def test_append_of_nothing():
@@ -91,7 +95,7 @@ def test_select_of_nothing():
 
 
 def reorder(layers, n=None, **kw):
-    a = dict(parent=P, len=P, fresh=P, out_batch=4, out=1 << 20, out_len=P)
+    a = dict(parent=2 * P, len=3 * P, fresh=4 * P, out_batch=4, out=1 << 20, out_len=1 << 21)
     a.update(kw)
     arr = (Pages * len(layers))(*layers)
     return library().nnhip_kv_reorder(arr, len(layers) if n is None else n, a["parent"], a["len"], a["fresh"],
@@ -105,7 +109,9 @@ def test_reorder_pages(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(parent=None), dict(len=None), dict(out=None), dict(out_len=None),
-                                 dict(out_batch=(1 << 24) + 1), dict(out=P), dict(out=P + 4 * 31), dict(out=P - 4 * 31)])
+                                 dict(out_batch=(1 << 24) + 1), dict(out=P), dict(out=P + 4 * 31), dict(out=P - 4 * 31),
+                                 dict(out_len=3 * P), dict(out_len=3 * P + 12), dict(out_len=2 * P - 12), dict(out_len=4 * P),
+                                 dict(out=2 * P), dict(out=4 * P - 4 * 31)])
 def test_reorder_arguments(bad):
     assert reorder([pages()], **bad) == -1
 
