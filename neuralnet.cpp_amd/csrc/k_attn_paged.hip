@@ -873,9 +873,12 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group, int 
     // Workgroups a CU: the streams of unshared sequences run best with 6 (attend of 24 sequences of 2500 to 5000:
     // 120 us with 2, 109 with 4, 103 with 6, 108 with 8). Ranges of shared positions cost a partial result of every
     // row, and a workgroup in bf16 parts has a CU to itself: 2 and 1. Beside shared positions the sequences' own are
-    // few: 1, and 2 in the launch of their own that they have beside bf16 parts.
-    auto ranges = [&](size_t others, size_t per_cu) {
-        const size_t want = (per_cu * cus + others - 1) / others, most_ranges = (most + 63) / 64;
+    // few: 1, and 2 in the launch of their own that they have beside bf16 parts. A range has at least 64 positions,
+    // one step of a workgroup's waves, and shared ones 128 once they fill the CUs (12 heads of 4 groups over 1000
+    // positions: 13.4 us with 64, 11.5 with 128; of one group over 300: 7.1 and 8.0).
+    auto ranges = [&](size_t others, size_t per_cu, bool long_ones = false) {
+        const size_t least = long_ones && others * ((most + 63) / 64) > cus ? 128 : 64;
+        const size_t want = (per_cu * cus + others - 1) / others, most_ranges = (most + least - 1) / least;
         return static_cast<unsigned>(want < most_ranges ? want : most_ranges);
     };
     auto blocks = [](size_t pieces, unsigned row_blocks) { return (pieces + 7) / 8 * 8 * row_blocks; };
@@ -888,7 +891,7 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group, int 
         p.shared_row_blocks = along_rows(rows, p.row_tiles, p.shared_row_waves);
         if (split) p.shared_row_waves = 1, p.shared_row_blocks = static_cast<unsigned>((rows + kTile * kSplitRows - 1) / (kTile * kSplitRows));
         const size_t sh = c.batch / group * c.heads;
-        p.n_shared = ranges(sh * p.shared_row_blocks, split ? 1 : 2);
+        p.n_shared = ranges(sh * p.shared_row_blocks, split ? 1 : 2, !split);
         p.shared_blocks = blocks(sh * p.n_shared, p.shared_row_blocks);
     }
     return p;
