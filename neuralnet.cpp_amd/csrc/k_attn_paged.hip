@@ -54,6 +54,7 @@ struct PagedArgs
     unsigned q_heads, group, n_shared, n_own, shared_blocks;
     // per: query heads of a key head; of the shared and the own parts: 8 row blocks, ranges
     FastDiv by_per, by_heads, by_shared_rows, by_own_rows, by_n_shared, by_n_own;
+    int q_rows;   // queries lie a token a row, 16-byte aligned
     int shared_row_waves, own_row_waves, own_wide;   // own_wide: own parts in RT row tiles a wave too
     float alpha;
 };
@@ -363,15 +364,27 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 #pragma unroll
             for (int y = 0; y < G::VW; ++y) w.o[x][y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (begin >= end) continue;
-        const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;
+        const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;   // rows that are not live are formed and dropped
+        if (MODE != kSingle && a.q_rows)
+        {
 #pragma unroll
-        for (int x = 0; x < KS; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int x = 0; x < KS; ++x)
             {
-                const int d = 16 * x + 4 * g + e;
-                w.q[x][e] = qp[(long)(d < dim ? d : 0) * a.q_f];   // rows that are not live are formed and dropped
+                const int d = 16 * x + 4 * g;
+                w.q[x] = *reinterpret_cast<const f32x4*>(qp + (d < dim ? d : 0));
             }
+        }
+        else
+        {
+#pragma unroll
+            for (int x = 0; x < KS; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    const int d = 16 * x + 4 * g + e;
+                    w.q[x][e] = qp[(long)(d < dim ? d : 0) * a.q_f];
+                }
+        }
     }
     if (begin < end)
     {
@@ -1001,6 +1014,7 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     a.shared_row_waves = p.shared_row_waves;
     a.own_row_waves = p.own_row_waves;
     a.own_wide = p.own_wide;
+    a.q_rows = q_f == 1 && q_t % 4 == 0 && aligned16(q);
     a.alpha = alpha;
     if (p.parts() > 1) a.part_o = ws + ml_floats(*c, q_heads, p);
     const size_t d = c->dim;

@@ -254,6 +254,22 @@ def test_attend(groups, beams, q_heads, heads, dim, page, prefix, own, share, sl
     assert np.all(np.abs(l - wl) <= wl * (4 * s_tol + 2 * max(lens) * U))
 
 
+@pytest.mark.parametrize("kind", ["token", "gaps", "feature", "strided"])
+@pytest.mark.parametrize("heads,per,beams,dim", [(2, 2, 3, 64), (1, 3, 2, 20), (2, 20, 2, 128), (1, 1, 1, 80), (2, 1, 40, 32)])
+def test_attend_query_layouts(heads, per, beams, dim, kind):
+    """Queries of any alignment beside aligned caches."""
+    rng = np.random.default_rng(dim + beams)
+    prefix, page = 70, 16
+    lens = [prefix + int(n) for n in rng.integers(0, 20, beams)]
+    table, pages = batch_of(rng, 1, beams, page, [prefix], lens, True)
+    K, V = (rng.normal(size=(pages * page, heads, dim)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(beams, heads * per, dim)).astype(np.float32)
+    c = dict(pages=pages, page=page, heads=heads, dim=dim)
+    O, _, _ = run_attend(c, q, K, V, table, lens, [prefix // page * page], beams, None, 0.2, kind)
+    wO, _, _, tol = ph.attend(q, K, V, table, page, pages, heads, lens, np.float32(0.2))
+    assert np.all(np.abs(O - wO) <= tol + 1e-30)
+
+
 # Many rows to a position (more than 32): the products are formed from bf16 parts, and again in float32 where these
 # do not hold the values.
 def many_rows(rng, beams, per, dim, prefix, own, page=16):
