@@ -532,14 +532,28 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
             for (int y = 0; y < G::VW; ++y) w.o[x][y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (i != wave) continue;   // a wave splits the queries of one row tile
         const float* qp = a.q + (long)b * a.q_t + (long)qh * dim * a.q_f;
+        floatx8 z[steps];
+        if (a.q_rows)
+        {
+#pragma unroll
+            for (int x = 0; x < steps; ++x)
+            {
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(qp + 32 * x + 8 * g), hi = *reinterpret_cast<const f32x4*>(qp + 32 * x + 8 * g + 4);
+                z[x] = floatx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int x = 0; x < steps; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[x][e] = qp[(long)(32 * x + 8 * g + e) * a.q_f];
+        }
 #pragma unroll
         for (int x = 0; x < steps; ++x)
         {
-            floatx8 z;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = qp[(long)(32 * x + 8 * g + e) * a.q_f];
             bf16x8 h, m, l;
-            split3(units, z, h, m, l);
+            split3(units, z[x], h, m, l);
             qparts[((i * 3 + 0) * steps + x) * 64 + lane] = h;
             qparts[((i * 3 + 1) * steps + x) * 64 + lane] = m;
             qparts[((i * 3 + 2) * steps + x) * 64 + lane] = l;
