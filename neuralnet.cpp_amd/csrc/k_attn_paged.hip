@@ -24,7 +24,7 @@
 //
 // Unshared sequences are bound by HBM: 24 of 2500 to 5000 positions, 8 heads of
 // 80, take 102 us, 4.9 TB/s. Few positions are bound by the latency of two
-// launches (4 beams of 321 positions: 7.5 us and 4). Shared ones that more than
+// launches (4 beams of 321 positions: 7.1 us and 4). Shared ones that more than
 // 32 rows read are bound by the products and the vector instructions around
 // them, which is why these rows have a walk in bf16 parts.
 #include "kv_pages.hpp"
@@ -473,11 +473,19 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 // of the second product: its k index 8 (l / 16) + e stands for position 16 (e / 4) + 4 (l / 16) + e % 4, which are
 // the ones that the lane's scores belong to.
 //
-// Values that the parts do not hold (inputs of 2^104 and above, sums of 2^80 and above, infinities, NaN) give scores
-// or sums that are not finite; the range is then walked again in float32.
+// A row's weights are taken against a fixed score, the largest of the wave's first tile that has any (with a slope, what
+// that would be at the range's end): sums in floats are as exact against any score that keeps them in range, and
+// nothing is scaled on the way, which took 15 us of 140 for the moves of the outputs between the matrix cores'
+// registers and the others. At the end they are scaled to the largest score.
 //
-// 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 146 us, 3.6 TB/s; 92 with the loads alone, 131 without
-// them. 512 rows over 6000: 110 us.
+// Values that the parts do not hold (queries and values of 2^104 and above, sums of 2^80 and above, infinities, NaN)
+// and scores that grow by more than some 70 over a range give scores or sums that are not finite, and scores that
+// fall short of the slope's by 40 small sums; the range is then walked again in float32. Keys are split as they are,
+// not times 2^24: of those below 2^-109 parts below 2^-126 are lost, less than 2^-22 of a score whatever the query.
+//
+// 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 120 us, 4.4 TB/s (92 with the loads alone); 512 rows over
+// 6000 take 93 us. Two waves a SIMD of 32 rows each took 160 (every wave splits all its keys and
+// values) and 170 (two waves split a tile in halves, exchanged through LDS).
 constexpr int kSplitRows = 4;   // row tiles of a wave
 
 template <int KS> struct SplitTile
@@ -493,7 +501,7 @@ template <int KS> struct SplitRow
     int len;
     float slope;
     bool counts;
-    float m, l;   // l: of the lane's positions alone, times kSplitScale
+    float m, top, l;   // the score that the weights are against, the largest; l: of the lane's positions, times kSplitScale
     f32x4 o[G::T][G::VW];
 };
 
@@ -524,7 +532,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
         w.len = live ? length_of(a.len[b], most) : 0;
         w.counts = live && w.len >= part.common;
         w.slope = a.slopes && live ? a.slopes[qh] : 0.0f;
-        w.m = kLowest;
+        w.m = w.top = kLowest;
         w.l = 0.0f;
 #pragma unroll
         for (int x = 0; x < G::T; ++x)
@@ -605,7 +613,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
     // -inf among the scores, which a sum too large for the parts may be too, shows in the smallest; NaN and +inf make
     // the row's l one that is not finite.
     float low = 0.0f;
-    const float alpha = a.alpha * kSplitUnscale;
+    const float alpha = a.alpha * (1.0f / kSplitScale);
     for (int p = p1; p < end; p += step)
     {
         f32x4 s[2][RT];
@@ -625,7 +633,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
             for (int u = 0; u < 2; ++u)
             {
                 const f32x4 lo = x.k[u][2 * k], hi = x.k[u][2 * k + 1];
-                split3(units, floatx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, kp[u][0], kp[u][1], kp[u][2]);
+                split3_scaled(units, floatx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, kp[u][0], kp[u][1], kp[u][2]);
             }
 #pragma unroll
             for (int c = 0; c < 6; ++c)
@@ -657,6 +665,20 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
 #pragma unroll
                         for (int y = 0; y < G::VW; ++y) x.v[u][e][i][y] = x.row[u][e] < 0 ? 0.0f : x.v[u][e][i][y];
         }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[u][i] *= alpha;
+        if (a.slopes)
+        {
+            asm volatile("");   // stays a branch
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s[u][i][q] -= rows[i].slope * (float)(rows[i].len - 1 - (p + kTile * u + 4 * g + q));
+        }
         bf16x8 pp[RT][3];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -668,33 +690,23 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
             for (int e = 0; e < 8; ++e)
             {
                 const int u = e / 4, q = e % 4;
-                float y = alpha * s[u][i][q];
-                if (a.slopes) y -= w.slope * (float)(w.len - 1 - (p + kTile * u + 4 * g + q));
+                const float y = s[u][i][q];
                 low = fminf(low, y);
                 z[e] = x.row[u][q] >= 0 && w.counts ? y : -__builtin_inff();
-                top = fmax_std(top, z[e]);
+                top = fmaxf(top, z[e]);
             }
-            top = fmax_std(top, __shfl_xor(top, 16, 64));
-            top = fmax_std(top, __shfl_xor(top, 32, 64));
-            const float mn = fmax_std(w.m, top);
-            const float f = __builtin_amdgcn_exp2f((w.m - mn) * kLog2e);
-            float sum = 0.0f;
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            w.top = fmaxf(w.top, top);
+            if (w.m == kLowest && top > kLowest)   // the first tile with a position
+                w.m = top + (a.slopes ? fmax_std(w.slope, 0.0f) * (float)(end - 1 - p) : 0.0f);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] - mn, kLog2e, 24.0f));   // times kSplitScale
-                sum += z[e];
+                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] - w.m, kLog2e, 24.0f));   // times kSplitScale
+                w.l += z[e];
             }
-            w.l = w.l * f + sum;
-            w.m = mn;
             split3_scaled(units, z, pp[i][0], pp[i][1], pp[i][2]);
-            if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
-            {
-#pragma unroll
-                for (int b = 0; b < G::T; ++b)
-#pragma unroll
-                    for (int y = 0; y < G::VW; ++y) w.o[b][y] *= f;
-            }
         }
 #pragma unroll
         for (int b = 0; b < G::T; ++b)
@@ -724,14 +736,19 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
     for (int i = 0; i < RT; ++i)
     {
         SplitRow<KS>& w = rows[i];
-        w.l *= 1.0f / kSplitScale;
+        const float f = __builtin_amdgcn_exp2f((w.m - w.top) * kLog2e);
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+        bad |= w.counts && w.m != kLowest && !(w.l >= kSplitScale * 0x1p-60f);
+        w.m = w.top;
+        w.l *= f * (1.0f / kSplitScale);
         float size = 0.0f;
 #pragma unroll
         for (int b = 0; b < G::T; ++b)
 #pragma unroll
             for (int y = 0; y < G::VW; ++y)
             {
-                w.o[b][y] *= kSplitUnscale;
+                w.o[b][y] *= f * kSplitUnscale;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) size += fabsf(w.o[b][y][e]) * 0x1p-12f;   // NaN or infinite if one is
             }
@@ -742,8 +759,6 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
     for (int i = 0; i < RT; ++i)
     {
         SplitRow<KS>& w = rows[i];
-        w.l += __shfl_xor(w.l, 16, 64);
-        w.l += __shfl_xor(w.l, 32, 64);
         join_waves<KS, kWhole>(a, part, sh, w.m, w.l, w.o, (part.rb * RT + i) * kTile, 1, 0, n_rows);
     }
     return true;

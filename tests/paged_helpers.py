@@ -74,7 +74,7 @@ def attend(q, K, V, table, page, pages, heads, lens, alpha, slopes=None):
                 size = abs(alpha) * (np.abs(k) @ np.abs(x))
                 if slopes is not None:
                     s = s - slopes[h] * (n - 1 - pos)
-                    size = size + 2 * slopes[h] * (n - 1 - pos)
+                    size = size + 2 * abs(slopes[h]) * (n - 1 - pos)
                 if s.max() == -np.inf:
                     continue
                 m[b, h] = s.max()

@@ -359,6 +359,34 @@ def test_attend_many_rows_range(what):
         assert np.isnan(O[4, 2]).all() and np.isfinite(np.delete(O.reshape(48, 64), 18, 0)).all()
 
 
+@pytest.mark.parametrize("slopes,falls,size", [(0, False, 0), (0, False, 60), (0, False, 600), (0, True, 60), (0, True, 600),
+                                               (0.25, False, 0), (3.0, False, 0), (3.0, True, 60), (3.0, True, 20000),
+                                               (-2.0, False, 0), (0.01, False, 300)])
+def test_attend_many_rows_far_scores(slopes, falls, size):
+    """Several tiles a wave, over which the scores grow or fall along the positions, by themselves or by the slope."""
+    rng = np.random.default_rng(int(size) + 7)
+    heads, per, beams, dim, n, page = 16, 4, 10, 32, 8000, 16
+    lens = [n + int(x) for x in rng.integers(1, 9, beams)]
+    table, pages = batch_of(rng, 1, beams, page, [n], lens, True)
+    K, V = (rng.normal(size=(pages * page, heads, dim)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(beams, heads * per, dim)).astype(np.float32) * np.float32(0.25)
+    ramp = np.linspace(size, 0, n) if falls else np.linspace(0, size, n)
+    for j in range(n):
+        K[ph.row_of(table, 0, j, page, pages), :, 0] = np.float32(ramp[j])
+    q[:, :, 0] = 1.0
+    sl = (slopes * np.linspace(0.5, 1, heads * per)).astype(np.float32) if slopes else None
+    c = dict(pages=pages, page=page, heads=heads, dim=dim)
+    O, m, l = run_attend(c, q, K, V, table, lens, [n], beams, sl, 1.0)
+    wO, wm, wl, tol = ph.attend(q, K, V, table, page, pages, heads, lens, 1.0, sl)
+    assert np.all(np.abs(O - wO) <= tol)
+    # as in test_attend; the slope's product with up to 8000 is rounded too
+    s_tol = (dim + 8) * U * np.abs(q).sum(axis=2) * np.abs(K).max() + 8 * U * np.abs(wm)
+    if slopes:
+        s_tol = s_tol + 2 * U * np.abs(sl)[None, :] * n
+    assert np.all(np.abs(m - wm) <= s_tol)
+    assert np.all(np.abs(l - wl) <= wl * (4 * s_tol + 2 * max(lens) * U))
+
+
 def test_attend_lengths_and_pages():
     """Lengths of zero, one, below the shared prefix, NaN, negative and beyond the table; pages that do not exist in
     the prefix, in a sequence's own part and at its end; infinities in rows that another sequence reads."""
