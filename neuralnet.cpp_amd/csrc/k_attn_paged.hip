@@ -649,22 +649,6 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
         load_k(r);
         __builtin_amdgcn_sched_barrier(0);
 
-        int least = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) least = min(least, x.row[u][e]);
-        if (__builtin_amdgcn_ballot_w64(least < 0))
-        {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int i = 0; i < G::T; ++i)
-#pragma unroll
-                        for (int y = 0; y < G::VW; ++y) x.v[u][e][i][y] = x.row[u][e] < 0 ? 0.0f : x.v[u][e][i][y];
-        }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -679,6 +663,34 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
 #pragma unroll
                     for (int q = 0; q < 4; ++q) s[u][i][q] -= rows[i].slope * (float)(rows[i].len - 1 - (p + kTile * u + 4 * g + q));
         }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) low = fminf(low, s[u][i][q]);
+        int least = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) least = min(least, x.row[u][e]);
+        if (__builtin_amdgcn_ballot_w64(least < 0))
+        {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s[u][i][q] = x.row[u][q] < 0 ? -__builtin_inff() : s[u][i][q];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < G::T; ++i)
+#pragma unroll
+                        for (int y = 0; y < G::VW; ++y) x.v[u][e][i][y] = x.row[u][e] < 0 ? 0.0f : x.v[u][e][i][y];
+        }
         bf16x8 pp[RT][3];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -689,10 +701,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                const int u = e / 4, q = e % 4;
-                const float y = s[u][i][q];
-                low = fminf(low, y);
-                z[e] = x.row[u][q] >= 0 && w.counts ? y : -__builtin_inff();
+                z[e] = s[e / 4][i][e % 4];
                 top = fmaxf(top, z[e]);
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -753,6 +762,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
                 for (int e = 0; e < 4; ++e) size += fabsf(w.o[b][y][e]) * 0x1p-12f;   // NaN or infinite if one is
             }
         bad |= w.counts && !(size + w.l <= kMaxF);
+        if (!w.counts) w.m = kLowest, w.l = 0.0f;   // whatever came of these rows
     }
     if (__syncthreads_or(bad)) return false;
 #pragma unroll
@@ -901,9 +911,8 @@ PagedPlan paged_plan(const nnhip_kv_pages& c, size_t q_heads, size_t group, int 
     PagedPlan p{};
     const size_t per = q_heads / c.heads, most = c.width * c.page, cus = device_cus();
     const size_t rows = group > 1 ? group * per : per;   // that read the same positions
-    // More than 32 rows: bf16 parts. In float32 and so, 128 wide heads: 24 rows over 16000 positions 75 us and 87, 32
-    // rows 77 and 84, 36 rows (of 4 key heads) 52 and 47, 128 rows 77 and 61, 64 rows over 65000 positions 208 and
-    // 165; 64 wide: 32 rows 42 and 54, 36 rows 33 and 32, 128 rows 47 and 41.
+    // More than 32 rows: bf16 parts. In float32 and so, over 16000 positions of 4 key heads: 128 wide 32 rows 37 us and
+    // 40, 36 rows 44 and 41, 128 rows 67 and 53; 64 wide 32 rows 21 and 28, 36 rows 26 and 28, 128 rows 43 and 38.
     const bool split = group > 1 && rows > 32 && mode == kWhole && c.dim % 32 == 0 && alpha_ok;
     p.row_tiles = split ? kSplitRows : rows > kTile ? 2 : 1;
     p.own_wide = per > kTile;
