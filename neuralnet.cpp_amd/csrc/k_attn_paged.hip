@@ -475,17 +475,18 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 //
 // A row's weights are taken against a fixed score, the largest of the wave's first tile that has any (with a slope, what
 // that would be at the range's end): sums in floats are as exact against any score that keeps them in range, and
-// nothing is scaled on the way, which took 15 us of 140 for the moves of the outputs between the matrix cores'
-// registers and the others. At the end they are scaled to the largest score.
+// nothing is scaled on the way, which took 15 us of 140 for moves of the outputs between the matrix cores' registers
+// and the others. At the end they are scaled to the largest score.
 //
 // Values that the parts do not hold (queries and values of 2^104 and above, sums of 2^80 and above, infinities, NaN)
 // and scores that grow by more than some 70 over a range give scores or sums that are not finite, and scores that
 // fall short of the slope's by 40 small sums; the range is then walked again in float32. Keys are split as they are,
-// not times 2^24: of those below 2^-109 parts below 2^-126 are lost, less than 2^-22 of a score whatever the query.
+// not times 2^24: of those below 2^-109 parts below 2^-126 are lost, dim alpha 2^-22 of a score at most with
+// the largest queries that the parts hold.
 //
 // 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 120 us, 4.4 TB/s (92 with the loads alone); 512 rows over
-// 6000 take 93 us. Two waves a SIMD of 32 rows each took 160 (every wave splits all its keys and
-// values) and 170 (two waves split a tile in halves, exchanged through LDS).
+// 6000 take 91 us. Two waves a SIMD of 32 rows each took 160 where one of 64 took 144 (every wave splits all its keys
+// and values), and 170 where two waves split a tile in halves, exchanged through LDS.
 constexpr int kSplitRows = 4;   // row tiles of a wave
 
 template <int KS> struct SplitTile
@@ -750,14 +751,14 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
         w.l += __shfl_xor(w.l, 32, 64);
         bad |= w.counts && w.m != kLowest && !(w.l >= kSplitScale * 0x1p-60f);
         w.m = w.top;
-        w.l *= f * (1.0f / kSplitScale);
+        w.l = w.l * (1.0f / kSplitScale) * f;   // one after the other: f times the scale may be below every float
         float size = 0.0f;
 #pragma unroll
         for (int b = 0; b < G::T; ++b)
 #pragma unroll
             for (int y = 0; y < G::VW; ++y)
             {
-                w.o[b][y] *= f * kSplitUnscale;
+                w.o[b][y] = w.o[b][y] * kSplitUnscale * f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) size += fabsf(w.o[b][y][e]) * 0x1p-12f;   // NaN or infinite if one is
             }

@@ -359,7 +359,8 @@ def test_attend_many_rows_range(what):
         assert np.isnan(O[4, 2]).all() and np.isfinite(np.delete(O.reshape(48, 64), 18, 0)).all()
 
 
-@pytest.mark.parametrize("slopes,falls,size", [(0, False, 0), (0, False, 60), (0, False, 600), (0, True, 60), (0, True, 600),
+@pytest.mark.parametrize("slopes,falls,size", [(0, False, 0), (0, False, 60), (0, False, 600), (0, False, 900), (0, False, 1000),
+                                               (0, False, 1100), (0, False, 1300), (0, True, 60), (0, True, 600),
                                                (0.25, False, 0), (3.0, False, 0), (3.0, True, 60), (3.0, True, 20000),
                                                (-2.0, False, 0), (0.01, False, 300)])
 def test_attend_many_rows_far_scores(slopes, falls, size):
