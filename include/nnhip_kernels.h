@@ -535,8 +535,9 @@ int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const floa
  *   table_out[b][i + 1 ..) = -1;  len_out[b] = n.
  * With fresh NULL entry i is the parent's page when n % page != 0, else -1, and nothing is copied. A parent
  * that is no sequence number gives a row of -1 and length 0; a fresh[b] that is no page number is stored as -1
- * and nothing is copied. table_out (out_batch, width) and len_out overlap no input (-1). The pages of fresh must differ
- * from each other and from every page that another sequence of the new batch continues or shares. */
+ * and nothing is copied. table_out (out_batch, width) and len_out overlap neither an input, the caches among
+ * them, nor each other (-1). The pages of fresh must differ from each other and from every page that another
+ * sequence of the new batch continues or shares. */
 int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float* parent, const float* len,
                      const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);
 

@@ -291,11 +291,16 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
     }
     const nnhip_kv_pages& c = layers[0];
     if (out_batch == 0) return 0;
-    if (!parent || !len || !table_out || !len_out || out_batch > kMaxIndex ||
-        overlap(c.table, c.batch * c.width, table_out, out_batch * c.width) || overlap(len, c.batch, len_out, out_batch) ||
-        overlap(parent, out_batch, table_out, out_batch * c.width) || overlap(parent, out_batch, len_out, out_batch) ||
-        (fresh && (overlap(fresh, out_batch, table_out, out_batch * c.width) || overlap(fresh, out_batch, len_out, out_batch))))
+    if (!parent || !len || !table_out || !len_out || out_batch > kMaxIndex) return -1;
+    // The workgroups of the tables read what the others' outputs would have overwritten, in any order.
+    auto over_outputs = [&](const float* x, size_t n) {
+        return x && (overlap(x, n, table_out, out_batch * c.width) || overlap(x, n, len_out, out_batch));
+    };
+    if (over_outputs(c.table, c.batch * c.width) || over_outputs(len, c.batch) || over_outputs(parent, out_batch) ||
+        over_outputs(fresh, out_batch) || overlap(table_out, out_batch * c.width, len_out, out_batch))
         return -1;
+    for (size_t i = 0; i < n_layers; ++i)
+        if (over_outputs(layers[i].K, c.pages * c.page * c.row) || over_outputs(layers[i].V, c.pages * c.page * c.row)) return -1;
     ReorderArgs a{};
     a.c = pages_of(c);
     a.parent = parent;

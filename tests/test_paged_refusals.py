@@ -122,3 +122,12 @@ def test_reorder_layers():
     for other in (dict(table=2 * P), dict(batch=5), dict(width=9), dict(pages=17), dict(page=8), dict(heads=2),
                   dict(dim=32), dict(row=512)):
         assert reorder([pages(), pages(**other)]) == -1
+
+
+@pytest.mark.parametrize("bad", [dict(out=3 * P), dict(out=3 * P - 4 * 31), dict(out=3 * P + 12), dict(out_len=P), dict(out_len=P - 12),
+                                 dict(out_len=P + 4 * 31), dict(out_len=1 << 20), dict(out_len=(1 << 20) + 4 * 31),
+                                 dict(out_len=(1 << 20) - 12), dict(out=P + (1 << 18) - 4), dict(out=(1 << 24) + (1 << 17)),
+                                 dict(out_len=P + (1 << 18) - 4), dict(out_len=(1 << 24) - 12)])
+def test_reorder_outputs_over_the_rest(bad):
+    """The table's output on the lengths, the lengths' on the table, one output on the other, either on the caches."""
+    assert reorder([pages()], **bad) == -1
