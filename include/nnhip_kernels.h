@@ -466,8 +466,8 @@ int nnhip_attn_query(const float* Q, const float* Kp, long kb, long kj, long kk,
  * of a row at h * dim. table (batch, width) holds page numbers: position p of sequence b is row
  * table[b * width + p / page] * page + p % page. A position whose table entry is no page number (negative,
  * NaN, >= pages) or that lies past width * page is absent: it is neither read nor written. Sequences may share
- * pages. width * page and pages are at most 2^24 (index tensors hold integers as floats), pages * page below
- * 2^31. */
+ * pages. width * page and pages are at most 2^24 (index tensors hold integers as floats), pages * page and
+ * heads * dim below 2^31, row at most 2^32. */
 typedef struct nnhip_kv_pages
 {
     float* K;

@@ -60,13 +60,13 @@ __device__ __forceinline__ int length_of(float f, int most)
     return f >= (float)most ? most : (int)f;
 }
 
-// The sizes that every entry point asks for.
+// The sizes that every entry point asks for: the kernels count pages, rows and a row's values in 32 bits.
 inline bool pages_ok(const nnhip_kv_pages* c, size_t max_dim)
 {
     return c && c->K && c->V && c->table && c->batch > 0 && c->width > 0 && c->pages > 0 && c->page > 0 &&
            c->heads > 0 && c->dim > 0 && c->dim <= max_dim && c->batch <= kMaxIndex && c->pages <= kMaxIndex &&
            c->page <= kMaxIndex && c->pages * c->page < (size_t)0x80000000u && c->width <= kMaxIndex && c->width * c->page <= kMaxIndex &&
-           c->heads <= kMaxIndex && c->row >= c->heads * c->dim && c->row <= ((size_t)1 << 32);
+           c->heads <= kMaxIndex && c->heads * c->dim < (size_t)0x80000000u && c->row >= c->heads * c->dim && c->row <= ((size_t)1 << 32);
 }
 
 inline Pages pages_of(const nnhip_kv_pages& c)

@@ -131,3 +131,9 @@ def test_reorder_layers():
 def test_reorder_outputs_over_the_rest(bad):
     """The table's output on the lengths, the lengths' on the table, one output on the other, either on the caches."""
     assert reorder([pages()], **bad) == -1
+
+
+@pytest.mark.parametrize("heads,dim", [(1 << 8, 1 << 24), (255, 1 << 24), (1 << 9, 1 << 23), (1 << 7, 1 << 24)])
+def test_reorder_rows_past_31_bits(heads, dim):
+    """Rows of 2^31 values and more: the kernel counts a row's values in 32 bits, up to 256 past the last."""
+    assert reorder([pages(K=1 << 48, V=1 << 56, heads=heads, dim=dim, row=heads * dim, pages=1, page=1)]) == -1
