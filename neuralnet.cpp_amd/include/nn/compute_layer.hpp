@@ -1350,6 +1350,22 @@ public:
         std::vector<Scalar> scores;
     };
 
+    // What beam_search asks of its sizes, before it runs any layer: the tokens that it will add (the last one is not
+    // fed; 0: no layer runs).
+    [[nodiscard]] Result<std::size_t> beam_steps(std::size_t n_prompt, std::size_t beams, std::size_t max_new) const
+    {
+        if (n_prompt == 0) return fail("GPTModel beam_search: empty prompt");
+        if (n_prompt > seq_len_) return fail("GPTModel beam_search: the prompt is longer than the context");
+        if (beams == 0 || beams > 256) return fail("GPTModel beam_search: 1 to 256 beams");
+        if (beams > vocab_) return fail("GPTModel beam_search: more beams than tokens to begin with");
+        if (!blocks_.empty() && d_model_ / blocks_[0]->attention().heads() > 128)
+            return fail("GPTModel beam_search: heads wider than 128");
+        const std::size_t steps = std::min(max_new, seq_len_ - n_prompt + 1);
+        if (steps > 0 && beam_rows_(n_prompt, beams, steps) >= (std::size_t{1} << 24))
+            return fail("GPTModel beam_search: too many cache rows");
+        return steps;
+    }
+
     // Beam search (no reference counterpart): the `beams` continuations of the prompt with the largest sum of log
     // probabilities among those that extend, token by token, the `beams` best so far. A continuation ends at eos (an
     // id past the vocabulary: none does), after max_new tokens or where the context is full, and keeps its total.
@@ -1363,15 +1379,10 @@ public:
     {
         constexpr std::size_t kPromptChunk = 64;
         const std::size_t P = prompt.size();
-        if (P == 0) return fail("GPTModel beam_search: empty prompt");
-        if (P > seq_len_) return fail("GPTModel beam_search: the prompt is longer than the context");
-        if (beams == 0 || beams > 256) return fail("GPTModel beam_search: 1 to 256 beams");
-        if (beams > vocab_) return fail("GPTModel beam_search: more beams than tokens to begin with");
-        const std::size_t steps = std::min(max_new, seq_len_ - P + 1);   // the last token is not fed
+        NN_TRY(steps, beam_steps(P, beams, max_new));
         Beams out{std::vector<std::vector<std::size_t>>(beams), std::vector<Scalar>(beams, Scalar{0})};
         if (steps == 0) return out;
-        const std::size_t rows = P + beams * (steps - 1);
-        if (rows >= (std::size_t{1} << 24)) return fail("GPTModel beam_search: too many cache rows");
+        const std::size_t rows = beam_rows_(P, beams, steps);
 
         std::vector<KvPages> caches(blocks_.size());
         for (KvPages& c : caches)
@@ -1497,6 +1508,11 @@ public:
     }
 
 private:
+    // Rows of a layer's cache: the prompt's, and one a beam for every token that is fed.
+    static std::size_t beam_rows_(std::size_t n_prompt, std::size_t beams, std::size_t steps)
+    {
+        return n_prompt + beams * (steps - 1);
+    }
     // Tokens ids (batch) of a step through the blocks: hidden states (d_model, batch).
     Result<Tensor> paged_hidden_(ComputeEngine& engine, const Tensor& ids, std::vector<KvPages>& caches,
                                  const PagedStep& step)

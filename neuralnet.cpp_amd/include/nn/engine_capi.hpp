@@ -668,7 +668,9 @@ try
         if (prompt[i] >= m->vocab_size()) return set_error("gpt_beam_search: prompt token out of range");
         pr[i] = static_cast<std::size_t>(prompt[i]);
     }
-    g->searched = true;
+    auto steps = m->beam_steps(n_prompt, beams, max_new);
+    if (!steps) return set_error(steps.error().message);
+    if (*steps > 0) g->searched = true;   // layers will run
     if (auto r = g->eng->begin_batch(); !r) return set_error(r.error().message);
     auto b = m->beam_search(*g->eng, pr, beams, max_new, static_cast<std::size_t>(eos));
     if (!b) return set_error(b.error().message);

@@ -204,3 +204,35 @@ def test_refusals(cpu):
     for call, msg in refusals(cpu):
         with pytest.raises(nnengine.EngineError, match=msg):
             call()
+
+
+def test_refused_search_leaves_the_forward_pass(cpu):
+    """A search that is refused, or asked for no token, has run no layer: the backward pass still has its inputs."""
+    cfg = dict(SMALL, pos_enc="learned")
+    g = cpu.gpt(**cfg)
+    g.set_params(params_of(cfg, 7))
+    toks = np.random.default_rng(0).integers(0, 23, (15, 2))
+    g.load_batch(toks[:14].astype(np.float32), toks[1:].T.reshape(-1))
+    g.forward_loss()
+    g.backward()
+    grads = g.grads()
+    for args in ([1] * 15, 2, 3), ([1], 257, 3), ([1], 24, 3), ([23], 2, 3), ([], 2, 3):
+        g.zero_grad()
+        g.forward_loss()
+        with pytest.raises(nnengine.EngineError):
+            g.beam_search(*args)
+        g.backward()
+        assert all(np.array_equal(a, b) for a, b in zip(grads, g.grads()))
+    g.zero_grad()
+    g.forward_loss()
+    f, one, n, s = cpu._f["gpt_beam_search"], (ctypes.c_uint64 * 1)(1), (ctypes.c_size_t * 3)(), (ctypes.c_float * 3)()
+    assert f(g._g, one, 1, 0, 3, 0, one, n, s) != 0
+    assert g.beam_search([1, 2], 3, 0) == [([], 0.0)] * 3
+    g.backward()
+    assert all(np.array_equal(a, b) for a, b in zip(grads, g.grads()))
+    wide = cpu.gpt(vocab_size=23, d_model=136, seq_len=14, num_heads=1, d_ff=8, num_layers=1, pos_enc="learned")
+    wide.load_batch(toks[:14].astype(np.float32), toks[1:].T.reshape(-1))
+    wide.forward_loss()
+    with pytest.raises(nnengine.EngineError, match="128"):
+        wide.beam_search([1], 2, 2)
+    wide.backward()
