@@ -447,7 +447,8 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
     };
 
     // The best segments. Bins of 1/32 over the 32 below the best total hold them, as a rule; the bin behind the
-    // one where their count is reached is taken too, for the half bin that a distance may be off.
+    // one where their count is reached is taken too, for the half bin that a distance may be off. Behind the last
+    // bin there is none: a count that is reached there is left to pick.
     auto bin_of = [&](float distance) {
         const float d = distance * 32.0f;
         return d > -1.0f && d < (float)kBins ? (unsigned)(int)d : (unsigned)kBins;
@@ -490,8 +491,8 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
         });
         __syncthreads();
         find_bin(s, k_seg, false);
-        const unsigned last = min(s.bin + 1, (unsigned)kBins - 1);
-        listed = !s.wide && s.bin < kBins && s.above + s.hist[s.bin] + (last > s.bin ? s.hist[last] : 0) <= kList;
+        const unsigned last = s.bin + 1;
+        listed = !s.wide && last < kBins && s.above + s.hist[s.bin] + s.hist[last] <= kList;
         if (listed)
         {
             if (stored)
