@@ -842,6 +842,10 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     else if constexpr (!kAll) walk<KS, MODE, 1>(a, part, sh);
 }
 
+// In place of the factor of a range of l = 0, whose O is anything. A factor that underflows to 0 is one: a value of its
+// range that is not finite makes O one that is not, as within a range.
+constexpr float kNoRange = -1.0f;
+
 // Joins the ranges of one row in order: blockIdx.x = sequence * q_heads + head. The ranges' factors go to LDS,
 // then 2 or 4 groups of threads sum every 2nd or 4th range.
 __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
@@ -865,12 +869,15 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
     m = fmax_std(fmax_std(red[0][0], red[0][1]), fmax_std(red[0][2], red[0][3]));
     for (unsigned c = 0; c < n; c += kChunk)
     {
-        float w = 0.0f;
+        float w = kNoRange;
         if (c + t < n)
         {
             const float li = ml[2 * (c + t) + 1];
-            if (li != 0.0f) w = __builtin_amdgcn_exp2f((ml[2 * (c + t)] - m) * kLog2e);
-            l += li * w;
+            if (li != 0.0f)
+            {
+                w = __builtin_amdgcn_exp2f((ml[2 * (c + t)] - m) * kLog2e);
+                l += li * w;
+            }
         }
         __syncthreads();
         w_s[t] = w;
@@ -880,7 +887,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a)
         for (int i = g; i < nc; i += groups)
         {
             const float x = po[(size_t)(c + i) * dim], f = w_s[i];
-            o += f == 0.0f ? 0.0f : x * f;   // where l is 0, O is anything
+            o += f == kNoRange ? 0.0f : x * f;
         }
     }
     l = wave_sum(l);
@@ -916,7 +923,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join_few(PagedArgs a)
 #pragma unroll
         for (int y = 0; y < 2; ++y) x[i][y] = po[(size_t)min(i, n - 1) * dim + min(lane + 64 * y, dim - 1)];
     const bool any = lane < (int)n && own.y != 0.0f;
-    const float m = wave_max(any ? own.x : kLowest), w = any ? __builtin_amdgcn_exp2f((own.x - m) * kLog2e) : 0.0f;
+    const float m = wave_max(any ? own.x : kLowest), w = any ? __builtin_amdgcn_exp2f((own.x - m) * kLog2e) : kNoRange;
     const float l = wave_sum(any ? own.y * w : 0.0f);
     float o[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -924,7 +931,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join_few(PagedArgs a)
     {
         const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
 #pragma unroll
-        for (int y = 0; y < 2; ++y) o[y] += f == 0.0f ? 0.0f : x[i][y] * f;   // where l is 0, O is anything
+        for (int y = 0; y < 2; ++y) o[y] += f == kNoRange ? 0.0f : x[i][y] * f;
     }
 #pragma unroll
     for (int y = 0; y < 2; ++y)
