@@ -1,6 +1,20 @@
 """nnhip_beam_select where its first pass puts segments of neighbouring tokens aside (csrc/k_beam.hip): distances at the
 edge of the range that is sorted at once, more segments than are kept in LDS, segments that grow, against the 64-bit form
-(paged_helpers.select)."""The last one taken lies just under 32 below the best total. Its beam has logits of 50000, where float32 distances
+(paged_helpers.select)."""
+import numpy as np
+import pytest
+
+import paged_helpers as ph
+from test_gpu_paged import check_select, run_select
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("beam_major,seg", [(False, 64), (True, 256)])
+@pytest.mark.parametrize("group", [0, 2])
+def test_select_at_the_last_distance(beam_major, seg, group):
+    """The last one taken lies just under 32 below the best total. Its beam has logits of 50000, where float32 distances
     are off by up to 1/512, and measures 32; another beam's candidate, a little worse, measures less than 32."""
     n_seg, take = 80, 3
     x = np.full((3, 2, n_seg * seg), -200.0, np.float32)
