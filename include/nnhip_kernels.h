@@ -498,9 +498,9 @@ int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f,
  * with m = lowest(), l = 0, O = 0 when there is no position or every s_j is -inf. q and O as the features of
  * nnhip_kv_append's q; m, l (batch, q_heads) may be NULL. The batch is batch / group groups of `group`
  * neighbouring sequences; shared (batch / group), when set, says how many first positions the group's
- * sequences have in common: the tables of the group name the same rows there, and these are read once for all
- * of them (through the table of the group's first sequence). A sequence shorter than that is read through its
- * own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
+ * sequences have in common: the tables of those that are as long name the same rows there, and these are read
+ * once for all of them (through the table of the first of them). A sequence shorter than that is read through
+ * its own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
  * O, m and l overlap no input. The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte
  * aligned; calls that may overlap in time need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
  * bits every time. */

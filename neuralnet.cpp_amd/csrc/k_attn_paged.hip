@@ -65,6 +65,20 @@ __device__ __forceinline__ int shared_of(const PagedArgs& a, unsigned b)
     return a.shared ? length_of(a.shared[b / a.group], (int)(a.c.width * a.c.page.d)) : 0;
 }
 
+// The first sequence of the group from b0 on that is as long as the positions it shares: a shorter one's table need not
+// name them. b0 + group where there is none.
+__device__ __forceinline__ unsigned reader_of(const PagedArgs& a, unsigned b0, int common)
+{
+    const unsigned lane = threadIdx.x & 63;
+    for (unsigned i = 0; i < a.group; i += 64)
+    {
+        const int len = length_of(a.len[b0 + min(i + lane, a.group - 1)], (int)(a.c.width * a.c.page.d));
+        const unsigned long long long_enough = __builtin_amdgcn_ballot_w64(i + lane < a.group && len >= common);
+        if (long_enough) return b0 + i + __builtin_ctzll(long_enough);
+    }
+    return b0 + a.group;
+}
+
 // KS: groups of 16 key dims. Value columns of a lane: VW neighbouring ones of every 16 VW; columns past dim are
 // formed and dropped.
 template <int KS> struct Geometry
@@ -245,6 +259,7 @@ __device__ __forceinline__ void use_values(const PagedArgs& a, Tile<KS>& x, f32x
 struct Part
 {
     unsigned b0, nb, h, rb, slot;   // sequences b0 .. b0 + nb - 1, key head, block of rows, range of all
+    unsigned by;                    // the sequence whose table is read
     int begin, end, common, row_waves;
     bool is_shared;
 };
@@ -398,7 +413,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
         }
         // Table entries are loaded two tiles ahead of their use, keys and values one: the entries' loads are then
         // older than the keys' and values' that are still on their way when the addresses are formed.
-        auto entry = [&](int p) { return a.c.entry_of(part.b0, p + j); };
+        auto entry = [&](int p) { return a.c.entry_of(part.by, p + j); };
         auto row_at = [&](float e, int p) {
             const int r = a.c.row_in(e, p + j);
             return p + j < end ? r : -1;
@@ -570,7 +585,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
     }
     __syncthreads();
 
-    auto entry = [&](int p) { return a.c.entry_of(part.b0, p + j); };
+    auto entry = [&](int p) { return a.c.entry_of(part.by, p + j); };
     auto row_at = [&](float e, int p) {
         const int r = a.c.row_in(e, p + j);
         return p + j < end ? r : -1;
@@ -805,8 +820,14 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     part.slot = part.is_shared ? c : a.n_shared + c;
     part.row_waves = part.is_shared ? a.shared_row_waves : a.own_row_waves;
     part.common = shared_of(a, part.b0);
+    part.by = part.b0;
     int lo = 0, hi = part.common;
-    if (!part.is_shared)
+    if (part.is_shared)
+    {
+        part.by = reader_of(a, part.b0, part.common);
+        if (part.by - part.b0 == a.group) hi = 0;   // for no one
+    }
+    else
     {
         hi = length_of(a.len[part.b0], (int)(a.c.width * a.c.page.d));
         lo = hi >= part.common ? part.common : 0;

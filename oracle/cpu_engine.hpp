@@ -253,12 +253,15 @@ public:
         {
             const std::size_t n = length_(P(len)[b], most);
             const std::size_t common = shared ? length_(P(*shared)[b / group], most) : 0;
+            std::size_t by = b;   // whose table names the shared positions: the group's first sequence as long as these
+            if (n >= common)
+                for (by = b / group * group; length_(P(len)[by], most) < common;) ++by;
             rows.clear();
             at.clear();
             for (std::size_t j = 0; j < n; ++j)
             {
                 std::size_t r;
-                if (!page_row_(c, n >= common && j < common ? b / group * group : b, j, r)) continue;
+                if (!page_row_(c, j < common ? by : b, j, r)) continue;
                 rows.push_back(r);
                 at.push_back(j);
             }

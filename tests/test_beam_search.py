@@ -236,3 +236,30 @@ def test_refused_search_leaves_the_forward_pass(cpu):
     with pytest.raises(nnengine.EngineError, match="128"):
         wide.beam_search([1], 2, 2)
     wide.backward()
+
+
+def orphan_first(e, beams):
+    """The first sequences of a group continue no one (a table row of -1, length 0); the others share a prefix."""
+    rng = np.random.default_rng(11)
+    heads, d, page, width, pages, n = 2, 32, 4, 12, 120, 37
+    x = dict(K=rng.normal(size=(pages * page, heads * d)), V=rng.normal(size=(pages * page, heads * d)),
+             q=rng.normal(size=(heads * d, beams)), table=np.full((1, width), -1.0), lens=np.array([[n]]))
+    x["table"][0, :n // page + 1] = rng.permutation(30)[:n // page + 1]
+    parent = np.zeros((beams, 1))
+    parent[:max(1, beams - 5)] = -1
+    x = {k: np.asarray(a, np.float32) for k, a in x.items()}
+    t = {k: e.tensor(a) for k, a in x.items()}
+    fresh = e.tensor(40.0 + np.arange(beams)[:, None])
+    table, lens = e.kv_reorder([(t["K"], t["V"])], t["table"], e.tensor(parent), t["lens"], fresh, page, heads)
+    got = e.attn_paged(t["K"], t["V"], table, t["q"], lens, 0.2, page, heads, shared=e.tensor(np.array([[n // page * page]])),
+                       group=beams).numpy()
+    K, V = (t[k].numpy().reshape(-1, heads, d) for k in "KV")
+    want, _, _, tol = ph.attend(x["q"].T.reshape(beams, heads, d), K, V, table.numpy(), page, pages, heads, lens.numpy()[:, 0],
+                                np.float32(0.2))
+    assert np.all(lens.numpy()[parent[:, 0] < 0] == 0) and np.all(np.abs(want[parent[:, 0] == 0]).sum(axis=(1, 2)) > 0)
+    assert np.all(np.abs(got.T.reshape(beams, heads, d) - want) <= tol)
+
+
+@pytest.mark.parametrize("beams", [2, 6, 70])
+def test_group_whose_first_sequence_has_no_parent(cpu, beams):
+    orphan_first(cpu, beams)

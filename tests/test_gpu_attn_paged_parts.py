@@ -33,3 +33,24 @@ def test_value_not_finite_under_a_small_weight(beams, n, shared, dim, value):
     assert not np.isfinite(wO[:, 0, 5]).any() and not np.isfinite(O[:, 0, 5]).any()
     rest = np.arange(dim) != 5
     assert np.all(np.abs(O[:, 0, rest] - wO[:, 0, rest]) <= tol[:, 0, rest])
+
+
+@pytest.mark.parametrize("beams,first,dim,per", [(4, 1, 64, 1), (4, 3, 30, 2), (40, 7, 64, 1), (140, 130, 32, 1), (9, 2, 128, 4)])
+@pytest.mark.parametrize("short", [0, 5, 95])
+def test_group_whose_first_sequences_are_short(beams, first, dim, per, short):
+    """The shared positions are read through the first sequence that has them all, whatever the tables of the shorter ones
+    in front of it name there; where no sequence has them all each is read through its own table."""
+    rng = np.random.default_rng(beams + dim)
+    page, width, n = 16, 8, 96
+    table = np.tile(rng.permutation(60)[:width].astype(np.float32), (beams, 1))
+    table[:first] = -1.0
+    table[:first, :short // page + 1] = 60 + np.arange(short // page + 1)     # rows of their own
+    table[1::2, 6:] = [[70, 71]]
+    K, V = (rng.normal(size=(80 * page, 1, dim)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(beams, per, dim)).astype(np.float32)
+    lens = np.array([short] * first + [n + int(x) for x in rng.integers(0, 20, beams - first)], np.float32)
+    c = dict(pages=80, page=page, heads=1, dim=dim)
+    for ls in (lens, np.minimum(lens, 95)):
+        O, m, l = run_attend(c, q, K, V, table, ls, [float(n)], beams, None, 0.125)
+        wO, wm, wl, tol = ph.attend(q, K, V, table, page, 80, 1, ls, 0.125)
+        assert np.all(np.abs(O - wO) <= tol)

@@ -75,3 +75,8 @@ def test_one_beam_is_greedy(hip):
     assert one[0][0] == g.generate(prompt, 12)
     best = g.beam_search(prompt, 8, 12)
     assert best[0][1] >= one[0][1] - 1e-3 and [s for _, s in best] == sorted((s for _, s in best), reverse=True)
+
+
+@pytest.mark.parametrize("beams", [2, 6, 40, 70])
+def test_group_whose_first_sequence_has_no_parent(hip, beams):
+    cpu_tests.orphan_first(hip, beams)
