@@ -493,11 +493,14 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 // nothing is scaled on the way, which took 15 us of 140 for moves of the outputs between the matrix cores' registers
 // and the others. At the end they are scaled to the largest score.
 //
-// Values that the parts do not hold (queries and values of 2^104 and above, sums of 2^80 and above, infinities, NaN)
-// and scores that grow by more than some 70 over a range give scores or sums that are not finite, and scores that
-// fall short of the slope's by 40 small sums; the range is then walked again in float32. Keys are split as they are,
-// not times 2^24: of those below 2^-109 parts below 2^-126 are lost, dim alpha 2^-22 of a score at most with
-// the largest queries that the parts hold.
+// Weights are split as they are and values times 2^48: 24 added to the exponents' arguments, for the parts' scale, would
+// cost these 4 bits, and parts of a weight that counts beside a sum of 2^-60 are normal without it.
+//
+// Values that the parts do not hold (queries of 2^104, values and sums of 2^80 and above, infinities, NaN) and scores that
+// grow by more than some 55 to 69 over a range give sums that are not finite, or above 2^100 (up to there the factor that
+// scales them back is a normal float), and scores that fall short of the slope's by 40 small sums; the range is then
+// walked again in float32. Keys are split as they are too: of those below 2^-109 parts below 2^-126 are lost, dim alpha
+// 2^-22 of a score at most with the largest queries that the parts hold.
 //
 // 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 120 us, 4.4 TB/s (92 with the loads alone); 512 rows over
 // 6000 take 91 us. Two waves a SIMD of 32 rows each took 160 where one of 64 took 144 (every wave splits all its keys
@@ -517,7 +520,7 @@ template <int KS> struct SplitRow
     int len;
     float slope;
     bool counts;
-    float m, top, l;   // the score that the weights are against, the largest; l: of the lane's positions, times kSplitScale
+    float m, top, l;   // the score that the weights are against, the largest; l: of the lane's positions
     f32x4 o[G::T][G::VW];
 };
 
@@ -728,7 +731,7 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] - w.m, kLog2e, 24.0f));   // times kSplitScale
+                z[e] = __builtin_amdgcn_exp2f((z[e] - w.m) * kLog2e);
                 w.l += z[e];
             }
             split3_scaled(units, z, pp[i][0], pp[i][1], pp[i][2]);
@@ -741,8 +744,8 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
                 bf16x8 vp[3];
                 floatx8 z;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = x.v[e / 4][e % 4][b][y];
-                split3(units, z, vp[0], vp[1], vp[2]);
+                for (int e = 0; e < 8; ++e) z[e] = x.v[e / 4][e % 4][b][y] * (1.0f / kSplitUnscale);
+                split3_scaled(units, z, vp[0], vp[1], vp[2]);
 #pragma unroll
                 for (int c = 0; c < 6; ++c)
 #pragma unroll
@@ -764,16 +767,16 @@ template <int KS> __device__ __forceinline__ bool walk_split(const PagedArgs& a,
         const float f = __builtin_amdgcn_exp2f((w.m - w.top) * kLog2e);
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
-        bad |= w.counts && w.m != kLowest && !(w.l >= kSplitScale * 0x1p-60f);
+        bad |= w.counts && w.m != kLowest && !(w.l >= 0x1p-60f && w.l <= 0x1p100f);
         w.m = w.top;
-        w.l = w.l * (1.0f / kSplitScale) * f;   // one after the other: f times the scale may be below every float
+        w.l *= f;
         float size = 0.0f;
 #pragma unroll
         for (int b = 0; b < G::T; ++b)
 #pragma unroll
             for (int y = 0; y < G::VW; ++y)
             {
-                w.o[b][y] = w.o[b][y] * kSplitUnscale * f;
+                w.o[b][y] = w.o[b][y] * kSplitUnscale * f;   // one after the other: f times that may be below every float
 #pragma unroll
                 for (int e = 0; e < 4; ++e) size += fabsf(w.o[b][y][e]) * 0x1p-12f;   // NaN or infinite if one is
             }

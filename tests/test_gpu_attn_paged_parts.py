@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import paged_helpers as ph
+import test_gpu_paged as tp
 from test_gpu_paged import run_attend
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +55,71 @@ def test_group_whose_first_sequences_are_short(beams, first, dim, per, short):
         O, m, l = run_attend(c, q, K, V, table, ls, [float(n)], beams, None, 0.125)
         wO, wm, wl, tol = ph.attend(q, K, V, table, page, 80, 1, ls, 0.125)
         assert np.all(np.abs(O - wO) <= tol)
+
+
+def two_positions(rows, dim):
+    """A group of `rows` sequences that share 64 positions, all absent but two of one tile: queries, caches, table, lengths."""
+    q = np.zeros((rows, 1, dim), np.float32)
+    K, V = np.zeros((64, 1, dim), np.float32), np.zeros((64, 1, dim), np.float32)
+    table = np.full((rows, 64), -1.0, np.float32)
+    table[:, 3], table[:, 9] = 3, 9
+    return q, K, V, table, [64] * rows, dict(pages=64, page=1, heads=1, dim=dim)
+
+
+@pytest.mark.parametrize("rows,dim", [(12, 64), (32, 64), (40, 64), (64, 128), (130, 32)])
+def test_weight_to_its_last_bits(rows, dim):
+    """Scores 0 and -x, values 0 and 1: O = z / (1 + z), z = exp(-x), 0.69 < x < 1.39. Score, products and sums are exact (one
+    factor has one bit); the exponent's argument, below 2, is off by its rounding, 2^-24, and log2(e)'s, 2^-25.1, times
+    ln 2, exp2 by a unit in its last place, 2^-23 of z, together 3.1 2^-24 of z and, times 1 / (1 + z) <= 0.8, 2.5 2^-24 of O;
+    1 + z and the quotient round once each, 2^-24: 4.5 2^-24 of O. The x are those at which an argument near 24 would round
+    by nearly 2^-20, 16 times as far."""
+    rng = np.random.default_rng(rows)
+    q, K, V, table, lens, c = two_positions(rows, dim)
+    x = rng.uniform(0.7, 1.38, 20000).astype(np.float32)
+    half = np.abs((24 - x.astype(np.float64) / np.log(2)) * 2.0 ** 19 % 1 - 0.5)
+    x = x[np.argsort(half)[:rows]]
+    q[:, 0, 1], K[9, 0, 1], V[9, 0] = -x, 1, 2.0 ** rng.integers(-3, 4, dim)
+    O, m, l = run_attend(c, q, K, V, table, lens, [64.0], rows, None, 1.0)
+    z = np.exp(-x.astype(np.float64))
+    assert np.all(m == 0) and np.all(np.abs(l[:, 0] - (1 + z)) <= (3.1 * z + 1.5) * U)
+    want = (z / (1 + z))[:, None] * V[9, 0].astype(np.float64)
+    assert np.all(np.abs(O[:, 0] - want) <= 4.5 * U * np.abs(want))
+
+
+@pytest.mark.parametrize("rows,dim", [(12, 64), (40, 64), (64, 128), (130, 32)])
+def test_every_part_of_the_products(rows, dim):
+    """As above with factors of 24 bits. A product of three bf16 parts each leaves out (2^-24 + 2^-34) of itself, and its
+    six terms' sum, smallest first, is rounded or cut, 2^-23 for the last addition and 5 2^-31 before: 3.1 2^-24. A score of
+    up to 1.39 is off by 4.4 2^-24, with the argument's and exp2's 3.1 2^-24 z by 7.5 2^-24, O by 0.8 times that, by 3.1 2^-24
+    for its own product and 2 2^-24 for 1 + z and the quotient: 11.1 2^-24. A third part left out anywhere is up to 2^-16."""
+    rng = np.random.default_rng(rows + 1)
+    q, K, V, table, lens, c = two_positions(rows, dim)
+    K[9, 0, 1] = np.float32(rng.uniform(1.2, 1.3))
+    q[:, 0, 1] = -rng.uniform(0.6, 1.06, rows)
+    V[9, 0] = rng.normal(size=dim)
+    O, m, l = run_attend(c, q, K, V, table, lens, [64.0], rows, None, 1.0)
+    z = np.exp(q[:, 0, 1].astype(np.float64) * float(K[9, 0, 1]))
+    assert z.max() < 0.5 and z.min() > 0.25
+    want = (z / (1 + z))[:, None] * V[9, 0].astype(np.float64)
+    assert np.all(np.abs(O[:, 0] - want) <= 11.1 * U * np.abs(want))
+    assert np.all(np.abs(l[:, 0] - (1 + z)) <= (7.5 * z + 1.5) * U)
+
+
+@pytest.mark.parametrize("size", [1100, 1250, 1340, 1360, 1380, 1400, 1420, 1450])
+def test_small_values_under_growing_scores(size):
+    """Values of 2^-100 under scores that grow by 69 to 91 over each of 16 ranges: neither the weights nor the products
+    overflow where the factor to the largest score is below every normal float."""
+    rng = np.random.default_rng(size)
+    heads, per, beams, dim, n, page = 16, 4, 10, 32, 8000, 16
+    lens = [n + int(x) for x in rng.integers(1, 9, beams)]
+    table, pages = tp.batch_of(rng, 1, beams, page, [n], lens, True)
+    K = (rng.normal(size=(pages * page, heads, dim)) * 0.1).astype(np.float32)
+    V = (rng.normal(size=(pages * page, heads, dim)) * 2.0 ** -100).astype(np.float32)
+    q = (rng.normal(size=(beams, heads * per, dim)) * 0.25).astype(np.float32)
+    q[:, :, 0] = 1.0
+    rows = [ph.row_of(table, 0, j, page, pages) for j in range(n)]
+    K[rows, :, 0] = np.linspace(0, size, n).astype(np.float32)[:, None]
+    c = dict(pages=pages, page=page, heads=heads, dim=dim)
+    O, m, l = run_attend(c, q, K, V, table, lens, [n], beams, None, 1.0)
+    wO, wm, wl, tol = ph.attend(q, K, V, table, page, pages, heads, lens, 1.0)
+    assert np.all(np.abs(O - wO) <= tol) and np.all(np.abs(wO).max(axis=2) > 2.0 ** -110)
