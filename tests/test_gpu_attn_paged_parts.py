@@ -1,5 +1,7 @@
 """nnhip_attn_paged over positions that several ranges, waves and walks take (csrc/k_attn_paged.hip), against the 64-bit
 form (paged_helpers.attend): what must not depend on how a call is cut."""
+import math
+
 import numpy as np
 import pytest
 
@@ -123,3 +125,55 @@ def test_small_values_under_growing_scores(size):
     O, m, l = run_attend(c, q, K, V, table, lens, [n], beams, None, 1.0)
     wO, wm, wl, tol = ph.attend(q, K, V, table, page, pages, heads, lens, 1.0)
     assert np.all(np.abs(O - wO) <= tol) and np.all(np.abs(wO).max(axis=2) > 2.0 ** -110)
+
+
+def check_stats(c, q, K, V, table, lens, shared, alpha, slopes=None):
+    """test_gpu_paged.check_many, and m and l: a score is off by what its products, the slope's and the sums round, l by
+    what its weights and their sum are (as in test_attend); without a position they are lowest() and 0."""
+    beams, dim = q.shape[0], q.shape[2]
+    O, m, l = run_attend(c, q, K, V, table, lens, shared, beams, slopes, alpha)
+    wO, wm, wl, tol = ph.attend(q, K, V, table, c["page"], c["pages"], 1, lens, alpha, slopes)
+    ok = np.isfinite(wO)
+    assert np.array_equal(np.isfinite(O), ok) and np.all(np.abs(O[ok] - wO[ok]) <= tol[ok])
+    fin = np.isfinite(wl)
+    assert np.array_equal(np.isfinite(l), fin)
+    size = np.zeros(wm.shape)
+    for b in range(beams):
+        rows = [ph.row_of(table, b, j, c["page"], c["pages"]) for j in range(ph.length_of(lens[b], table.shape[1] * c["page"]))]
+        k = np.abs(K[[r for r in rows if r is not None], 0].astype(np.float64))
+        if len(k):
+            with np.errstate(invalid="ignore"):
+                size[b] = abs(alpha) * (k @ np.abs(q[b].astype(np.float64)).T).max(axis=0)
+    s_tol = (dim + 8) * U * size + 8 * U * np.abs(wm)
+    if slopes is not None:
+        s_tol = s_tol + 2 * U * np.abs(slopes)[None, :] * max(lens)
+    n = max(lens)
+    assert np.all(np.abs(m[fin] - wm[fin]) <= s_tol[fin])
+    assert np.all(np.abs(l[fin] - wl[fin]) <= wl[fin] * (4 * s_tol[fin] + 2 * n * U))
+    none = wl == 0
+    assert np.all(l[none] == 0) and np.all(m[none] == np.float32(-3.4028234663852886e38))
+    return O
+
+
+@pytest.mark.parametrize("beams,per,dim,prefix,own", [(9, 4, 32, 130, 20), (33, 1, 64, 400, 9), (40, 3, 96, 700, 5),
+                                                     (16, 4, 128, 1500, 40), (70, 2, 128, 333, 3), (40, 1, 80, 200, 7),
+                                                     (3, 20, 128, 200, 50)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_many_rows_m_and_l(beams, per, dim, prefix, own, slopes):
+    """The bf16 walk's m and l: also of a sequence shorter than the shared positions, of one of length 0, beside rows past
+    the last one."""
+    rng = np.random.default_rng(beams * 100 + dim + 1)
+    c, q, K, V, table, lens, shared = tp.many_rows(rng, beams, per, dim, prefix, own)
+    tp.poison(K, V, table, lens, c["page"], c["pages"])
+    lens[1] = shared[0] - 3
+    lens[2] = 0
+    sl = (2.0 ** -np.arange(3, per + 3)).astype(np.float32) if slopes else None
+    O = check_stats(c, q, K, V, table, lens, shared, 1 / math.sqrt(dim), sl)
+    assert np.all(O[2] == 0)
+
+
+@pytest.mark.parametrize("what", tp.test_attend_many_rows_range.pytestmark[0].args[1])
+def test_many_rows_range_m_and_l(what, monkeypatch):
+    """The same where the bf16 parts do not hold the values and the range is walked again."""
+    monkeypatch.setattr(tp, "check_many", check_stats)
+    tp.test_attend_many_rows_range(what)
