@@ -822,18 +822,19 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
     part.b0 = i * part.nb;
     part.slot = part.is_shared ? c : a.n_shared + c;
     part.row_waves = part.is_shared ? a.shared_row_waves : a.own_row_waves;
+    const int len0 = length_of(a.len[part.b0], (int)(a.c.width * a.c.page.d));   // on its way with the shared length
     part.common = shared_of(a, part.b0);
     part.by = part.b0;
     int lo = 0, hi = part.common;
-    if (part.is_shared)
+    if (!part.is_shared)
+    {
+        hi = len0;
+        lo = hi >= part.common ? part.common : 0;
+    }
+    else if (len0 < part.common)
     {
         part.by = reader_of(a, part.b0, part.common);
         if (part.by - part.b0 == a.group) hi = 0;   // for no one
-    }
-    else
-    {
-        hi = length_of(a.len[part.b0], (int)(a.c.width * a.c.page.d));
-        lo = hi >= part.common ? part.common : 0;
     }
     constexpr int kStep = 4 * kTile;
     const int steps = (hi - lo + kStep - 1) / kStep;
