@@ -500,10 +500,11 @@ int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f,
  * neighbouring sequences; shared (batch / group), when set, says how many first positions the group's
  * sequences have in common: the tables of those that are as long name the same rows there, and these are read
  * once for all of them (through the table of the first of them). A sequence shorter than that is read through
- * its own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128.
- * O, m and l overlap no input. The workspace is nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte
- * aligned; calls that may overlap in time need one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same
- * bits every time. */
+ * its own table. A len or shared that is negative or NaN counts as 0, one past width * page as that. dim <= 128,
+ * batch * heads below 2^24 (a workgroup each, or several). O, m and l overlap no input. The workspace is
+ * nnhip_attn_paged_workspace_bytes (0 where none is needed), 16-byte aligned; calls that may overlap in time need
+ * one each. Results do not depend on the other sequences of the batch beyond rounding, and are the same bits every
+ * time. */
 size_t nnhip_attn_paged_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t group);
 int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, const float* len,
                      const float* shared, size_t group, const float* slopes, float alpha, float* O, long o_t,
@@ -537,7 +538,7 @@ int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const floa
  * that is no sequence number gives a row of -1 and length 0; a fresh[b] that is no page number is stored as -1
  * and nothing is copied. table_out (out_batch, width) and len_out overlap neither an input, the caches among
  * them, nor each other (-1). The pages of fresh must differ from each other and from every page that another
- * sequence of the new batch continues or shares. */
+ * sequence of the new batch continues or shares. out_batch below 2^17, out_batch * width below 2^31. */
 int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float* parent, const float* len,
                      const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);
 

@@ -1093,7 +1093,7 @@ extern "C" int nnhip_attn_paged(const nnhip_kv_pages* c, const float* q, long q_
     const PagedPlan p = paged_plan(*c, q_heads, shared ? group : 1, mode, __builtin_fabsf(alpha) >= 0x1p-64f);
     const size_t need = paged_workspace(*c, q_heads, p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
-    if (p.shared_blocks + p.own_blocks > 0x7fffffffu) return -1;
+    if (p.shared_blocks + p.own_blocks > kGridMost || (p.parts() > kFewParts && c->batch * q_heads > kGridMost)) return -1;
     auto* ws = static_cast<float*>(workspace);
     PagedArgs a{};
     a.c = pages_of(*c);

@@ -329,7 +329,7 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
         a.splits = static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
         const size_t blocks = tables + a.splits * pages;
         if (blocks == 0) break;
-        if (blocks > 0x7fffffffu) return -1;
+        if (blocks > kGridMost) return -1;   // of the first launch, if of any: it has the tables and the most layers
         a.table_blocks = static_cast<unsigned>(tables);
         hipLaunchKernelGGL(k_kv_reorder, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                            static_cast<hipStream_t>(stream), a);

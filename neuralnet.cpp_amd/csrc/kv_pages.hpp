@@ -60,6 +60,8 @@ __device__ __forceinline__ int length_of(float f, int most)
     return f >= (float)most ? most : (int)f;
 }
 
+constexpr size_t kGridMost = 0xffffff;   // workgroups of 256: a launch has fewer than 2^32 threads along an axis
+
 // The sizes that every entry point asks for: the kernels count pages, rows and a row's values in 32 bits.
 inline bool pages_ok(const nnhip_kv_pages* c, size_t max_dim)
 {

@@ -137,3 +137,18 @@ def test_reorder_outputs_over_the_rest(bad):
 def test_reorder_rows_past_31_bits(heads, dim):
     """Rows of 2^31 values and more: the kernel counts a row's values in 32 bits, up to 256 past the last."""
     assert reorder([pages(K=1 << 48, V=1 << 56, heads=heads, dim=dim, row=heads * dim, pages=1, page=1)]) == -1
+
+
+@pytest.mark.parametrize("batch,q_heads", [(1 << 20, 16), (1 << 21, 8), (1 << 24, 1), ((1 << 20) - 16, 16)])
+def test_attend_more_workgroups_than_a_grid_has(batch, q_heads):
+    """A workgroup of 256 a sequence and key head, and a grid of fewer than 2^32 threads. One short of that is not refused."""
+    refused = batch * q_heads >= 1 << 24
+    rc = attend(pages(batch=batch, width=1, heads=q_heads, row=64 * q_heads), q_heads=q_heads, shared=None, group=1)
+    assert (rc == -1) == refused
+
+
+def test_reorder_more_workgroups_than_a_grid_has():
+    big = dict(K=1 << 50, V=1 << 54, table=1 << 58, page=1, pages=16)
+    assert reorder([pages(batch=1 << 10, width=1 << 22, **big)], out_batch=1 << 10, out=1 << 44, out_len=1 << 43) == -1
+    assert reorder([pages(batch=1 << 10, width=1 << 21, **big)], out_batch=1 << 10, out=1 << 44, out_len=1 << 43) != -1
+    assert reorder([pages(batch=4, width=8, **dict(big, page=2))] * 32, out_batch=1 << 18, out=1 << 44, out_len=1 << 43) == -1
