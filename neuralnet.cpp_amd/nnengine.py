@@ -501,6 +501,7 @@ class GptSession:
         eng._check(self._f["gpt_create"](eng._e, ctypes.byref(cfg), ctypes.byref(g)))
         self._g = g
         self.vocab_size = vocab_size
+        self.seq_len = seq_len
 
     def num_params(self) -> int:
         return self._f["gpt_num_params"](self._g)
@@ -606,6 +607,7 @@ class GptSession:
         """The `beams` best continuations of the prompt: a list of (token ids, sum of log probabilities), best first."""
         if beams < 1 or max_new < 0:
             raise EngineError("beam_search: 1 to 256 beams, max_new not negative")
+        max_new = min(int(max_new), self.seq_len)   # more never fit behind a prompt
         pr = np.ascontiguousarray(np.asarray(prompt, dtype=np.uint64))
         out = np.zeros(max(1, beams * max_new), dtype=np.uint64)
         n = (ctypes.c_size_t * max(1, beams))()

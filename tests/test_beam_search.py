@@ -263,3 +263,13 @@ def orphan_first(e, beams):
 @pytest.mark.parametrize("beams", [2, 6, 70])
 def test_group_whose_first_sequence_has_no_parent(cpu, beams):
     orphan_first(cpu, beams)
+
+
+def test_any_number_of_new_tokens(cpu):
+    """More tokens than the context has room for are what fits, however many are asked for."""
+    cfg = dict(SMALL, pos_enc="rope")
+    g = cpu.gpt(**cfg)
+    g.set_params(params_of(cfg, 5))
+    want = g.beam_search([1, 2, 3], 4, 12, 5)
+    for n in (13, 14, 10 ** 6, 10 ** 15, 2 ** 64 - 1):
+        assert g.beam_search([1, 2, 3], 4, n, 5) == want
