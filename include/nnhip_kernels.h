@@ -465,8 +465,8 @@ int nnhip_attn_query(const float* Q, const float* Kp, long kb, long kj, long kk,
  * incremental inference hold them: K and V have pages * page rows, `row` floats apart (>= heads * dim), head h
  * of a row at h * dim. table (batch, width) holds page numbers: position p of sequence b is row
  * table[b * width + p / page] * page + p % page. A position whose table entry is no page number (negative,
- * NaN, >= pages) or that lies past width * page is absent: it is neither read nor written. Sequences may share
- * pages. width * page and pages are at most 2^24 (index tensors hold integers as floats), pages * page and
+ * NaN, >= pages) or that lies past width * page is absent: nothing is written for it, and no result depends on
+ * it (row 0 of the caches may be read in its place, and counts for nothing). Sequences may share pages. width * page and pages are at most 2^24 (index tensors hold integers as floats), pages * page and
  * heads * dim below 2^31, row at most 2^32. */
 typedef struct nnhip_kv_pages
 {
@@ -483,8 +483,10 @@ typedef struct nnhip_kv_pages
  * j and j + rope_dim / 2 (j < rope_dim / 2) of each head of k and q as RotaryEmbedding does
  * (compute_layer.hpp:884-984): x_j c - x_{j+r/2} s and x_{j+r/2} c + x_j s; the others, and v, are stored as
  * they are. Without (cos and sin NULL, rope_dim 0) nothing is turned. q and q_out may both be NULL; q_out may
- * be q itself with the same strides. A token whose sequence, position, page or, with a rotation, table row does not exist is padding:
- * nothing of it is written. Two tokens of one call must not name the same row, and K must not be V. dim <= 256. */
+ * be q itself with the same strides; but for that nothing that is written overlaps an input. A token whose
+ * sequence, position, page or, with a rotation, table row does not exist is padding: nothing of it is written,
+ * but its k, v and q may be read. Two tokens of one call must not name the same row, and K must not be V.
+ * dim <= 256. */
 int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f, const float* v, long v_t, long v_f,
                     const float* q, long q_t, long q_f, float* q_out, long o_t, long o_f, size_t q_heads,
                     size_t tokens, const float* seq, const float* pos, const float* cos, const float* sin,
@@ -495,7 +497,8 @@ int nnhip_kv_append(const nnhip_kv_pages* c, const float* k, long k_t, long k_f,
  * h / (q_heads / heads)), over the positions j < len[b] that are not absent:
  *   s_j = alpha * (q_bh . k_j) - slopes[h] * (len[b] - 1 - j)     (no second term when slopes is NULL)
  *   m = max_j s_j, l = sum_j exp(s_j - m), O = sum_j exp(s_j - m) v_j / l
- * with m = lowest(), l = 0, O = 0 when there is no position or every s_j is -inf. q and O as the features of
+ * with m = lowest(), l = 0, O = 0 when there is no position or every s_j is -inf (a value that is not finite at a
+ * position whose s_j is -inf may make O so, or not). q and O as the features of
  * nnhip_kv_append's q; m, l (batch, q_heads) may be NULL. The batch is batch / group groups of `group`
  * neighbouring sequences; shared (batch / group), when set, says how many first positions the group's
  * sequences have in common: the tables of those that are as long name the same rows there, and these are read

@@ -330,7 +330,9 @@ __device__ __forceinline__ void rank_list(PickShared& s, unsigned k)
 // One workgroup a group. The kernel runs once over little data, so its time is that of the loads it waits for one
 // after another, of its instructions (one CU's) and of fetching them: loads go several at a time, loops stay loops,
 // and most items are put aside by a float32 distance from the best total, before any 64-bit total is formed. 13 us for
-// 4 x 1024 logits, 20 for 16 x 32000 and for 32 groups of 8 x 100003.
+// 4 x 1024 logits, 20 for 16 x 32000 and for 32 groups of 8 x 100003. Of these, by the cycle counter (2.4 GHz): the
+// sums 4.9, 5.6 and 5.6, log-sum-exps and distances 1.8, 1.5 and 1.8, the best segments 0.6 (64 are ranked at once), 5.1
+// and 4.1, their rank 1.3, 1.2 and 1.2, the best segments' tokens 2.3, 3.9 and 4.3, the last rank 0.7, and the launch.
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(BeamArgs a)
 {
     constexpr unsigned kWaves = kPickThreads / 64;
