@@ -502,7 +502,7 @@ __device__ __forceinline__ void walk(const PagedArgs& a, const Part& part, PartS
 // walked again in float32. Keys are split as they are too: of those below 2^-109 parts below 2^-126 are lost, dim alpha
 // 2^-22 of a score at most with the largest queries that the parts hold.
 //
-// 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 122 us by themselves, 4.4 TB/s (92 with the loads alone); 512 rows over
+// 64 rows over 65000 positions of 8 heads of 128 (532 MB) take 120 us by themselves, 4.4 TB/s (92 with the loads alone); 512 rows over
 // 6000 take 93 us. Two waves a SIMD of 32 rows each took 160 where one of 64 took 144 (every wave splits all its keys
 // and values), and 170 where two waves split a tile in halves, exchanged through LDS.
 constexpr int kSplitRows = 4;   // row tiles of a wave
@@ -831,9 +831,9 @@ template <int KS, int MODE, int RT> __global__ __launch_bounds__(256, MODE == kS
         hi = len0;
         lo = hi >= part.common ? part.common : 0;
     }
-    else if (len0 < part.common)
+    else if (__builtin_expect(len0 < part.common, 0))   // marked seldom, 64 rows over 65000 positions take 120 us instead of 122
     {
-        part.by = reader_of(a, part.b0, part.common);
+        part.by = __builtin_amdgcn_readfirstlane(reader_of(a, part.b0, part.common));
         if (part.by - part.b0 == a.group) hi = 0;   // for no one
     }
     constexpr int kStep = 4 * kTile;
