@@ -299,8 +299,9 @@ extern "C" int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, c
     if (over_outputs(c.table, c.batch * c.width) || over_outputs(len, c.batch) || over_outputs(parent, out_batch) ||
         over_outputs(fresh, out_batch) || overlap(table_out, out_batch * c.width, len_out, out_batch))
         return -1;
+    const size_t extent = (c.pages * c.page - 1) * c.row + c.heads * c.dim;   // of a cache: nothing behind its last row's heads
     for (size_t i = 0; i < n_layers; ++i)
-        if (over_outputs(layers[i].K, c.pages * c.page * c.row) || over_outputs(layers[i].V, c.pages * c.page * c.row)) return -1;
+        if (over_outputs(layers[i].K, extent) || over_outputs(layers[i].V, extent)) return -1;
     ReorderArgs a{};
     a.c = pages_of(c);
     a.parent = parent;

@@ -152,3 +152,13 @@ def test_reorder_more_workgroups_than_a_grid_has():
     assert reorder([pages(batch=1 << 10, width=1 << 22, **big)], out_batch=1 << 10, out=1 << 44, out_len=1 << 43) == -1
     assert reorder([pages(batch=1 << 10, width=1 << 21, **big)], out_batch=1 << 10, out=1 << 44, out_len=1 << 43) != -1
     assert reorder([pages(batch=4, width=8, **dict(big, page=2))] * 32, out_batch=1 << 18, out=1 << 44, out_len=1 << 43) == -1
+
+
+def test_reorder_outputs_behind_the_caches():
+    """Values interleaved with keys, V behind K's heads in rows of twice their width: an output right behind the last row
+    is not on it, one on its last value is."""
+    kv = dict(K=1 << 30, V=(1 << 30) + 4 * 256, row=512)
+    end = (1 << 30) + 4 * 512 * 16 * 16
+    for at, refused in ((end, False), (end - 4, True), ((1 << 30) - 4 * 32, False), ((1 << 30) - 4 * 31, True)):
+        assert (reorder([pages(**kv)], out=at) == -1) == refused
+        assert (reorder([pages(**kv), pages(**kv)], out=at) == -1) == refused
