@@ -273,3 +273,38 @@ def test_any_number_of_new_tokens(cpu):
     want = g.beam_search([1, 2, 3], 4, 12, 5)
     for n in (13, 14, 10 ** 6, 10 ** 15, 2 ** 64 - 1):
         assert g.beam_search([1, 2, 3], 4, n, 5) == want
+
+
+def through_views(e):
+    """Caches, tokens and tables that are slices of other tensors, or are sliced before they are written: a slice is a
+    copy, whatever is written afterwards on either side."""
+    rng = np.random.default_rng(21)
+    heads, d, page, pages, n = 2, 4, 2, 8, 8
+    both = e.tensor(rng.normal(size=(2 * pages * page, heads * d)).astype(np.float32))
+    tables = e.tensor(np.arange(4 * 4, dtype=np.float32).reshape(4, 4) % pages)
+    out = {}
+    K, V = e.slice_rows(both, 0, pages * page), e.slice_rows(both, pages * page, pages * page)
+    table = e.slice_rows(tables, 1, 2)
+    k, v = e.slice_rows(K, 0, heads * d), e.slice_rows(both, 3, heads * d)     # (heads * d, 8 tokens)
+    before = e.slice_rows(K, 2, 9)
+    seq = e.tensor((np.arange(n) % 2).astype(np.float32)[:, None])
+    pos = e.tensor((np.arange(n) // 2).astype(np.float32)[:, None])
+    cos, sin = (e.tensor(rng.normal(size=(8, 2)).astype(np.float32)) for _ in range(2))
+    out["q"] = e.kv_append(K, V, table, k, v, pos, page, heads, q=k, cos=cos, sin=sin, seq=seq)
+    after = e.slice_rows(K, 2, 9)
+    lens = e.tensor(np.array([[3.0], [4]]))
+    q2 = e.slice_rows(both, 5, 2)                                               # (2, 8): as (heads * d, batch) below
+    out["O"] = e.attn_paged(K, V, table, e.transpose(q2), lens, 0.5, page, heads)
+    out["table2"], out["lens2"] = e.kv_reorder([(K, V)], table, e.tensor(np.array([[1.0], [0]])), lens,
+                                               e.tensor(np.array([[3.0], [6]])), page, heads)
+    out.update(K=K, V=V, k=k, v=v, before=before, after=after, both=both, tables=tables)
+    return {n: t.numpy() for n, t in out.items()}
+
+
+def test_slices_are_copies(cpu):
+    got = through_views(cpu)
+    rng = np.random.default_rng(21)
+    both = rng.normal(size=(32, 8)).astype(np.float32)
+    assert np.array_equal(got["both"], both) and np.array_equal(got["before"], both[2:11])
+    assert np.array_equal(got["k"], both[:8]) and np.array_equal(got["v"], both[3:11])
+    assert not np.array_equal(got["after"], both[2:11])

@@ -80,3 +80,11 @@ def test_one_beam_is_greedy(hip):
 @pytest.mark.parametrize("beams", [2, 6, 40, 70])
 def test_group_whose_first_sequence_has_no_parent(hip, beams):
     cpu_tests.orphan_first(hip, beams)
+
+
+def test_slices_are_copies(hip, cpu):
+    h, c = cpu_tests.through_views(hip), cpu_tests.through_views(cpu)
+    for n in ("table2", "lens2", "k", "v", "before", "both", "tables"):
+        assert np.array_equal(h[n], c[n]), n
+    for n in ("q", "O", "K", "V", "after"):
+        assert nrm_err(h[n], c[n]) <= 1e-6, n
