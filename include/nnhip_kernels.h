@@ -545,6 +545,86 @@ int nnhip_beam_select(const float* logits, size_t ld, int beam_major, const floa
 int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float* parent, const float* len,
                      const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);
 
+/* ── 8-bit caches, chunks of new tokens, drafted tokens (no CUDA counterpart) ──
+ * A paged cache as nnhip_kv_pages with a byte a value: value j of head h of a row stands for
+ * K[row * r + h * dim + j] * K_scale[r * heads + h] (V alike). K and V have pages * page rows, `row` bytes apart
+ * (>= heads * dim), the scales (pages * page, heads). Table and limits as there. */
+typedef struct nnhip_kv8_pages
+{
+    signed char* K;
+    signed char* V;
+    float* K_scale;
+    float* V_scale;
+    const float* table;
+    size_t batch, width, pages, page, heads, dim, row;
+} nnhip_kv8_pages;
+
+/* nnhip_kv_append into an 8-bit cache: arguments, padding, rotation and q_out as there. Of each token and head the scale is
+ * (largest |x_j|) / 127 rounded to float32, and a byte is x_j / scale rounded to the nearest integer, ties to even, within
+ * [-127, 127]; k is turned, and both quotients are formed, in float64, so that the bytes do not depend on float32's
+ * rounding. A head whose values are all 0 (or so small that the scale is) has scale 0 and bytes 0; one with a value that
+ * is not finite has scale NaN and bytes 0. K, V, K_scale and V_scale must differ (-1). dim <= 256. */
+int nnhip_kv8_append(const nnhip_kv8_pages* c, const float* k, long k_t, long k_f, const float* v, long v_t, long v_f,
+                     const float* q, long q_t, long q_f, float* q_out, long o_t, long o_f, size_t q_heads,
+                     size_t tokens, const float* seq, const float* pos, const float* cos, const float* sin,
+                     size_t rope_rows, size_t rope_dim, void* stream);
+
+/* What an 8-bit cache holds of position pos[n] of sequence seq[n] (seq NULL: of sequence n): byte * scale, rounded once,
+ * to features of k and v as nnhip_kv_append reads them (heads * dim, a k_f, v_f apart, tokens k_t, v_t). Either of k and
+ * v may be NULL. Of a token whose sequence, position or page does not exist nothing is written. The outputs overlap
+ * neither the cache nor each other; dim <= 256. */
+int nnhip_kv8_read(const nnhip_kv8_pages* c, float* k, long k_t, long k_f, float* v, long v_t, long v_f, size_t tokens,
+                   const float* seq, const float* pos, void* stream);
+
+/* Attention of a chunk of new tokens of every sequence against the sequence's pages, into which they have been appended
+ * (chunked prompts, drafted tokens; with one token a sequence nnhip_attn_paged without sharing). Sequence b has the
+ * tokens start[b] .. start[b + 1) of q (start: batch + 1 ascending numbers), at most `most` of them, which are the last of
+ * its len[b] positions: with n of them, token i is at p = len[b] - n + i and sees the positions j <= p. For head h
+ * (reading key head h / (q_heads / heads)), over these positions but the absent ones:
+ *   s_j = alpha * (q . k_j) - slopes[h] * (p - j)     (no second term when slopes is NULL)
+ *   m = max_j s_j, l = sum_j exp(s_j - m), O = sum_j exp(s_j - m) v_j / l
+ * with m = lowest(), l = 0, O = 0 when there is no position or every s_j is -inf. What lies at positions that a token does
+ * not see does not change its results, whatever it is. q and O as the features of nnhip_kv_append's q; m, l (tokens,
+ * q_heads) may be NULL. Tokens that no sequence has, behind the last one's or past `most`, are left as they are. A start
+ * that is negative or NaN counts as 0, one past `tokens` as that, a len as nnhip_attn_paged's. 1 <= most <= tokens; dim <=
+ * 128; tokens * q_heads below 2^31. O, m and l overlap no input. The workspace is nnhip_attn_chunk_workspace_bytes (0
+ * where none is needed), 16-byte aligned; calls that may overlap in time need one each. Results are the same bits every
+ * time. */
+size_t nnhip_attn_chunk_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t tokens, size_t most);
+int nnhip_attn_chunk(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, size_t tokens,
+                     const float* start, size_t most, const float* len, const float* slopes, float alpha, float* O,
+                     long o_t, long o_f, float* m, float* l, void* workspace, size_t workspace_bytes, void* stream);
+/* The same over an 8-bit cache. */
+size_t nnhip_attn_chunk8_workspace_bytes(const nnhip_kv8_pages* c, size_t q_heads, size_t tokens, size_t most);
+int nnhip_attn_chunk8(const nnhip_kv8_pages* c, const float* q, long q_t, long q_f, size_t q_heads, size_t tokens,
+                      const float* start, size_t most, const float* len, const float* slopes, float alpha, float* O,
+                      long o_t, long o_f, float* m, float* l, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens (speculative sampling). The target's logits of token n lie in row n of a (tokens, vocab)
+ * matrix (token_major) or in column n of a (vocab, tokens) matrix, the layout of the output head's logits, t_ld floats
+ * from a row to the next; the draft's alike with d_ld. Sequence b was fed the tokens fed[start[b] .. start[b + 1)), at most
+ * `most`, of which all but the first were drafted: row n's distributions are those of the token after it, so that
+ * fed[n + 1] was drawn from the draft's row n. With p = softmax(target / temperature) and q = softmax(draft /
+ * temperature), both in float64, the token x after row n stands if accept[n] * q(x) < p(x). At the first row whose token
+ * does not stand, the next token is drawn from max(p - q, 0) (from p where that is 0 throughout), behind the last row
+ * from p: the smallest v whose cumulative sum exceeds pick[b] times the whole sum. out_accepted[b] is the number of tokens
+ * that stand, out_token[b] the token drawn: these many drafted tokens and that one continue the sequence, distributed as
+ * if drawn from the target. Without drafted tokens (one row a sequence) this is sampling.
+ * draft NULL: the tokens were chosen without probabilities; q is 1 at the drafted token. temperature 0: a token stands if
+ * it is the target's largest logit (the lowest index of equal ones), and that of the first row whose token is another
+ * comes next; draft, accept and pick are not used and may be NULL. A logit that is NaN counts as -inf; of rows with +inf
+ * these share p; a row of nothing but -inf has p = 0 and draws token 0. A drafted token that is no index below vocab does
+ * not stand, and takes nothing from p where draft is NULL. pick below 0 or NaN counts as 0, 1 and above as the largest number below 1. A sequence without rows
+ * has out_accepted 0 and out_token -1. start as nnhip_attn_chunk's; 1 <= most <= 1024, vocab and tokens at most 2^24,
+ * temperature finite and not negative. The draft's last row of a sequence is not used (it may be anything that can be
+ * read). The outputs overlap no input. The workspace is nnhip_draft_verify_workspace_bytes, 16-byte aligned; calls that
+ * may overlap in time need one each. */
+size_t nnhip_draft_verify_workspace_bytes(size_t tokens, size_t batch, size_t most, size_t vocab);
+int nnhip_draft_verify(const float* target, size_t t_ld, const float* draft, size_t d_ld, int token_major, size_t vocab,
+                       size_t tokens, const float* fed, const float* start, size_t batch, size_t most, float temperature,
+                       const float* accept, const float* pick, float* out_accepted, float* out_token, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ── column softmax / sparse cross-entropy (no CUDA counterpart) ─────────
  * cpu_engine.hpp:922-945 and :948-1006. Workspace from nnhip_col_softmax_workspace_bytes. */
 size_t nnhip_col_softmax_workspace_bytes(size_t C, size_t N);

@@ -85,4 +85,51 @@ inline Pages pages_of(const nnhip_kv_pages& c)
                  FastDiv(static_cast<unsigned>(c.page))};
 }
 
+// An 8-bit cache (nnhip_kv8_pages): the table's part as Pages has it (its K and V are not set), a byte a value in rows
+// t.row apart, and a scale a row and head.
+struct Pages8
+{
+    Pages t;
+    signed char *K, *V;
+    float *K_scale, *V_scale;
+};
+
+inline bool pages8_ok(const nnhip_kv8_pages* c, size_t max_dim)
+{
+    if (!c || !c->K || !c->V || !c->K_scale || !c->V_scale) return false;
+    auto* some = c->K_scale;   // stands for the caches in the checks of the sizes
+    const nnhip_kv_pages t{some, some, c->table, c->batch, c->width, c->pages, c->page, c->heads, c->dim, c->row};
+    return pages_ok(&t, max_dim);
+}
+
+inline Pages8 pages8_of(const nnhip_kv8_pages& c)
+{
+    const nnhip_kv_pages t{nullptr, nullptr, c.table, c.batch, c.width, c.pages, c.page, c.heads, c.dim, c.row};
+    return Pages8{pages_of(t), c.K, c.V, c.K_scale, c.V_scale};
+}
+
+// The tokens of a call that name positions of sequences. rope_rows: rows of the rotation's tables, 0 without one.
+struct Tokens
+{
+    const float *seq, *pos;
+    unsigned n, rope_rows;
+
+    // Where token i goes: its row, or -1 for padding, and its position.
+    __device__ __forceinline__ int row(const Pages& c, unsigned i, unsigned& at) const
+    {
+        size_t p = 0, b = i;
+        const bool seq_ok = seq ? row_index(seq[i], c.batch, b) : i < c.batch;
+        const bool ok = row_index(pos[i], kMaxIndex, p) && seq_ok && (!rope_rows || p < rope_rows);
+        at = (unsigned)p;
+        return ok ? c.row_of((unsigned)b, at) : -1;
+    }
+};
+
+// Features of tokens: floats from a token and from a feature to the next.
+struct Features
+{
+    float* p;
+    long t, f;
+};
+
 } // namespace nnhip
