@@ -9,7 +9,7 @@ namespace nnhip
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kTile = 16;          // positions and rows of a product
 constexpr int kChunkMaxDim = 128;
 
@@ -302,9 +302,13 @@ template <int KS> struct WalkShared
     float ml[4][kTile][2];
 };
 
-// Where a row's results go: m, l and values d .. d + 3 of O, unnormalised.
+// Where a row's results go: m, l and values d .. d + 3 of O, unnormalised. LOG2: m is a score times log2(e). The results of
+// k_attn_chunk_wide's ranges (WIDE) are joined so: a score's product with log2(e) is rounded once, before the ranges part.
+template <bool WIDE, bool LOG2>
 __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int row, int d, f32x4 o, float m, float l, bool stats)
 {
+    if (LOG2 && a.ranges == 1 && m != kLowest) m *= kLn2;
+    if (WIDE && !LOG2 && a.ranges > 1 && m != kLowest) m *= kLog2e;
     const unsigned i = a.by_per.div(row), qh = part.h * a.by_per.d + (row - i * a.by_per.d);
     const size_t n = part.chunk.first + i, at = n * a.q_heads + qh;
     const int dim = a.c.t.dim;
@@ -332,7 +336,7 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int ro
 
 // The waves' results for 16 rows of each row wave (rows first + rv * apart on) are joined through LDS, in the order
 // of their positions, and written: 16 threads a row, 4 neighbouring values at a time.
-template <int KS>
+template <int KS, bool WIDE>
 __device__ __forceinline__ void join_waves(const ChunkArgs& a, const Part& part, WalkShared<KS>& sh, float m, float l,
                                            const f32x4 (&o)[Geometry<KS>::T][Geometry<KS>::VW], int first, int rws, int apart)
 {
@@ -378,14 +382,14 @@ __device__ __forceinline__ void join_waves(const ChunkArgs& a, const Part& part,
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 if (any[k]) z += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
-            put(a, part, row, d, z, mm, ll, d == 0);
+            put<WIDE, false>(a, part, row, d, z, mm, ll, d == 0);
         }
     }
 }
 
 // One range of positions. row_waves of the 4 waves lie along the rows, RT tiles each; the others take 16 positions
 // each in turn.
-template <int BITS, int KS, bool VEC, int RT>
+template <int BITS, int KS, bool VEC, int RT, bool WIDE>
 __device__ __forceinline__ void walk(const ChunkArgs& a, const Part& part, int rws, WalkShared<KS>& sh)
 {
     using G = Geometry<KS>;
@@ -466,7 +470,7 @@ __device__ __forceinline__ void walk(const ChunkArgs& a, const Part& part, int r
         Row<KS>& w = rows[i];
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
-        join_waves<KS>(a, part, sh, w.m, w.l, w.o, part.first + i * kTile, rws, RT * kTile);
+        join_waves<KS, WIDE>(a, part, sh, w.m, w.l, w.o, part.first + i * kTile, rws, RT * kTile);
     }
 }
 

@@ -36,7 +36,7 @@ template <int BITS, int KS, bool VEC, int RT> __global__ __launch_bounds__(256, 
     const int rows_here = kTile * RT * a.row_waves;
     part.first = block * rows_here;
     if (part.n_rows > a.wide_from || (int)part.first >= part.n_rows || !cut_range<4 * kTile>(a, part, rows_here)) return;
-    walk<BITS, KS, VEC, RT>(a, part, a.row_waves, sh);
+    walk<BITS, KS, VEC, RT, false>(a, part, a.row_waves, sh);
 }
 
 // In place of the factor of a range of l = 0, whose O is anything. A factor that underflows to 0 is one: a value of its
@@ -54,7 +54,9 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
     if (b < 0) return;
     const Chunk c = chunk_of(a, b);
     if (n >= c.first + c.n) return;   // no sequence's
-    const unsigned ranges = c.n * (int)a.by_per.d > a.wide_from ? wide : narrow;
+    const bool is_wide = c.n * (int)a.by_per.d > a.wide_from;   // m is a score times log2(e)
+    const unsigned ranges = is_wide ? wide : narrow;
+    const float to_log2 = is_wide ? 1.0f : kLog2e;
     if (ranges == 1) return;   // written already
     const float* ml = a.part_ml + 2 * (size_t)at * a.slots;
     const float* po = a.part_o + (size_t)at * a.slots * dim;
@@ -67,7 +69,7 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
         float w = kNoRange;
         if (c0 + lane < ranges && ml[2 * (c0 + lane) + 1] != 0.0f)
         {
-            w = __builtin_amdgcn_exp2f((ml[2 * (c0 + lane)] - m) * kLog2e);
+            w = __builtin_amdgcn_exp2f((ml[2 * (c0 + lane)] - m) * to_log2);
             l += ml[2 * (c0 + lane) + 1] * w;
         }
         const int nc = min(ranges - c0, 64u);
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
         const int d = lane + 64 * y;
         if (d < dim) a.O[(long)n * a.o_t + ((long)h * dim + d) * a.o_f] = l == 0.0f ? 0.0f : o[y] / l;
     }
-    if (lane == 0 && a.m) a.m[at] = m;
+    if (lane == 0 && a.m) a.m[at] = is_wide && m != kLowest ? m * kLn2 : m;
     if (lane == 0 && a.l) a.l[at] = l;
 }
 

@@ -41,17 +41,21 @@ typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPos = 32;      // positions of a tile
 constexpr int kNone = -200;   // exponent of nothing but zeros: below every float's
-__device__ __forceinline__ int ref_of(int e) { return e == kNone ? 0 : e; }
 
-// Two parts of eight floats that are scaled already.
+// Two parts of eight floats that are scaled already. What rounding leaves of a pair, x - f16(x), is exact: the pair's dot
+// product with (-1, 0) or (0, -1) added to x, one instruction each.
 __device__ __forceinline__ void split2(const floatx8& x, half8& h, half8& l)
 {
+    unsigned c0 = 0x0000bc00u, c1 = 0xbc000000u;
+    asm("" : "+s"(c0));
+    asm("" : "+s"(c1));
+    const half2_t e0 = __builtin_bit_cast(half2_t, c0), e1 = __builtin_bit_cast(half2_t, c1);
     uintx4 hv, lv;
 #pragma unroll
     for (int p = 0; p < 4; ++p)
     {
         const half2_t a = __builtin_convertvector((floatx2){x[2 * p], x[2 * p + 1]}, half2_t);
-        const floatx2 left = {__builtin_fmaf((float)a[0], -1.0f, x[2 * p]), __builtin_fmaf((float)a[1], -1.0f, x[2 * p + 1])};
+        const floatx2 left = {__builtin_amdgcn_fdot2(a, e0, x[2 * p], false), __builtin_amdgcn_fdot2(a, e1, x[2 * p + 1], false)};
         hv[p] = __builtin_bit_cast(unsigned, a);
         lv[p] = __builtin_bit_cast(unsigned, __builtin_convertvector(left, half2_t));
     }
@@ -64,7 +68,39 @@ __device__ __forceinline__ unsigned halves_of(unsigned two)
     const half2_t z = __builtin_bit_cast(half2_t, two ^ 0x64806480u) - (half2_t){(_Float16)1152, (_Float16)1152};
     return __builtin_bit_cast(unsigned, z);
 }
-__device__ __forceinline__ int exponent_of(float x) { return __builtin_amdgcn_frexp_expf(x); }   // x < 2^e
+// e with |x| < 2^e, and 2^(e - 1) <= |x| but for denormals. What is not finite has 129.
+__device__ __forceinline__ int exponent_of(float x) { return (int)max(__builtin_bit_cast(unsigned, x) >> 23 & 255u, 1u) - 126; }
+
+// The largest of N neighbouring lanes' numbers, none negative, in all of them: without LDS, which the shuffles take.
+template <int CTRL> __device__ __forceinline__ float max_dpp(float x)
+{
+    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 15, 15, true)));
+}
+template <int N> __device__ __forceinline__ float max_of(float x)
+{
+    x = max_dpp<0xb1>(x);                           // lanes 1, 0, 3, 2 of each 4
+    x = max_dpp<0x4e>(x);                           // 2, 3, 0, 1
+    if constexpr (N >= 8) x = max_dpp<0x141>(x);    // each 8 mirrored
+    if constexpr (N >= 16) x = max_dpp<0x140>(x);   // each 16 mirrored
+    if constexpr (N >= 32)
+    {
+        const int a = __builtin_bit_cast(int, x);   // 4 rows of 16 lanes, as whole numbers in the order of the floats
+        const int lo = max(__builtin_amdgcn_readlane(a, 0), __builtin_amdgcn_readlane(a, 16));
+        const int hi = max(__builtin_amdgcn_readlane(a, 32), __builtin_amdgcn_readlane(a, 48));
+        if constexpr (N == 64) x = __builtin_bit_cast(float, max(lo, hi));
+        else x = __builtin_bit_cast(float, (threadIdx.x & 32) ? hi : lo);
+    }
+    return x;
+}
+// Both halves of the wave: f of the lane's value and that of lane l ^ 32.
+template <class F> __device__ __forceinline__ float across(float x, F&& f)
+{
+    unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+    asm("" : "+v"(b));   // of one value twice the compiler takes both results to be the same
+    const auto z = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    const unsigned lo = z[0], hi = z[1];
+    return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
 __device__ __forceinline__ floatx16 mfma32(const half8& x, const half8& y, const floatx16& c)
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
@@ -76,10 +112,9 @@ template <int BITS, int KS> struct WideShared
     // Operands by lane: [buffer][step or block of 32 dims and k step][part][lane's place]
     half8 k[2][KS][P][64];
     half8 v[2][KS / 2][2][P][64];
-    float k_scale[2][kPos];        // of the scores: relative to k_ref
+    float k_scale[2][kPos];        // of the scores
     float v_scale[2][kPos];        // BITS 8: of the values
     int v_top[2][4];               // exponents of the values: of each group of 8 positions; BITS 8: all [0]
-    int k_ref;                     // exponent of the first tile's largest key
 };
 
 // What a thread holds of a tile on its way to LDS. Keys: 8 dims of one position each; values: VD dims of the 8 positions of
@@ -115,8 +150,18 @@ template <int BITS, int KS> struct Wide
     // Position e of the wave's group of values.
     __device__ __forceinline__ int value_pos(int e) const { return 8 * (2 * (wave >> 1) + e / 4) + 4 * (wave & 1) + e % 4; }
 
-    // row: of position lane % 32, -1 where there is none.
-    __device__ __forceinline__ void load(int row, R& r) const
+    // row: of position lane % 32, -1 where there is none. key_rows: those of the thread's pieces.
+    __device__ __forceinline__ void key_rows(int row, int (&kr)[R::KI]) const
+    {
+#pragma unroll
+        for (int i = 0; i < R::KI; ++i)
+        {
+            int p, d;
+            piece(i, p, d);
+            kr[i] = max(__shfl(row, p & 31, 64), 0);
+        }
+    }
+    __device__ __forceinline__ void load(int row, const int (&kr)[R::KI], R& r) const
     {
         const int dim = a.c.t.dim;
         const bool vec = a.vec;
@@ -125,8 +170,7 @@ template <int BITS, int KS> struct Wide
         {
             int p, d;
             piece(i, p, d);
-            const int kr = max(__shfl(row, p & 31, 64), 0);
-            const size_t at = (size_t)kr * a.c.t.row + (size_t)part.h * dim;
+            const size_t at = (size_t)kr[i] * a.c.t.row + (size_t)part.h * dim;
             if constexpr (BITS == 32)
             {
                 const float* from = a.c.t.K + at;
@@ -200,10 +244,10 @@ template <int BITS, int KS> struct Wide
     }
 
     // The tile's parts into buffer b; there: which of its positions exist. Absent ones, and dims past the last, are 0.
-    // first: k_ref is formed, and the keys' scales are left to a second step.
-    __device__ __forceinline__ void stage(const R& r, int b, unsigned there, bool first)
+    __device__ __forceinline__ void stage(const R& r, int b, unsigned there)
     {
         const int dim = a.c.t.dim;
+        const bool whole = there == 0xffffffffu && dim == 16 * KS;
 #pragma unroll
         for (int i = 0; i < R::KI; ++i)
         {
@@ -214,15 +258,18 @@ template <int BITS, int KS> struct Wide
             if constexpr (BITS == 32)
             {
                 floatx8 z;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = r.k[i][e];
+                if (!whole)
+                {
+                    asm volatile("");   // stays a branch
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = ok && d + e < dim ? z[e] : 0.0f;
+                }
                 float top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    z[e] = ok && d + e < dim ? r.k[i][e] : 0.0f;
-                    top = fmaxf(top, fabsf(z[e]));
-                }
-#pragma unroll
-                for (int o = 1; o < R::CP; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(z[e]));
+                top = max_of<R::CP>(top);
                 const int ke = top > 0.0f ? exponent_of(top) : kNone;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) z[e] = __builtin_ldexpf(z[e], 15 - ke);
@@ -232,15 +279,7 @@ template <int BITS, int KS> struct Wide
                 {
                     sh.k[b][step][0][place] = hi;
                     sh.k[b][step][P - 1][place] = lo;
-                    if (d == 0)
-                    {
-                        if (first)
-                        {
-                            sh.k_scale[b][p] = __builtin_bit_cast(float, ke);
-                            atomicMax(&sh.k_ref, ke);
-                        }
-                        else sh.k_scale[b][p] = __builtin_ldexpf(1.0f, ke - ref_of(sh.k_ref));
-                    }
+                    if (d == 0) sh.k_scale[b][p] = __builtin_ldexpf(1.0f, ke - 20);
                 }
             }
             else
@@ -272,12 +311,20 @@ template <int BITS, int KS> struct Wide
 #pragma unroll
                 for (int y = 0; y < R::VD; ++y)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                    {
-                        z[y][e] = (ok >> e & 1) && d0 + y < dim ? r.v[e][y] : 0.0f;
-                        top = fmaxf(top, fabsf(z[y][e]));
-                    }
-                for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+                    for (int e = 0; e < 8; ++e) z[y][e] = r.v[e][y];
+                if (!whole)
+                {
+                    asm volatile("");
+#pragma unroll
+                    for (int y = 0; y < R::VD; ++y)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) z[y][e] = (ok >> e & 1) && d0 + y < dim ? z[y][e] : 0.0f;
+                }
+#pragma unroll
+                for (int y = 0; y < R::VD; ++y)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(z[y][e]));
+                top = max_of<64>(top);
                 ve = top > 0.0f ? exponent_of(top) : kNone;
             }
 #pragma unroll
@@ -317,15 +364,9 @@ template <int BITS, int KS> struct Wide
             {
                 const bool ok = there >> (lane & 31) & 1;
                 const float s = ok ? r.scale : 0.0f;
-                float top = fabsf(s) <= kMaxF ? fabsf(s) : 0.0f;
-#pragma unroll
-                for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+                const float top = max_of<32>(fabsf(s) <= kMaxF ? fabsf(s) : 0.0f);
                 const int e = top > 0.0f ? exponent_of(top) : kNone;   // of the keys' scales, of the values'
-                if (lane < 32)
-                {
-                    if (first && lane == 0) sh.k_ref = e;
-                    sh.k_scale[b][lane] = __builtin_ldexpf(s, -ref_of(first ? e : sh.k_ref));
-                }
+                if (lane < 32) sh.k_scale[b][lane] = s * 0x1p-5f;
                 else
                 {
                     sh.v_scale[b][lane - 32] = s;
@@ -389,10 +430,12 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     };
     auto mask_of = [](int r) { return (unsigned)__builtin_amdgcn_ballot_w64(r >= 0); };
     float ahead = entry(begin + kPos);
-    int at = row_at(entry(begin), begin);
+    int at = row_at(entry(begin), begin), kr[W::R::KI];
     unsigned there = mask_of(at);   // of the tile in `raw`
-    w.load(at, raw);
+    w.key_rows(at, kr);
+    w.load(at, kr, raw);
     at = row_at(ahead, begin + kPos);
+    w.key_rows(at, kr);
     ahead = entry(begin + 2 * kPos);
 
     // The queries' parts: row l % 32, dims 16 k + 8 (l / 32) + e.
@@ -423,8 +466,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
                 top = fmaxf(top, fabsf(z[k][e]));
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        qe = exponent_of(top);
+        qe = exponent_of(across(top, [](float x, float y) { return fmaxf(x, y); }));
 #pragma unroll
         for (int k = 0; k < KS; ++k)
         {
@@ -434,24 +476,17 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         }
     }
 
-    if (t == 0) sh.k_ref = kNone;
-    __syncthreads();
-    w.stage(raw, 0, there, true);
+    w.stage(raw, 0, there);
     const unsigned there0 = there;
     there = mask_of(at);
-    w.load(at, raw);
+    w.load(at, kr, raw);
     at = row_at(ahead, begin + 2 * kPos);
+    w.key_rows(at, kr);
     ahead = entry(begin + 3 * kPos);
     __syncthreads();
-    const int ref = ref_of(sh.k_ref);
-    if constexpr (BITS == 32)
-    {
-        if (t < kPos) sh.k_scale[0][t] = __builtin_ldexpf(1.0f, __builtin_bit_cast(int, sh.k_scale[0][t]) - ref);
-        __syncthreads();
-    }
     unsigned now = there0;          // the positions of the tile whose parts are used
     const float slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
-    const float scale = __builtin_ldexpf(a.alpha * kLog2e, ref + qe - (BITS == 32 ? 30 : 15));   // scores times log2(e)
+    const float scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);   // scores times log2(e)
     float m = kLowest, l = 0.0f;
     int top = kNone;                // exponent that the values are held against
     floatx16 o[NB];
@@ -468,10 +503,11 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         if (i + 1 < tiles)
         {
             next = there;
-            w.stage(raw, buf ^ 1, there, false);
+            w.stage(raw, buf ^ 1, there);
             there = mask_of(at);
-            w.load(at, raw);
+            w.load(at, kr, raw);
             at = row_at(ahead, p0 + 3 * kPos);
+            w.key_rows(at, kr);
             ahead = entry(p0 + 4 * kPos);
         }
         if (p0 < most)
@@ -516,7 +552,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             float high = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
-            high = fmaxf(high, __shfl_xor(high, 32, 64));
+            high = across(high, [](float x, float y) { return fmaxf(x, y); });
             const float mn = fmaxf(m, high);
             float f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -588,8 +624,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         __syncthreads();
     }
 
-    l += __shfl_xor(l, 32, 64);
-    m = m == kLowest ? m : m * (1.0f / kLog2e);
+    l = across(l, [](float x, float y) { return x + y; });
     const int unscale = top - (BITS == 32 ? 30 : 15);
     bool bad = false;
 #pragma unroll
@@ -605,7 +640,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         bad = live && (bad || !(l <= kMaxF));
         if (__syncthreads_or(bad))
         {
-            walk<32, KS, false, 2>(a, part, 4, *reinterpret_cast<WalkShared<KS>*>(lds));
+            walk<32, KS, false, 2, true>(a, part, 4, *reinterpret_cast<WalkShared<KS>*>(lds));
             return;
         }
     }
@@ -614,7 +649,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            put(a, part, row, 32 * b + 8 * q + 4 * g, f32x4{o[b][4 * q], o[b][4 * q + 1], o[b][4 * q + 2], o[b][4 * q + 3]}, m, l,
+            put<true, true>(a, part, row, 32 * b + 8 * q + 4 * g, f32x4{o[b][4 * q], o[b][4 * q + 1], o[b][4 * q + 2], o[b][4 * q + 3]}, m, l,
                 b == 0 && q == 0 && g == 0);
 }
 
