@@ -28,7 +28,7 @@ struct ChunkArgs
     FastDiv by_per, by_heads, by_row_blocks, by_ranges;   // by_row_blocks: 8 of them
     int q_rows;                      // queries lie a token a row, 16-byte aligned
     int vec;                         // the cache's rows can be read in pieces of 4 values
-    int row_waves;
+    int page4;                       // pages have a multiple of 4 rows
     float alpha;
 };
 
@@ -303,7 +303,7 @@ template <int KS> struct WalkShared
 };
 
 // Where a row's results go: m, l and values d .. d + 3 of O, unnormalised. LOG2: m is a score times log2(e). The results of
-// k_attn_chunk_wide's ranges (WIDE) are joined so: a score's product with log2(e) is rounded once, before the ranges part.
+// ranges that others form so (WIDE) are joined so: a score's product with log2(e) is rounded once, before the ranges part.
 template <bool WIDE, bool LOG2>
 __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int row, int d, f32x4 o, float m, float l, bool stats)
 {
@@ -476,13 +476,13 @@ __device__ __forceinline__ void walk(const ChunkArgs& a, const Part& part, int r
 
 // The positions of range `slot` of `ranges` for rows up to `last`: whole steps of `step` positions; empty ones are marked
 // for the join and give false.
-template <int STEP> __device__ __forceinline__ bool cut_range(const ChunkArgs& a, Part& part, int rows_here)
+__device__ __forceinline__ bool cut_range(const ChunkArgs& a, Part& part, int rows_here, int step)
 {
     const int last = min((int)part.first + rows_here, part.n_rows) - 1;
     const int hi = max(part.chunk.seen + (int)a.by_per.div(last), 0);
-    const int steps = (hi + STEP - 1) / STEP;
-    part.begin = (int)((long)steps * part.slot / a.ranges) * STEP;
-    part.end = min(hi, (int)((long)steps * (part.slot + 1) / a.ranges) * STEP);
+    const int steps = (hi + step - 1) / step;
+    part.begin = (int)((long)steps * part.slot / a.ranges) * step;
+    part.end = min(hi, (int)((long)steps * (part.slot + 1) / a.ranges) * step);
     if (part.begin < part.end || a.ranges == 1) return true;
     for (int row = part.first + threadIdx.x; row <= last; row += blockDim.x)
     {
@@ -494,7 +494,24 @@ template <int STEP> __device__ __forceinline__ bool cut_range(const ChunkArgs& a
     return false;
 }
 
-// k_attn_chunk_wide: rows of a workgroup, and its launch.
+// A workgroup of the kernels of few rows: all rows of a sequence and key head, one range of positions in steps of `step`.
+// False: nothing is left to do.
+__device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int step)
+{
+    // Ranges of a piece run on the XCDs in turn.
+    const unsigned next = a.by_ranges.div(blockIdx.x);
+    part.slot = blockIdx.x - next * a.ranges;
+    part.b = a.by_heads.div(next);
+    part.h = next - part.b * a.c.t.heads;
+    if (part.b >= a.c.t.batch) return false;
+    part.chunk = chunk_of(a, part.b);
+    part.n_rows = part.chunk.n * a.by_per.d;
+    part.first = 0;
+    return part.n_rows > 0 && part.n_rows <= a.wide_from && cut_range(a, part, part.n_rows, step);
+}
+
+// k_attn_chunk8, and k_attn_chunk_wide: their launches; rows of a workgroup.
+void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s);
 constexpr int kWideRows = 128;
 void chunk_wide(const ChunkArgs& a, int bits, unsigned blocks, hipStream_t s);
 

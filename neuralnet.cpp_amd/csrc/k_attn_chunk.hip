@@ -17,26 +17,15 @@ namespace nnhip
 namespace
 {
 
-template <int BITS, int KS, bool VEC, int RT> __global__ __launch_bounds__(256, VEC ? 2 : 1) void k_attn_chunk(ChunkArgs a)
+// Sequences of up to kNarrowRows rows.
+template <int BITS, int KS, bool VEC> __global__ __launch_bounds__(256, VEC ? 2 : 1) void k_attn_chunk(ChunkArgs a)
 {
     __shared__ WalkShared<KS> sh;
     Part part;
-    // The blocks of rows that read the same keys and values run on one XCD (workgroups go to the 8 in turn), so that its
-    // L2 holds them once; the pieces are padded to a multiple of 8.
-    unsigned i = blockIdx.x;
-    const unsigned eight = a.by_row_blocks.div(i), block = (i - eight * a.by_row_blocks.d) / 8;
-    i = eight * 8 + i % 8;
-    unsigned next = a.by_ranges.div(i);
-    part.slot = i - next * a.ranges;
-    part.b = a.by_heads.div(next);
-    part.h = next - part.b * a.c.t.heads;
-    if (part.b >= a.c.t.batch) return;
-    part.chunk = chunk_of(a, part.b);
-    part.n_rows = part.chunk.n * a.by_per.d;
-    const int rows_here = kTile * RT * a.row_waves;
-    part.first = block * rows_here;
-    if (part.n_rows > a.wide_from || (int)part.first >= part.n_rows || !cut_range<4 * kTile>(a, part, rows_here)) return;
-    walk<BITS, KS, VEC, RT, false>(a, part, a.row_waves, sh);
+    if (!narrow_part(a, part, 4 * kTile)) return;
+    // Ranges of an 8-bit cache are joined in the order of k_attn_chunk8.
+    if (part.n_rows <= kTile) walk<BITS, KS, VEC, 1, BITS == 8>(a, part, 1, sh);
+    else walk<BITS, KS, VEC, 2, BITS == 8>(a, part, 1, sh);
 }
 
 // In place of the factor of a range of l = 0, whose O is anything. A factor that underflows to 0 is one: a value of its
@@ -54,9 +43,9 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
     if (b < 0) return;
     const Chunk c = chunk_of(a, b);
     if (n >= c.first + c.n) return;   // no sequence's
-    const bool is_wide = c.n * (int)a.by_per.d > a.wide_from;   // m is a score times log2(e)
+    const bool is_wide = c.n * (int)a.by_per.d > a.wide_from, log2 = is_wide || a.c.K;   // m is a score times log2(e)
     const unsigned ranges = is_wide ? wide : narrow;
-    const float to_log2 = is_wide ? 1.0f : kLog2e;
+    const float to_log2 = log2 ? 1.0f : kLog2e;
     if (ranges == 1) return;   // written already
     const float* ml = a.part_ml + 2 * (size_t)at * a.slots;
     const float* po = a.part_o + (size_t)at * a.slots * dim;
@@ -91,7 +80,7 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
         const int d = lane + 64 * y;
         if (d < dim) a.O[(long)n * a.o_t + ((long)h * dim + d) * a.o_f] = l == 0.0f ? 0.0f : o[y] / l;
     }
-    if (lane == 0 && a.m) a.m[at] = is_wide && m != kLowest ? m * kLn2 : m;
+    if (lane == 0 && a.m) a.m[at] = log2 && m != kLowest ? m * kLn2 : m;
     if (lane == 0 && a.l) a.l[at] = l;
 }
 
@@ -101,13 +90,14 @@ struct ChunkCall
     Pages8 c;
     int bits;
     bool vec;          // rows can be read in pieces of 4 values
+    bool wide_bytes;   // and 16 bytes
     size_t q_heads, tokens, most;
 };
 
 struct ChunkPlan
 {
-    int row_tiles, row_waves, wide_from;
-    unsigned row_blocks, narrow, wide;   // ranges of the two kernels' rows, 0: it is not launched
+    int wide_from;
+    unsigned narrow, wide;   // ranges of the two kernels' rows, 0: it is not launched
     size_t blocks, wide_row_blocks, wide_blocks;
     unsigned slots() const { return std::max(narrow, wide); }
 };
@@ -120,14 +110,10 @@ ChunkPlan chunk_plan(const ChunkCall& c)
     ChunkPlan p{};
     const size_t per = c.q_heads / c.c.t.heads, batch = c.c.t.batch, heads = c.c.t.heads;
     const size_t positions = (size_t)c.c.t.width * c.c.t.page.d, cus = device_cus();
-    const size_t rows = std::min(c.most * per, kNarrowRows);
     p.wide_from = kNarrowRows;
-    p.row_tiles = rows > kTile ? 2 : 1;
-    p.row_waves = 1;
-    p.row_blocks = 1;
     const size_t want = (4 * cus + batch * heads - 1) / (batch * heads), most_ranges = (positions + 63) / 64;
     p.narrow = static_cast<unsigned>(std::min<size_t>(std::min(want, most_ranges), 256));
-    p.blocks = (batch * heads * p.narrow + 7) / 8 * 8;
+    p.blocks = batch * heads * p.narrow;
     if (c.most * per > kNarrowRows)
     {
         p.wide_row_blocks = c.tokens * per / kWideRows + batch;
@@ -154,32 +140,28 @@ bool chunk_ok(const ChunkCall& c, size_t heads)
 bool chunk_call(const nnhip_kv_pages* c, size_t q_heads, size_t tokens, size_t most, ChunkCall& out)
 {
     if (!pages_ok(c, kChunkMaxDim)) return false;
-    out = {Pages8{pages_of(*c), nullptr, nullptr, nullptr, nullptr}, 32, c->dim % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V),
+    out = {Pages8{pages_of(*c), nullptr, nullptr, nullptr, nullptr}, 32, c->dim % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V), false,
            q_heads, tokens, most};
     return chunk_ok(out, c->heads);
 }
 bool chunk_call(const nnhip_kv8_pages* c, size_t q_heads, size_t tokens, size_t most, ChunkCall& out)
 {
     if (!pages8_ok(c, kChunkMaxDim)) return false;
-    out = {pages8_of(*c), 8, c->dim % 4 == 0 && c->row % 4 == 0 && ((reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V)) & 3) == 0,
+    const uintptr_t at = reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V);
+    out = {pages8_of(*c), 8, c->dim % 4 == 0 && c->row % 4 == 0 && (at & 3) == 0, c->dim % 16 == 0 && c->row % 16 == 0 && (at & 15) == 0,
            q_heads, tokens, most};
     return chunk_ok(out, c->heads);
 }
 
-template <int BITS, int KS, bool VEC> void chunk_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s)
-{
-    const dim3 grid(static_cast<unsigned>(p.blocks));
-    if (p.row_tiles == 1) hipLaunchKernelGGL((k_attn_chunk<BITS, KS, VEC, 1>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_chunk<BITS, KS, VEC, 2>), grid, dim3(256), 0, s, a);
-}
 template <int BITS, bool VEC> void chunk_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s)
 {
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.blocks)), dim3(256), 0, s, a); };
     switch ((a.c.t.dim + 31) / 32)
     {
-    case 1: chunk_launch<BITS, 2, VEC>(a, p, s); break;
-    case 2: chunk_launch<BITS, 4, VEC>(a, p, s); break;
-    case 3: chunk_launch<BITS, 6, VEC>(a, p, s); break;
-    default: chunk_launch<BITS, 8, VEC>(a, p, s); break;
+    case 1: go(k_attn_chunk<BITS, 2, VEC>); break;
+    case 2: go(k_attn_chunk<BITS, 4, VEC>); break;
+    case 3: go(k_attn_chunk<BITS, 6, VEC>); break;
+    default: go(k_attn_chunk<BITS, 8, VEC>); break;
     }
 }
 
@@ -224,17 +206,17 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     a.wide_from = p.wide_from;
     a.by_per = FastDiv(static_cast<unsigned>(q_heads / c->heads));
     a.by_heads = FastDiv(call.c.t.heads);
-    a.by_row_blocks = FastDiv(8 * p.row_blocks);
     a.by_ranges = FastDiv(std::max(p.narrow, 1u));
     a.q_rows = q_f == 1 && q_t % 4 == 0 && aligned16(q) && c->dim % 4 == 0;
-    a.row_waves = p.row_waves;
+    a.page4 = c->page % 4 == 0;
     a.vec = call.vec;
     a.alpha = alpha;
     auto s = static_cast<hipStream_t>(stream);
     if (p.narrow)
     {
         if (call.bits == 32) call.vec ? chunk_launch<32, true>(a, p, s) : chunk_launch<32, false>(a, p, s);
-        else call.vec ? chunk_launch<8, true>(a, p, s) : chunk_launch<8, false>(a, p, s);
+        else if (call.wide_bytes) chunk8(a, static_cast<unsigned>(p.blocks), s);
+        else chunk_launch<8, false>(a, p, s);
         if (int rc = launch_status()) return rc;
     }
     if (p.wide)

@@ -1,0 +1,380 @@
+// k_attn_chunk8.hip — chunk attention of sequences with few rows over an 8-bit
+// cache (single tokens above all), bound by the cache's bytes.
+//
+// As in the float32 walk (attn_chunk.hpp) a wave forms both products transposed
+// and a workgroup's four waves take 32 positions each in turn, but on the
+// float16 matrix cores (16 x 16 x 32): bytes are float16 as they are, so that
+// queries and weights in two parts (f16_parts.hpp) make float32's accuracy of
+// two products, eight times faster than the float32 cores'. With their single
+// products a key head's 16 positions would take 2048 cycles, which 5 TB/s of
+// bytes do not leave.
+//
+// Lane l = 16 g + j has the scores of row j and of the positions 16 u + 4 g + r
+// (u < 2, r < 4), which stand behind the k index 8 g + 4 u + r of the second
+// product. Block b of the output's dims are those that leave the remainder b by
+// VB, so that the lane's VB neighbouring bytes of a value row serve one block
+// each.
+#include "attn_chunk.hpp"
+#include "f16_parts.hpp"
+
+namespace nnhip
+{
+namespace
+{
+
+constexpr int kPos = 32;   // positions of a tile
+
+__device__ __forceinline__ f32x4 mfma16(const half8& x, const half8& y, const f32x4& c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+}
+
+// KS: groups of 16 dims, even. VB: value bytes of a lane and position, and blocks of dims; up to 16 VB dims.
+template <int KS> struct Bytes
+{
+    static constexpr int VB = KS <= 2 ? 2 : KS <= 4 ? 4 : 8, VW = (VB + 3) / 4, steps = KS / 2;
+    // Keys are loaded 16 bytes at a time where whole pairs of steps let them: bytes 0 to 7 are the first step's.
+    static constexpr bool WIDE = KS % 4 == 0;
+    static __device__ __forceinline__ int dim_of(int step, int g) { return WIDE ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 32 * step + 8 * g; }
+};
+
+template <int KS> struct Row8
+{
+    half8 q[KS / 2][2];
+    int seen;
+    float slope, scale, m, l;   // slope, scale and m: times log2(e)
+    f32x4 o[Bytes<KS>::VB];
+};
+
+template <int KS> struct Shared8
+{
+    using B = Bytes<KS>;
+    union
+    {
+        float scales[4][2][kPos];   // by wave: the keys', the values'
+        float o[4][kTile][16 * B::VB + 4];
+    };
+    float ml[4][kTile][2];
+};
+
+// One tile's bytes on their way.
+template <int KS> struct Tile8
+{
+    using B = Bytes<KS>;
+    unsigned k[2][B::steps][2], v[8][B::VW];
+    float scale;   // lane p < 32: position p's of the keys; lane 32 + p: of the values
+};
+
+template <int KS> __device__ __forceinline__ void load_keys8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS>& x)
+{
+    using B = Bytes<KS>;
+    const int j = lane & 15, g = lane >> 4, dim = a.c.t.dim;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+    {
+        const signed char* from = a.c.K + (size_t)max(__shfl(row, 16 * u + j, 64), 0) * a.c.t.row + (size_t)h * dim;
+#pragma unroll
+        for (int s = 0; s < B::steps; s += B::WIDE ? 2 : 1)
+        {
+            const int d = B::dim_of(s, g);
+            const signed char* at = from + (d < dim ? d : 0);
+            if constexpr (B::WIDE)
+            {
+                const uintx4 z = *reinterpret_cast<const uintx4*>(at);
+                x.k[u][s][0] = z[0];
+                x.k[u][s][1] = z[1];
+                x.k[u][s + 1][0] = z[2];
+                x.k[u][s + 1][1] = z[3];
+            }
+            else
+            {
+                const uint2 z = *reinterpret_cast<const uint2*>(at);
+                x.k[u][s][0] = z.x;
+                x.k[u][s][1] = z.y;
+            }
+        }
+    }
+    const float z = (lane < 32 ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
+    x.scale = row >= 0 ? z : 0.0f;
+}
+template <int KS> __device__ __forceinline__ void load_values8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS>& x)
+{
+    using B = Bytes<KS>;
+    const int j = lane & 15, g = lane >> 4, dim = a.c.t.dim, d = B::VB * j;
+    auto load = [&](int e, size_t r) {
+        const signed char* at = a.c.V + r * a.c.t.row + (size_t)h * dim + (d < dim ? d : 0);
+        if constexpr (B::VB == 8)
+        {
+            const uint2 z = *reinterpret_cast<const uint2*>(at);
+            x.v[e][0] = z.x;
+            x.v[e][B::VW - 1] = z.y;
+        }
+        else if constexpr (B::VB == 4) x.v[e][0] = *reinterpret_cast<const unsigned*>(at);
+        else x.v[e][0] = *reinterpret_cast<const unsigned short*>(at);
+    };
+    if (a.page4)   // four neighbouring positions lie in neighbouring rows
+    {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+        {
+            const int r = __shfl(row, 16 * u + 4 * g, 64);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) load(4 * u + e, r < 0 ? 0 : (size_t)r + e);
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) load(e, max(__shfl(row, 16 * (e / 4) + 4 * g + e % 4, 64), 0));
+    }
+}
+
+// 8 bytes as float16, in the order of the bytes.
+__device__ __forceinline__ half8 halves8(unsigned lo, unsigned hi)
+{
+    uintx4 z;
+    z[0] = halves_of(__builtin_amdgcn_perm(0u, lo, 0x0c010c00u));
+    z[1] = halves_of(__builtin_amdgcn_perm(0u, lo, 0x0c030c02u));
+    z[2] = halves_of(__builtin_amdgcn_perm(0u, hi, 0x0c010c00u));
+    z[3] = halves_of(__builtin_amdgcn_perm(0u, hi, 0x0c030c02u));
+    return __builtin_bit_cast(half8, z);
+}
+
+template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs& a, const Part& part, Shared8<KS>& sh)
+{
+    using B = Bytes<KS>;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 15, g = lane >> 4;
+    const int dim = a.c.t.dim, begin = part.begin, end = part.end, step = 4 * kPos;
+    Row8<KS> rows[RT];
+    int all = 0x7fffffff;
+    const int p1 = begin + wave * kPos;
+    // Lane p and lane 32 + p: the table's entry and the row of position p of a tile.
+    auto entry = [&](int p) { return a.c.t.entry_of(part.b, p + (lane & 31)); };
+    auto row_at = [&](float e, int p) {
+        const int r = a.c.t.row_in(e, p + (lane & 31));
+        return p + (lane & 31) < end ? r : -1;
+    };
+    Tile8<KS> x;
+    float ahead = entry(p1 + step);
+    int row = row_at(entry(p1), p1);
+    unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
+    load_keys8<KS>(a, row, part.h, lane, x);
+    load_values8<KS>(a, row, part.h, lane, x);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        Row8<KS>& w = rows[i];
+        const int r = part.first + i * kTile + j;
+        const bool live = r < part.n_rows;
+        const unsigned n = live ? a.by_per.div(r) : 0, qh = part.h * a.by_per.d + (live ? r - n * a.by_per.d : 0);
+        w.seen = live ? max(part.chunk.seen + (int)n, 0) : 0;
+        all = min(all, live ? w.seen : 0x7fffffff);
+        const float* from = a.q + (long)(part.chunk.first + n) * a.q_t + (long)qh * dim * a.q_f;   // rows that are none are formed and dropped
+        floatx8 z[B::steps];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < B::steps; ++s)
+        {
+            const int d = B::dim_of(s, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[s][e] = from[(long)(d + e < dim ? d + e : 0) * a.q_f];
+        }
+#pragma unroll
+        for (int s = 0; s < B::steps; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                z[s][e] = B::dim_of(s, g) + e < dim ? z[s][e] : 0.0f;   // dims past the last one
+                top = fmaxf(top, fabsf(z[s][e]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const int qe = exponent_of(top);
+#pragma unroll
+        for (int s = 0; s < B::steps; ++s)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[s][e] = __builtin_ldexpf(z[s][e], 15 - qe);
+            split2(z[s], w.q[s][0], w.q[s][1]);
+        }
+        w.slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
+        w.scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);
+        w.m = kLowest;
+        w.l = 0.0f;
+#pragma unroll
+        for (int b = 0; b < B::VB; ++b) w.o[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int o = 1; o < 16; o *= 2) all = min(all, __shfl_xor(all, o, 64));
+    all = __builtin_amdgcn_readfirstlane(all);
+    int top = kNone;   // exponent that the values' scales are held against
+    for (int p = p1; p < end; p += step)
+    {
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) s[i][0] = s[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // The scales, from a lane a position to a lane's positions, through LDS: the wave's own part of it.
+        (&sh.scales[wave][0][0])[lane] = lane < 32 ? x.scale * 0x1p-5f : x.scale;
+        const float vs_top = max_of<64>(lane >= 32 && fabsf(x.scale) <= kMaxF ? fabsf(x.scale) : 0.0f);
+#pragma unroll
+        for (int k = 0; k < B::steps; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+            {
+                const half8 z = halves8(x.k[u][k][0], x.k[u][k][1]);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) s[i][u] = mfma16(z, rows[i].q[k][1], s[i][u]);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) s[i][u] = mfma16(z, rows[i].q[k][0], s[i][u]);
+            }
+        f32x4 ks[2], vs[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+        {
+            ks[u] = *reinterpret_cast<const f32x4*>(&sh.scales[wave][0][16 * u + 4 * g]);
+            vs[u] = *reinterpret_cast<const f32x4*>(&sh.scales[wave][1][16 * u + 4 * g]);
+        }
+        const float further = entry(p + 2 * step);
+        row = row_at(ahead, p + step);
+        const unsigned now = there;
+        there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
+        load_keys8<KS>(a, row, part.h, lane, x);
+        __builtin_amdgcn_sched_barrier(0);
+
+        const bool odd = a.slopes || now != 0xffffffffu || p + kPos > all;
+        const int new_top = max(top, vs_top > 0.0f ? exponent_of(vs_top) : kNone);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vs[u][e] = __builtin_ldexpf(vs[u][e], 15 - new_top);
+        half8 pp[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+        {
+            Row8<KS>& w = rows[i];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
+            if (odd)
+            {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        const int q = 16 * u + 4 * g + e;
+                        const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q));
+                        s[i][u][e] = (now >> q & 1) && p + q < w.seen ? z : -__builtin_inff();
+                    }
+            }
+            float high = kLowest;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) high = fmaxf(high, s[i][u][e]);
+            high = fmaxf(high, __shfl_xor(high, 16, 64));
+            high = fmaxf(high, __shfl_xor(high, 32, 64));
+            const float mn = fmaxf(w.m, high);
+            float f = __builtin_amdgcn_exp2f(w.m - mn), sum = 0.0f;
+            w.m = mn;
+            floatx8 z;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    const float y = __builtin_amdgcn_exp2f(s[i][u][e] - mn);
+                    sum += y;
+                    z[4 * u + e] = y == 0.0f ? 0.0f : y * vs[u][e];   // a weight of 0 stays 0, whatever the scale is
+                }
+            w.l = w.l * f + sum;
+            f = __builtin_ldexpf(f, top - new_top);
+            if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
+            {
+#pragma unroll
+                for (int b = 0; b < B::VB; ++b) w.o[b] *= f;
+            }
+            split2(z, pp[i][0], pp[i][1]);
+        }
+        top = new_top;
+#pragma unroll
+        for (int b = 0; b < B::VB; ++b)
+        {
+            uintx4 z;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+            {
+                const unsigned pick = 0x0c040c00u + 0x00010001u * (b % 4);
+                z[e / 2] = halves_of(__builtin_amdgcn_perm(x.v[e + 1][b / 4], x.v[e][b / 4], pick));
+            }
+            const half8 y = __builtin_bit_cast(half8, z);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) rows[i].o[b] = mfma16(y, pp[i][1], rows[i].o[b]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) rows[i].o[b] = mfma16(y, pp[i][0], rows[i].o[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_values8<KS>(a, row, part.h, lane, x);
+        ahead = further;
+    }
+
+    // The waves joined in the order of their positions: 16 threads a row, 4 neighbouring values at a time.
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        Row8<KS>& w = rows[i];
+        w.l += __shfl_xor(w.l, 16, 64);
+        w.l += __shfl_xor(w.l, 32, 64);
+        __syncthreads();
+        if (g == 0)
+        {
+            sh.ml[wave][j][0] = w.m;
+            sh.ml[wave][j][1] = w.l;
+        }
+#pragma unroll
+        for (int b = 0; b < B::VB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], top - 15);
+        __syncthreads();
+        const int jr = t >> 4, r = part.first + i * kTile + jr;
+        if (r >= part.n_rows) continue;
+        float mm = kLowest, ll = 0.0f, f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mm = fmaxf(mm, sh.ml[k][jr][0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            f[k] = sh.ml[k][jr][1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sh.ml[k][jr][0] - mm);
+            ll += sh.ml[k][jr][1] * f[k];
+        }
+#pragma unroll
+        for (int d0 = 0; d0 < 16 * B::VB; d0 += 64)
+        {
+            const int d = d0 + 4 * (t & 15);
+            if (d >= 16 * B::VB) continue;
+            f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (sh.ml[k][jr][1] != 0.0f) z += *reinterpret_cast<const f32x4*>(&sh.o[k][jr][d]) * f[k];
+            put<true, true>(a, part, r, d, z, mm, ll, d == 0);
+        }
+    }
+}
+
+template <int KS> __global__ __launch_bounds__(256, 2) void k_attn_chunk8(ChunkArgs a)
+{
+    __shared__ Shared8<KS> sh;
+    Part part;
+    if (!narrow_part(a, part, 4 * kPos)) return;
+    if (part.n_rows <= kTile) walk8<KS, 1>(a, part, sh);
+    else walk8<KS, 2>(a, part, sh);
+}
+
+} // namespace
+
+void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s)
+{
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, s, a); };
+    const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
+    groups == 1 ? go(k_attn_chunk8<2>) : groups == 2 ? go(k_attn_chunk8<4>) : groups == 3 ? go(k_attn_chunk8<6>) : go(k_attn_chunk8<8>);
+}
+
+} // namespace nnhip
