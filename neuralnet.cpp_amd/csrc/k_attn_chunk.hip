@@ -17,71 +17,118 @@ namespace nnhip
 namespace
 {
 
-// Sequences of up to kNarrowRows rows.
-template <int BITS, int KS, bool VEC> __global__ __launch_bounds__(256, VEC ? 2 : 1) void k_attn_chunk(ChunkArgs a)
+// Sequences of up to 16 RT rows.
+template <int BITS, int KS, bool VEC, int RT> __global__ __launch_bounds__(256, VEC ? 2 : 1) void k_attn_chunk(ChunkArgs a)
 {
     __shared__ WalkShared<KS> sh;
     Part part;
     if (!narrow_part(a, part, 4 * kTile)) return;
     // Ranges of an 8-bit cache are joined in the order of k_attn_chunk8.
-    if (part.n_rows <= kTile) walk<BITS, KS, VEC, 1, BITS == 8>(a, part, 1, sh);
-    else walk<BITS, KS, VEC, 2, BITS == 8>(a, part, 1, sh);
+    if (RT == 1 || part.n_rows <= kTile) walk<BITS, KS, VEC, 1, BITS == 8>(a, part, 1, sh);
+    else walk<BITS, KS, VEC, RT, BITS == 8>(a, part, 1, sh);
 }
 
 // In place of the factor of a range of l = 0, whose O is anything. A factor that underflows to 0 is one: a value of its
 // range that is not finite makes O one that is not, as within a range.
 constexpr float kNoRange = -1.0f;
+constexpr size_t kMostRanges = 256;
 
-// Joins the ranges of a row in order: a wave a row. narrow, wide: the ranges of the rows of either kernel.
-__global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned narrow, unsigned wide)
+// The joins: narrow, wide: the ranges of the rows of either kernel. A row's ranges, 0 where it has nothing to join: written
+// already, or no sequence's token.
+struct Joined
+{
+    unsigned ranges;
+    bool log2;   // m is a score times log2(e)
+};
+__device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigned narrow, unsigned wide)
+{
+    const int b = last_of(a.c.t.batch, [&](unsigned i) { return length_of(a.start[i], a.tokens) <= (int)n; });
+    if (b < 0) return {0, false};
+    const Chunk c = chunk_of(a, b);
+    if (n >= c.first + c.n) return {0, false};
+    const bool is_wide = c.n * (int)a.by_per.d > a.wide_from;
+    const unsigned ranges = is_wide ? wide : narrow;
+    return {ranges == 1 ? 0 : ranges, is_wide || a.c.K};
+}
+
+// Up to kFewParts ranges: a wave a row, everything it needs on its way at once, the search for the token's sequence too.
+constexpr unsigned kFewParts = 16;
+__global__ __launch_bounds__(256) void k_attn_chunk_join_few(ChunkArgs a, unsigned narrow, unsigned wide)
 {
     const unsigned at = blockIdx.x * 4 + threadIdx.x / 64;
-    const unsigned n = at / a.q_heads, h = at - n * a.q_heads;
+    const unsigned n = a.by_q_heads.div(at), h = at - n * a.q_heads;
     if (n >= a.tokens) return;
     const int lane = threadIdx.x & 63, dim = a.c.t.dim;
-    const int b = last_of(a.c.t.batch, [&](unsigned i) { return length_of(a.start[i], a.tokens) <= (int)n; });
-    if (b < 0) return;
-    const Chunk c = chunk_of(a, b);
-    if (n >= c.first + c.n) return;   // no sequence's
-    const bool is_wide = c.n * (int)a.by_per.d > a.wide_from, log2 = is_wide || a.c.K;   // m is a score times log2(e)
-    const unsigned ranges = is_wide ? wide : narrow;
-    const float to_log2 = log2 ? 1.0f : kLog2e;
-    if (ranges == 1) return;   // written already
-    const float* ml = a.part_ml + 2 * (size_t)at * a.slots;
+    const float2 own = reinterpret_cast<const float2*>(a.part_ml)[(size_t)at * a.slots + min((unsigned)lane, a.slots - 1)];
     const float* po = a.part_o + (size_t)at * a.slots * dim;
-    float m = kLowest, l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (unsigned i = lane; i < ranges; i += 64)
-        if (ml[2 * i + 1] != 0.0f) m = fmax_std(m, ml[2 * i]);
-    m = wave_max(m);
-    for (unsigned c0 = 0; c0 < ranges; c0 += 64)
-    {
-        float w = kNoRange;
-        if (c0 + lane < ranges && ml[2 * (c0 + lane) + 1] != 0.0f)
-        {
-            w = __builtin_amdgcn_exp2f((ml[2 * (c0 + lane)] - m) * to_log2);
-            l += ml[2 * (c0 + lane) + 1] * w;
-        }
-        const int nc = min(ranges - c0, 64u);
-        for (int i = 0; i < nc; ++i)
-        {
-            const float f = __shfl(w, i, 64);
+    float x[kFewParts][2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-            {
-                const float x = po[(size_t)(c0 + i) * dim + min(lane + 64 * y, dim - 1)];
-                o[y] += f == kNoRange ? 0.0f : x * f;
-            }
-        }
+    for (unsigned i = 0; i < kFewParts; ++i)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) x[i][y] = po[(size_t)min(i, a.slots - 1) * dim + min(lane + 64 * y, dim - 1)];
+    const Joined r = joined(a, n, narrow, wide);
+    if (r.ranges == 0) return;
+    const bool any = lane < (int)r.ranges && own.y != 0.0f;
+    const float m = wave_max(any ? own.x : kLowest);
+    const float w = any ? __builtin_amdgcn_exp2f((own.x - m) * (r.log2 ? 1.0f : kLog2e)) : kNoRange;
+    const float l = wave_sum(any ? own.y * w : 0.0f);
+    float o[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (unsigned i = 0; i < kFewParts; ++i)
+    {
+        const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+#pragma unroll
+        for (int y = 0; y < 2; ++y) o[y] += f == kNoRange ? 0.0f : x[i][y] * f;
     }
-    l = wave_sum(l);
 #pragma unroll
     for (int y = 0; y < 2; ++y)
     {
         const int d = lane + 64 * y;
         if (d < dim) a.O[(long)n * a.o_t + ((long)h * dim + d) * a.o_f] = l == 0.0f ? 0.0f : o[y] / l;
     }
-    if (lane == 0 && a.m) a.m[at] = log2 && m != kLowest ? m * kLn2 : m;
+    if (lane == 0 && a.m) a.m[at] = r.log2 && m != kLowest ? m * kLn2 : m;
     if (lane == 0 && a.l) a.l[at] = l;
+}
+
+// More: a workgroup a row. The ranges' factors go to LDS, then 2 or 4 groups of threads sum every 2nd or 4th range.
+__global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned narrow, unsigned wide)
+{
+    static_assert(kMostRanges <= 256);
+    __shared__ float w_s[256], red[2][4], o_s[256];
+    const unsigned at = blockIdx.x, n = a.by_q_heads.div(at), h = at - n * a.q_heads;
+    const Joined r = joined(a, n, narrow, wide);
+    if (r.ranges == 0) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, dim = a.c.t.dim;
+    const int cols = dim <= 64 ? 64 : 128, groups = 256 / cols, d = t % cols, g = t / cols;
+    const float2 own = reinterpret_cast<const float2*>(a.part_ml)[(size_t)at * a.slots + min((unsigned)t, r.ranges - 1)];
+    const float* po = a.part_o + (size_t)at * a.slots * dim + (d < dim ? d : 0);
+    const bool any = t < (int)r.ranges && own.y != 0.0f;
+    float m = wave_max(any ? own.x : kLowest);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = fmax_std(fmax_std(red[0][0], red[0][1]), fmax_std(red[0][2], red[0][3]));
+    const float w = any ? __builtin_amdgcn_exp2f((own.x - m) * (r.log2 ? 1.0f : kLog2e)) : kNoRange;
+    float l = wave_sum(any ? own.y * w : 0.0f), o = 0.0f;
+    w_s[t] = w;
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = g; i < (int)r.ranges; i += groups)
+    {
+        const float x = po[(size_t)i * dim], f = w_s[i];
+        o += f == kNoRange ? 0.0f : x * f;
+    }
+    o_s[t] = o;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    if (t < dim)
+    {
+        o = 0.0f;
+        for (int i = 0; i < groups; ++i) o += o_s[i * cols + t];
+        a.O[(long)n * a.o_t + ((long)h * dim + t) * a.o_f] = l == 0.0f ? 0.0f : o / l;
+    }
+    if (t == 0 && a.m) a.m[at] = r.log2 && m != kLowest ? m * kLn2 : m;
+    if (t == 0 && a.l) a.l[at] = l;
 }
 
 // A call's sizes, whichever cache it is over.
@@ -110,15 +157,21 @@ ChunkPlan chunk_plan(const ChunkCall& c)
     ChunkPlan p{};
     const size_t per = c.q_heads / c.c.t.heads, batch = c.c.t.batch, heads = c.c.t.heads;
     const size_t positions = (size_t)c.c.t.width * c.c.t.page.d, cus = device_cus();
-    p.wide_from = kNarrowRows;
-    const size_t want = (4 * cus + batch * heads - 1) / (batch * heads), most_ranges = (positions + 63) / 64;
-    p.narrow = static_cast<unsigned>(std::min<size_t>(std::min(want, most_ranges), 256));
-    p.blocks = batch * heads * p.narrow;
+    // No sequence has more rows: those of up to 16 have a kernel that holds fewer registers.
+    p.wide_from = static_cast<int>(std::min(kNarrowRows, (c.most * per + kTile - 1) / kTile * kTile));
+    // Workgroups a CU. Where the key heads alone fill the CUs, float32 caches stream best with 8 (48 sequences of 4000 to 8000
+    // positions, 8 heads of 128: 466 us with 2, 440 with 4, 400 with 8), bytes with 4 (143 us with 2 to 8; 5 rows a head 192
+    // with 2, 188 with 4, 213 with 8); where they do not, ranges are more results to join (one sequence of 60000: 95 to 103
+    // us with 2 and 3, 107 with 8; in bytes 34 and 36, 50 with 8; 4 of 3000, 12 heads of 64: 22 and 20, 25 with 8).
+    const size_t pieces = batch * heads, per_cu = pieces < cus ? 3 : c.bits == 32 ? 8 : 4;
+    const size_t want = (per_cu * cus + pieces - 1) / pieces, most_ranges = (positions + 63) / 64;
+    p.narrow = static_cast<unsigned>(std::min<size_t>(std::min(want, most_ranges), kMostRanges));
+    p.blocks = (batch * p.narrow + 7) / 8 * 8 * heads;
     if (c.most * per > kNarrowRows)
     {
         p.wide_row_blocks = c.tokens * per / kWideRows + batch;
         const size_t others = heads * std::max<size_t>(c.tokens * per / kWideRows, 1), most_wide = (positions + 255) / 256;
-        p.wide = static_cast<unsigned>(std::min<size_t>(std::min(std::max<size_t>(2 * cus / others, 1), most_wide), 256));
+        p.wide = static_cast<unsigned>(std::min<size_t>(std::min(std::max<size_t>(2 * cus / others, 1), most_wide), kMostRanges));
         p.wide_blocks = (p.wide_row_blocks * heads * p.wide + 7) / 8 * 8;
         if (batch == 1) p.narrow = 0, p.wide_from = 0;   // one launch, however few tokens the sequence has
     }
@@ -153,16 +206,21 @@ bool chunk_call(const nnhip_kv8_pages* c, size_t q_heads, size_t tokens, size_t 
     return chunk_ok(out, c->heads);
 }
 
-template <int BITS, bool VEC> void chunk_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s)
+template <int BITS, bool VEC, int RT> void chunk_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.blocks)), dim3(256), 0, s, a); };
     switch ((a.c.t.dim + 31) / 32)
     {
-    case 1: go(k_attn_chunk<BITS, 2, VEC>); break;
-    case 2: go(k_attn_chunk<BITS, 4, VEC>); break;
-    case 3: go(k_attn_chunk<BITS, 6, VEC>); break;
-    default: go(k_attn_chunk<BITS, 8, VEC>); break;
+    case 1: go(k_attn_chunk<BITS, 2, VEC, RT>); break;
+    case 2: go(k_attn_chunk<BITS, 4, VEC, RT>); break;
+    case 3: go(k_attn_chunk<BITS, 6, VEC, RT>); break;
+    default: go(k_attn_chunk<BITS, 8, VEC, RT>); break;
     }
+}
+template <int BITS, bool VEC> void chunk_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s)
+{
+    if (a.wide_from <= kTile) chunk_launch<BITS, VEC, 1>(a, p, s);
+    else chunk_launch<BITS, VEC, 2>(a, p, s);
 }
 
 template <class C> size_t chunk_bytes(const C* c, size_t q_heads, size_t tokens, size_t most)
@@ -181,7 +239,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     const ChunkPlan p = chunk_plan(call);
     const size_t need = chunk_workspace(call, p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
-    if (p.blocks > kGridMost || p.wide_blocks > kGridMost || tokens * q_heads / 4 + 1 > kGridMost) return -1;
+    if (p.blocks > kGridMost || p.wide_blocks > kGridMost || (p.slots() > kFewParts ? tokens * q_heads : tokens * q_heads / 4 + 1) > kGridMost) return -1;
     auto* ws = static_cast<float*>(workspace);
     ChunkArgs a{};
     a.c = call.c;
@@ -206,6 +264,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     a.wide_from = p.wide_from;
     a.by_per = FastDiv(static_cast<unsigned>(q_heads / c->heads));
     a.by_heads = FastDiv(call.c.t.heads);
+    a.by_q_heads = FastDiv(a.q_heads);
     a.by_ranges = FastDiv(std::max(p.narrow, 1u));
     a.q_rows = q_f == 1 && q_t % 4 == 0 && aligned16(q) && c->dim % 4 == 0;
     a.page4 = c->page % 4 == 0;
@@ -229,7 +288,9 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
         if (int rc = launch_status()) return rc;
     }
     if (p.slots() == 1) return 0;
-    hipLaunchKernelGGL(k_attn_chunk_join, dim3(static_cast<unsigned>((tokens * q_heads + 3) / 4)), dim3(256), 0, s, a, p.narrow, p.wide);
+    const size_t rows = tokens * q_heads;
+    if (p.slots() <= kFewParts) hipLaunchKernelGGL(k_attn_chunk_join_few, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a, p.narrow, p.wide);
+    else hipLaunchKernelGGL(k_attn_chunk_join, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a, p.narrow, p.wide);
     return launch_status();
 }
 

@@ -359,13 +359,14 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
     }
 }
 
-template <int KS> __global__ __launch_bounds__(256, 2) void k_attn_chunk8(ChunkArgs a)
+// RT 1: no sequence has more than 16 rows.
+template <int KS, int RT> __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void k_attn_chunk8(ChunkArgs a)
 {
     __shared__ Shared8<KS> sh;
     Part part;
     if (!narrow_part(a, part, 4 * kPos)) return;
-    if (part.n_rows <= kTile) walk8<KS, 1>(a, part, sh);
-    else walk8<KS, 2>(a, part, sh);
+    if (RT == 1 || part.n_rows <= kTile) walk8<KS, 1>(a, part, sh);
+    else walk8<KS, RT>(a, part, sh);
 }
 
 } // namespace
@@ -374,7 +375,8 @@ void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, s, a); };
     const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
-    groups == 1 ? go(k_attn_chunk8<2>) : groups == 2 ? go(k_attn_chunk8<4>) : groups == 3 ? go(k_attn_chunk8<6>) : go(k_attn_chunk8<8>);
+    if (a.wide_from <= kTile) groups == 1 ? go(k_attn_chunk8<2, 1>) : groups == 2 ? go(k_attn_chunk8<4, 1>) : groups == 3 ? go(k_attn_chunk8<6, 1>) : go(k_attn_chunk8<8, 1>);
+    else groups == 1 ? go(k_attn_chunk8<2, 2>) : groups == 2 ? go(k_attn_chunk8<4, 2>) : groups == 3 ? go(k_attn_chunk8<6, 2>) : go(k_attn_chunk8<8, 2>);
 }
 
 } // namespace nnhip
