@@ -500,7 +500,7 @@ __device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int 
 {
     // The key heads of one range run on one XCD (workgroups go to the 8 in turn), one after another: neighbouring heads have
     // parts of the same lines, of a row's bytes up to 64 wide and of its scales. 48 sequences of 6000 positions, 8 heads of 64
-    // bytes: 119 us with a piece's ranges side by side, 74 so.
+    // bytes: 119 us with a piece's ranges side by side, 88 so.
     const unsigned y = blockIdx.x >> 3, group = a.by_heads.div(y), q = 8 * group + (blockIdx.x & 7);
     part.h = y - group * a.c.t.heads;
     part.b = a.by_ranges.div(q);

@@ -18,7 +18,6 @@ namespace
 {
 
 constexpr int kThreads = 256;
-constexpr int kAtOnce = 16;          // logits that a thread holds
 constexpr unsigned kMostSegments = 1024;
 constexpr size_t kMostRows = 1024;   // of a sequence
 
@@ -28,29 +27,66 @@ struct Decision
 {
     int row, accepted, drafted, token;
     float mt, md;
-    double st, sd;
+    double pt, pd;   // 1 / the sums, 0 where these are
 };
 
 struct VerifyArgs
 {
     const float *target, *draft, *fed, *start, *accept, *pick;
     size_t t_row, t_col, d_row, d_col;   // floats from a row's logits to the next row's, and from one logit to the next
-    unsigned vocab, tokens, batch, most, seg, n_seg;
-    int log2_cols, rows_along;           // logits by columns: 2^log2_cols of them to a workgroup
-    FastDiv by_seg;
-    double inv;                          // 1 / temperature; 0: the largest logit
+    unsigned vocab, tokens, batch, most, seg, n_seg, left_seg, n_left;   // tokens of a segment, segments: of the sums, of what is left
+    int log2_cols;                       // logits by columns: 2^log2_cols of them to a workgroup
+    FastDiv by_seg, by_left;
+    double scale;                        // 32 / (temperature ln 2); 0: the largest logit
     float* part_m;                       // per (model, row, segment): largest logit; and sum, or the largest one's index
     double* part_s;
     Decision* decision;                  // per sequence
-    double* left;                        // per (sequence, segment): sum of max(p - q, 0)
+    double* left;                        // per (sequence, piece): sum of max(p - q, 0)
     float *out_accepted, *out_token;
 };
 
-// exp((z - m) / temperature) for m >= z; NaN counts as -inf, and +inf beside +inf as equal.
-__device__ __forceinline__ double term(const VerifyArgs& a, float z, float m)
+// 2^(i / 32), by the exponential's series.
+struct Powers
 {
-    if (!(z > -__builtin_inff())) return 0.0;
-    return z == m ? 1.0 : exp(((double)z - (double)m) * a.inv);
+    double p[32];
+    constexpr Powers() : p{}
+    {
+        for (int i = 0; i < 32; ++i)
+        {
+            const double x = i * 0.6931471805599453 / 32;
+            double term = 1.0, sum = 0.0;
+            for (int k = 1; k < 30; ++k)
+            {
+                sum += term;
+                term *= x / k;
+            }
+            p[i] = sum;
+        }
+    }
+};
+__constant__ const Powers kPowers;
+
+// exp((z - m) / temperature) for m >= z; NaN counts as -inf, and +inf beside +inf as equal. With x = (z - m) / temperature
+// in units of ln 2 / 32 and n the nearest whole number this is 2^(n / 32), from a table, times exp of (x - n) ln 2 / 32,
+// which is below 0.011: 1 + r + r^2 (1/2 + r/6 + r^2/24), the last in float32. Off by 2^-37 at most. No branch, so that a
+// thread's values go side by side. 144 rows of 100003 twice, first launch: 40 us with the series to r^13 in float64, 30 so;
+// the library's exp, one value after another, took 54.
+using Table = double[32];
+__device__ __forceinline__ double term(const VerifyArgs& a, const Table& powers, float z, float m)
+{
+    constexpr double kUnit = 0.6931471805599453 / 32;
+    const double d = z == m ? 0.0 : (double)z - (double)m;
+    const double x = z > -__builtin_inff() ? fmax(d * a.scale, -36932.0) : -36932.0;   // exp(-800), as every number below -746: 0
+    const double n = rint(x), left = x - n;
+    const int i = (int)n;
+    const float r = (float)left * (float)kUnit;
+    const float square = r * r * __builtin_fmaf(r, __builtin_fmaf(r, 1.0f / 24, 1.0f / 6), 0.5f);
+    const double p = powers[i & 31];
+    return __builtin_ldexp(__builtin_fma(p, __builtin_fma(left, kUnit, (double)square), p), i >> 5);
+}
+__device__ __forceinline__ void load_powers(Table& powers)   // a barrier follows
+{
+    if (threadIdx.x < 32) powers[threadIdx.x] = kPowers.p[threadIdx.x];
 }
 __device__ __forceinline__ float larger(float m, float z) { return z > m ? z : m; }   // of NaN and m, m
 
@@ -59,70 +95,67 @@ struct Sum
     float m;
     double s;   // or the index of m
 };
-template <bool GREEDY> __device__ __forceinline__ Sum join(const VerifyArgs& a, Sum x, Sum y)
+
+// What f makes of the values of all threads that have the thread's column: lanes at distances of 2^log2_cols, then waves.
+template <int NT, class T, class F> __device__ __forceinline__ T of_column(const VerifyArgs& a, T x, T (&wave_s)[NT / 2], F&& f)
 {
-    Sum r;
-    r.m = larger(x.m, y.m);
-    if constexpr (GREEDY) r.s = x.m == y.m ? fmin(x.s, y.s) : x.m > y.m ? x.s : y.s;
-    else r.s = x.s * term(a, x.m, r.m) + y.s * term(a, y.m, r.m);
-    return r;
+    const int t = threadIdx.x, cols = 1 << a.log2_cols, col = t & (cols - 1);
+    for (int o = 32; o >= cols; o >>= 1) x = f(x, __shfl_xor(x, o, 64));
+    __syncthreads();
+    if ((t & 63) < cols) wave_s[(t >> 6) * cols + col] = x;
+    __syncthreads();
+    x = wave_s[col];
+    for (int w = 1; w < NT / 64; ++w) x = f(x, wave_s[w * cols + col]);
+    return x;
 }
 
-// What a thread's logits come to: get(k) gives logit k of n and its index.
-template <bool GREEDY, class F> __device__ __forceinline__ Sum sum_of(const VerifyArgs& a, unsigned v0, unsigned step, unsigned end, F&& get)
+// One segment of a row (logits by rows) or of up to 32 rows' columns; a thread takes PER logits of a row at once, on their
+// way together. blockIdx.y: the target's, the draft's.
+template <bool GREEDY, int PER, int NT> __global__ __launch_bounds__(NT) void k_verify_sums(VerifyArgs a)
 {
-    Sum r{-__builtin_inff(), GREEDY ? (double)v0 : 0.0};
-    for (unsigned v = v0; v < end; v += kAtOnce * step)
-    {
-        float z[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) z[k] = v + k * step < end ? get(v + k * step) : -__builtin_inff();
-        Sum c{-__builtin_inff(), GREEDY ? (double)v : 0.0};
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k)
-        {
-            if (GREEDY && z[k] > c.m) c.s = v + k * step;
-            c.m = larger(c.m, z[k]);
-        }
-        if constexpr (!GREEDY)
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) c.s += term(a, z[k], c.m);
-        r = v == v0 ? c : join<GREEDY>(a, r, c);
-    }
-    return r;
-}
-
-// One segment of a row (logits by rows) or of up to 64 rows' columns. blockIdx.y: the target's, the draft's.
-template <bool GREEDY> __global__ __launch_bounds__(kThreads) void k_verify_sums(VerifyArgs a)
-{
-    __shared__ float m_s[kThreads];
-    __shared__ double s_s[kThreads];
+    __shared__ float m_s[NT / 2];
+    __shared__ double s_s[NT / 2];
+    __shared__ Table powers;
+    load_powers(powers);   // of_column has barriers
     const int t = threadIdx.x;
     const unsigned outer = a.by_seg.div(blockIdx.x), seg = blockIdx.x - outer * a.n_seg;
-    const unsigned cols = 1u << a.log2_cols, parts = kThreads >> a.log2_cols;
+    const unsigned cols = 1u << a.log2_cols, parts = NT >> a.log2_cols;
     const unsigned part = t >> a.log2_cols, n = outer * cols + (t & (cols - 1));
     const float* p = blockIdx.y ? a.draft : a.target;
     const size_t row = blockIdx.y ? a.d_row : a.t_row, col = blockIdx.y ? a.d_col : a.t_col;
     const unsigned v0 = seg * a.seg, end = min(v0 + a.seg, a.vocab);
-    Sum r{-__builtin_inff(), (double)v0};
-    if (n < a.tokens)
+    const float* x = p + (size_t)min(n, a.tokens - 1) * row;
+    Sum r{-__builtin_inff(), GREEDY ? (double)v0 : 0.0};
+    for (unsigned v = v0; v < end; v += PER * parts)
     {
-        const float* x = p + (size_t)n * row;
-        r = sum_of<GREEDY>(a, v0 + part, parts, end, [&](unsigned v) { return x[(size_t)v * col]; });
-    }
-    m_s[t] = r.m;
-    s_s[t] = r.s;
-    for (unsigned half = parts / 2; half > 0; half /= 2)
-    {
-        __syncthreads();
-        if (part < half)
+        float z[PER], m = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) z[k] = x[(size_t)min(v + part + k * parts, end - 1) * col];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) z[k] = v + part + k * parts < end ? z[k] : -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) m = larger(m, z[k]);
+        m = larger(r.m, of_column<NT>(a, m, m_s, larger));
+        if constexpr (GREEDY)
         {
-            const unsigned o = t + (half << a.log2_cols);
-            r = join<GREEDY>(a, r, Sum{m_s[o], s_s[o]});
-            m_s[t] = r.m;
-            s_s[t] = r.s;
+            double at = a.vocab;
+#pragma unroll
+            for (int k = PER - 1; k >= 0; --k)
+                if (z[k] == m) at = v + part + k * parts;
+            at = of_column<NT>(a, at, s_s, [](double u, double w) { return fmin(u, w); });
+            if (m > r.m) r.s = at;
         }
+        else
+        {
+            double s = 0.0;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) s += term(a, powers, z[k], m);
+            if (v != v0) s += r.s * term(a, powers, r.m, m);
+            r.s = s;
+        }
+        r.m = m;
     }
+    if constexpr (!GREEDY) r.s = of_column<NT>(a, r.s, s_s, [](double u, double w) { return u + w; });
     if (part == 0 && n < a.tokens)
     {
         const size_t at = ((size_t)blockIdx.y * a.tokens + n) * a.n_seg + seg;
@@ -136,32 +169,6 @@ __device__ __forceinline__ double wave_sum64(double v)
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-// A wave: a row's segments together.
-__device__ __forceinline__ Sum row_sum(const VerifyArgs& a, int model, unsigned n)
-{
-    const unsigned lane = threadIdx.x & 63;
-    const size_t at = ((size_t)model * a.tokens + n) * a.n_seg;
-    Sum r{-__builtin_inff(), 0.0};
-    for (unsigned i = lane; i < a.n_seg; i += 64) r.m = larger(r.m, a.part_m[at + i]);
-    r.m = wave_max(r.m);
-    for (unsigned i = lane; i < a.n_seg; i += 64) r.s += a.part_s[at + i] * term(a, a.part_m[at + i], r.m);
-    r.s = wave_sum64(r.s);
-    return r;
-}
-__device__ __forceinline__ unsigned row_best(const VerifyArgs& a, unsigned n)
-{
-    const unsigned lane = threadIdx.x & 63;
-    const size_t at = (size_t)n * a.n_seg;
-    float m = -__builtin_inff();
-    for (unsigned i = lane; i < a.n_seg; i += 64) m = larger(m, a.part_m[at + i]);
-    m = wave_max(m);
-    double best = a.vocab;
-    for (unsigned i = lane; i < a.n_seg; i += 64)
-        if (a.part_m[at + i] == m) best = fmin(best, a.part_s[at + i]);
-    for (int o = 32; o > 0; o >>= 1) best = fmin(best, __shfl_xor(best, o, 64));
-    return (unsigned)best;
-}
-
 // The drafted token behind row n, -1 where it is none.
 __device__ __forceinline__ int drafted(const VerifyArgs& a, unsigned n)
 {
@@ -169,98 +176,138 @@ __device__ __forceinline__ int drafted(const VerifyArgs& a, unsigned n)
     return row_index(a.fed[n + 1], a.vocab, x) ? (int)x : -1;
 }
 
-// A workgroup: what becomes of sequence b. shared: kMostRows places.
-template <bool GREEDY> __device__ __forceinline__ Decision decide(const VerifyArgs& a, unsigned b, int& first_s, Decision& d_s)
+constexpr int kRowsAtOnce = kThreads / 32;   // rows that a workgroup decides on together: 16 lanes a model's row
+struct DecideShared
 {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int lo = length_of(a.start[b], a.tokens), hi = length_of(a.start[b + 1], a.tokens);
-    const int n = min(hi - lo, (int)a.most);
-    if (t == 0) first_s = n - 1;
-    __syncthreads();
-    for (int i = wave; i < n - 1; i += kThreads / 64)
+    float m[2 * kRowsAtOnce];
+    double s[2 * kRowsAtOnce];   // or the index of m
+    int first;
+};
+// A workgroup: what becomes of sequence b.
+template <bool GREEDY> __device__ __forceinline__ Decision decide(const VerifyArgs& a, const Table& powers, unsigned b, DecideShared& sh)
+{
+    const int t = threadIdx.x, group = t >> 4, lane = t & 15, model = group & 1;
+    const int lo = length_of(a.start[b], a.tokens), hi = length_of(a.start[b + 1], a.tokens), n = min(hi - lo, (int)a.most);
+    Decision d{};
+    d.row = -1;
+    d.token = -1;
+    d.mt = d.md = -__builtin_inff();
+    for (int i0 = 0; i0 < n; i0 += kRowsAtOnce)
     {
-        const unsigned row = lo + i;
-        const int x = drafted(a, row);
-        bool stands;
-        if constexpr (GREEDY) stands = (int)row_best(a, row) == x;
-        else
+        const int i = i0 + (group >> 1);
+        if (i < n && (model == 0 || (a.draft && i < n - 1)))
         {
-            const Sum p = row_sum(a, 0, row);
-            const double px = x < 0 || p.s == 0.0 ? 0.0 : term(a, a.target[(size_t)row * a.t_row + (size_t)x * a.t_col], p.m) / p.s;
-            double qx = 1.0;
-            if (a.draft)
+            // The row's segments together.
+            const size_t at = ((size_t)model * a.tokens + lo + i) * a.n_seg;
+            float m = -__builtin_inff();
+            for (unsigned k = lane; k < a.n_seg; k += 16) m = larger(m, a.part_m[at + k]);
+            for (int o = 8; o > 0; o >>= 1) m = larger(m, __shfl_xor(m, o, 16));
+            double s = GREEDY ? (double)a.vocab : 0.0;
+            for (unsigned k = lane; k < a.n_seg; k += 16)
             {
-                const Sum q = row_sum(a, 1, row);
-                qx = x < 0 || q.s == 0.0 ? 0.0 : term(a, a.draft[(size_t)row * a.d_row + (size_t)x * a.d_col], q.m) / q.s;
+                const float mk = a.part_m[at + k];
+                const double sk = a.part_s[at + k];
+                if constexpr (GREEDY) s = mk == m ? fmin(s, sk) : s;
+                else s += sk * term(a, powers, mk, m);
             }
-            stands = (double)a.accept[row] * qx < px;
-        }
-        if (!stands)
-        {
-            if (lane == 0) atomicMin(&first_s, i);   // in LDS: the smallest, in whatever order
-            break;
-        }
-    }
-    __syncthreads();
-    const int f = first_s;
-    if (wave == 0)
-    {
-        Decision d{};
-        d.row = n > 0 ? lo + f : -1;
-        d.accepted = n > 0 ? f : 0;
-        d.drafted = f < n - 1;
-        d.token = d.drafted ? drafted(a, lo + f) : -1;
-        d.mt = d.md = -__builtin_inff();
-        if (n > 0)
-        {
-            if constexpr (GREEDY) d.token = (int)row_best(a, lo + f);
-            else
+            for (int o = 8; o > 0; o >>= 1)
             {
-                const Sum p = row_sum(a, 0, lo + f);
-                d.mt = p.m;
-                d.st = p.s;
-                if (d.drafted && a.draft)
+                const double y = __shfl_xor(s, o, 16);
+                s = GREEDY ? fmin(s, y) : s + y;
+            }
+            if (lane == 0)
+            {
+                sh.m[group] = m;
+                sh.s[group] = s;
+            }
+        }
+        if (t == 0) sh.first = n;
+        __syncthreads();
+        if (t < 64)   // a row a lane
+        {
+            const bool there = t < kRowsAtOnce && i0 + t < n;
+            bool stands = false;
+            if (there && i0 + t < n - 1)
+            {
+                const unsigned row = lo + i0 + t;
+                const int x = drafted(a, row);
+                if constexpr (GREEDY) stands = (int)sh.s[2 * t] == x;
+                else
                 {
-                    const Sum q = row_sum(a, 1, lo + f);
-                    d.md = q.m;
-                    d.sd = q.s;
+                    auto p_of = [&](const float* z, size_t r, size_t c, int k) {
+                        return x < 0 || sh.s[k] == 0.0 ? 0.0 : term(a, powers, z[row * r + (size_t)x * c], sh.m[k]) * (1.0 / sh.s[k]);
+                    };
+                    const double px = p_of(a.target, a.t_row, a.t_col, 2 * t), qx = a.draft ? p_of(a.draft, a.d_row, a.d_col, 2 * t + 1) : 1.0;
+                    stands = (double)a.accept[row] * qx < px;
                 }
             }
+            const unsigned long long ends = __builtin_amdgcn_ballot_w64(there && !stands);
+            if (t == 0 && ends) sh.first = i0 + __builtin_ctzll(ends);
         }
-        if (lane == 0) d_s = d;
+        __syncthreads();
+        const int f = sh.first, k = 2 * (f - i0);
+        if (f < n)   // the last row ends the search if none does before
+        {
+            d.row = lo + f;
+            d.accepted = f;
+            d.drafted = f < n - 1;
+            if constexpr (GREEDY) d.token = (int)sh.s[k];
+            else
+            {
+                d.token = d.drafted ? drafted(a, lo + f) : -1;
+                d.mt = sh.m[k];
+                d.pt = sh.s[k] == 0.0 ? 0.0 : 1.0 / sh.s[k];
+                if (d.drafted && a.draft)
+                {
+                    d.md = sh.m[k + 1];
+                    d.pd = sh.s[k + 1] == 0.0 ? 0.0 : 1.0 / sh.s[k + 1];
+                }
+            }
+            break;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    return d_s;
+    return d;
 }
 
 // max(p - q, 0) of logit v of the decision's row.
-__device__ __forceinline__ double left_of(const VerifyArgs& a, const Decision& d, unsigned v)
+__device__ __forceinline__ double left_of(const VerifyArgs& a, const Table& powers, const Decision& d, unsigned v)
 {
-    const double p = d.st == 0.0 ? 0.0 : term(a, a.target[(size_t)d.row * a.t_row + (size_t)v * a.t_col], d.mt) / d.st;
-    double q = 0.0;
-    if (!a.draft) q = (int)v == d.token ? 1.0 : 0.0;
-    else if (d.sd != 0.0) q = term(a, a.draft[(size_t)d.row * a.d_row + (size_t)v * a.d_col], d.md) / d.sd;
+#pragma clang fp contract(off)   // p = q has to leave 0
+    const double p = term(a, powers, a.target[(size_t)d.row * a.t_row + (size_t)v * a.t_col], d.mt) * d.pt;
+    double q = (int)v == d.token ? 1.0 : 0.0;
+    if (a.draft) q = term(a, powers, a.draft[(size_t)d.row * a.d_row + (size_t)v * a.d_col], d.md) * d.pd;
     return fmax(p - q, 0.0);
 }
 
-// Segment sums of what is left of p, blockIdx.x = sequence * n_seg + segment.
+// Sums of what is left of p over kLeft tokens, blockIdx.x = sequence * n_left + piece.
+constexpr unsigned kLeft = 8 * kThreads;
 __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
 {
-    __shared__ int first_s;
-    __shared__ Decision d_s;
+    __shared__ DecideShared sh;
     __shared__ double s_s[kThreads / 64];
+    __shared__ Table powers;
     const int t = threadIdx.x;
-    const unsigned b = a.by_seg.div(blockIdx.x), seg = blockIdx.x - b * a.n_seg;
-    const Decision d = decide<false>(a, b, first_s, d_s);
-    if (seg == 0 && t == 0) a.decision[b] = d;
+    load_powers(powers);
+    __syncthreads();
+    const unsigned b = a.by_left.div(blockIdx.x), piece = blockIdx.x - b * a.n_left;
+    const Decision d = decide<false>(a, powers, b, sh);
+    if (piece == 0 && t == 0) a.decision[b] = d;
     if (!d.drafted) return;
-    const unsigned end = min((seg + 1) * a.seg, a.vocab);
+    const unsigned v0 = piece * a.left_seg, end = min(v0 + a.left_seg, a.vocab);
     double s = 0.0;
-    for (unsigned v = seg * a.seg + t; v < end; v += kThreads) s += left_of(a, d, v);
+    for (unsigned v = v0 + t; v < end; v += kLeft)
+    {
+        double x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = left_of(a, powers, d, min(v + i * kThreads, end - 1));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v + i * kThreads < end ? x[i] : 0.0;
+    }
     s = wave_sum64(s);
     if ((t & 63) == 0) s_s[t >> 6] = s;
     __syncthreads();
-    if (t == 0) a.left[(size_t)b * a.n_seg + seg] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+    if (t == 0) a.left[(size_t)b * a.n_left + piece] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
 }
 
 // Sums of all threads' values up to and with the thread's own.
@@ -285,16 +332,43 @@ __device__ __forceinline__ double scan(double x, double (&wave_s)[kThreads / 64]
     return before + x;
 }
 
+// The smallest of all threads' `first`, the largest of their `last`.
+struct Found
+{
+    unsigned first, last;
+};
+__device__ __forceinline__ Found found(unsigned first, unsigned last, unsigned (&first_w)[kThreads / 64], unsigned (&last_w)[kThreads / 64])
+{
+    for (int o = 32; o > 0; o >>= 1)
+    {
+        first = min(first, (unsigned)__shfl_xor((int)first, o, 64));
+        last = max(last, (unsigned)__shfl_xor((int)last, o, 64));
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+    {
+        first_w[threadIdx.x >> 6] = first;
+        last_w[threadIdx.x >> 6] = last;
+    }
+    __syncthreads();
+    return {min(min(first_w[0], first_w[1]), min(first_w[2], first_w[3])), max(max(last_w[0], last_w[1]), max(last_w[2], last_w[3]))};
+}
+
 // The next token of sequence blockIdx.x.
 template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a)
 {
-    __shared__ int first_s;
-    __shared__ Decision d_s;
+    __shared__ DecideShared sh;
     __shared__ double wave_s[kThreads / 64], before_s;
-    __shared__ unsigned at_s, last_s;
+    __shared__ unsigned first_w[kThreads / 64], last_w[kThreads / 64];
+    __shared__ Table powers;
     const int t = threadIdx.x;
+    if constexpr (!GREEDY)
+    {
+        load_powers(powers);
+        __syncthreads();
+    }
     const unsigned b = blockIdx.x;
-    const Decision d = DECIDE ? decide<GREEDY>(a, b, first_s, d_s) : a.decision[b];
+    const Decision d = DECIDE ? decide<GREEDY>(a, powers, b, sh) : a.decision[b];
     if (t == 0) a.out_accepted[b] = (float)d.accepted;
     if (GREEDY || d.row < 0)
     {
@@ -304,14 +378,14 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     const size_t at = (size_t)d.row * a.n_seg;
     bool left = d.drafted;   // whether p is lessened by q
     auto of_segment = [&](unsigned i) -> double {
-        if (i >= a.n_seg) return 0.0;
-        return left ? a.left[(size_t)b * a.n_seg + i] : a.part_s[at + i] * term(a, a.part_m[at + i], d.mt);
+        if (i >= (left ? a.n_left : a.n_seg)) return 0.0;
+        return left ? a.left[(size_t)b * a.n_left + i] : a.part_s[at + i] * term(a, powers, a.part_m[at + i], d.mt);
     };
     double whole = 0.0;
     for (int again = 0; again < 2; ++again)
     {
         whole = 0.0;
-        for (unsigned i = 0; i < a.n_seg; i += kThreads)
+        for (unsigned i = 0; i < (left ? a.n_left : a.n_seg); i += kThreads)
         {
             double all;
             scan(of_segment(i + t), wave_s, all);
@@ -323,63 +397,83 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     const float w = a.pick[b];
     const double want = (w >= 1.0f ? 1.0 - 0x1p-53 : w > 0.0f ? (double)w : 0.0) * whole;
     // The first segment whose cumulative sum is above that, the last one with anything where rounding leaves none.
-    if (t == 0) at_s = a.n_seg, last_s = 0, before_s = 0.0;
-    __syncthreads();
-    double sum = 0.0;
-    for (unsigned i = 0; i < a.n_seg; i += kThreads)
+    const unsigned segs = left ? a.n_left : a.n_seg, size = left ? a.left_seg : a.seg;
+    Found in{segs, 0};
+    double sum = 0.0, base = 0.0;
+    for (unsigned i = 0; i < segs && in.first == segs; i += kThreads)
     {
         double all;
         const double x = of_segment(i + t), up = sum + scan(x, wave_s, all);
-        if (x > 0.0)
-        {
-            atomicMax(&last_s, i + t);
-            if (up > want) atomicMin(&at_s, i + t);
-        }
+        const Found here = found(x > 0.0 && up > want ? i + t : segs, x > 0.0 ? i + t : 0, first_w, last_w);
+        in.first = min(in.first, here.first);
+        in.last = max(in.last, here.last);
+        if (in.first == i + t) before_s = up - x;
         __syncthreads();
-        if (at_s == i + t) before_s = up - x;
-        __syncthreads();
-        if (at_s < a.n_seg) break;
+        base = before_s;
         sum += all;
     }
-    const bool found = at_s < a.n_seg;
-    const unsigned seg = found ? at_s : last_s;
-    const double base = before_s;
-    __syncthreads();
-    // The token, alike: 'want' lies past the last one with anything where no cumulative sum is above it.
-    if (t == 0) at_s = a.vocab, last_s = 0;
-    __syncthreads();
-    const unsigned end = min((seg + 1) * a.seg, a.vocab);
-    sum = found ? base : -__builtin_inf();
-    for (unsigned v0 = seg * a.seg; v0 < end; v0 += kThreads)
+    const bool some = in.first < segs;
+    const unsigned seg = some ? in.first : in.last;
+    // The token, alike: a thread takes kEach neighbouring ones.
+    constexpr int kEach = 8;
+    const unsigned end = min((seg + 1) * size, a.vocab);
+    in = {a.vocab, 0};
+    sum = some ? base : -__builtin_inf();
+    for (unsigned v0 = seg * size; v0 < end && in.first == a.vocab; v0 += kThreads * kEach)
     {
-        double all;
-        const unsigned v = v0 + t;
-        double x = 0.0;
-        if (v < end) x = left ? left_of(a, d, v) : term(a, a.target[(size_t)d.row * a.t_row + (size_t)v * a.t_col], d.mt);
-        const double up = sum + scan(x, wave_s, all);
-        if (x > 0.0)
+        double x[kEach], mine = 0.0, all;
+        const unsigned v = v0 + kEach * t;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
         {
-            atomicMax(&last_s, v);
-            if (up > want) atomicMin(&at_s, v);
+            const unsigned at = min(v + i, end - 1);
+            x[i] = left ? left_of(a, powers, d, at) : term(a, powers, a.target[(size_t)d.row * a.t_row + (size_t)at * a.t_col], d.mt);
+            if (v + i >= end) x[i] = 0.0;
+            mine += x[i];
         }
-        __syncthreads();
-        if (at_s < a.vocab) break;
+        double up = sum + (scan(mine, wave_s, all) - mine);
+        unsigned first = a.vocab, last = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            up += x[i];
+            if (x[i] > 0.0)
+            {
+                last = v + i;
+                if (up > want) first = min(first, v + i);
+            }
+        }
+        const Found here = found(first, last, first_w, last_w);
+        in.first = min(in.first, here.first);
+        in.last = max(in.last, here.last);
         sum += all;
     }
-    if (t == 0) a.out_token[b] = (float)(at_s < a.vocab ? at_s : last_s);
+    if (t == 0) a.out_token[b] = (float)(in.first < a.vocab ? in.first : in.last);
 }
 
 struct VerifyPlan
 {
-    unsigned seg, n_seg;
+    unsigned seg, n_seg, left_seg, n_left;
+    int log2_cols, per, threads;   // the first launch: columns and threads of a workgroup, logits that a thread takes at once
 };
-VerifyPlan verify_plan(size_t tokens, size_t vocab)
+VerifyPlan verify_plan(size_t tokens, size_t vocab, bool token_major)
 {
-    // Some 8 workgroups a CU for the first launch, of 512 logits at least to a row.
-    size_t seg = 512;
-    while (seg < 4096 && 2 * tokens * ((vocab + seg - 1) / seg) > 8 * (size_t)device_cus()) seg *= 2;
+    VerifyPlan p{};
+    if (!token_major)
+        while (p.log2_cols < 5 && ((size_t)1 << p.log2_cols) < tokens) ++p.log2_cols;
+    // 16 logits a thread once they fill the CUs' threads (verify of 144 rows of 100003: PER), else 4.
+    p.per = 2 * tokens * vocab < ((size_t)1 << 22) ? 4 : 16;
+    // Of several columns more threads, for as few segments: every sequence reads its rows' twice more.
+    p.threads = p.log2_cols >= 2 ? 1024 : kThreads;
+    size_t seg = (size_t)(p.threads >> p.log2_cols) * p.per;
     while ((vocab + seg - 1) / seg > kMostSegments) seg *= 2;
-    return {static_cast<unsigned>(seg), static_cast<unsigned>((vocab + seg - 1) / seg)};
+    p.seg = static_cast<unsigned>(seg);
+    p.n_seg = static_cast<unsigned>((vocab + seg - 1) / seg);
+    size_t left = kLeft;
+    while ((vocab + left - 1) / left > kMostSegments) left *= 2;
+    p.left_seg = static_cast<unsigned>(left);
+    p.n_left = static_cast<unsigned>((vocab + left - 1) / left);
+    return p;
 }
 
 struct VerifySpace
@@ -392,7 +486,7 @@ VerifySpace verify_space(size_t tokens, size_t batch, const VerifyPlan& p)
     s.part_m = 2 * tokens * p.n_seg * sizeof(double);
     s.decision = (s.part_m + 2 * tokens * p.n_seg * sizeof(float) + 15) / 16 * 16;
     s.left = s.decision + batch * sizeof(Decision);
-    s.all = s.left + batch * p.n_seg * sizeof(double);
+    s.all = s.left + batch * p.n_left * sizeof(double);
     return s;
 }
 static_assert(sizeof(Decision) % 8 == 0);
@@ -410,7 +504,10 @@ using namespace nnhip;
 
 extern "C" size_t nnhip_draft_verify_workspace_bytes(size_t tokens, size_t batch, size_t most, size_t vocab)
 {
-    return verify_ok(tokens, batch, most, vocab) ? verify_space(tokens, batch, verify_plan(tokens, vocab)).all : 0;
+    if (!verify_ok(tokens, batch, most, vocab)) return 0;
+    const size_t rows = verify_space(tokens, batch, verify_plan(tokens, vocab, true)).all;   // enough for either layout
+    const size_t columns = verify_space(tokens, batch, verify_plan(tokens, vocab, false)).all;
+    return rows > columns ? rows : columns;
 }
 
 extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float* draft, size_t d_ld, int token_major,
@@ -425,7 +522,7 @@ extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float*
         t_ld > ((size_t)1 << 32) || (draft && (d_ld < least_ld || d_ld > ((size_t)1 << 32))) || !(temperature >= 0.0f) ||
         temperature > kMaxF || (temperature > 0.0f && (!accept || !pick)))
         return -1;
-    const VerifyPlan plan = verify_plan(tokens, vocab);
+    const VerifyPlan plan = verify_plan(tokens, vocab, token_major != 0);
     const VerifySpace space = verify_space(tokens, batch, plan);
     if (!workspace || workspace_bytes < space.all || !aligned16(workspace)) return -1;
     const bool greedy = temperature == 0.0f;
@@ -446,10 +543,12 @@ extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float*
     a.most = static_cast<unsigned>(most);
     a.seg = plan.seg;
     a.n_seg = plan.n_seg;
+    a.left_seg = plan.left_seg;
+    a.n_left = plan.n_left;
     a.by_seg = FastDiv(plan.n_seg);
-    if (!token_major)
-        while (a.log2_cols < 5 && ((size_t)1 << a.log2_cols) < tokens) ++a.log2_cols;
-    a.inv = greedy ? 0.0 : 1.0 / static_cast<double>(temperature);
+    a.by_left = FastDiv(plan.n_left);
+    a.log2_cols = plan.log2_cols;
+    a.scale = greedy ? 0.0 : 32.0 / (static_cast<double>(temperature) * 0.6931471805599453);
     auto* ws = static_cast<char*>(workspace);
     a.part_s = reinterpret_cast<double*>(ws);
     a.part_m = reinterpret_cast<float*>(ws + space.part_m);
@@ -458,25 +557,30 @@ extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float*
     a.out_accepted = out_accepted;
     a.out_token = out_token;
     const size_t cols = (size_t)1 << a.log2_cols, blocks = (tokens + cols - 1) / cols * plan.n_seg;
-    if (blocks > kGridMost || batch * plan.n_seg > kGridMost) return -1;
+    if (blocks * plan.threads / kThreads > kGridMost || batch * plan.n_left > kGridMost) return -1;
     auto s = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(blocks), a.draft ? 2 : 1);
     const dim3 all(static_cast<unsigned>(batch));
+    auto sums = [&](auto few, auto many, auto few_cols, auto many_cols) {
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(static_cast<unsigned>(plan.threads)), 0, s, a); };
+        if (plan.threads == kThreads) plan.per == 4 ? go(few) : go(many);
+        else plan.per == 4 ? go(few_cols) : go(many_cols);
+    };
     if (greedy)
     {
-        hipLaunchKernelGGL(k_verify_sums<true>, grid, dim3(kThreads), 0, s, a);
+        sums(k_verify_sums<true, 4, kThreads>, k_verify_sums<true, 16, kThreads>, k_verify_sums<true, 4, 1024>, k_verify_sums<true, 16, 1024>);
         if (int rc = launch_status()) return rc;
         hipLaunchKernelGGL((k_verify_pick<true, true>), all, dim3(kThreads), 0, s, a);
         return launch_status();
     }
-    hipLaunchKernelGGL(k_verify_sums<false>, grid, dim3(kThreads), 0, s, a);
+    sums(k_verify_sums<false, 4, kThreads>, k_verify_sums<false, 16, kThreads>, k_verify_sums<false, 4, 1024>, k_verify_sums<false, 16, 1024>);
     if (int rc = launch_status()) return rc;
     if (most == 1)
     {
         hipLaunchKernelGGL((k_verify_pick<false, true>), all, dim3(kThreads), 0, s, a);
         return launch_status();
     }
-    hipLaunchKernelGGL(k_verify_left, dim3(static_cast<unsigned>(batch * plan.n_seg)), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(k_verify_left, dim3(static_cast<unsigned>(batch * plan.n_left)), dim3(kThreads), 0, s, a);
     if (int rc = launch_status()) return rc;
     hipLaunchKernelGGL((k_verify_pick<false, false>), all, dim3(kThreads), 0, s, a);
     return launch_status();
