@@ -76,8 +76,19 @@ enum nnhip_op {
                                 * has_slopes  out O */
     NNHIP_OP_BEAM_SELECT = 33, /* in logits (vocab, groups*beams),scores[,done]; args groups,take,eos
                                 * out totals,beams,tokens (groups, take) */
-    NNHIP_OP_KV_REORDER = 34   /* in table,parent,len[,fresh],K0,V0,K1,V1,..; args page,heads,layers,has_fresh
+    NNHIP_OP_KV_REORDER = 34,  /* in table,parent,len[,fresh],K0,V0,K1,V1,..; args page,heads,layers,has_fresh
                                 * out table,len (K, V in place) */
+    /* Chunks of new tokens (start: a float more than there are sequences), 8-bit caches (K, V pages * page rows of
+     * floats of four bytes each, K_scale, V_scale (pages * page, heads); values of `dim` bytes a head) and drafted
+     * tokens. Results of tokens that no sequence has, or whose position does not exist, are 0 (q: as it was). */
+    NNHIP_OP_ATTN_CHUNK = 35,  /* in K,V,table,q,start,len[,slopes]; args page,heads,most,alpha,has_slopes  out O */
+    NNHIP_OP_KV8_APPEND = 36,  /* in K,V,K_scale,V_scale,table,k,v,pos[,q][,cos,sin][,seq]; args page,heads,dim,has_q,
+                                * has_rope,has_seq  out [q turned] (K, V, K_scale, V_scale in place) */
+    NNHIP_OP_KV8_READ = 37,    /* in K,V,K_scale,V_scale,table,pos[,seq]; args page,heads,dim  out k,v */
+    NNHIP_OP_ATTN_CHUNK8 = 38, /* in K,V,K_scale,V_scale,table,q,start,len[,slopes]; args page,heads,dim,most,alpha,
+                                * has_slopes  out O */
+    NNHIP_OP_DRAFT_VERIFY = 39 /* in target,fed,start[,draft][,accept,pick]; args most,temperature,token_major,has_draft,
+                                * has_random  out accepted,tokens (a sequence each) */
 };
 
 const char* nnhip_last_error(void);
@@ -212,6 +223,19 @@ int nnhip_gpt_reset_cache(nnhip_gpt* g);
  * backward pass after it is refused until the next forward pass. */
 int nnhip_gpt_beam_search(nnhip_gpt* g, const uint64_t* prompt, size_t n_prompt, size_t beams, size_t max_new,
                           uint64_t eos, uint64_t* out, size_t* out_len, float* out_scores);
+/* Speculative decoding with a draft session of the same engine and vocabulary (no reference counterpart): continues n
+ * prompts (one after another in prompts, prompt_len tokens each, 1 to seq_len) by up to max_new tokens, distributed as if
+ * each were drawn from this session's softmax(logits / temperature); temperature 0 takes the largest logit, as
+ * _generate does. The draft proposes draft_len tokens (1 to 1023) at a time, which this model verifies in one pass. A
+ * sequence ends at eos (an id past the vocabulary: none does), after max_new tokens or where the context is full
+ * (seq_len - prompt_len + 1 tokens); the draft's context has to hold it too. cache_bits 32: float32 caches; 8: a byte a
+ * value (nnhip_kv8_append), for both models. seed: of the random numbers. out (n * max_new places, sequence i's tokens
+ * from i * max_new on, eos not among them), out_len (n), stats (or NULL): passes of the target model, drafted tokens
+ * and those of them that stood. 1 to 1024 prompts; heads at most 128 wide. Caches (_forward_step) and backward passes,
+ * of both sessions, as with _beam_search. */
+int nnhip_gpt_speculate(nnhip_gpt* g, nnhip_gpt* draft, const uint64_t* prompts, const size_t* prompt_len, size_t n,
+                        size_t max_new, size_t draft_len, float temperature, uint64_t eos, uint64_t seed,
+                        size_t cache_bits, uint64_t* out, size_t* out_len, uint64_t* stats);
 int nnhip_gpt_generate(nnhip_gpt* g, const uint64_t* prompt, size_t n_prompt, size_t max_new, float temperature,
                        uint64_t eos, size_t min_new, uint64_t seed, uint64_t* out, size_t out_cap, size_t* n_out);
 

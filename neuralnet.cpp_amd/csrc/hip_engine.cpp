@@ -2293,6 +2293,123 @@ Result<Tensor> HipEngine::kv_reorder(std::span<KvPages> layers, const Tensor& pa
     return out;
 }
 
+// ── chunks of new tokens, 8-bit caches, drafted tokens (no reference counterpart) ──
+namespace
+{
+nnhip_kv8_pages pages8_of(const KvPages8& c)
+{
+    return nnhip_kv8_pages{reinterpret_cast<signed char*>(W(c.K)),
+                           reinterpret_cast<signed char*>(W(c.V)),
+                           W(c.K_scale),
+                           W(c.V_scale),
+                           D(c.table),
+                           c.table.rows(),
+                           c.table.cols(),
+                           c.K.rows() / c.page,
+                           c.page,
+                           c.heads,
+                           c.dim,
+                           4 * c.K.cols()};
+}
+} // namespace
+
+Result<Tensor> HipEngine::attn_chunk(const KvPages& c, const Tensor& q, const Tensor& start, std::size_t most,
+                                     const Tensor& len, const Tensor* slopes, Scalar alpha)
+{
+    const std::size_t dim = paged::dim_of(c), n = q.cols();
+    NN_TRY(heads, paged::check_chunk("attn_chunk", dim, c.heads, c.table.rows(), q, start, most, len, slopes));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.table, &q, &start, &len, slopes}, "attn_chunk"));
+    NN_TRY(out, alloc_(q.rows(), n));
+    NN_CHECK(kernel_(nnhip_fill(W(out), out.size(), 0.0f, stream_), "attn_chunk"));   // tokens that no sequence has
+    const nnhip_kv_pages p = pages_of(c, dim);
+    const std::size_t need = nnhip_attn_chunk_workspace_bytes(&p, heads, n, most);
+    NN_TRY(ws, scratch_(need));
+    NN_CHECK(kernel_(nnhip_attn_chunk(&p, D(q), 1, static_cast<long>(n), heads, n, D(start), most, D(len),
+                                      slopes ? D(*slopes) : nullptr, alpha, W(out), 1, static_cast<long>(n), nullptr,
+                                      nullptr, ws->data(), need, stream_),
+                     "attn_chunk"));
+    return out;
+}
+
+Result<Tensor> HipEngine::kv8_append(KvPages8& c, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                                     const Tensor* seq, const Tensor* cos, const Tensor* sin)
+{
+    NN_TRY(s, paged::check_append8(c, k, v, q, pos, seq, cos, sin));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &k, &v, q, &pos, seq, cos, sin}, "kv8_append"));
+    for (const Tensor* t : {&c.K, &c.V, &c.K_scale, &c.V_scale}) NN_CHECK(settle_write_(*t));
+    if (W(c.K) == W(c.V) || W(c.K_scale) == W(c.V_scale) || W(c.K) == W(c.K_scale) || W(c.K) == W(c.V_scale) ||
+        W(c.V) == W(c.K_scale) || W(c.V) == W(c.V_scale))
+        return fail("kv8_append: two of K, V and their scales are one tensor");
+    const std::size_t n = k.cols();
+    const long t = 1, f = static_cast<long>(n);
+    Tensor out;
+    if (q)
+    {
+        NN_TRY(o, alloc_(q->rows(), n));
+        // The tokens that are padding are not written.
+        if (q->size()) NN_CHECK(kernel_(nnhip_copy(D(*q), W(o), q->size(), stream_), "kv8_append"));
+        out = o;
+    }
+    const nnhip_kv8_pages p = pages8_of(c);
+    NN_CHECK(kernel_(nnhip_kv8_append(&p, D(k), t, f, D(v), t, f, q ? D(*q) : nullptr, t, f, q ? W(out) : nullptr, t, f,
+                                      s.q_heads, n, seq ? D(*seq) : nullptr, D(pos), cos ? D(*cos) : nullptr,
+                                      sin ? D(*sin) : nullptr, cos ? cos->rows() : 0, 2 * s.half, stream_),
+                     "kv8_append"));
+    return out;
+}
+
+Result<Tensor> HipEngine::kv8_read(const KvPages8& c, const Tensor& pos, const Tensor* seq, Tensor& v_out)
+{
+    NN_TRY(n, paged::check_read8(c, pos, seq));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &pos, seq}, "kv8_read"));
+    NN_TRY(k, alloc_(c.heads * c.dim, n));
+    NN_TRY(v, alloc_(c.heads * c.dim, n));
+    for (const Tensor* t : {&k, &v}) NN_CHECK(kernel_(nnhip_fill(W(*t), t->size(), 0.0f, stream_), "kv8_read"));
+    const nnhip_kv8_pages p = pages8_of(c);
+    const long f = static_cast<long>(n);
+    NN_CHECK(kernel_(nnhip_kv8_read(&p, W(k), 1, f, W(v), 1, f, n, seq ? D(*seq) : nullptr, D(pos), stream_), "kv8_read"));
+    v_out = v;
+    return k;
+}
+
+Result<Tensor> HipEngine::attn_chunk8(const KvPages8& c, const Tensor& q, const Tensor& start, std::size_t most,
+                                      const Tensor& len, const Tensor* slopes, Scalar alpha)
+{
+    const std::size_t n = q.cols();
+    NN_TRY(heads, paged::check_chunk("attn_chunk8", paged::dim_of8(c), c.heads, c.table.rows(), q, start, most, len, slopes));
+    NN_CHECK(need_gpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &q, &start, &len, slopes}, "attn_chunk8"));
+    NN_TRY(out, alloc_(q.rows(), n));
+    NN_CHECK(kernel_(nnhip_fill(W(out), out.size(), 0.0f, stream_), "attn_chunk8"));   // tokens that no sequence has
+    const nnhip_kv8_pages p = pages8_of(c);
+    const std::size_t need = nnhip_attn_chunk8_workspace_bytes(&p, heads, n, most);
+    NN_TRY(ws, scratch_(need));
+    NN_CHECK(kernel_(nnhip_attn_chunk8(&p, D(q), 1, static_cast<long>(n), heads, n, D(start), most, D(len),
+                                       slopes ? D(*slopes) : nullptr, alpha, W(out), 1, static_cast<long>(n), nullptr,
+                                       nullptr, ws->data(), need, stream_),
+                     "attn_chunk8"));
+    return out;
+}
+
+Result<Tensor> HipEngine::draft_verify(const Tensor& target, const Tensor* draft, bool token_major, const Tensor& fed,
+                                       const Tensor& start, std::size_t most, Scalar temperature, const Tensor* accept,
+                                       const Tensor* pick, Tensor& tokens_out)
+{
+    NN_TRY(batch, paged::check_verify(target, draft, token_major, fed, start, most, temperature, accept, pick));
+    NN_CHECK(need_gpu_({&target, draft, &fed, &start, accept, pick}, "draft_verify"));
+    const std::size_t n = fed.size(), vocab = target.size() / n, most_here = std::min(most, n);
+    NN_TRY(accepted, alloc_(batch, 1));
+    NN_TRY(tokens, alloc_(batch, 1));
+    const std::size_t need = nnhip_draft_verify_workspace_bytes(n, batch, most_here, vocab);
+    NN_TRY(ws, scratch_(need));
+    NN_CHECK(kernel_(nnhip_draft_verify(D(target), target.cols(), draft ? D(*draft) : nullptr, draft ? draft->cols() : 0,
+                                        token_major ? 1 : 0, vocab, n, D(fed), D(start), batch, most_here, temperature,
+                                        accept ? D(*accept) : nullptr, pick ? D(*pick) : nullptr, W(accepted), W(tokens),
+                                        ws->data(), need, stream_),
+                     "draft_verify"));
+    tokens_out = tokens;
+    return accepted;
+}
+
 // ── layout (cpu_engine.hpp:226-287) ─────────────────────────────────────────
 Result<Tensor> HipEngine::rearrange_3d(const Tensor& x, std::size_t M, std::size_t B, std::size_t N, bool inverse)
 {

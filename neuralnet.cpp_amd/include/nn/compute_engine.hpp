@@ -41,6 +41,14 @@ struct KvPages
     std::size_t page = 1, heads = 1;
 };
 
+// The same with a byte a value (nnhip_kv8_pages): K and V (pages * page, at least heads * dim / 4 floats, each of four
+// bytes), a scale a row and head (pages * page, heads).
+struct KvPages8
+{
+    Tensor K, V, K_scale, V_scale, table;
+    std::size_t page = 1, heads = 1, dim = 1;
+};
+
 class ComputeEngine
 {
 public:
@@ -193,6 +201,47 @@ public:
     {
         (void)layers, (void)parent, (void)len, (void)fresh, (void)len_out;
         return fail("kv_reorder: not supported by this engine");
+    }
+    // Attention of a chunk of new tokens of every sequence: q (q_heads * dim, tokens), of which sequence b has start[b] ..
+    // start[b + 1) (start: batch + 1 numbers), at most `most`, the last of its len[b] positions; each sees the positions
+    // up to its own. O (q_heads * dim, tokens), zeros for tokens that no sequence has.
+    [[nodiscard]] virtual Result<Tensor> attn_chunk(const KvPages& cache, const Tensor& q, const Tensor& start,
+                                                    std::size_t most, const Tensor& len, const Tensor* slopes, Scalar alpha)
+    {
+        (void)cache, (void)q, (void)start, (void)most, (void)len, (void)slopes, (void)alpha;
+        return fail("attn_chunk: not supported by this engine");
+    }
+    // kv_append into 8-bit pages; what they hold of tokens' positions, k and v (heads * dim, tokens), zeros where there is
+    // no such row; attn_chunk over them.
+    [[nodiscard]] virtual Result<Tensor> kv8_append(KvPages8& cache, const Tensor& k, const Tensor& v, const Tensor* q,
+                                                    const Tensor& pos, const Tensor* seq, const Tensor* cos,
+                                                    const Tensor* sin)
+    {
+        (void)cache, (void)k, (void)v, (void)q, (void)pos, (void)seq, (void)cos, (void)sin;
+        return fail("kv8_append: not supported by this engine");
+    }
+    [[nodiscard]] virtual Result<Tensor> kv8_read(const KvPages8& cache, const Tensor& pos, const Tensor* seq, Tensor& v_out)
+    {
+        (void)cache, (void)pos, (void)seq, (void)v_out;
+        return fail("kv8_read: not supported by this engine");
+    }
+    [[nodiscard]] virtual Result<Tensor> attn_chunk8(const KvPages8& cache, const Tensor& q, const Tensor& start,
+                                                     std::size_t most, const Tensor& len, const Tensor* slopes, Scalar alpha)
+    {
+        (void)cache, (void)q, (void)start, (void)most, (void)len, (void)slopes, (void)alpha;
+        return fail("attn_chunk8: not supported by this engine");
+    }
+    // Which drafted tokens stand, and the token that comes after them (nnhip_draft_verify): the logits (vocab, tokens), or
+    // (tokens, vocab) if token_major; start (batch + 1). draft may be null (tokens without probabilities), accept (tokens)
+    // and pick (batch) where temperature is 0. Numbers of tokens that stand (batch), and the drawn ones in tokens_out.
+    [[nodiscard]] virtual Result<Tensor> draft_verify(const Tensor& target, const Tensor* draft, bool token_major,
+                                                      const Tensor& fed, const Tensor& start, std::size_t most,
+                                                      Scalar temperature, const Tensor* accept, const Tensor* pick,
+                                                      Tensor& tokens_out)
+    {
+        (void)target, (void)draft, (void)token_major, (void)fed, (void)start, (void)most, (void)temperature, (void)accept;
+        (void)pick, (void)tokens_out;
+        return fail("draft_verify: not supported by this engine");
     }
 
     // Queues everything t's values depend on, as a read through the engine

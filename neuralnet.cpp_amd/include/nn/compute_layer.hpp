@@ -464,6 +464,22 @@ struct PagedStep
     std::size_t group = 1;
 };
 
+// One step of a batch of sequences, any number of new tokens each: the tokens' positions and sequences, where each
+// sequence's tokens start among them (batch + 1), the most that one has, the lengths after them, and the rotation's tables
+// and slopes as above.
+struct ChunkStep
+{
+    Tensor pos, seq, start, len, cos, sin, slopes;
+    std::size_t most = 1;
+};
+// A layer's cache in 8 bits or float32.
+struct ChunkCache
+{
+    KvPages f32;
+    KvPages8 b8;
+    bool eight = false;
+};
+
 // ── multi-head attention core (reference compute_layer.hpp:1016-1412) ─────
 class AttentionBase : public Layer
 {
@@ -683,6 +699,24 @@ public:
                                         use_rope_ ? &step.cos : nullptr, use_rope_ ? &step.sin : nullptr));
         NN_TRY(o, engine.attn_paged(cache, use_rope_ ? turned : q0, step.len, step.shared.valid() ? &step.shared : nullptr,
                                     step.group, step.slopes.valid() ? &step.slopes : nullptr, scale_));
+        return w_o_.forward(engine, o);
+    }
+    // The same for chunks of new tokens, x (d_model, tokens): kv_append or kv8_append, then attn_chunk or attn_chunk8.
+    Result<Tensor> forward_chunk(ComputeEngine& engine, const Tensor& x, ChunkCache& cache, const ChunkStep& step)
+    {
+        NN_TRY(q0, w_q_.forward(engine, x));
+        NN_TRY(k, w_k_.forward(engine, x));
+        NN_TRY(v, w_v_.forward(engine, x));
+        const Tensor *q = use_rope_ ? &q0 : nullptr, *cos = use_rope_ ? &step.cos : nullptr,
+                     *sin = use_rope_ ? &step.sin : nullptr, *slopes = step.slopes.valid() ? &step.slopes : nullptr;
+        if (cache.eight)
+        {
+            NN_TRY(turned, engine.kv8_append(cache.b8, k, v, q, step.pos, &step.seq, cos, sin));
+            NN_TRY(o, engine.attn_chunk8(cache.b8, q ? turned : q0, step.start, step.most, step.len, slopes, scale_));
+            return w_o_.forward(engine, o);
+        }
+        NN_TRY(turned, engine.kv_append(cache.f32, k, v, q, step.pos, &step.seq, cos, sin));
+        NN_TRY(o, engine.attn_chunk(cache.f32, q ? turned : q0, step.start, step.most, step.len, slopes, scale_));
         return w_o_.forward(engine, o);
     }
     [[nodiscard]] std::size_t heads() const { return num_heads_; }
@@ -982,6 +1016,16 @@ public:
     {
         NN_TRY(n1, norm1_->forward(engine, x));
         NN_TRY(a, attn_.forward_paged(engine, n1, cache, step));
+        NN_TRY(r2, engine.elementwise_binary(BinaryOp::Add, x, a));
+        NN_TRY(n2, norm2_->forward(engine, r2));
+        NN_TRY(f, ff_.forward(engine, n2));
+        return engine.elementwise_binary(BinaryOp::Add, r2, f);
+    }
+
+    Result<Tensor> forward_chunk(ComputeEngine& engine, const Tensor& x, ChunkCache& cache, const ChunkStep& step)
+    {
+        NN_TRY(n1, norm1_->forward(engine, x));
+        NN_TRY(a, attn_.forward_chunk(engine, n1, cache, step));
         NN_TRY(r2, engine.elementwise_binary(BinaryOp::Add, x, a));
         NN_TRY(n2, norm2_->forward(engine, r2));
         NN_TRY(f, ff_.forward(engine, n2));
@@ -1507,6 +1551,250 @@ public:
         return out;
     }
 
+    // What speculate found: the sequences' tokens without the prompts and eos, and how many times the target model ran
+    // over drafted tokens, how many there were and how many of them stood.
+    struct Drafted
+    {
+        std::vector<std::vector<std::size_t>> tokens;
+        std::size_t passes = 0, drafted = 0, accepted = 0;
+    };
+
+    // What speculate asks of its sizes, before it runs any layer.
+    [[nodiscard]] Result<void> can_speculate(const GPTModel& draft, const std::vector<std::vector<std::size_t>>& prompts,
+                                             std::size_t max_new, std::size_t draft_len, Scalar temperature,
+                                             std::size_t cache_bits) const
+    {
+        auto bad = [](const char* why) { return fail(std::string("GPTModel speculate: ") + why); };
+        if (prompts.empty() || prompts.size() > kMostPrompts) return bad("1 to 1024 prompts");
+        if (draft_len == 0 || draft_len > 1023) return bad("1 to 1023 drafted tokens");
+        if (!(temperature >= 0) || temperature > std::numeric_limits<Scalar>::max()) return bad("temperature out of range");
+        if (cache_bits != 8 && cache_bits != 32) return bad("caches of 8 or 32 bits");
+        if (draft.vocab_ != vocab_) return bad("the draft's vocabulary is another");
+        for (const GPTModel* m : {this, &draft})
+            if (m->blocks_.empty() || m->d_model_ / m->blocks_[0]->attention().heads() > 128)
+                return bad("heads wider than 128");
+        std::size_t longest = 0;
+        for (const auto& p : prompts)
+        {
+            if (p.empty()) return bad("empty prompt");
+            if (p.size() > seq_len_) return bad("a prompt is longer than the context");
+            for (std::size_t t : p)
+                if (t >= vocab_) return bad("prompt token out of range");
+            longest = std::max(longest, p.size());
+        }
+        if (max_new == 0) return {};
+        const std::size_t fed = fed_(longest, max_new), rows = prompts.size() * std::min(draft_len + 1, std::min(max_new, seq_len_));
+        if (max_new > 1 && draft.seq_len_ < fed) return bad("the draft's context is shorter than the sequences");
+        if (vocab_ >= (std::size_t{1} << 24) || rows * vocab_ >= std::size_t{1} << 31)
+            return bad("too many logits: fewer prompts or drafted tokens");
+        if (prompts.size() * (fed / kServePage + 1) * kServePage >= std::size_t{1} << 24) return bad("too many cache rows");
+        return {};
+    }
+
+    // Speculative decoding (no reference counterpart): continues every prompt by up to max_new tokens, distributed as
+    // if each were drawn from this model's softmax(logits / temperature) (temperature 0: its largest logit). The draft
+    // model, cheaper to run and of the same vocabulary, proposes draft_len tokens one by one; this model then runs over
+    // all of them at once, and draft_verify keeps those that stand and draws the next one. A sequence ends at eos (an id
+    // past the vocabulary: none does), after max_new tokens or where the context is full.
+    //
+    // Both models' caches are paged and hold float32 or, with cache_bits 8, a byte a value and a scale a row and head.
+    // Prompts go in by chunks. What a rejected token left in a cache lies past its sequence's length and is written over
+    // by the next chunk. The host learns of a round once, by its two results a sequence: drafted tokens stay on the device.
+    Result<Drafted> speculate(ComputeEngine& engine, GPTModel& draft, const std::vector<std::vector<std::size_t>>& prompts,
+                              std::size_t max_new, std::size_t draft_len, Scalar temperature, std::size_t eos,
+                              std::uint64_t seed, std::size_t cache_bits)
+    {
+        constexpr std::size_t kPromptTokens = 1024;   // of all sequences together, in a pass
+        NN_CHECK(can_speculate(draft, prompts, max_new, draft_len, temperature, cache_bits));
+        const std::size_t B = prompts.size();
+        Drafted out;
+        out.tokens.resize(B);
+        if (max_new == 0) return out;
+
+        std::vector<std::vector<std::size_t>> text(prompts);   // with what was found
+        std::vector<std::size_t> most(B), in_draft(B, 0);      // tokens to add, and positions in the draft's caches
+        std::size_t longest = 0;
+        for (std::size_t b = 0; b < B; ++b)
+        {
+            most[b] = std::min(max_new, seq_len_ - prompts[b].size() + 1);
+            longest = std::max(longest, prompts[b].size());
+        }
+        Serving big, small;
+        NN_CHECK(serve_(engine, B, fed_(longest, max_new), cache_bits == 8, big));
+        NN_CHECK(draft.serve_(engine, B, std::min(draft.seq_len_, fed_(longest, max_new)), cache_bits == 8, small));
+        std::mt19937_64 rng{seed};
+        auto uniform = [&](std::size_t n) {   // multiples of 2^-24 below 1
+            Matrix m(n, 1);
+            for (std::size_t i = 0; i < n; ++i) m.data()[i] = static_cast<Scalar>(rng() >> 40) * Scalar{0x1p-24f};
+            return engine.from_matrix(m);
+        };
+        auto column = [&](const std::vector<std::size_t>& x) {
+            Matrix m(x.size(), 1);
+            for (std::size_t i = 0; i < x.size(); ++i) m.data()[i] = static_cast<Scalar>(x[i]);
+            return engine.from_matrix(m);
+        };
+        auto tokens_of = [&](const std::vector<Range>& r) {
+            std::vector<std::size_t> ids;
+            for (std::size_t b = 0; b < B; ++b)
+                ids.insert(ids.end(), text[b].begin() + static_cast<std::ptrdiff_t>(r[b].at),
+                           text[b].begin() + static_cast<std::ptrdiff_t>(r[b].at + r[b].n));
+            return column(ids);
+        };
+
+        // The prompts but their last tokens, which the first round feeds.
+        const std::size_t chunk = std::max<std::size_t>(1, kPromptTokens / B);
+        std::vector<Range> r(B);
+        for (std::size_t at = 0; at + 1 < longest; at += chunk)
+        {
+            for (std::size_t b = 0; b < B; ++b)
+            {
+                const std::size_t P = prompts[b].size() - 1;
+                r[b] = {std::min(at, P), std::min(chunk, P - std::min(at, P))};
+            }
+            NN_TRY(ids, tokens_of(r));
+            NN_CHECK(chunk_hidden_(engine, ids, r, big));
+            if (max_new > 1) NN_CHECK(draft.chunk_hidden_(engine, ids, r, small));
+        }
+        for (std::size_t b = 0; b < B; ++b) in_draft[b] = prompts[b].size() - 1;
+
+        std::vector<char> ended(B, 0);
+        for (;;)
+        {
+            // Of each live sequence: its last token, and as many drafted ones behind it as it has room for.
+            std::vector<Range> fed(B);
+            std::vector<std::size_t> first(B), order;   // its first row; the rows' last tokens, or 0 for drafted ones
+            std::size_t rows = 0, steps = 0;
+            for (std::size_t b = 0; b < B; ++b)
+            {
+                first[b] = rows;
+                const std::size_t left = most[b] - out.tokens[b].size();
+                fed[b] = {text[b].size() - 1, ended[b] || left == 0 ? 0 : std::min(draft_len, left - 1) + 1};
+                if (fed[b].n == 0) continue;
+                order.push_back(text[b].back());
+                order.resize(rows + fed[b].n, 0);
+                rows += fed[b].n;
+                steps = std::max(steps, fed[b].n - 1);
+            }
+            if (rows == 0) break;
+            NN_TRY(tokens, column(order));
+            Tensor guess;   // the draft's logits, a row for each of the target's
+            if (temperature > 0 && steps > 0)
+            {
+                guess = engine.create_tensor(rows, vocab_);
+                NN_CHECK(engine.zero(guess));
+            }
+
+            // Drafting. The first step also brings in the token that the draft has not seen, where all of its last ones
+            // stood.
+            Tensor prev;
+            std::vector<std::size_t> live;
+            for (std::size_t i = 0; i < steps; ++i)
+            {
+                std::vector<std::size_t> now, from, to, last;
+                std::size_t n = 0;
+                for (std::size_t b = 0; b < B; ++b)
+                {
+                    r[b] = {0, 0};
+                    if (fed[b].n < i + 2) continue;
+                    r[b] = i == 0 ? Range{in_draft[b], text[b].size() - in_draft[b]} : Range{text[b].size() - 1 + i, 1};
+                    n += r[b].n;
+                    last.push_back(n - 1);
+                    to.push_back(first[b] + i);
+                    if (i > 0) from.push_back(static_cast<std::size_t>(std::lower_bound(live.begin(), live.end(), b) - live.begin()));
+                    now.push_back(b);
+                }
+                Tensor ids = prev;
+                if (i == 0)
+                {
+                    NN_TRY(t, tokens_of(r));
+                    ids = t;
+                }
+                else if (now.size() != live.size())
+                {
+                    NN_TRY(f, column(from));
+                    NN_TRY(t, engine.gather_rows(prev, f));
+                    ids = t;
+                }
+                NN_TRY(x0, draft.chunk_hidden_(engine, ids, r, small));
+                Tensor x = x0;
+                if (n != now.size())
+                {
+                    NN_TRY(xt, engine.transpose(x0));
+                    NN_TRY(at, column(last));
+                    NN_TRY(g, engine.gather_rows(xt, at));
+                    NN_TRY(xl, engine.transpose(g));
+                    x = xl;
+                }
+                NN_TRY(logits, draft.paged_logits_(engine, x));
+                std::vector<std::size_t> starts(now.size() + 1);
+                for (std::size_t j = 0; j < starts.size(); ++j) starts[j] = j;
+                NN_TRY(st, column(starts));
+                NN_TRY(rt, column(to));
+                Tensor accept, pick, next;
+                if (temperature > 0)
+                {
+                    NN_TRY(u, uniform(now.size()));
+                    accept = pick = u;   // (there is nothing to accept)
+                    NN_TRY(lt, engine.transpose(logits));
+                    NN_CHECK(engine.scatter_add_rows(guess, rt, lt));
+                }
+                NN_CHECK(engine.draft_verify(logits, nullptr, false, rt, st, 1, temperature, accept.valid() ? &accept : nullptr,
+                                             pick.valid() ? &pick : nullptr, next));
+                for (std::size_t& t : to) ++t;
+                NN_TRY(behind, column(to));
+                NN_CHECK(engine.scatter_add_rows(tokens, behind, next));
+                prev = next;
+                live = now;
+            }
+
+            // The target over all of it.
+            NN_TRY(x, chunk_hidden_(engine, tokens, fed, big));
+            NN_TRY(logits, paged_logits_(engine, x));
+            std::vector<std::size_t> starts(first);
+            starts.push_back(rows);
+            NN_TRY(st, column(starts));
+            Tensor accept, pick, next, lt = logits;
+            if (temperature > 0)
+            {
+                NN_TRY(a, uniform(rows));
+                NN_TRY(p, uniform(B));
+                NN_TRY(t, engine.transpose(logits));
+                accept = a;
+                pick = p;
+                lt = t;
+            }
+            NN_TRY(stand, engine.draft_verify(lt, guess.valid() ? &guess : nullptr, temperature > 0, tokens, st,
+                                              std::min(rows, draft_len + 1), temperature, accept.valid() ? &accept : nullptr,
+                                              pick.valid() ? &pick : nullptr, next));
+            NN_TRY(sm, engine.to_matrix(stand));
+            NN_TRY(nm, engine.to_matrix(next));
+            NN_TRY(tm, engine.to_matrix(tokens));
+            ++out.passes;
+            for (std::size_t b = 0; b < B; ++b)
+            {
+                if (fed[b].n == 0) continue;
+                const std::size_t ok = std::min(static_cast<std::size_t>(sm.data()[b]), fed[b].n - 1);
+                const std::size_t had = text[b].size();
+                out.drafted += fed[b].n - 1;
+                out.accepted += ok;
+                for (std::size_t i = 0; i <= ok && !ended[b]; ++i)
+                {
+                    const Scalar f = i < ok ? tm.data()[first[b] + 1 + i] : nm.data()[b];
+                    const auto t = static_cast<std::size_t>(f < Scalar{0} ? Scalar{0} : f);
+                    if (t == eos)
+                        ended[b] = 1;
+                    else
+                    {
+                        text[b].push_back(t);
+                        out.tokens[b].push_back(t);
+                    }
+                }
+                in_draft[b] = std::min(had + fed[b].n - 2, text[b].size() - 1);
+            }
+        }
+        return out;
+    }
+
 private:
     // Rows of a layer's cache: the prompt's, and one a beam for every token that is fed.
     static std::size_t beam_rows_(std::size_t n_prompt, std::size_t beams, std::size_t steps)
@@ -1524,6 +1812,96 @@ private:
         for (std::size_t i = 0; i < blocks_.size(); ++i)
         {
             NN_TRY(y, blocks_[i]->forward_paged(engine, x, caches[i], step));
+            x = y;
+        }
+        return x;
+    }
+    // Positions [at, at + n) of a sequence.
+    struct Range
+    {
+        std::size_t at = 0, n = 0;
+    };
+    // What a batch of sequences keeps while it is continued: the layers' caches, and what every step has alike.
+    struct Serving
+    {
+        std::vector<ChunkCache> caches;
+        ChunkStep step;
+    };
+    static constexpr std::size_t kMostPrompts = 1024, kServePage = 16;
+
+    // The positions that a sequence feeds at most: all but its last token's.
+    [[nodiscard]] std::size_t fed_(std::size_t n_prompt, std::size_t max_new) const
+    {
+        return max_new >= seq_len_ - n_prompt + 1 ? seq_len_ : n_prompt + max_new - 1;
+    }
+    // Caches for `batch` sequences of up to `positions`, page i of sequence b being page b * width + i.
+    Result<void> serve_(ComputeEngine& engine, std::size_t batch, std::size_t positions, bool eight, Serving& s)
+    {
+        const std::size_t width = (positions + kServePage - 1) / kServePage, rows = batch * width * kServePage;
+        const CausalSelfAttention& attn = blocks_[0]->attention();
+        Matrix m(batch, width);
+        for (std::size_t i = 0; i < m.size(); ++i) m.data()[i] = static_cast<Scalar>(i);
+        NN_TRY(table, engine.from_matrix(m));
+        s.caches.resize(blocks_.size());
+        for (ChunkCache& c : s.caches)
+        {
+            c.eight = eight;
+            if (eight)
+                c.b8 = KvPages8{engine.create_tensor(rows, (d_model_ + 3) / 4), engine.create_tensor(rows, (d_model_ + 3) / 4),
+                                engine.create_tensor(rows, attn.heads()), engine.create_tensor(rows, attn.heads()), table,
+                                kServePage, attn.heads(), d_model_ / attn.heads()};
+            else
+                c.f32 = KvPages{engine.create_tensor(rows, d_model_), engine.create_tensor(rows, d_model_), table, kServePage,
+                                attn.heads()};
+            if (eight)
+                for (Tensor* t : {&c.b8.K, &c.b8.V, &c.b8.K_scale, &c.b8.V_scale}) NN_CHECK(engine.zero(*t));
+            else
+                for (Tensor* t : {&c.f32.K, &c.f32.V}) NN_CHECK(engine.zero(*t));
+        }
+        if (attn.rope()) NN_CHECK(attn.rope()->table(engine, std::min(seq_len_, positions), s.step.cos, s.step.sin));
+        if (!attn.slopes().empty())
+        {
+            Matrix sl(attn.slopes().size(), 1);
+            std::copy(attn.slopes().begin(), attn.slopes().end(), sl.data());
+            NN_TRY(t, engine.from_matrix(sl));
+            s.step.slopes = t;
+        }
+        return {};
+    }
+    // Tokens ids, the positions r of each sequence one after another, through the blocks: hidden states (d_model, tokens).
+    Result<Tensor> chunk_hidden_(ComputeEngine& engine, const Tensor& ids, const std::vector<Range>& r, Serving& s)
+    {
+        const std::size_t n = ids.size(), B = r.size();
+        Matrix pos(n, 1), seq(n, 1), start(B + 1, 1), len(B, 1);
+        std::size_t i = 0;
+        s.step.most = 1;
+        for (std::size_t b = 0; b < B; ++b)
+        {
+            start.data()[b] = static_cast<Scalar>(i);
+            len.data()[b] = static_cast<Scalar>(r[b].at + r[b].n);
+            s.step.most = std::max(s.step.most, r[b].n);
+            for (std::size_t j = 0; j < r[b].n; ++j, ++i)
+            {
+                pos.data()[i] = static_cast<Scalar>(r[b].at + j);
+                seq.data()[i] = static_cast<Scalar>(b);
+            }
+        }
+        start.data()[B] = static_cast<Scalar>(i);
+        NN_TRY(pt, engine.from_matrix(pos));
+        NN_TRY(qt, engine.from_matrix(seq));
+        NN_TRY(tt, engine.from_matrix(start));
+        NN_TRY(lt, engine.from_matrix(len));
+        s.step.pos = pt;
+        s.step.seq = qt;
+        s.step.start = tt;
+        s.step.len = lt;
+        NN_TRY(emb, engine.gather_rows(token_emb_, ids));
+        NN_TRY(x0, engine.transpose(emb));
+        NN_TRY(xp, pos_->apply_positions(engine, x0, s.step.pos));
+        Tensor x = xp;
+        for (std::size_t b = 0; b < blocks_.size(); ++b)
+        {
+            NN_TRY(y, blocks_[b]->forward_chunk(engine, x, s.caches[b], s.step));
             x = y;
         }
         return x;

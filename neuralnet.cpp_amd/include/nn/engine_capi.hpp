@@ -248,6 +248,63 @@ inline int engine_op(EngineHandle* e, int op, void* const* in, std::size_t n_in,
         out[1] = new_tensor(len);
         return 0;
     }
+    case 35:   // args page, heads, most, alpha, with slopes: K, V, table, q, start, len[, slopes]
+    {
+        if (!need(6, 1, 5)) return 1;
+        const bool slopes = flag(4);
+        if (!need(slopes ? 7 : 6, 1, 5)) return 1;
+        const KvPages c{in_t(0), in_t(1), in_t(2), sz(0), sz(1)};
+        auto r = E.attn_chunk(c, in_t(3), in_t(4), sz(2), in_t(5), slopes ? &in_t(6) : nullptr, sc(3));
+        return put(0, r);
+    }
+    case 36:   // args page, heads, dim, with q, with cos and sin, with seq: K, V, K_scale, V_scale, table, k, v, pos[, q]
+               // [, cos, sin][, seq]
+    {
+        if (!need(8, 0, 6)) return 1;
+        const bool q = flag(3), rope = flag(4), seq = flag(5);
+        if (!need(8 + (q ? 1 : 0) + (rope ? 2 : 0) + (seq ? 1 : 0), q ? 1 : 0, 6)) return 1;
+        KvPages8 c{in_t(0), in_t(1), in_t(2), in_t(3), in_t(4), sz(0), sz(1), sz(2)};
+        std::size_t i = 8;
+        const Tensor *tq = q ? &in_t(i++) : nullptr, *cos = rope ? &in_t(i++) : nullptr, *sin = rope ? &in_t(i++) : nullptr;
+        auto r = E.kv8_append(c, in_t(5), in_t(6), tq, in_t(7), seq ? &in_t(i) : nullptr, cos, sin);
+        if (!r) return set_error(r.error().message);
+        if (q) out[0] = new_tensor(*r);
+        return 0;
+    }
+    case 37:   // args page, heads, dim: K, V, K_scale, V_scale, table, pos[, seq]
+    {
+        if (!need(6, 2, 3)) return 1;
+        const KvPages8 c{in_t(0), in_t(1), in_t(2), in_t(3), in_t(4), sz(0), sz(1), sz(2)};
+        Tensor v;
+        auto r = E.kv8_read(c, in_t(5), opt_mask(6), v);
+        if (put(0, r)) return 1;
+        out[1] = new_tensor(v);
+        return 0;
+    }
+    case 38:   // args page, heads, dim, most, alpha, with slopes: K, V, K_scale, V_scale, table, q, start, len[, slopes]
+    {
+        if (!need(8, 1, 6)) return 1;
+        const bool slopes = flag(5);
+        if (!need(slopes ? 9 : 8, 1, 6)) return 1;
+        const KvPages8 c{in_t(0), in_t(1), in_t(2), in_t(3), in_t(4), sz(0), sz(1), sz(2)};
+        auto r = E.attn_chunk8(c, in_t(5), in_t(6), sz(3), in_t(7), slopes ? &in_t(8) : nullptr, sc(4));
+        return put(0, r);
+    }
+    case 39:   // args most, temperature, token major, with draft, with accept and pick: target, fed, start[, draft]
+               // [, accept, pick]
+    {
+        if (!need(3, 2, 5)) return 1;
+        const bool draft = flag(3), random = flag(4);
+        if (!need(3 + (draft ? 1 : 0) + (random ? 2 : 0), 2, 5)) return 1;
+        std::size_t i = 3;
+        const Tensor *d = draft ? &in_t(i++) : nullptr, *accept = random ? &in_t(i++) : nullptr,
+                     *pick = random ? &in_t(i) : nullptr;
+        Tensor k;
+        auto r = E.draft_verify(in_t(0), d, flag(2), in_t(1), in_t(2), sz(0), sc(1), accept, pick, k);
+        if (put(0, r)) return 1;
+        out[1] = new_tensor(k);
+        return 0;
+    }
     default:
         return set_error("engine_op: unknown op " + std::to_string(op));
     }
@@ -310,7 +367,7 @@ struct GptSession
     std::size_t vocab = 0, seq = 0, batch = 0, num_valid = 0;
     Tensor tokens, labels, mask, logits;
     bool has_batch = false, has_mask = false;
-    bool searched = false;   // a beam search took the layers' inputs since the last forward pass
+    bool searched = false;   // a beam search or drafting took the layers' inputs since the last forward pass
     GptConfigC cfg{};
 };
 
@@ -688,6 +745,54 @@ catch (const std::exception& e)
     return set_error(std::string("gpt_beam_search: ") + e.what());
 }
 
+// GPTModel::speculate: the prompts one after another, the sequences' tokens from i * max_new on; stats (passes, drafted,
+// accepted) may be null.
+inline int gpt_speculate(GptSession* g, GptSession* draft, const std::uint64_t* prompts, const std::size_t* prompt_len,
+                         std::size_t n, std::size_t max_new, std::size_t draft_len, float temperature, std::uint64_t eos,
+                         std::uint64_t seed, std::size_t cache_bits, std::uint64_t* out, std::size_t* out_len,
+                         std::uint64_t* stats)
+try
+{
+    GPTModel *m = g ? gpt_model(g) : nullptr, *d = draft ? gpt_model(draft) : nullptr;
+    if (!m || !d) return set_error("gpt_speculate: a session holds no GPT model");
+    if (g->eng != draft->eng) return set_error("gpt_speculate: the draft session is on another engine");
+    if (!prompts || !prompt_len || !out || !out_len) return set_error("gpt_speculate: null argument");
+    if (n == 0 || n > 1024) return set_error("gpt_speculate: 1 to 1024 prompts");
+    std::vector<std::vector<std::size_t>> pr(n);
+    for (std::size_t i = 0; i < n; prompts += prompt_len[i++])
+    {
+        if (prompt_len[i] > m->seq_len()) return set_error("gpt_speculate: a prompt is longer than the context");
+        for (std::size_t j = 0; j < prompt_len[i]; ++j)
+        {
+            if (prompts[j] >= m->vocab_size()) return set_error("gpt_speculate: prompt token out of range");
+            pr[i].push_back(static_cast<std::size_t>(prompts[j]));
+        }
+    }
+    if (auto r = m->can_speculate(*d, pr, max_new, draft_len, temperature, cache_bits); !r)
+        return set_error(r.error().message);
+    if (max_new > 0) g->searched = draft->searched = true;   // layers will run
+    if (auto r = g->eng->begin_batch(); !r) return set_error(r.error().message);
+    auto s = m->speculate(*g->eng, *d, pr, max_new, draft_len, temperature, static_cast<std::size_t>(eos), seed, cache_bits);
+    if (!s) return set_error(s.error().message);
+    if (auto r = g->eng->end_batch(); !r) return set_error(r.error().message);
+    for (std::size_t i = 0; i < n; ++i)
+    {
+        out_len[i] = s->tokens[i].size();
+        std::copy(s->tokens[i].begin(), s->tokens[i].end(), out + i * max_new);
+    }
+    if (stats)
+    {
+        stats[0] = s->passes;
+        stats[1] = s->drafted;
+        stats[2] = s->accepted;
+    }
+    return 0;
+}
+catch (const std::exception& e)
+{
+    return set_error(std::string("gpt_speculate: ") + e.what());
+}
+
 inline int gpt_step(GptSession* g)
 {
     if (auto r = g->eng->begin_batch(); !r) return set_error(r.error().message);
@@ -986,6 +1091,14 @@ inline int layer_program(const char* name, std::uint32_t param, std::uint8_t* in
     {                                                                                                               \
         return nn::capi::gpt_beam_search(static_cast<nn::capi::GptSession*>(g), prompt, n_prompt, beams, max_new,  \
                                          eos, out, out_len, out_scores);                                            \
+    }                                                                                                               \
+    int NN_CAPI_CAT(P, gpt_speculate)(void* g, void* draft, const uint64_t* prompts, const size_t* prompt_len, size_t n, \
+                                      size_t max_new, size_t draft_len, float temperature, uint64_t eos, uint64_t seed, \
+                                      size_t cache_bits, uint64_t* out, size_t* out_len, uint64_t* stats)           \
+    {                                                                                                               \
+        return nn::capi::gpt_speculate(static_cast<nn::capi::GptSession*>(g),                                      \
+                                       static_cast<nn::capi::GptSession*>(draft), prompts, prompt_len, n, max_new,  \
+                                       draft_len, temperature, eos, seed, cache_bits, out, out_len, stats);         \
     }                                                                                                               \
     int NN_CAPI_CAT(P, gpt_generate)(void* g, const uint64_t* prompt, size_t n_prompt, size_t max_new,             \
                                      float temperature, uint64_t eos, size_t min_new, uint64_t seed, uint64_t* out,  \

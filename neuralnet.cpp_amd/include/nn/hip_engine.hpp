@@ -92,6 +92,16 @@ public:
                                std::size_t take, std::size_t eos, Tensor& beams_out, Tensor& tokens_out) override;
     Result<Tensor> kv_reorder(std::span<KvPages> layers, const Tensor& parent, const Tensor& len, const Tensor* fresh,
                               Tensor& len_out) override;
+    Result<Tensor> attn_chunk(const KvPages& cache, const Tensor& q, const Tensor& start, std::size_t most,
+                              const Tensor& len, const Tensor* slopes, Scalar alpha) override;
+    Result<Tensor> kv8_append(KvPages8& cache, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                              const Tensor* seq, const Tensor* cos, const Tensor* sin) override;
+    Result<Tensor> kv8_read(const KvPages8& cache, const Tensor& pos, const Tensor* seq, Tensor& v_out) override;
+    Result<Tensor> attn_chunk8(const KvPages8& cache, const Tensor& q, const Tensor& start, std::size_t most,
+                               const Tensor& len, const Tensor* slopes, Scalar alpha) override;
+    Result<Tensor> draft_verify(const Tensor& target, const Tensor* draft, bool token_major, const Tensor& fed,
+                                const Tensor& start, std::size_t most, Scalar temperature, const Tensor* accept,
+                                const Tensor* pick, Tensor& tokens_out) override;
 
     Result<Tensor> matmul(const Tensor& A, const Tensor& B, bool transA, bool transB) override;
     Result<Tensor> batched_matmul(const Tensor& A, const Tensor& B, std::size_t batch, bool transA, bool transB,

@@ -30,7 +30,8 @@ OP = dict(CLONE=1, SLICE_ROWS=2, INSERT_ROWS=3, GATHER_ROWS=4, SCATTER_ADD_ROWS=
           BMM_BWD_KV=14, COL_SOFTMAX_DENOM=15, COL_SOFTMAX_SPARSE=16, ADD_INPLACE=17, SCALE_INPLACE=18,
           AXPY_INPLACE=19, ZERO=20, ROW_REDUCE_SUM=21, COL_REDUCE_SUM=22, ROW_REDUCE_MAX=23,
           COL_REDUCE_MAX=24, BROADCAST_ROW=25, BROADCAST_COL=26, UNARY=27, BINARY=28, BINARY_SCALAR=29,
-          SELECT_SCALAR_COND=30, KV_APPEND=31, ATTN_PAGED=32, BEAM_SELECT=33, KV_REORDER=34)
+          SELECT_SCALAR_COND=30, KV_APPEND=31, ATTN_PAGED=32, BEAM_SELECT=33, KV_REORDER=34,
+          ATTN_CHUNK=35, KV8_APPEND=36, KV8_READ=37, ATTN_CHUNK8=38, DRAFT_VERIFY=39)
 
 # Enum values of compute_engine.hpp:43-82.
 UNARY = dict(Neg=0, Exp=1, Log=2, Sqrt=3, Rsqrt=4, Abs=5, Tanh=6)
@@ -127,6 +128,8 @@ def _bind(lib: ctypes.CDLL, prefix: str):
         "gpt_reset_cache": (i32, [vp]),
         "gpt_generate": (i32, [vp, u64p, sz, sz, ctypes.c_float, ctypes.c_uint64, sz, ctypes.c_uint64, u64p, sz,
                                ctypes.POINTER(ctypes.c_size_t)]),
+        "gpt_speculate": (i32, [vp, vp, u64p, ctypes.POINTER(sz), sz, sz, sz, ctypes.c_float, ctypes.c_uint64,
+                                ctypes.c_uint64, sz, u64p, ctypes.POINTER(sz), u64p]),
         "gpt_beam_search": (i32, [vp, u64p, sz, sz, sz, ctypes.c_uint64, u64p, ctypes.POINTER(sz), fp]),
         "build_attention_mask": (i32, [sz, sz, sz, i32, fp, ctypes.POINTER(ctypes.c_uint64), sz, fp]),
     }
@@ -367,6 +370,47 @@ class Engine:
         """caches: (K, V) of each layer. Returns (table, lens) of the sequences that continue parent."""
         ins = [table, parent, lens] + ([fresh] if fresh is not None else []) + [t for kv in caches for t in kv]
         return tuple(self._op("KV_REORDER", ins, 2, [page, heads, len(caches), fresh is not None]))
+
+    def attn_chunk(self, K, V, table, q, start, lens, most, alpha, page=1, heads=1, slopes=None):
+        """Attention of each sequence's new tokens start[b] .. start[b + 1) of q (q_heads * dim, tokens), the last of its
+        lens[b] positions, over the positions up to their own."""
+        ins = [K, V, table, q, start, lens] + ([slopes] if slopes is not None else [])
+        return self._op("ATTN_CHUNK", ins, 1, [page, heads, most, alpha, slopes is not None])[0]
+
+    def kv8_cache(self, pages, page, heads, dim):
+        """(K, V, K_scale, V_scale) of an 8-bit paged cache, zeroed: bytes in floats of four, a scale a row and head."""
+        out = [self.create_tensor(pages * page, n) for n in ((heads * dim + 3) // 4,) * 2 + (heads,) * 2]
+        for t in out:
+            self.zero(t)
+        return tuple(out)
+
+    def kv8_append(self, cache, table, k, v, pos, page, heads, dim, q=None, cos=None, sin=None, seq=None):
+        """kv_append into an 8-bit cache (K, V, K_scale, V_scale, in place)."""
+        if (cos is None) != (sin is None):
+            raise EngineError("kv8_append: cos and sin go together")
+        ins = [*cache, table, k, v, pos] + [t for t in (q, cos, sin, seq) if t is not None]
+        out = self._op("KV8_APPEND", ins, 0 if q is None else 1,
+                       [page, heads, dim, q is not None, cos is not None, seq is not None])
+        return out[0] if out else None
+
+    def kv8_read(self, cache, table, pos, page, heads, dim, seq=None):
+        """(k, v), (heads * dim, tokens) each: what an 8-bit cache holds of the tokens' positions."""
+        return tuple(self._op("KV8_READ", [*cache, table, pos] + ([seq] if seq is not None else []), 2, [page, heads, dim]))
+
+    def attn_chunk8(self, cache, table, q, start, lens, most, alpha, page, heads, dim, slopes=None):
+        """attn_chunk over an 8-bit cache (K, V, K_scale, V_scale)."""
+        ins = [*cache, table, q, start, lens] + ([slopes] if slopes is not None else [])
+        return self._op("ATTN_CHUNK8", ins, 1, [page, heads, dim, most, alpha, slopes is not None])[0]
+
+    def draft_verify(self, target, fed, start, most, temperature=0.0, draft=None, accept=None, pick=None,
+                     token_major=False):
+        """Which drafted tokens stand: (accepted, tokens), the number of them and the token that comes next, a sequence
+        each. target and draft: logits (vocab, tokens), or (tokens, vocab) if token_major."""
+        if (accept is None) != (pick is None):
+            raise EngineError("draft_verify: accept and pick go together")
+        ins = [target, fed, start] + [t for t in (draft, accept, pick) if t is not None]
+        return tuple(self._op("DRAFT_VERIFY", ins, 2, [most, temperature, token_major, draft is not None,
+                                                       accept is not None]))
 
     # -- pure host helpers ------------------------------------------------------
     def build_attention_mask(self, batch, seq, heads, use_alibi, slopes=(), doc_ids=()):
@@ -616,6 +660,26 @@ class GptSession:
         self._eng._check(self._f["gpt_beam_search"](self._g, pr.ctypes.data_as(u64p), pr.size, int(beams), int(max_new),
                                                     int(eos), out.ctypes.data_as(u64p), n, _fptr(scores)))
         return [(out[i * max_new:i * max_new + n[i]].astype(np.int64).tolist(), float(scores[i])) for i in range(beams)]
+
+    def speculate(self, draft: "GptSession", prompts, max_new: int, draft_len: int = 4, temperature: float = 0.0,
+                  eos: int = 2 ** 64 - 1, seed: int = 0, cache_bits: int = 32):
+        """Speculative decoding: continues the prompts (lists of token ids) by up to max_new tokens each, `draft`, a session
+        of the same engine and vocabulary, proposing draft_len tokens at a time. Returns (lists of token ids, dict of
+        passes, drafted and accepted)."""
+        prompts = [np.asarray(p, dtype=np.uint64).reshape(-1) for p in prompts]
+        if max_new < 0 or draft_len < 0 or not prompts:
+            raise EngineError("speculate: no prompts, or max_new or draft_len negative")
+        max_new = min(int(max_new), self.seq_len)   # more never fit behind a prompt
+        flat = np.ascontiguousarray(np.concatenate(prompts + [np.zeros(1, np.uint64)]))
+        lens = (ctypes.c_size_t * len(prompts))(*[p.size for p in prompts])
+        out = np.zeros(max(1, len(prompts) * max_new), dtype=np.uint64)
+        n, stats = (ctypes.c_size_t * len(prompts))(), (ctypes.c_uint64 * 3)()
+        u64p = ctypes.POINTER(ctypes.c_uint64)
+        self._eng._check(self._f["gpt_speculate"](self._g, draft._g, flat.ctypes.data_as(u64p), lens, len(prompts), max_new,
+                                                  int(draft_len), float(temperature), int(eos), int(seed), int(cache_bits),
+                                                  out.ctypes.data_as(u64p), n, stats))
+        return ([out[i * max_new:i * max_new + n[i]].astype(np.int64).tolist() for i in range(len(prompts))],
+                dict(zip(("passes", "drafted", "accepted"), map(int, stats))))
 
     def backward_scaled(self, grad_scale: float) -> None:
         """Backward of one accumulated micro-batch: loss gradient scaled by grad_scale first."""

@@ -81,11 +81,77 @@ class CpuEngine final : public ComputeEngine
     // Row of position pos of the table's row b; false where there is none.
     static bool page_row_(const KvPages& c, std::size_t b, std::size_t pos, std::size_t& row)
     {
-        const std::size_t i = pos / c.page;
+        return page_row_(c.table, c.page, c.K.rows() / c.page, b, pos, row);
+    }
+    static bool page_row_(const Tensor& table, std::size_t page, std::size_t pages, std::size_t b, std::size_t pos,
+                          std::size_t& row)
+    {
+        const std::size_t i = pos / page;
         std::size_t p;
-        if (i >= c.table.cols() || !row_index(P(c.table)[b * c.table.cols() + i], c.K.rows() / c.page, p)) return false;
-        row = p * c.page + pos % c.page;
+        if (i >= table.cols() || !row_index(P(table)[b * table.cols() + i], pages, p)) return false;
+        row = p * page + pos % page;
         return true;
+    }
+    // Byte e of head h in a row of an 8-bit cache's K or V.
+    static int byte_(const KvPages8& c, const Tensor& x, std::size_t row, std::size_t h, std::size_t e)
+    {
+        return reinterpret_cast<const signed char*>(P(x))[row * 4 * x.cols() + h * c.dim + e];
+    }
+    // attn_chunk over either cache; at(tensor, scales, row, head, feature) is a value of it.
+    template <class At>
+    static Result<Tensor> chunk_(const Tensor& table, std::size_t page, std::size_t pages, std::size_t heads, std::size_t d,
+                                 std::size_t H, const Tensor& q, const Tensor& start, std::size_t most, const Tensor& len,
+                                 const Tensor* slopes, Scalar alpha, At&& at, const Tensor& K, const Tensor* K_scale,
+                                 const Tensor& V, const Tensor* V_scale)
+    {
+        const std::size_t N = q.cols(), per = H / heads;
+        const double none = -std::numeric_limits<double>::infinity();
+        Matrix out(q.rows(), N);
+        std::vector<std::size_t> rows, pos;
+        std::vector<double> s, o(d);
+        for (std::size_t b = 0; b < table.rows(); ++b)
+        {
+            const std::size_t first = length_(P(start)[b], N), end = length_(P(start)[b + 1], N),
+                              length = length_(P(len)[b], table.cols() * page), n = end > first ? end - first : 0;
+            for (std::size_t i = 0; i < std::min(n, most); ++i)
+            {
+                if (length + i + 1 <= n) continue;   // in front of the first position
+                const std::size_t p = length + i - n;
+                rows.clear();
+                pos.clear();
+                for (std::size_t j = 0; j <= p; ++j)
+                {
+                    std::size_t r;
+                    if (!page_row_(table, page, pages, b, j, r)) continue;
+                    rows.push_back(r);
+                    pos.push_back(j);
+                }
+                for (std::size_t h = 0; h < H; ++h)
+                {
+                    s.assign(rows.size(), 0.0);
+                    double m = none, l = 0.0;
+                    for (std::size_t x = 0; x < rows.size(); ++x)
+                    {
+                        double dot = 0.0;
+                        for (std::size_t e = 0; e < d; ++e)
+                            dot += static_cast<double>(P(q)[(h * d + e) * N + first + i]) * at(K, K_scale, rows[x], h / per, e);
+                        s[x] = alpha * dot - (slopes ? static_cast<double>(P(*slopes)[h]) * static_cast<double>(p - pos[x]) : 0.0);
+                        m = std::max(m, s[x]);
+                    }
+                    std::fill(o.begin(), o.end(), 0.0);
+                    if (m != none)
+                        for (std::size_t x = 0; x < rows.size(); ++x)
+                        {
+                            const double w = std::exp(s[x] - m);
+                            l += w;
+                            for (std::size_t e = 0; e < d; ++e) o[e] += w * at(V, V_scale, rows[x], h / per, e);
+                        }
+                    for (std::size_t e = 0; e < d; ++e)
+                        out.data()[(h * d + e) * N + first + i] = l == 0.0 ? 0.0f : static_cast<float>(o[e] / l);
+                }
+            }
+        }
+        return Tensor::from_matrix(std::move(out));
     }
     static bool on_cpu_(std::initializer_list<const Tensor*> ts)
     {
@@ -362,6 +428,202 @@ public:
         }
         len_out = Tensor::from_matrix(std::move(lens));
         return Tensor::from_matrix(std::move(out));
+    }
+
+    // Chunks of new tokens, 8-bit caches, drafted tokens (no reference counterpart): plain loops, sums in float64.
+    Result<Tensor> attn_chunk(const KvPages& c, const Tensor& q, const Tensor& start, std::size_t most, const Tensor& len,
+                              const Tensor* slopes, Scalar alpha) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.table, &q, &start, &len, slopes})) return fail("attn_chunk: tensors are not CPU");
+        const std::size_t d = paged::dim_of(c);
+        NN_TRY(H, paged::check_chunk("attn_chunk", d, c.heads, c.table.rows(), q, start, most, len, slopes));
+        return chunk_(c.table, c.page, c.K.rows() / c.page, c.heads, d, H, q, start, most, len, slopes, alpha,
+                      [&](const Tensor& x, const Tensor*, std::size_t row, std::size_t h, std::size_t e) -> double {
+                          return P(x)[row * x.cols() + h * d + e];
+                      },
+                      c.K, nullptr, c.V, nullptr);
+    }
+    Result<Tensor> attn_chunk8(const KvPages8& c, const Tensor& q, const Tensor& start, std::size_t most, const Tensor& len,
+                               const Tensor* slopes, Scalar alpha) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &q, &start, &len, slopes}))
+            return fail("attn_chunk8: tensors are not CPU");
+        NN_TRY(H, paged::check_chunk("attn_chunk8", paged::dim_of8(c), c.heads, c.table.rows(), q, start, most, len, slopes));
+        return chunk_(c.table, c.page, c.K.rows() / c.page, c.heads, c.dim, H, q, start, most, len, slopes, alpha,
+                      [&](const Tensor& x, const Tensor* scale, std::size_t row, std::size_t h, std::size_t e) -> double {
+                          return static_cast<double>(byte_(c, x, row, h, e)) * P(*scale)[row * c.heads + h];
+                      },
+                      c.K, &c.K_scale, c.V, &c.V_scale);
+    }
+    Result<Tensor> kv8_append(KvPages8& c, const Tensor& k, const Tensor& v, const Tensor* q, const Tensor& pos,
+                              const Tensor* seq, const Tensor* cos, const Tensor* sin) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &k, &v, q, &pos, seq, cos, sin}))
+            return fail("kv8_append: tensors are not CPU");
+        NN_TRY(s, paged::check_append8(c, k, v, q, pos, seq, cos, sin));
+        const Matrix* const all[] = {&c.K.cpu_matrix(), &c.V.cpu_matrix(), &c.K_scale.cpu_matrix(), &c.V_scale.cpu_matrix()};
+        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < i; ++j)
+                if (all[i] == all[j]) return fail("kv8_append: two of K, V and their scales are one tensor");
+        const std::size_t N = k.cols(), d = s.dim, h = s.half;
+        Tensor out;
+        if (q) out = Tensor::from_matrix(Matrix(q->cpu_matrix()));
+        std::vector<double> y(d);
+        for (std::size_t n = 0; n < N; ++n)
+        {
+            std::size_t b = n, p, row;
+            if (seq ? !row_index(P(*seq)[n], c.table.rows(), b) : n >= c.table.rows()) continue;
+            if (!row_index(P(pos)[n], paged::kMaxIndex, p) || (cos && p >= cos->rows()) ||
+                !page_row_(c.table, c.page, c.K.rows() / c.page, b, p, row))
+                continue;
+            auto head = [&](const Tensor& x, std::size_t e, bool turn) {
+                for (std::size_t j = 0; j < d; ++j)
+                {
+                    y[j] = P(x)[(e * d + j) * N + n];
+                    if (!turn || j >= 2 * h) continue;
+                    const std::size_t i = j < h ? j : j - h;
+                    const double o = P(x)[(e * d + (j < h ? j + h : i)) * N + n], co = P(*cos)[p * h + i], si = P(*sin)[p * h + i];
+                    y[j] = j < h ? y[j] * co - o * si : y[j] * co + o * si;
+                }
+            };
+            auto store = [&](Tensor& to, Tensor& scales, std::size_t e) {
+                double most = 0.0;
+                bool finite = true;
+                for (double x : y)
+                {
+                    most = std::max(most, std::abs(x));
+                    finite = finite && std::isfinite(x);
+                }
+                const float scale = finite ? static_cast<float>(most / 127.0) : std::numeric_limits<float>::quiet_NaN();
+                W(scales)[row * c.heads + e] = scale;
+                auto* to8 = reinterpret_cast<signed char*>(W(to)) + row * 4 * to.cols() + e * d;
+                for (std::size_t j = 0; j < d; ++j)
+                    to8[j] = !(scale > 0.0f) ? 0 : static_cast<signed char>(std::clamp(std::nearbyint(y[j] / scale), -127.0, 127.0));
+            };
+            for (std::size_t e = 0; e < c.heads; ++e)
+            {
+                head(k, e, true);
+                store(c.K, c.K_scale, e);
+                head(v, e, false);
+                store(c.V, c.V_scale, e);
+            }
+            for (std::size_t e = 0; e < s.q_heads; ++e)
+            {
+                head(*q, e, true);
+                for (std::size_t j = 0; j < d; ++j) W(out)[(e * d + j) * N + n] = static_cast<float>(y[j]);
+            }
+        }
+        return out;
+    }
+    Result<Tensor> kv8_read(const KvPages8& c, const Tensor& pos, const Tensor* seq, Tensor& v_out) override
+    {
+        if (!on_cpu_({&c.K, &c.V, &c.K_scale, &c.V_scale, &c.table, &pos, seq})) return fail("kv8_read: tensors are not CPU");
+        NN_TRY(N, paged::check_read8(c, pos, seq));
+        Matrix k(c.heads * c.dim, N), v(c.heads * c.dim, N);
+        for (std::size_t n = 0; n < N; ++n)
+        {
+            std::size_t b = n, p, row;
+            if (seq ? !row_index(P(*seq)[n], c.table.rows(), b) : n >= c.table.rows()) continue;
+            if (!row_index(P(pos)[n], paged::kMaxIndex, p) || !page_row_(c.table, c.page, c.K.rows() / c.page, b, p, row)) continue;
+            for (std::size_t f = 0; f < c.heads * c.dim; ++f)
+            {
+                const std::size_t e = f / c.dim, j = f % c.dim;
+                k.data()[f * N + n] = static_cast<float>(byte_(c, c.K, row, e, j)) * P(c.K_scale)[row * c.heads + e];
+                v.data()[f * N + n] = static_cast<float>(byte_(c, c.V, row, e, j)) * P(c.V_scale)[row * c.heads + e];
+            }
+        }
+        v_out = Tensor::from_matrix(std::move(v));
+        return Tensor::from_matrix(std::move(k));
+    }
+    Result<Tensor> draft_verify(const Tensor& target, const Tensor* draft, bool token_major, const Tensor& fed,
+                                const Tensor& start, std::size_t most, Scalar temperature, const Tensor* accept,
+                                const Tensor* pick, Tensor& tokens_out) override
+    {
+        if (!on_cpu_({&target, draft, &fed, &start, accept, pick})) return fail("draft_verify: tensors are not CPU");
+        NN_TRY(B, paged::check_verify(target, draft, token_major, fed, start, most, temperature, accept, pick));
+        const std::size_t N = fed.size(), V = target.size() / N;
+        const double none = -std::numeric_limits<double>::infinity();
+        auto logit = [&](const Tensor& x, std::size_t n, std::size_t v) -> double {
+            const float f = P(x)[token_major ? n * V + v : v * N + n];
+            return f != f ? none : static_cast<double>(f);
+        };
+        auto softmax = [&](const Tensor& x, std::size_t n, std::vector<double>& p) {
+            double m = none, sum = 0.0;
+            for (std::size_t v = 0; v < V; ++v) m = std::max(m, logit(x, n, v));
+            p.assign(V, 0.0);
+            if (m == none) return;
+            for (std::size_t v = 0; v < V; ++v)
+            {
+                const double a = logit(x, n, v);
+                p[v] = std::isinf(m) ? (a == m ? 1.0 : 0.0) : std::exp((a - m) / temperature);
+                sum += p[v];
+            }
+            for (double& a : p) a /= sum;
+        };
+        Matrix accepted(B, 1), tokens(B, 1);
+        std::vector<double> p, q;
+        for (std::size_t b = 0; b < B; ++b)
+        {
+            const std::size_t first = length_(P(start)[b], N), end = length_(P(start)[b + 1], N),
+                              rows = end > first ? std::min(end - first, most) : 0;
+            std::size_t stand = 0;
+            float token = -1.0f;
+            for (std::size_t i = 0; i < rows; ++i)
+            {
+                const std::size_t n = first + i;
+                std::size_t x = 0;
+                const bool drafted = i + 1 < rows, known = drafted && row_index(P(fed)[n + 1], V, x);
+                if (temperature == 0)
+                {
+                    std::size_t best = 0;
+                    for (std::size_t v = 1; v < V; ++v)
+                        if (logit(target, n, v) > logit(target, n, best)) best = v;
+                    if (known && x == best)
+                    {
+                        ++stand;
+                        continue;
+                    }
+                    token = static_cast<float>(best);
+                    break;
+                }
+                softmax(target, n, p);
+                q.assign(V, 0.0);
+                if (drafted && draft) softmax(*draft, n, q);
+                if (known && !draft) q[x] = 1.0;
+                if (known && static_cast<double>(P(*accept)[n]) * q[x] < p[x])
+                {
+                    ++stand;
+                    continue;
+                }
+                double sum = 0.0;
+                if (drafted)
+                {
+                    for (std::size_t v = 0; v < V; ++v) sum += q[v] = std::max(p[v] - q[v], 0.0);
+                    if (sum > 0.0) p.swap(q);
+                }
+                if (!(sum > 0.0))
+                {
+                    sum = 0.0;
+                    for (double a : p) sum += a;
+                }
+                const float u = P(*pick)[b];
+                const double at = (!(u > 0.0f) ? 0.0 : u >= 1.0f ? std::nextafter(1.0, 0.0) : u) * sum;
+                double upto = 0.0;
+                std::size_t v = 0, last = 0;
+                for (; v < V; ++v)
+                {
+                    upto += p[v];
+                    if (p[v] > 0.0) last = v;
+                    if (upto > at) break;
+                }
+                token = static_cast<float>(v < V ? v : last);
+                break;
+            }
+            accepted.data()[b] = static_cast<float>(stand);
+            tokens.data()[b] = token;
+        }
+        tokens_out = Tensor::from_matrix(std::move(tokens));
+        return Tensor::from_matrix(std::move(accepted));
     }
 
     // reference :226-279
