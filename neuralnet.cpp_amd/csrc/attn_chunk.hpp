@@ -25,6 +25,9 @@ struct ChunkArgs
     unsigned q_heads, tokens, most;
     unsigned ranges, slots;          // that the kernel cuts positions into; and results of a row
     int wide_from;                   // sequences of more rows are k_attn_chunk_wide's
+    char* images;                    // its keys' and values' parts: `tiles` a piece, of the pieces (slot and key head)
+    unsigned tiles, first_piece, pieces;   // that the launch is for
+    int slots_by_batch;              // a slot a sequence
     FastDiv by_per, by_heads, by_q_heads, by_row_blocks, by_ranges;   // by_row_blocks: of k_attn_chunk_wide
     int q_rows;                      // queries lie a token a row, 16-byte aligned
     int vec;                         // the cache's rows can be read in pieces of 4 values
@@ -515,6 +518,9 @@ __device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int 
 // k_attn_chunk8, and k_attn_chunk_wide: their launches; rows of a workgroup.
 void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s);
 constexpr int kWideRows = 128;
+constexpr int kNarrowRows = 32;   // of a sequence and key head that the kernels of few rows take at most
+size_t chunk_image_bytes(int bits, unsigned dim);
+void chunk_parts(const ChunkArgs& a, int bits, unsigned pieces, unsigned blocks, hipStream_t s);
 void chunk_wide(const ChunkArgs& a, int bits, unsigned blocks, hipStream_t s);
 
 } // namespace nnhip

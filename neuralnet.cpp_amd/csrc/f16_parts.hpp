@@ -24,6 +24,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNone = -200;   // exponent of nothing but zeros: below every float's
+constexpr int kLeastTop = -108;   // values below 2^kLeastTop are held against that: 2^(17 - kLeastTop) is a float
 
 // Two parts of eight floats that are scaled already. What rounding leaves of a pair, x - f16(x), is exact: the pair's dot
 // product with (-1, 0) or (0, -1) added to x, one instruction each.
@@ -55,10 +56,11 @@ __device__ __forceinline__ unsigned halves_of(unsigned two)
 __device__ __forceinline__ int exponent_of(float x) { return (int)max(__builtin_bit_cast(unsigned, x) >> 23 & 255u, 1u) - 126; }
 
 // The largest of N neighbouring lanes' numbers, none negative, in all of them: without LDS, which the shuffles take.
-template <int CTRL> __device__ __forceinline__ float max_dpp(float x)
+template <int CTRL> __device__ __forceinline__ float swap_dpp(float x)
 {
-    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 15, 15, true)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 15, 15, true));
 }
+template <int CTRL> __device__ __forceinline__ float max_dpp(float x) { return fmaxf(x, swap_dpp<CTRL>(x)); }
 template <int N> __device__ __forceinline__ float max_of(float x)
 {
     x = max_dpp<0xb1>(x);                           // lanes 1, 0, 3, 2 of each 4
@@ -83,6 +85,23 @@ template <class F> __device__ __forceinline__ float across(float x, F&& f)
     const auto z = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     const unsigned lo = z[0], hi = z[1];
     return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+// The largest over the wave of each of 8 numbers a lane, none negative: lane l has the number l % 8's.
+__device__ __forceinline__ float max_of_8(const float (&x)[8], int lane)
+{
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = fmaxf(lane & 4 ? x[4 + i] : x[i], swap_dpp<0x141>(lane & 4 ? x[i] : x[4 + i]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = fmaxf(lane & 2 ? a[2 + i] : a[i], swap_dpp<0x4e>(lane & 2 ? a[i] : a[2 + i]));
+    float r = fmaxf(lane & 1 ? b[1] : b[0], swap_dpp<0xb1>(lane & 1 ? b[0] : b[1]));
+    r = max_dpp<0x128>(r);   // each 16 turned by 8
+    unsigned u = __builtin_bit_cast(unsigned, r), v = u;
+    asm("" : "+v"(v));
+    const auto z = __builtin_amdgcn_permlane16_swap(u, v, false, false);
+    const unsigned lo = z[0], hi = z[1];
+    r = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+    return across(r, [](float y, float w) { return fmaxf(y, w); });
 }
 
 } // namespace nnhip

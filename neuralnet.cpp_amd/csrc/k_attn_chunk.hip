@@ -146,10 +146,13 @@ struct ChunkPlan
     int wide_from;
     unsigned narrow, wide;   // ranges of the two kernels' rows, 0: it is not launched
     size_t blocks, wide_row_blocks, wide_blocks;
+    size_t image_slots, image_tiles, image_pieces;   // of the parts; pieces that are formed at a time
     unsigned slots() const { return std::max(narrow, wide); }
 };
 
-constexpr size_t kNarrowRows = 32;   // of a sequence and key head that the walk takes
+// Parts of keys and values that are formed at a time, or those of one piece: past this a call takes several launches. They are
+// as large as the float32 cache of the sequences with many rows, which may be any of the batch's.
+constexpr size_t kImageBytes = (size_t)2 << 30;
 
 // How a call is cut, from its sizes alone: the lengths are on the device.
 ChunkPlan chunk_plan(const ChunkCall& c)
@@ -158,7 +161,7 @@ ChunkPlan chunk_plan(const ChunkCall& c)
     const size_t per = c.q_heads / c.c.t.heads, batch = c.c.t.batch, heads = c.c.t.heads;
     const size_t positions = (size_t)c.c.t.width * c.c.t.page.d, cus = device_cus();
     // No sequence has more rows: those of up to 16 have a kernel that holds fewer registers.
-    p.wide_from = static_cast<int>(std::min(kNarrowRows, (c.most * per + kTile - 1) / kTile * kTile));
+    p.wide_from = static_cast<int>(std::min<size_t>(kNarrowRows, (c.most * per + kTile - 1) / kTile * kTile));
     // Workgroups a CU. Where the key heads alone fill the CUs, float32 caches stream best with 8 (48 sequences of 4000 to 8000
     // positions, 8 heads of 128: 466 us with 2, 440 with 4, 400 with 8), bytes with 4 (143 us with 2 to 8; 5 rows a head 192
     // with 2, 188 with 4, 213 with 8); where they do not, ranges are more results to join (one sequence of 60000: 95 to 103
@@ -174,15 +177,23 @@ ChunkPlan chunk_plan(const ChunkCall& c)
         p.wide = static_cast<unsigned>(std::min<size_t>(std::min(std::max<size_t>(2 * cus / others, 1), most_wide), kMostRanges));
         p.wide_blocks = (p.wide_row_blocks * heads * p.wide + 7) / 8 * 8;
         if (batch == 1) p.narrow = 0, p.wide_from = 0;   // one launch, however few tokens the sequence has
+        p.image_slots = std::min(batch, c.tokens * per / (kNarrowRows + 1) + 1);
+        p.image_tiles = (positions + 31) / 32;
+        p.image_pieces = std::min(p.image_slots * heads, std::max<size_t>(kImageBytes / (p.image_tiles * chunk_image_bytes(c.bits, c.c.t.dim)), 1));
     }
     return p;
 }
 
 // m and l of every row and range, in whole 16 bytes.
 size_t ml_floats(const ChunkCall& c, const ChunkPlan& p) { return (2 * c.tokens * c.q_heads * p.slots() + 3) / 4 * 4; }
+// The ranges' results, in whole 16 bytes, and behind them the parts.
+size_t chunk_results(const ChunkCall& c, const ChunkPlan& p)
+{
+    return p.slots() == 1 ? 0 : (ml_floats(c, p) + (c.tokens * c.q_heads * p.slots() * c.c.t.dim + 3) / 4 * 4) * sizeof(float);
+}
 size_t chunk_workspace(const ChunkCall& c, const ChunkPlan& p)
 {
-    return p.slots() == 1 ? 0 : (ml_floats(c, p) + c.tokens * c.q_heads * p.slots() * c.c.t.dim) * sizeof(float);
+    return chunk_results(c, p) + p.image_pieces * p.image_tiles * chunk_image_bytes(c.bits, c.c.t.dim);
 }
 
 bool chunk_ok(const ChunkCall& c, size_t heads)
@@ -284,8 +295,20 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
         w.ranges = p.wide;
         w.by_ranges = FastDiv(p.wide);
         w.by_row_blocks = FastDiv(static_cast<unsigned>(p.wide_row_blocks));
-        chunk_wide(w, call.bits, static_cast<unsigned>(p.wide_blocks), s);
-        if (int rc = launch_status()) return rc;
+        w.images = static_cast<char*>(workspace) + chunk_results(call, p);
+        w.tiles = static_cast<unsigned>(p.image_tiles);
+        w.slots_by_batch = p.image_slots == call.c.t.batch;
+        const size_t all = p.image_slots * call.c.t.heads;
+        for (size_t at = 0; at < all; at += p.image_pieces)
+        {
+            const size_t pieces = std::min(p.image_pieces, all - at), each = std::min(p.image_tiles, (8 * device_cus() + pieces - 1) / pieces);
+            w.first_piece = static_cast<unsigned>(at);
+            w.pieces = static_cast<unsigned>(pieces);
+            chunk_parts(w, call.bits, w.pieces, static_cast<unsigned>(each), s);
+            if (int rc = launch_status()) return rc;
+            chunk_wide(w, call.bits, static_cast<unsigned>(p.wide_blocks), s);
+            if (int rc = launch_status()) return rc;
+        }
     }
     if (p.slots() == 1) return 0;
     const size_t rows = tokens * q_heads;

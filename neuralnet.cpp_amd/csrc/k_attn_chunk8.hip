@@ -42,6 +42,7 @@ template <int KS> struct Row8
 {
     half8 q[KS / 2][2];
     int seen;
+    int top;                    // exponent that the values' scales are held against: of those that the row sees
     float slope, scale, m, l;   // slope, scale and m: times log2(e)
     f32x4 o[Bytes<KS>::VB];
 };
@@ -199,6 +200,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
         }
         w.slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
         w.scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);
+        w.top = kNone;
         w.m = kLowest;
         w.l = 0.0f;
 #pragma unroll
@@ -206,7 +208,6 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
     }
     for (int o = 1; o < 16; o *= 2) all = min(all, __shfl_xor(all, o, 64));
     all = __builtin_amdgcn_readfirstlane(all);
-    int top = kNone;   // exponent that the values' scales are held against
     for (int p = p1; p < end; p += step)
     {
         f32x4 s[RT][2];
@@ -240,12 +241,8 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
         load_keys8<KS>(a, row, part.h, lane, x);
         __builtin_amdgcn_sched_barrier(0);
 
-        const bool odd = a.slopes || now != 0xffffffffu || p + kPos > all;
-        const int new_top = max(top, vs_top > 0.0f ? exponent_of(vs_top) : kNone);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vs[u][e] = __builtin_ldexpf(vs[u][e], 15 - new_top);
+        const bool part_seen = now != 0xffffffffu || p + kPos > all, odd = a.slopes || part_seen;
+        const int tile_top = vs_top > 0.0f ? exponent_of(vs_top) : kNone;
         half8 pp[RT][2];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -253,18 +250,30 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
             Row8<KS>& w = rows[i];
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
+            int new_top = tile_top;
             if (odd)
             {
+                float size = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                     {
                         const int q = 16 * u + 4 * g + e;
-                        const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q));
-                        s[i][u][e] = (now >> q & 1) && p + q < w.seen ? z : -__builtin_inff();
+                        const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q)), v = fabsf(vs[u][e]);
+                        const bool sees = (now >> q & 1) && p + q < w.seen;
+                        s[i][u][e] = sees ? z : -__builtin_inff();
+                        size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
                     }
+                if (part_seen)
+                {
+                    size = fmaxf(size, __shfl_xor(size, 16, 64));
+                    size = fmaxf(size, __shfl_xor(size, 32, 64));
+                    new_top = size > 0.0f ? exponent_of(size) : kNone;
+                }
             }
+            new_top = max(max(w.top, new_top), kLeastTop);
+            const float to = __builtin_ldexpf(1.0f, 15 - new_top);
             float high = kLowest;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -283,10 +292,11 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
                 {
                     const float y = __builtin_amdgcn_exp2f(s[i][u][e] - mn);
                     sum += y;
-                    z[4 * u + e] = y == 0.0f ? 0.0f : y * vs[u][e];   // a weight of 0 stays 0, whatever the scale is
+                    z[4 * u + e] = y == 0.0f ? 0.0f : y * vs[u][e] * to;   // a weight of 0 stays 0, whatever the scale is
                 }
             w.l = w.l * f + sum;
-            f = __builtin_ldexpf(f, top - new_top);
+            f = __builtin_ldexpf(f, w.top - new_top);
+            w.top = new_top;
             if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
             {
 #pragma unroll
@@ -294,7 +304,6 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
             }
             split2(z, pp[i][0], pp[i][1]);
         }
-        top = new_top;
 #pragma unroll
         for (int b = 0; b < B::VB; ++b)
         {
@@ -332,7 +341,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
 #pragma unroll
         for (int b = 0; b < B::VB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], top - 15);
+            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], w.top - 15);
         __syncthreads();
         const int jr = t >> 4, r = part.first + i * kTile + jr;
         if (r >= part.n_rows) continue;

@@ -1,18 +1,34 @@
 // k_attn_chunk_wide.hip — chunk attention of sequences with many rows: both
-// products on the float16 matrix cores, from parts (f16_parts.hpp): three float16 products for a float32 one, two over an 8-bit
-// cache.
+// products on the float16 matrix cores, from parts (f16_parts.hpp): three float16
+// products for a float32 one, two over an 8-bit cache.
 //
-// The scales are exact: a key's goes into its scores, a value's into its
-// position's weights, relative to the largest so far (the outputs are rescaled
-// when that grows, as they are when a row's largest score does).
+// k_attn_chunk_parts forms the parts of 32 positions of a key head at a time, once
+// for all of its blocks of rows, in the order of the matrix cores' operands. It
+// reads the cache and writes as much again (2048 tokens behind 6000, 8 heads of
+// 128: 24 us), and takes the scaling, the rounding and the pages' table out of the
+// loop below, of whose vector instructions they were two thirds: with parts formed
+// by every block of 128 rows the call took 951 us, so 712, and 8 sequences of 192
+// rows a key head behind 2000 positions 200 and 181.
 //
-// A workgroup takes 128 rows, 32 to a wave, and 32 positions at a time. Its waves
-// form the positions' parts together and leave them in LDS in the order of the
-// matrix cores' operands. Both products are formed transposed (S^T = K Q^T, O^T =
-// V^T P^T), 32 x 32 x 16 at a time: lane l has the scores of row l % 32 and of
-// the positions 8 (r / 4) + 4 (l / 32) + r % 4, r < 16, and its weights are the
-// second product's operand as they lie, if its k index 8 (l / 32) + e of step t
+// Scales are exact: a key's goes into its scores, a value's into its position's
+// weights, relative to the largest that the row has seen (a row's outputs are
+// rescaled when that grows, as they are when its largest score does). Both are a
+// position's own, so that what a row does not see takes no accuracy from what it does.
+//
+// A workgroup of k_attn_chunk_wide takes 128 rows, 32 to a wave, and 32 positions at
+// a time, copied to LDS a tile ahead. Both products are formed transposed (S^T = K
+// Q^T, O^T = V^T P^T), 32 x 32 x 16 at a time: lane l has the scores of row l % 32
+// and of the positions 8 (r / 4) + 4 (l / 32) + r % 4, r < 16, and its weights are
+// the second product's operand as they lie, if its k index 8 (l / 32) + e of step t
 // stands for position 8 (2 t + e / 4) + 4 (l / 32) + e % 4.
+//
+// What bounds it: the matrix cores are busy for 55 % of the cycles, the vector
+// instructions of the softmax and of the weights' parts (some 160 a tile and wave,
+// the exponentials at a quarter of the rate) for 40 %, and as the clock falls under
+// both (1.8 GHz) two waves a SIMD hardly hide one behind the other: time is 190 us
+// and 4.1 us a dim for 2048 tokens behind 6000 of 32 heads (dims 32, 64, 128: 291,
+// 411, 712 us). No order of reads, products and priorities changed it by 2 %; four
+// waves of 64 rows each, with half the reads from LDS, ran 1503 us.
 //
 // Of a float32 cache, results that are not finite are formed again by the float32
 // walk: infinities and NaN among keys, queries and values, also at positions
@@ -32,18 +48,20 @@ __device__ __forceinline__ floatx16 mfma32(const half8& x, const half8& y, const
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
 }
 
-template <int BITS, int KS> struct WideShared
+// A tile's parts, of one key head.
+template <int BITS, int KS> struct alignas(16) Image
 {
     static constexpr int P = BITS == 32 ? 2 : 1;   // parts
-    // Operands by lane: [buffer][step or block of 32 dims and k step][part][lane's place]
-    half8 k[2][KS][P][64];
-    half8 v[2][KS / 2][2][P][64];
-    float k_scale[2][kPos];        // of the scores
-    float v_scale[2][kPos];        // BITS 8: of the values
-    int v_top[2][4];               // exponents of the values: of each group of 8 positions; BITS 8: all [0]
+    // Operands by lane: [step or block of 32 dims and k step][part][lane's place]
+    half8 k[KS][P][64];
+    half8 v[KS / 2][2][P][64];
+    float k_scale[kPos];           // of the scores
+    float v_scale[kPos];           // of the weights: the values' scales; BITS 32: a quarter of 2^(exponent of the position's values)
+    int v_top[4];                  // exponents of the values: of each group of 8 positions; BITS 8: all [0]
+    unsigned there[4];             // [0]: which positions exist
 };
 
-// What a thread holds of a tile on its way to LDS. Keys: 8 dims of one position each; values: VD dims of the 8 positions of
+// What a thread of k_attn_chunk_parts holds of a tile. Keys: 8 dims of one position each; values: VD dims of the 8 positions of
 // the wave's group.
 template <int BITS, int KS> struct Raw
 {
@@ -57,12 +75,11 @@ template <int BITS, int KS> struct Raw
 template <int BITS, int KS> struct Wide
 {
     using R = Raw<BITS, KS>;
-    using S = WideShared<BITS, KS>;
+    using S = Image<BITS, KS>;
     static constexpr int P = S::P, NB = KS / 2;
 
     const ChunkArgs& a;
     const Part& part;
-    S& sh;
     int t, lane, wave;
 
     // Whether this thread has piece i of the keys, of which position, and its first dim.
@@ -169,8 +186,8 @@ template <int BITS, int KS> struct Wide
         }
     }
 
-    // The tile's parts into buffer b; there: which of its positions exist. Absent ones, and dims past the last, are 0.
-    __device__ __forceinline__ void stage(const R& r, int b, unsigned there)
+    // The tile's parts; there: which of its positions exist. Absent ones, and dims past the last, are 0.
+    __device__ __forceinline__ void stage(const R& r, S& sh, unsigned there)
     {
         const int dim = a.c.t.dim;
         const bool whole = there == 0xffffffffu && dim == 16 * KS;
@@ -203,9 +220,9 @@ template <int BITS, int KS> struct Wide
                 split2(z, hi, lo);
                 if (mine)
                 {
-                    sh.k[b][step][0][place] = hi;
-                    sh.k[b][step][P - 1][place] = lo;
-                    if (d == 0) sh.k_scale[b][p] = __builtin_ldexpf(1.0f, ke - 20);
+                    sh.k[step][0][place] = hi;
+                    sh.k[step][P - 1][place] = lo;
+                    if (d == 0) sh.k_scale[p] = __builtin_ldexpf(1.0f, ke - 20);
                 }
             }
             else
@@ -220,7 +237,7 @@ template <int BITS, int KS> struct Wide
                     z[2 * w] = halves_of(__builtin_amdgcn_perm(0u, x, 0x0c010c00u));
                     z[2 * w + 1] = halves_of(__builtin_amdgcn_perm(0u, x, 0x0c030c02u));
                 }
-                if (mine) sh.k[b][step][0][place] = __builtin_bit_cast(half8, z);
+                if (mine) sh.k[step][0][place] = __builtin_bit_cast(half8, z);
             }
         }
         {
@@ -230,8 +247,7 @@ template <int BITS, int KS> struct Wide
 #pragma unroll
             for (int e = 0; e < 8; ++e) ok |= (there >> value_pos(e) & 1u) << e;
             floatx8 z[R::VD];
-            float top = 0.0f;
-            int ve = 0;
+            int ve[8] = {};
             if constexpr (BITS == 32)
             {
 #pragma unroll
@@ -246,12 +262,25 @@ template <int BITS, int KS> struct Wide
 #pragma unroll
                         for (int e = 0; e < 8; ++e) z[y][e] = (ok >> e & 1) && d0 + y < dim ? z[y][e] : 0.0f;
                 }
+                float top[8];
 #pragma unroll
-                for (int y = 0; y < R::VD; ++y)
+                for (int e = 0; e < 8; ++e)
+                {
+                    top[e] = fabsf(z[0][e]);
+                    if constexpr (R::VD == 2) top[e] = fmaxf(top[e], fabsf(z[R::VD - 1][e]));
+                }
+                const float mine = max_of_8(top, lane);   // position lane % 8's
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(z[y][e]));
-                top = max_of<64>(top);
-                ve = top > 0.0f ? exponent_of(top) : kNone;
+                for (int e = 0; e < 8; ++e)
+                {
+                    const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), e));
+                    ve[e] = x > 0.0f ? exponent_of(x) : kNone;
+                }
+                if (lane < 8) sh.v_scale[value_pos(lane)] = mine > 0.0f ? __builtin_ldexpf(0.25f, exponent_of(mine)) : 0.0f;
+                int highest = ve[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) highest = max(highest, ve[e]);
+                if (lane == 0) sh.v_top[group] = highest;
             }
 #pragma unroll
             for (int y = 0; y < R::VD; ++y)
@@ -259,11 +288,11 @@ template <int BITS, int KS> struct Wide
                 const int d = d0 + y;
                 if (d >= 16 * KS) continue;
                 const int slot = d % 32 + 32 * (group & 1), place = slot ^ (slot >> 3 & 7);
-                half8(&to)[P][64] = sh.v[b][d / 32][group >> 1];
+                half8(&to)[P][64] = sh.v[d / 32][group >> 1];
                 if constexpr (BITS == 32)
                 {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[y][e] = __builtin_ldexpf(z[y][e], 15 - ve);
+                    for (int e = 0; e < 8; ++e) z[y][e] = __builtin_ldexpf(z[y][e], 15 - ve[e]);
                     half8 hi, lo;
                     split2(z[y], hi, lo);
                     to[0][place] = hi;
@@ -282,8 +311,6 @@ template <int BITS, int KS> struct Wide
                     to[0][place] = __builtin_bit_cast(half8, x);
                 }
             }
-            if constexpr (BITS == 32)
-                if (lane == 0) sh.v_top[b][group] = ve;
         }
         if constexpr (BITS == 8)
             if (wave == 0)
@@ -292,26 +319,78 @@ template <int BITS, int KS> struct Wide
                 const float s = ok ? r.scale : 0.0f;
                 const float top = max_of<32>(fabsf(s) <= kMaxF ? fabsf(s) : 0.0f);
                 const int e = top > 0.0f ? exponent_of(top) : kNone;   // of the keys' scales, of the values'
-                if (lane < 32) sh.k_scale[b][lane] = s * 0x1p-5f;
+                if (lane < 32) sh.k_scale[lane] = s * 0x1p-5f;
                 else
                 {
-                    sh.v_scale[b][lane - 32] = s;
-                    if (lane == 32) sh.v_top[b][0] = e;
+                    sh.v_scale[lane - 32] = s;
+                    if (lane == 32) sh.v_top[0] = e;
                 }
             }
     }
 };
 
-template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chunk_wide(ChunkArgs a)
+// The place of a sequence among those whose parts are formed: its own number, or, as these have more than kNarrowRows rows
+// each, its first row's share of them.
+__device__ __forceinline__ unsigned slot_of(const ChunkArgs& a, unsigned b)
+{
+    if (a.slots_by_batch) return b;
+    return (unsigned)((size_t)length_of(a.start[b], a.tokens) * a.by_per.d / (kNarrowRows + 1));
+}
+
+// The parts of every tile, once for all blocks of rows, of the pieces (slot and key head) from a.first_piece on. blocks:
+// workgroups of a piece.
+template <int BITS, int KS> __global__ __launch_bounds__(256) void k_attn_chunk_parts(ChunkArgs a, FastDiv blocks)
 {
     using W = Wide<BITS, KS>;
-    using S = WideShared<BITS, KS>;
+    using S = Image<BITS, KS>;
+    __shared__ S sh;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31;
+    Part part{};
+    const unsigned piece = blocks.div(blockIdx.x), first = blockIdx.x - piece * blocks.d;
+    const unsigned slot = a.by_heads.div(a.first_piece + piece);
+    part.h = a.first_piece + piece - slot * a.c.t.heads;
+    int b = slot;
+    if (!a.slots_by_batch)
+    {
+        b = last_of(a.c.t.batch, [&](unsigned i) { return slot_of(a, i) <= slot; });
+        if (b < 0 || slot_of(a, b) != slot) return;
+    }
+    part.b = b;
+    part.chunk = chunk_of(a, part.b);
+    if (part.chunk.n * (int)a.by_per.d <= a.wide_from) return;
+    const int end = max(part.chunk.seen + part.chunk.n - 1, 0), tiles = (end + kPos - 1) / kPos;
+    W w{a, part, t, lane, wave};
+    S* to = reinterpret_cast<S*>(a.images) + (size_t)piece * a.tiles;
+    for (int i = first; i < tiles; i += blocks.d)
+    {
+        const int p = kPos * i + j;
+        int row = a.c.t.row_in(a.c.t.entry_of(part.b, p), p);
+        if (p >= end) row = -1;
+        int kr[W::R::KI];
+        typename W::R raw;
+        w.key_rows(row, kr);
+        w.load(row, kr, raw);
+        const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
+        w.stage(raw, sh, there);
+        if (t < 4) sh.there[t] = there;
+        __syncthreads();
+        const f32x4* from = reinterpret_cast<const f32x4*>(&sh);
+        f32x4* out = reinterpret_cast<f32x4*>(to + i);
+        for (int x = t; x < (int)(sizeof(S) / 16); x += 256) out[x] = from[x];
+        __syncthreads();
+    }
+}
+
+template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chunk_wide(ChunkArgs a)
+{
+    using S = Image<BITS, KS>;
     constexpr int NB = KS / 2, P = S::P;
-    constexpr size_t kLds = BITS == 32 && sizeof(WalkShared<KS>) > sizeof(S) ? sizeof(WalkShared<KS>) : sizeof(S);
+    constexpr size_t kLds = BITS == 32 && sizeof(WalkShared<KS>) > 2 * sizeof(S) ? sizeof(WalkShared<KS>) : 2 * sizeof(S);
     __shared__ __attribute__((aligned(16))) char lds[kLds];
-    S& sh = *reinterpret_cast<S*>(lds);
+    S* const sh = reinterpret_cast<S*>(lds);
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, g = lane >> 5;
     Part part;
+    const S* images;
     // Workgroups go to the 8 XCDs in turn: each takes neighbouring pieces of work, the blocks of rows of one range of one key
     // head after another (they read the same keys and values), the rows that see most first.
     {
@@ -329,7 +408,9 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         part.chunk = chunk_of(a, part.b);
         part.n_rows = part.chunk.n * a.by_per.d;
         const unsigned block = x - base(b);
-        if (part.n_rows <= a.wide_from || block >= (unsigned)(part.n_rows + kWideRows - 1) / kWideRows) return;
+        const unsigned at_piece = slot_of(a, part.b) * a.c.t.heads + part.h - a.first_piece;
+        if (part.n_rows <= a.wide_from || at_piece >= a.pieces || block >= (unsigned)(part.n_rows + kWideRows - 1) / kWideRows) return;
+        images = reinterpret_cast<const S*>(a.images) + (size_t)at_piece * a.tiles;
         part.first = block * kWideRows;
         if (!cut_range(a, part, kWideRows, 64)) return;
     }
@@ -347,22 +428,27 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     all = __builtin_amdgcn_readfirstlane(all);
     most = __builtin_amdgcn_readfirstlane(most);
 
-    W w{a, part, sh, t, lane, wave};
-    typename W::R raw;
-    auto entry = [&](int p) { return a.c.t.entry_of(part.b, p + j); };
-    auto row_at = [&](float e, int p) {
-        const int r = a.c.t.row_in(e, p + j);
-        return p + j < end ? r : -1;
+    const int tiles = (end - begin + kPos - 1) / kPos;
+    // A thread's 16-byte pieces of a tile's keys and then of its values, and of what is behind them.
+    constexpr int kHalf = sizeof(S::k) / 16, kPieces = (kHalf + 255) / 256, kTail = sizeof(S) / 16 - 2 * kHalf;
+    static_assert(sizeof(S::v) == sizeof(S::k) && kHalf % 64 == 0);
+    const f32x4* image = reinterpret_cast<const f32x4*>(images + begin / kPos);
+    f32x4 piece[kPieces], tail;
+    auto fetch = [&](int i, int half) __attribute__((always_inline)) {
+        const f32x4* from = image + (size_t)min(i, tiles - 1) * (sizeof(S) / 16) + half * kHalf;
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x)
+            if (256 * x + 256 <= kHalf || 256 * x + 64 * wave < kHalf) piece[x] = from[256 * x + t];
+        if (half == 1) tail = from[kHalf + min(lane, kTail - 1)];
     };
-    auto mask_of = [](int r) { return (unsigned)__builtin_amdgcn_ballot_w64(r >= 0); };
-    float ahead = entry(begin + kPos);
-    int at = row_at(entry(begin), begin), kr[W::R::KI];
-    unsigned there = mask_of(at);   // of the tile in `raw`
-    w.key_rows(at, kr);
-    w.load(at, kr, raw);
-    at = row_at(ahead, begin + kPos);
-    w.key_rows(at, kr);
-    ahead = entry(begin + 2 * kPos);
+    auto place = [&](S& to, int half) __attribute__((always_inline)) {
+        f32x4* at = reinterpret_cast<f32x4*>(&to) + half * kHalf;
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x)
+            if (256 * x + 256 <= kHalf || 256 * x + 64 * wave < kHalf) at[256 * x + t] = piece[x];
+        if (half == 1 && wave == 0 && lane < kTail) at[kHalf + lane] = tail;
+    };
+    fetch(0, 0);
 
     // The queries' parts: row l % 32, dims 16 k + 8 (l / 32) + e.
     half8 qp[KS][2];
@@ -397,156 +483,177 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         for (int k = 0; k < KS; ++k)
         {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[k][e] = __builtin_ldexpf(z[k][e], 15 - qe);
+            for (int e = 0; e < 8; ++e) z[k][e] = __builtin_ldexpf(a.alpha < 0.0f ? -z[k][e] : z[k][e], 15 - qe);
             split2(z[k], qp[k][0], qp[k][1]);
         }
     }
 
-    w.stage(raw, 0, there);
-    const unsigned there0 = there;
-    there = mask_of(at);
-    w.load(at, kr, raw);
-    at = row_at(ahead, begin + 2 * kPos);
-    w.key_rows(at, kr);
-    ahead = entry(begin + 3 * kPos);
+    place(sh[0], 0);
+    fetch(0, 1);
+    place(sh[0], 1);
+    fetch(1, 0);
     __syncthreads();
-    unsigned now = there0;          // the positions of the tile whose parts are used
     const float slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
-    const float scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);   // scores times log2(e)
+    // Scores times log2(e); not 0, which would make a masked score's product NaN (alpha 0: 2^-149 of at most 2^127 is none).
+    const float scale = fmaxf(__builtin_ldexpf(fabsf(a.alpha) * kLog2e, qe - 10), 0x1p-149f);
+    const float by = a.slopes ? 1.0f : scale;   // of the scores as the softmax sees them
     float m = kLowest, l = 0.0f;
-    int top = kNone;                // exponent that the values are held against
+    int top = kNone;                // exponent that the row's values are held against
     floatx16 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[b][r] = 0.0f;
 
-    const int tiles = (end - begin + kPos - 1) / kPos;
     for (int i = 0; i < tiles; ++i)
     {
-        const int p0 = begin + kPos * i, buf = i & 1;
-        unsigned next = 0;
-        if (i + 1 < tiles)
-        {
-            next = there;
-            w.stage(raw, buf ^ 1, there);
-            there = mask_of(at);
-            w.load(at, kr, raw);
-            at = row_at(ahead, p0 + 3 * kPos);
-            w.key_rows(at, kr);
-            ahead = entry(p0 + 4 * kPos);
-        }
-        if (p0 < most)
-        {
-            floatx16 s;
+        const int p0 = begin + kPos * i;
+        const S& in = sh[i & 1];
+        const unsigned now = __builtin_amdgcn_readfirstlane(in.there[0]);
+        S& out = sh[(i & 1) ^ 1];
+        // The next tile's parts: its keys were loaded during the last tile's second product, its values are during this one's
+        // softmax.
+        auto turn = [&](int half) __attribute__((always_inline)) {
+            place(out, half);   // behind the last tile, too: nothing reads it
+            fetch(i + 1 + half, half ^ 1);
+        };
+        const bool work = p0 < most;   // some row of the wave sees some of it
+        floatx16 s;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        if (work)
+        {
+            // Operands are read kDeep steps before their products.
+            constexpr int kDeep = 2;
+            half8 ks[kDeep + 1][P];
+            auto keys = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 0; x < P; ++x) ks[k % (kDeep + 1)][x] = in.k[k][x][lane ^ ((2 * k + g) & 7)];
+            };
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) keys(k);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
             {
-                const int place0 = lane ^ ((2 * k + g) & 7);
-                const half8 hi = sh.k[buf][k][0][place0];
-                if constexpr (BITS == 32)
-                {
-                    const half8 lo = sh.k[buf][k][P - 1][place0];
-                    s = mfma32(lo, qp[k][0], s);
-                }
-                s = mfma32(hi, qp[k][1], s);
-                s = mfma32(hi, qp[k][0], s);
+                if (k + kDeep < KS) keys(k + kDeep);
+                __builtin_amdgcn_sched_barrier(0);
+                const half8(&x)[P] = ks[k % (kDeep + 1)];
+                if constexpr (BITS == 32) s = mfma32(x[P - 1], qp[k][0], s);
+                s = mfma32(x[0], qp[k][1], s);
+                s = mfma32(x[0], qp[k][0], s);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q)
             {
-                const f32x4 f = *reinterpret_cast<const f32x4*>(&sh.k_scale[buf][8 * q + 4 * g]);
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&in.k_scale[8 * q + 4 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * q + e] = s[4 * q + e] * f[e] * scale;
+                for (int e = 0; e < 4; ++e) s[4 * q + e] *= f[e];
             }
+        }
+        turn(0);
+        if (work)
+        {
             if (a.slopes)
             {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] -= slope * (float)(seen - 1 - (p0 + 8 * (r / 4) + 4 * g + r % 4));
+                for (int r = 0; r < 16; ++r) s[r] = s[r] * scale - slope * (float)(seen - 1 - (p0 + 8 * (r / 4) + 4 * g + r % 4));
             }
+            f32x4 vs[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) vs[q] = *reinterpret_cast<const f32x4*>(&in.v_scale[8 * q + 4 * g]);
+            int new_top = in.v_top[0];
+            if constexpr (BITS == 32) new_top = max(max(new_top, in.v_top[1]), max(in.v_top[2], in.v_top[3]));
             if (now != 0xffffffffu || p0 + kPos > all)
             {
+                // Of the values, too, only those that the row sees count.
+                float size = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                 {
                     const int p = 8 * (r / 4) + 4 * g + r % 4;
-                    s[r] = (now >> p & 1) && p0 + p < seen ? s[r] : -__builtin_inff();
+                    const bool sees = (now >> p & 1) && p0 + p < seen;
+                    s[r] = sees ? s[r] : -__builtin_inff();
+                    const float v = fabsf(vs[r / 4][r % 4]);
+                    size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
                 }
+                size = across(size, [](float x, float y) { return fmaxf(x, y); });
+                new_top = size > 0.0f ? exponent_of(size) + (BITS == 32 ? 1 : 0) : kNone;
             }
             float high = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
             high = across(high, [](float x, float y) { return fmaxf(x, y); });
-            const float mn = fmaxf(m, high);
+            const float mn = fmaxf(m, high * by);
             float f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
+            // What rounding the largest score took away is added to the weights' exponents: of scores past 2^20 it may be
+            // more than an exponent holds, and these are rounded first.
+            float once = by;
+            if (__builtin_amdgcn_ballot_w64(fabsf(mn) > 0x1p20f && mn != kLowest))
+            {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= by;
+                once = 1.0f;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
             {
-                s[r] = __builtin_amdgcn_exp2f(s[r] - mn);
+                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], once, -mn));
                 sum += s[r];
             }
             l = l * f + sum;
-            // The values' scales. Weights that are 0 stay so, whatever their position's scale is.
-            int new_top = sh.v_top[buf][0];
-            if constexpr (BITS == 32) new_top = max(max(new_top, sh.v_top[buf][1]), max(sh.v_top[buf][2], sh.v_top[buf][3]));
-            new_top = max(top, __builtin_amdgcn_readfirstlane(new_top));
-            if (new_top != top) f = __builtin_ldexpf(f, top - new_top);
+            new_top = max(max(top, new_top), kLeastTop);
+            f = __builtin_ldexpf(f, top - new_top);
             top = new_top;
             if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
             {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) o[b] *= f;
             }
+            // The values' scales, into the weights. Weights that are 0 stay so, whatever their position's scale is.
+            const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - top);
+            const int place1 = lane ^ (lane >> 3 & 7);
+            half8 vh[NB], vl[NB];
+            auto values = [&](int st, int x, half8(&to)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) to[b] = in.v[b][st][x][place1];
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto product = [&](const half8(&x)[NB], const half8& y) __attribute__((always_inline)) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[b] = mfma32(x[b], y, o[b]);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            values(0, 0, vh);
+            if constexpr (BITS == 32) values(0, P - 1, vl);
             half8 pp[2][2];
 #pragma unroll
             for (int st = 0; st < 2; ++st)
             {
                 floatx8 z;
-                if constexpr (BITS == 32)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
                 {
-                    const float to = __builtin_ldexpf(1.0f, sh.v_top[buf][2 * st + g] - top + 15);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = s[8 * st + e] * to;
-                }
-                else
-                {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q)
-                    {
-                        const f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.v_scale[buf][8 * (2 * st + q) + 4 * g]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                        {
-                            const float x = s[8 * st + 4 * q + e], y = x * __builtin_ldexpf(vs[e], 15 - top);
-                            z[4 * q + e] = x == 0.0f ? 0.0f : y;
-                        }
-                    }
+                    const float x = s[8 * st + e], y = x * vs[2 * st + e / 4][e % 4] * to;
+                    z[e] = BITS == 8 && x == 0.0f ? 0.0f : y;
                 }
                 split2(z, pp[st][0], pp[st][1]);
             }
-            const int place1 = lane ^ (lane >> 3 & 7);
-#pragma unroll
-            for (int st = 0; st < 2; ++st)
+            product(vh, pp[0][1]);
+            product(vh, pp[0][0]);
+            values(1, 0, vh);
+            if constexpr (BITS == 32)
             {
-                half8 hi[NB];
-#pragma unroll
-                for (int b = 0; b < NB; ++b) hi[b] = sh.v[buf][b][st][0][place1];
-                if constexpr (BITS == 32)
-                {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) o[b] = mfma32(sh.v[buf][b][st][P - 1][place1], pp[st][0], o[b]);
-                }
-#pragma unroll
-                for (int b = 0; b < NB; ++b) o[b] = mfma32(hi[b], pp[st][1], o[b]);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) o[b] = mfma32(hi[b], pp[st][0], o[b]);
+                product(vl, pp[0][0]);
+                values(1, P - 1, vl);
             }
+            product(vh, pp[1][1]);
+            product(vh, pp[1][0]);
+            if constexpr (BITS == 32) product(vl, pp[1][0]);
         }
-        now = next;
+        turn(1);
         __syncthreads();
     }
 
@@ -580,6 +687,20 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 }
 
 } // namespace
+
+size_t chunk_image_bytes(int bits, unsigned dim)
+{
+    const size_t groups = (dim + 31) / 32;
+    return groups * (bits == 32 ? 8192 : 4096) + sizeof(float) * 2 * kPos + sizeof(int) * 8;
+}
+
+void chunk_parts(const ChunkArgs& a, int bits, unsigned pieces, unsigned blocks, hipStream_t s)
+{
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(pieces * blocks), dim3(256), 0, s, a, FastDiv(blocks)); };
+    const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
+    if (bits == 32) groups == 1 ? go(k_attn_chunk_parts<32, 2>) : groups == 2 ? go(k_attn_chunk_parts<32, 4>) : groups == 3 ? go(k_attn_chunk_parts<32, 6>) : go(k_attn_chunk_parts<32, 8>);
+    else groups == 1 ? go(k_attn_chunk_parts<8, 2>) : groups == 2 ? go(k_attn_chunk_parts<8, 4>) : groups == 3 ? go(k_attn_chunk_parts<8, 6>) : go(k_attn_chunk_parts<8, 8>);
+}
 
 void chunk_wide(const ChunkArgs& a, int bits, unsigned blocks, hipStream_t s)
 {

@@ -323,6 +323,50 @@ def test_what_a_token_does_not_see(new, past, per, dim, value):
                 assert ok.all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("new,past,per,dim", [(9, 20, 1, 64), (5, 0, 4, 30), (20, 3, 1, 48), (40, 100, 1, 64), (70, 10, 2, 128), (200, 33, 1, 96)])
+def test_large_values_that_a_token_does_not_see(new, past, per, dim, bits):
+    """Finite keys and values of 1e30 among ordinary ones: the tokens in front of them are as exact as without."""
+    rng = np.random.default_rng(new + dim)
+    page, heads = 16, 2
+    lens, start = [new + past], [0, new]
+    x, table, pages = cache_for(rng, lens, page, heads, dim, bits)
+    c = dict(pages=pages, page=page, heads=heads, dim=dim)
+    q = rng.normal(size=(new, heads * per, dim)).astype(np.float32)
+    want = ch.attend(q, x["K64"], x["V64"], table, page, pages, heads, start, new, lens, 0.125)
+    for at in sorted({1, new // 2, new - 1}):
+        r = ch.row_of(table, 0, past + at, page, pages)
+        for which in "VK":
+            y = {n: a.copy() for n, a in x.items()}
+            if bits == 32:
+                y[which][r] *= np.float32(1e30)
+                y[which + "64"][r] = y[which][r]
+            else:
+                y[which + "s"][r] *= np.float32(1e30)
+                y[which + "64"][r] = y[which][r].astype(np.float64) * y[which + "s"][r].astype(np.float64)[:, None]
+            got = run_chunk(y, c, table, q, start, new, lens, None, 0.125)
+            assert np.all(np.abs(got[0][:at] - want[0][:at]) <= want[3][:at])
+            w2 = ch.attend(q, y["K64"], y["V64"], table, page, pages, heads, start, new, lens, 0.125)
+            if bits == 8:      # bytes are held against the largest scale, not the largest product of one with its byte
+                w2 = (*w2[:3], w2[3] + len(y["V64"]) * 2.0 ** -39 * 127 * np.abs(y["Vs"][np.isfinite(y["Vs"])]).max(), *w2[4:])
+            check_chunk(got, w2, stats=False)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_table_of_many_positions(bits):
+    """Tables that reach 2^24 positions: the keys' and values' parts are formed a sequence and key head at a time."""
+    rng = np.random.default_rng(bits)
+    page, heads, dim, new, past = 16, 2, 32, [40, 3, 100], [70, 50, 0]
+    lens = [n + p for n, p in zip(new, past)]
+    x, table, pages = cache_for(rng, lens, page, heads, dim, bits)
+    wide = np.full((3, 1 << 20), -1, np.float32)
+    wide[:, :table.shape[1]] = table
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = rng.normal(size=(int(start[-1]), 4, dim)).astype(np.float32)
+    got = run_chunk(x, dict(pages=pages, page=page, heads=heads, dim=dim), wide, q, start, 100, lens, None, 0.2)
+    check_chunk(got, ch.attend(q, x["K64"], x["V64"], table, page, pages, heads, start, 100, lens, 0.2))
+
+
 @pytest.mark.parametrize("new,past,per,dim", [(9, 20, 1, 64), (5, 0, 4, 30), (40, 100, 1, 64), (200, 33, 1, 96)])
 def test_scales_that_are_not_finite(new, past, per, dim):
     """An 8-bit row that was not finite when it was stored (scale NaN) makes the tokens that see it NaN, and no other."""
