@@ -515,8 +515,9 @@ __device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int 
     return part.n_rows > 0 && part.n_rows <= a.wide_from && cut_range(a, part, part.n_rows, step);
 }
 
-// k_attn_chunk8, and k_attn_chunk_wide: their launches; rows of a workgroup.
-void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s);
+// k_attn_chunk8 (bytes: what rows, heads and caches are aligned to, 4, 8 or 16), and k_attn_chunk_wide: their launches; rows
+// of a workgroup.
+void chunk8(const ChunkArgs& a, int bytes, unsigned blocks, hipStream_t s);
 constexpr int kWideRows = 128;
 constexpr int kNarrowRows = 32;   // of a sequence and key head that the kernels of few rows take at most
 size_t chunk_image_bytes(int bits, unsigned dim);

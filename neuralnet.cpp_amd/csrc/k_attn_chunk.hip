@@ -147,7 +147,7 @@ struct ChunkCall
     Pages8 c;
     int bits;
     bool vec;          // rows can be read in pieces of 4 values
-    bool wide_bytes;   // and 16 bytes
+    int bytes;         // 8 bits: and in pieces of so many bytes, 16, 8 or 4, or 1
     size_t q_heads, tokens, most;
 };
 
@@ -214,15 +214,16 @@ bool chunk_ok(const ChunkCall& c, size_t heads)
 bool chunk_call(const nnhip_kv_pages* c, size_t q_heads, size_t tokens, size_t most, ChunkCall& out)
 {
     if (!pages_ok(c, kChunkMaxDim)) return false;
-    out = {Pages8{pages_of(*c), nullptr, nullptr, nullptr, nullptr}, 32, c->dim % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V), false,
+    out = {Pages8{pages_of(*c), nullptr, nullptr, nullptr, nullptr}, 32, c->dim % 4 == 0 && c->row % 4 == 0 && aligned16(c->K) && aligned16(c->V), 0,
            q_heads, tokens, most};
     return chunk_ok(out, c->heads);
 }
 bool chunk_call(const nnhip_kv8_pages* c, size_t q_heads, size_t tokens, size_t most, ChunkCall& out)
 {
     if (!pages8_ok(c, kChunkMaxDim)) return false;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V);
-    out = {pages8_of(*c), 8, c->dim % 4 == 0 && c->row % 4 == 0 && (at & 3) == 0, c->dim % 16 == 0 && c->row % 16 == 0 && (at & 15) == 0,
+    const uintptr_t at = reinterpret_cast<uintptr_t>(c->K) | reinterpret_cast<uintptr_t>(c->V) | c->dim | c->row;
+    const int bytes = at % 16 == 0 ? 16 : at % 8 == 0 ? 8 : at % 4 == 0 ? 4 : 1;
+    out = {pages8_of(*c), 8, bytes >= 4, bytes,
            q_heads, tokens, most};
     return chunk_ok(out, c->heads);
 }
@@ -295,7 +296,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     if (p.narrow)
     {
         if (call.bits == 32) call.vec ? chunk_launch<32, true>(a, p, s) : chunk_launch<32, false>(a, p, s);
-        else if (call.wide_bytes) chunk8(a, static_cast<unsigned>(p.blocks), s);
+        else if (call.bytes >= 4) chunk8(a, call.bytes, static_cast<unsigned>(p.blocks), s);
         else chunk_launch<8, false>(a, p, s);
         if (int rc = launch_status()) return rc;
     }

@@ -14,6 +14,10 @@
 // product. Block b of the output's dims are those that leave the remainder b by
 // VB, so that the lane's VB neighbouring bytes of a value row serve one block
 // each.
+//
+// Rows are read 16, 8 or 4 bytes at a time, as heads begin (32 sequences of 3000
+// positions, 12 heads: of 64 bytes 38 us, of 40 39, of 36 43; the float32 walk,
+// which takes heads of odd widths byte by byte, took 183 us for 40).
 #include "attn_chunk.hpp"
 #include "f16_parts.hpp"
 
@@ -29,27 +33,28 @@ __device__ __forceinline__ f32x4 mfma16(const half8& x, const half8& y, const f3
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
 }
 
-// KS: groups of 16 dims, even. VB: value bytes of a lane and position, and blocks of dims; up to 16 VB dims.
-template <int KS> struct Bytes
+// KS: groups of 16 dims, even. W: rows, heads and the caches themselves begin at multiples of W bytes, 16, 8 or 4, which is what
+// a lane loads at a time. VB: value bytes of a lane and position, and blocks of dims; up to 16 VB dims.
+template <int KS, int W> struct Bytes
 {
     static constexpr int VB = KS <= 2 ? 2 : KS <= 4 ? 4 : 8, VW = (VB + 3) / 4, steps = KS / 2;
     // Keys are loaded 16 bytes at a time where whole pairs of steps let them: bytes 0 to 7 are the first step's.
-    static constexpr bool WIDE = KS % 4 == 0;
+    static constexpr bool WIDE = KS % 4 == 0 && W == 16;
     static __device__ __forceinline__ int dim_of(int step, int g) { return WIDE ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 32 * step + 8 * g; }
 };
 
-template <int KS> struct Row8
+template <int KS, int W> struct Row8
 {
     half8 q[KS / 2][2];
     int seen;
     int top;                    // exponent that the values' scales are held against: of those that the row sees
     float slope, scale, m, l;   // slope, scale and m: times log2(e)
-    f32x4 o[Bytes<KS>::VB];
+    f32x4 o[Bytes<KS, W>::VB];
 };
 
-template <int KS> struct Shared8
+template <int KS, int W> struct Shared8
 {
-    using B = Bytes<KS>;
+    using B = Bytes<KS, W>;
     union
     {
         float scales[4][2][kPos];   // by wave: the keys', the values'
@@ -59,16 +64,16 @@ template <int KS> struct Shared8
 };
 
 // One tile's bytes on their way.
-template <int KS> struct Tile8
+template <int KS, int W> struct Tile8
 {
-    using B = Bytes<KS>;
+    using B = Bytes<KS, W>;
     unsigned k[2][B::steps][2], v[8][B::VW];
     float scale;   // lane p < 32: position p's of the keys; lane 32 + p: of the values
 };
 
-template <int KS> __device__ __forceinline__ void load_keys8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS>& x)
+template <int KS, int W> __device__ __forceinline__ void load_keys8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS, W>& x)
 {
-    using B = Bytes<KS>;
+    using B = Bytes<KS, W>;
     const int j = lane & 15, g = lane >> 4, dim = a.c.t.dim;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -87,24 +92,34 @@ template <int KS> __device__ __forceinline__ void load_keys8(const ChunkArgs& a,
                 x.k[u][s + 1][0] = z[2];
                 x.k[u][s + 1][1] = z[3];
             }
-            else
+            else if constexpr (W >= 8)
             {
                 const uint2 z = *reinterpret_cast<const uint2*>(at);
                 x.k[u][s][0] = z.x;
                 x.k[u][s][1] = z.y;
+            }
+            else
+            {
+                x.k[u][s][0] = *reinterpret_cast<const unsigned*>(at);
+                x.k[u][s][1] = *reinterpret_cast<const unsigned*>(from + (d + 4 < dim ? d + 4 : 0));
             }
         }
     }
     const float z = (lane < 32 ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
     x.scale = row >= 0 ? z : 0.0f;
 }
-template <int KS> __device__ __forceinline__ void load_values8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS>& x)
+template <int KS, int W> __device__ __forceinline__ void load_values8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS, W>& x)
 {
-    using B = Bytes<KS>;
+    using B = Bytes<KS, W>;
     const int j = lane & 15, g = lane >> 4, dim = a.c.t.dim, d = B::VB * j;
     auto load = [&](int e, size_t r) {
         const signed char* at = a.c.V + r * a.c.t.row + (size_t)h * dim + (d < dim ? d : 0);
-        if constexpr (B::VB == 8)
+        if constexpr (B::VB == 8 && W == 4)
+        {
+            x.v[e][0] = *reinterpret_cast<const unsigned*>(at);
+            x.v[e][B::VW - 1] = *reinterpret_cast<const unsigned*>(at + (d + 4 < dim ? 4 : 0));
+        }
+        else if constexpr (B::VB == 8)
         {
             const uint2 z = *reinterpret_cast<const uint2*>(at);
             x.v[e][0] = z.x;
@@ -141,12 +156,12 @@ __device__ __forceinline__ half8 halves8(unsigned lo, unsigned hi)
     return __builtin_bit_cast(half8, z);
 }
 
-template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs& a, const Part& part, Shared8<KS>& sh)
+template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const ChunkArgs& a, const Part& part, Shared8<KS, W>& sh)
 {
-    using B = Bytes<KS>;
+    using B = Bytes<KS, W>;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 15, g = lane >> 4;
     const int dim = a.c.t.dim, begin = part.begin, end = part.end, step = 4 * kPos;
-    Row8<KS> rows[RT];
+    Row8<KS, W> rows[RT];
     int all = 0x7fffffff;
     const int p1 = begin + wave * kPos;
     // Lane p and lane 32 + p: the table's entry and the row of position p of a tile.
@@ -155,16 +170,16 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
         const int r = a.c.t.row_in(e, p + (lane & 31));
         return p + (lane & 31) < end ? r : -1;
     };
-    Tile8<KS> x;
+    Tile8<KS, W> x;
     float ahead = entry(p1 + step);
     int row = row_at(entry(p1), p1);
     unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
-    load_keys8<KS>(a, row, part.h, lane, x);
-    load_values8<KS>(a, row, part.h, lane, x);
+    load_keys8<KS, W>(a, row, part.h, lane, x);
+    load_values8<KS, W>(a, row, part.h, lane, x);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
     {
-        Row8<KS>& w = rows[i];
+        Row8<KS, W>& w = rows[i];
         const int r = part.first + i * kTile + j;
         const bool live = r < part.n_rows;
         const unsigned n = live ? a.by_per.div(r) : 0, qh = part.h * a.by_per.d + (live ? r - n * a.by_per.d : 0);
@@ -238,7 +253,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
         row = row_at(ahead, p + step);
         const unsigned now = there;
         there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
-        load_keys8<KS>(a, row, part.h, lane, x);
+        load_keys8<KS, W>(a, row, part.h, lane, x);
         __builtin_amdgcn_sched_barrier(0);
 
         const bool part_seen = now != 0xffffffffu || p + kPos > all, odd = a.slopes || part_seen;
@@ -247,7 +262,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
 #pragma unroll
         for (int i = 0; i < RT; ++i)
         {
-            Row8<KS>& w = rows[i];
+            Row8<KS, W>& w = rows[i];
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
             int new_top = tile_top;
@@ -321,7 +336,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
             for (int i = 0; i < RT; ++i) rows[i].o[b] = mfma16(y, pp[i][0], rows[i].o[b]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_values8<KS>(a, row, part.h, lane, x);
+        load_values8<KS, W>(a, row, part.h, lane, x);
         ahead = further;
     }
 
@@ -329,7 +344,7 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
 #pragma unroll
     for (int i = 0; i < RT; ++i)
     {
-        Row8<KS>& w = rows[i];
+        Row8<KS, W>& w = rows[i];
         w.l += __shfl_xor(w.l, 16, 64);
         w.l += __shfl_xor(w.l, 32, 64);
         __syncthreads();
@@ -369,23 +384,30 @@ template <int KS, int RT> __device__ __forceinline__ void walk8(const ChunkArgs&
 }
 
 // RT 1: no sequence has more than 16 rows.
-template <int KS, int RT> __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void k_attn_chunk8(ChunkArgs a)
+template <int KS, int W, int RT> __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void k_attn_chunk8(ChunkArgs a)
 {
-    __shared__ Shared8<KS> sh;
+    __shared__ Shared8<KS, W> sh;
     Part part;
     if (!narrow_part(a, part, 4 * kPos)) return;
-    if (RT == 1 || part.n_rows <= kTile) walk8<KS, 1>(a, part, sh);
-    else walk8<KS, RT>(a, part, sh);
+    if (RT == 1 || part.n_rows <= kTile) walk8<KS, W, 1>(a, part, sh);
+    else walk8<KS, W, RT>(a, part, sh);
 }
 
 } // namespace
 
-void chunk8(const ChunkArgs& a, unsigned blocks, hipStream_t s)
+template <int W> void launch8(const ChunkArgs& a, unsigned blocks, hipStream_t s)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, s, a); };
+    constexpr int W8 = W < 8 ? W : 8;   // odd numbers of 32 dims are loaded 8 bytes at a time at most
     const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
-    if (a.wide_from <= kTile) groups == 1 ? go(k_attn_chunk8<2, 1>) : groups == 2 ? go(k_attn_chunk8<4, 1>) : groups == 3 ? go(k_attn_chunk8<6, 1>) : go(k_attn_chunk8<8, 1>);
-    else groups == 1 ? go(k_attn_chunk8<2, 2>) : groups == 2 ? go(k_attn_chunk8<4, 2>) : groups == 3 ? go(k_attn_chunk8<6, 2>) : go(k_attn_chunk8<8, 2>);
+    if (a.wide_from <= kTile) groups == 1 ? go(k_attn_chunk8<2, W8, 1>) : groups == 2 ? go(k_attn_chunk8<4, W, 1>) : groups == 3 ? go(k_attn_chunk8<6, W8, 1>) : go(k_attn_chunk8<8, W, 1>);
+    else groups == 1 ? go(k_attn_chunk8<2, W8, 2>) : groups == 2 ? go(k_attn_chunk8<4, W, 2>) : groups == 3 ? go(k_attn_chunk8<6, W8, 2>) : go(k_attn_chunk8<8, W, 2>);
+}
+void chunk8(const ChunkArgs& a, int bytes, unsigned blocks, hipStream_t s)
+{
+    if (bytes >= 16) launch8<16>(a, blocks, s);
+    else if (bytes == 8) launch8<8>(a, blocks, s);
+    else launch8<4>(a, blocks, s);
 }
 
 } // namespace nnhip

@@ -256,6 +256,20 @@ def test_chunk(new, past, q_heads, heads, dim, page, slopes, kind, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dim", [4, 8, 24, 28, 40, 44, 68, 72, 90, 100, 104, 116, 120, 127])
+def test_head_widths(dim, bits):
+    """Every width of the pieces that rows are read in, with up to 16, up to 32 and more rows of a key head."""
+    rng = np.random.default_rng(dim)
+    for new, past in (([4, 1], [90, 300]), ([7], [200]), ([7, 40, 1], [5, 60, 33])):
+        lens, start = [n + p for n, p in zip(new, past)], np.concatenate([[0], np.cumsum(new)])
+        x, table, pages = cache_for(rng, lens, 8, 2, dim, bits, holes=True)
+        q = rng.normal(size=(int(start[-1]), 6, dim)).astype(np.float32)
+        alpha = np.float32(1.0 / math.sqrt(dim))
+        got = run_chunk(x, dict(pages=pages, page=8, heads=2, dim=dim), table, q, start, max(new), lens, None, alpha)
+        check_chunk(got, ch.attend(q, x["K64"], x["V64"], table, 8, pages, 2, start, max(new), lens, float(alpha)))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("most,tokens", [(4, 40), (6, 70), (40, 200)])
 def test_tokens_of_no_sequence(bits, most, tokens):
     """Tokens before the first sequence, behind the last, past `most`; sequences shorter than their chunk, of length 0, of
