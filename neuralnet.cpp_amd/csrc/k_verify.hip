@@ -69,7 +69,7 @@ __constant__ const Powers kPowers;
 // exp((z - m) / temperature) for m >= z; NaN counts as -inf, and +inf beside +inf as equal. With x = (z - m) / temperature
 // in units of ln 2 / 32 and n the nearest whole number this is 2^(n / 32), from a table, times exp of (x - n) ln 2 / 32,
 // which is below 0.011: 1 + r + r^2 (1/2 + r/6 + r^2/24), the last in float32. Off by 2^-37 at most. No branch, so that a
-// thread's values go side by side. 144 rows of 100003 twice, first launch: 40 us with the series to r^13 in float64, 30 so;
+// thread's values go side by side. 144 rows of 100003 twice, first launch: 40 us with the series to r^13 in float64, 33 so;
 // the library's exp, one value after another, took 54.
 using Table = double[32];
 __device__ __forceinline__ double term(const VerifyArgs& a, const Table& powers, float z, float m)
@@ -280,21 +280,12 @@ __device__ __forceinline__ double left_of(const VerifyArgs& a, const Table& powe
     return fmax(p - q, 0.0);
 }
 
-// Sums of what is left of p over kLeft tokens, blockIdx.x = sequence * n_left + piece.
+// A workgroup's sum of what is left of p over the tokens from v0 to end; the first thread has it.
 constexpr unsigned kLeft = 8 * kThreads;
-__global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
+__device__ __forceinline__ double left_sum(const VerifyArgs& a, const Table& powers, const Decision& d, unsigned v0, unsigned end,
+                                           double (&s_s)[kThreads / 64])
 {
-    __shared__ DecideShared sh;
-    __shared__ double s_s[kThreads / 64];
-    __shared__ Table powers;
     const int t = threadIdx.x;
-    load_powers(powers);
-    __syncthreads();
-    const unsigned b = a.by_left.div(blockIdx.x), piece = blockIdx.x - b * a.n_left;
-    const Decision d = decide<false>(a, powers, b, sh);
-    if (piece == 0 && t == 0) a.decision[b] = d;
-    if (!d.drafted) return;
-    const unsigned v0 = piece * a.left_seg, end = min(v0 + a.left_seg, a.vocab);
     double s = 0.0;
     for (unsigned v = v0 + t; v < end; v += kLeft)
     {
@@ -307,7 +298,25 @@ __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
     s = wave_sum64(s);
     if ((t & 63) == 0) s_s[t >> 6] = s;
     __syncthreads();
-    if (t == 0) a.left[(size_t)b * a.n_left + piece] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+    return (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+}
+
+// These sums over kLeft tokens, blockIdx.x = sequence * n_left + piece.
+__global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
+{
+    __shared__ DecideShared sh;
+    __shared__ double s_s[kThreads / 64];
+    __shared__ Table powers;
+    const int t = threadIdx.x;
+    load_powers(powers);
+    __syncthreads();
+    const unsigned b = a.by_left.div(blockIdx.x), piece = blockIdx.x - b * a.n_left;
+    const Decision d = decide<false>(a, powers, b, sh);
+    if (piece == 0 && t == 0) a.decision[b] = d;
+    if (!d.drafted) return;
+    const unsigned v0 = piece * a.left_seg;
+    const double s = left_sum(a, powers, d, v0, min(v0 + a.left_seg, a.vocab), s_s);
+    if (t == 0) a.left[(size_t)b * a.n_left + piece] = s;
 }
 
 // Sums of all threads' values up to and with the thread's own.
@@ -354,7 +363,8 @@ __device__ __forceinline__ Found found(unsigned first, unsigned last, unsigned (
     return {min(min(first_w[0], first_w[1]), min(first_w[2], first_w[3])), max(max(last_w[0], last_w[1]), max(last_w[2], last_w[3]))};
 }
 
-// The next token of sequence blockIdx.x.
+// The next token of sequence blockIdx.x. DECIDE: without the second launch, which has nothing to do for single rows, and no
+// more for a vocabulary of one piece than this one can do for itself (4 drafted tokens of 1024: 22 us a call, 15 so).
 template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a)
 {
     __shared__ DecideShared sh;
@@ -377,8 +387,12 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     }
     const size_t at = (size_t)d.row * a.n_seg;
     bool left = d.drafted;   // whether p is lessened by q
+    double one = 0.0;
+    if constexpr (DECIDE)
+        if (left) one = left_sum(a, powers, d, 0, a.vocab, wave_s);
     auto of_segment = [&](unsigned i) -> double {
         if (i >= (left ? a.n_left : a.n_seg)) return 0.0;
+        if (DECIDE && left) return one;
         return left ? a.left[(size_t)b * a.n_left + i] : a.part_s[at + i] * term(a, powers, a.part_m[at + i], d.mt);
     };
     double whole = 0.0;
@@ -575,7 +589,7 @@ extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float*
     }
     sums(k_verify_sums<false, 4, kThreads>, k_verify_sums<false, 16, kThreads>, k_verify_sums<false, 4, 1024>, k_verify_sums<false, 16, 1024>);
     if (int rc = launch_status()) return rc;
-    if (most == 1)
+    if (most == 1 || plan.n_left == 1)
     {
         hipLaunchKernelGGL((k_verify_pick<false, true>), all, dim3(kThreads), 0, s, a);
         return launch_status();
