@@ -475,8 +475,10 @@ VerifyPlan verify_plan(size_t tokens, size_t vocab, bool token_major)
     VerifyPlan p{};
     if (!token_major)
         while (p.log2_cols < 5 && ((size_t)1 << p.log2_cols) < tokens) ++p.log2_cols;
-    // 16 logits a thread once they fill the CUs' threads (verify of 144 rows of 100003: PER), else 4.
-    p.per = 2 * tokens * vocab < ((size_t)1 << 22) ? 4 : 16;
+    // 16 logits a thread, for their way together and for fewer segments, or 4 where 16 leave CUs without work. A call with 4 and
+    // with 16, by columns: 5 rows of 1024 20 and 22 us, 4 rows of 50257 (no draft) 15 and 19, 5 of 50257 both 26, 40 of 50257 44 and
+    // 31; by rows: 20 of 32000 22 both, 144 of 100003 82 and 62.
+    p.per = tokens * vocab < ((size_t)1 << 19) ? 4 : 16;
     // Of several columns more threads, for as few segments: every sequence reads its rows' twice more.
     p.threads = p.log2_cols >= 2 ? 1024 : kThreads;
     size_t seg = (size_t)(p.threads >> p.log2_cols) * p.per;
