@@ -546,6 +546,7 @@ int nnhip_kv_reorder(const nnhip_kv_pages* layers, size_t n_layers, const float*
                      const float* fresh, size_t out_batch, float* table_out, float* len_out, void* stream);
 
 /* ── 8-bit caches, chunks of new tokens, drafted tokens (no CUDA counterpart) ──
+ * Here, too, all is float32 but the caches' bytes. A call that would take more than 2^24 workgroups is refused (-1).
  * A paged cache as nnhip_kv_pages with a byte a value: value j of head h of a row stands for
  * K[row * r + h * dim + j] * K_scale[r * heads + h] (V alike). K and V have pages * page rows, `row` bytes apart
  * (>= heads * dim), the scales (pages * page, heads). Table and limits as there. */
@@ -609,7 +610,7 @@ int nnhip_attn_chunk8(const nnhip_kv8_pages* c, const float* q, long q_t, long q
  * from a row to the next; the draft's alike with d_ld. Sequence b was fed the tokens fed[start[b] .. start[b + 1)), at most
  * `most`, of which all but the first were drafted: row n's distributions are those of the token after it, so that
  * fed[n + 1] was drawn from the draft's row n. With p = softmax(target / temperature) and q = softmax(draft /
- * temperature), both in float64, the token x after row n stands if accept[n] * q(x) < p(x). At the first row whose token
+ * temperature), both in float64, the token x after row n stands if accept[n] * q(x) < p(x) (of NaN it does not). At the first row whose token
  * does not stand, the next token is drawn from max(p - q, 0) (from p where that is 0 throughout), behind the last row
  * from p: the smallest v whose cumulative sum exceeds pick[b] times the whole sum. out_accepted[b] is the number of tokens
  * that stand, out_token[b] the token drawn: these many drafted tokens and that one continue the sequence, distributed as

@@ -57,7 +57,7 @@ __device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigne
 constexpr unsigned kFewParts = 16;
 __global__ __launch_bounds__(256) void k_attn_chunk_join_few(ChunkArgs a, unsigned narrow, unsigned wide)
 {
-    const unsigned at = blockIdx.x * 4 + threadIdx.x / 64;
+    const unsigned at = (blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64;
     const unsigned n = a.by_q_heads.div(at), h = at - n * a.q_heads;
     if (n >= a.tokens) return;
     Joined r{};
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
 {
     static_assert(kMostRanges <= 256);
     __shared__ float w_s[256], red[2][4], o_s[256];
-    const unsigned at = blockIdx.x, n = a.by_q_heads.div(at), h = at - n * a.q_heads;
+    const unsigned at = blockIdx.y * gridDim.x + blockIdx.x, n = a.by_q_heads.div(at), h = at - n * a.q_heads;
+    if (n >= a.tokens) return;
     const Joined r = joined(a, n, narrow, wide);
     if (r.ranges == 0) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, dim = a.c.t.dim;
@@ -261,7 +262,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     const ChunkPlan p = chunk_plan(call);
     const size_t need = chunk_workspace(call, p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
-    if (p.blocks > kGridMost || p.wide_blocks > kGridMost || (p.slots() > kFewParts ? tokens * q_heads : tokens * q_heads / 4 + 1) > kGridMost) return -1;
+    if (p.blocks > kGridMost || p.wide_blocks > kGridMost) return -1;
     auto* ws = static_cast<float*>(workspace);
     ChunkArgs a{};
     a.c = call.c;
@@ -322,9 +323,10 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
         }
     }
     if (p.slots() == 1) return 0;
-    const size_t rows = tokens * q_heads;
-    if (p.slots() <= kFewParts) hipLaunchKernelGGL(k_attn_chunk_join_few, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a, p.narrow, p.wide);
-    else hipLaunchKernelGGL(k_attn_chunk_join, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, a, p.narrow, p.wide);
+    const bool few = p.slots() <= kFewParts;
+    const size_t blocks = few ? (tokens * q_heads + 3) / 4 : tokens * q_heads, x = std::min(blocks, (size_t)1 << 20);
+    const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>((blocks + x - 1) / x));
+    hipLaunchKernelGGL(few ? k_attn_chunk_join_few : k_attn_chunk_join, grid, dim3(256), 0, s, a, p.narrow, p.wide);
     return launch_status();
 }
 

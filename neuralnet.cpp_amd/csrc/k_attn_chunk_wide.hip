@@ -435,7 +435,8 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     const f32x4* image = reinterpret_cast<const f32x4*>(images + begin / kPos);
     f32x4 piece[kPieces], tail;
     auto fetch = [&](int i, int half) __attribute__((always_inline)) {
-        const f32x4* from = image + (size_t)min(i, tiles - 1) * (sizeof(S) / 16) + half * kHalf;
+        // (a sequence whose length is 0 has no tile: the first one's place is read for it)
+        const f32x4* from = image + (size_t)max(min(i, tiles - 1), 0) * (sizeof(S) / 16) + half * kHalf;
 #pragma unroll
         for (int x = 0; x < kPieces; ++x)
             if (256 * x + 256 <= kHalf || 256 * x + 64 * wave < kHalf) piece[x] = from[256 * x + t];

@@ -367,6 +367,21 @@ def test_large_values_that_a_token_does_not_see(new, past, per, dim, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("new,lens", [([40], [0]), ([40], [float("nan")]), ([200], [-3]), ([200], [90]), ([50, 60, 3, 2], [0, 300, 0, 40]),
+                                      ([50, 60, 70], [0, 0, 0]), ([40, 0, 33], [45, 20, 12])])
+def test_lengths_below_the_chunks(new, lens, bits):
+    """Sequences that are shorter than their chunk: tokens in front of the first position see nothing."""
+    rng = np.random.default_rng(len(new))
+    page, heads, dim = 16, 2, 64
+    held = [int(n) if n > 0 else 0 for n in lens]
+    x, table, pages = cache_for(rng, held, page, heads, dim, bits)
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = rng.normal(size=(int(start[-1]), 2, dim)).astype(np.float32)
+    got = run_chunk(x, dict(pages=pages, page=page, heads=heads, dim=dim), table, q, start, max(new), lens, None, 0.2)
+    check_chunk(got, ch.attend(q, x["K64"], x["V64"], table, page, pages, heads, start, max(new), held, 0.2))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_table_of_many_positions(bits):
     """Tables that reach 2^24 positions: the keys' and values' parts are formed a sequence and key head at a time."""
     rng = np.random.default_rng(bits)
