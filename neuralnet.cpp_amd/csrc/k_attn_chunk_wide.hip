@@ -480,11 +480,12 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             }
         }
         qe = exponent_of(across(top, [](float x, float y) { return fmaxf(x, y); }));
+        const float sign = a.alpha < 0.0f ? -1.0f : a.alpha == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
         {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[k][e] = __builtin_ldexpf(a.alpha < 0.0f ? -z[k][e] : z[k][e], 15 - qe);
+            for (int e = 0; e < 8; ++e) z[k][e] = __builtin_ldexpf(z[k][e] * sign, 15 - qe);
             split2(z[k], qp[k][0], qp[k][1]);
         }
     }
@@ -495,8 +496,9 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     fetch(1, 0);
     __syncthreads();
     const float slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
-    // Scores times log2(e); not 0, which would make a masked score's product NaN (alpha 0: 2^-149 of at most 2^127 is none).
-    const float scale = fmaxf(__builtin_ldexpf(fabsf(a.alpha) * kLog2e, qe - 10), 0x1p-149f);
+    // Scores times log2(e), of queries that have alpha's sign (0 of an alpha of 0); not 0, which would make a masked score's
+    // product NaN.
+    const float by_alpha = __builtin_ldexpf(fabsf(a.alpha) * kLog2e, qe - 10), scale = by_alpha == 0.0f ? 0x1p-149f : by_alpha;
     const float by = a.slopes ? 1.0f : scale;   // of the scores as the softmax sees them
     float m = kLowest, l = 0.0f;
     int top = kNone;                // exponent that the row's values are held against

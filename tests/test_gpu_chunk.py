@@ -382,6 +382,55 @@ def test_lengths_below_the_chunks(new, lens, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("new,past,per", [(5, 60, 2), (9, 40, 3), (70, 33, 1), (50, 9, 4)])
+def test_factors_of_the_scores(new, past, per, bits):
+    """alpha 0, negative and NaN; a query that is not finite, which changes its own row alone."""
+    rng = np.random.default_rng(new)
+    page, heads, dim = 16, 2, 48
+    lens, start = [new + past], [0, new]
+    x, table, pages = cache_for(rng, lens, page, heads, dim, bits)
+    c = dict(pages=pages, page=page, heads=heads, dim=dim)
+    q = rng.normal(size=(new, heads * per, dim)).astype(np.float32)
+    sl = (2.0 ** -np.arange(1, heads * per + 1)).astype(np.float32)
+    for alpha in (0.0, -0.3):
+        for slopes in (None, sl):
+            got = run_chunk(x, c, table, q, start, new, lens, slopes, np.float32(alpha))
+            check_chunk(got, ch.attend(q, x["K64"], x["V64"], table, page, pages, heads, start, new, lens, float(np.float32(alpha)), slopes))
+    assert np.isnan(run_chunk(x, c, table, q, start, new, lens, None, np.float32("nan"))[0]).all()
+    clean = run_chunk(x, c, table, q, start, new, lens, None, np.float32(0.2))[0]
+    want = ch.attend(q, x["K64"], x["V64"], table, page, pages, heads, start, new, lens, float(np.float32(0.2)))
+    for value in (np.nan, np.inf):
+        y = q.copy()
+        y[2, 1, 3] = value
+        O = run_chunk(x, c, table, y, start, new, lens, None, np.float32(0.2))[0]
+        rest = np.ones(O.shape[:2], bool)
+        rest[2, 1] = False
+        assert np.all(np.abs(O - want[0])[rest] <= want[3][rest]) and np.all(np.abs(clean - want[0]) <= want[3])
+        if bits == 8 or np.isnan(value):
+            assert np.isnan(O[2, 1]).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_rows(bits):
+    """Four million rows, long and single ones, the join's grid in two dimensions: some of them against the 64-bit form."""
+    rng = np.random.default_rng(bits)
+    page, heads, dim, qh, new, past = 64, 8, 4, 128, [8300, 1, 8300, 16600, 3], [5, 700, 0, 40, 90]
+    lens, start = [n + p for n, p in zip(new, past)], np.concatenate([[0], np.cumsum(new)])
+    x, table, pages = cache_for(rng, lens, page, heads, dim, bits)
+    N = int(start[-1])
+    assert N * qh > 1 << 22
+    q = rng.normal(size=(N, qh, dim)).astype(np.float32)
+    O, m, l = run_chunk(x, dict(pages=pages, page=page, heads=heads, dim=dim), table, q, start, max(new), lens, None, 0.5)
+    for n in (0, 1, 8299, 8300, 8301, 12000, 16600, 16601, 30000, 33200, 33201, 33202, N - 1):
+        b = int(np.searchsorted(start, n, side="right")) - 1
+        seen = lens[b] - new[b] + n - int(start[b]) + 1
+        for h in (0, 77, 127):   # the token alone, as the last of what it sees
+            w = ch.attend(q[n:n + 1, h:h + 1], x["K64"][:, h // 16:h // 16 + 1], x["V64"][:, h // 16:h // 16 + 1], table[b:b + 1], page, pages, 1,
+                          [0, 1], 1, [seen], 0.5)
+            assert np.all(np.abs(O[n, h] - w[0][0, 0]) <= w[3][0, 0]) and abs(m[n, h] - w[1][0, 0]) <= w[4][0, 0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_table_of_many_positions(bits):
     """Tables that reach 2^24 positions: the keys' and values' parts are formed a sequence and key head at a time."""
     rng = np.random.default_rng(bits)

@@ -183,3 +183,63 @@ def test_calls_between_graphs_and_streams(hip):
         for k in outs:
             assert torch.equal(got[0][k], got[1][k]), (i, k)
         assert got[0]["o"].abs().sum() > 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_prompts_in_a_graph(hip, bits):
+    """A prompt's chunk beside single tokens, every kernel of the attention, captured and replayed with other contents and
+    lengths: the same bits as the eager calls."""
+    import torch
+
+    import chunk_helpers as ch
+    from test_gpu_paged import dev, ptr
+    lib = ch.library()
+    new, qh, heads, dim, page, width = [70, 1, 1, 40], 4, 2, 64, 16, 40
+    B, N, pages = len(new), sum(new), len(new) * width
+    rng = np.random.default_rng(bits)
+    table, start = dev(rng.permutation(pages).reshape(B, width)), dev(np.concatenate([[0], np.cumsum(new)]))
+    q, o, lens = torch.zeros(N, qh * dim).cuda(), torch.zeros(N, qh * dim).cuda(), torch.zeros(B).cuda()
+    if bits == 32:
+        K, V = (torch.zeros(pages * page, heads * dim).cuda() for _ in range(2))
+        c = ch.Pages(ptr(K), ptr(V), ptr(table), B, width, pages, page, heads, dim, heads * dim)
+        need, call = lib.nnhip_attn_chunk_workspace_bytes(c, qh, N, 70), lib.nnhip_attn_chunk
+    else:
+        K, V = (torch.zeros(pages * page, heads * dim, dtype=torch.int8).cuda() for _ in range(2))
+        Ks, Vs = (torch.zeros(pages * page, heads).cuda() for _ in range(2))
+        c = ch.Pages8(ptr(K), ptr(V), ptr(Ks), ptr(Vs), ptr(table), B, width, pages, page, heads, dim, heads * dim)
+        need, call = lib.nnhip_attn_chunk8_workspace_bytes(c, qh, N, 70), lib.nnhip_attn_chunk8
+    ws = torch.full((need // 4 + 4,), float("nan")).cuda()
+
+    def step():
+        assert call(c, ptr(q), qh * dim, 1, qh, N, ptr(start), 70, ptr(lens), None, 0.125, ptr(o), qh * dim, 1, None, None, ptr(ws), need,
+                    torch.cuda.current_stream().cuda_stream) == 0
+
+    def load(i):
+        r = np.random.default_rng(50 + i)
+        q.copy_(dev(r.normal(size=(N, qh * dim))))
+        lens.copy_(dev(np.array(new) + [100 * i, 30, 500 - 100 * i, 0]))
+        for t in (K, V):
+            t.copy_(dev(r.normal(size=tuple(t.shape))) if bits == 32 else torch.as_tensor(r.integers(-127, 128, tuple(t.shape)).astype(np.int8)).cuda())
+        if bits == 8:
+            for t in (Ks, Vs):
+                t.copy_(dev(r.uniform(0.005, 0.02, tuple(t.shape))))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        load(0)
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    torch.cuda.synchronize()
+    for i in range(4):
+        got = []
+        for replay in (True, False):
+            load(i)
+            o.fill_(3.0)
+            torch.cuda.synchronize()
+            graph.replay() if replay else step()
+            torch.cuda.synchronize()
+            got.append(o.clone())
+        assert torch.equal(*got) and got[0].abs().sum() > 0
