@@ -17,7 +17,9 @@ namespace nnhip
 namespace
 {
 
-// Sequences of up to 16 RT rows.
+// Sequences of up to 16 RT rows, bound by the cache's bytes: 32 single tokens behind 3000 positions, 12 heads of 64, take 100 us
+// (460 MB, 4.6 TB/s), 48 of 4000 to 8000, 8 heads of 128, 400 (5.9); five tokens of one sequence behind 700, 7 and the join's
+// 3 of latency.
 template <int BITS, int KS, bool VEC, int RT> __global__ __launch_bounds__(256, VEC ? 2 : 1) void k_attn_chunk(ChunkArgs a)
 {
     __shared__ WalkShared<KS> sh;

@@ -10,6 +10,11 @@
 // falls into, and the token within it. Sums, probabilities and comparisons are
 // in float64: float32's would move the border between two tokens by 2^-24 of
 // the whole, far more than most tokens' probability.
+//
+// The first launch is bound by its exponentials (144 rows of 100003 of either
+// model: 32 us, 3.5 TB/s; 144 of 32000 by columns 17), the others by latency:
+// a sequence's decision, a scan of its row's sums and a search by one
+// workgroup, 10 to 18 us each.
 #include "kv_pages.hpp"
 
 namespace nnhip
