@@ -285,28 +285,8 @@ __device__ __forceinline__ double left_of(const VerifyArgs& a, const Table& powe
     return fmax(p - q, 0.0);
 }
 
-// A workgroup's sum of what is left of p over the tokens from v0 to end; the first thread has it.
+// Sums of what is left of p over kLeft tokens, blockIdx.x = sequence * n_left + piece.
 constexpr unsigned kLeft = 8 * kThreads;
-__device__ __forceinline__ double left_sum(const VerifyArgs& a, const Table& powers, const Decision& d, unsigned v0, unsigned end,
-                                           double (&s_s)[kThreads / 64])
-{
-    const int t = threadIdx.x;
-    double s = 0.0;
-    for (unsigned v = v0 + t; v < end; v += kLeft)
-    {
-        double x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = left_of(a, powers, d, min(v + i * kThreads, end - 1));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += v + i * kThreads < end ? x[i] : 0.0;
-    }
-    s = wave_sum64(s);
-    if ((t & 63) == 0) s_s[t >> 6] = s;
-    __syncthreads();
-    return (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
-}
-
-// These sums over kLeft tokens, blockIdx.x = sequence * n_left + piece.
 __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
 {
     __shared__ DecideShared sh;
@@ -319,9 +299,20 @@ __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
     const Decision d = decide<false>(a, powers, b, sh);
     if (piece == 0 && t == 0) a.decision[b] = d;
     if (!d.drafted) return;
-    const unsigned v0 = piece * a.left_seg;
-    const double s = left_sum(a, powers, d, v0, min(v0 + a.left_seg, a.vocab), s_s);
-    if (t == 0) a.left[(size_t)b * a.n_left + piece] = s;
+    const unsigned v0 = piece * a.left_seg, end = min(v0 + a.left_seg, a.vocab);
+    double s = 0.0;
+    for (unsigned v = v0 + t; v < end; v += kLeft)
+    {
+        double x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = left_of(a, powers, d, min(v + i * kThreads, end - 1));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v + i * kThreads < end ? x[i] : 0.0;
+    }
+    s = wave_sum64(s);
+    if ((t & 63) == 0) s_s[t >> 6] = s;
+    __syncthreads();
+    if (t == 0) a.left[(size_t)b * a.n_left + piece] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
 }
 
 // Sums of all threads' values up to and with the thread's own.
@@ -368,8 +359,9 @@ __device__ __forceinline__ Found found(unsigned first, unsigned last, unsigned (
     return {min(min(first_w[0], first_w[1]), min(first_w[2], first_w[3])), max(max(last_w[0], last_w[1]), max(last_w[2], last_w[3]))};
 }
 
-// The next token of sequence blockIdx.x. DECIDE: without the second launch, which has nothing to do for single rows, and no
-// more for a vocabulary of one piece than this one can do for itself (4 drafted tokens of 1024: 22 us a call, 15 so).
+// The next token of sequence blockIdx.x. DECIDE: without the second launch, which has nothing to do for single rows, and for
+// a vocabulary of one piece no more than this one does on its way: its threads hold all of it, so that it is read once
+// (4 drafted tokens of 1024: 22 us a call with three launches, 15 with two that read it twice, 13 so).
 template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a)
 {
     __shared__ DecideShared sh;
@@ -392,12 +384,52 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     }
     const size_t at = (size_t)d.row * a.n_seg;
     bool left = d.drafted;   // whether p is lessened by q
-    double one = 0.0;
-    if constexpr (DECIDE)
-        if (left) one = left_sum(a, powers, d, 0, a.vocab, wave_s);
+    constexpr int kEach = 8;   // neighbouring tokens of a thread
+    // The weights of tokens from v on, and their sum.
+    auto weights = [&](unsigned v, unsigned end, double (&x)[kEach]) -> double {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            const unsigned at = min(v + i, end - 1);
+            x[i] = left ? left_of(a, powers, d, at) : term(a, powers, a.target[(size_t)d.row * a.t_row + (size_t)at * a.t_col], d.mt);
+            if (v + i >= end) x[i] = 0.0;
+            sum += x[i];
+        }
+        return sum;
+    };
+    // Of these the first whose cumulative sum, of `up` before the first, is above `want`, and the last with anything.
+    auto search = [&](unsigned v, const double (&x)[kEach], double up, double want) -> Found {
+        unsigned first = a.vocab, last = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            up += x[i];
+            if (x[i] > 0.0)
+            {
+                last = v + i;
+                if (up > want) first = min(first, v + i);
+            }
+        }
+        return found(first, last, first_w, last_w);
+    };
+    const float w = a.pick[b];
+    const double share = w >= 1.0f ? 1.0 - 0x1p-53 : w > 0.0f ? (double)w : 0.0;
+    if (DECIDE && a.vocab <= kEach * kThreads)
+    {
+        double x[kEach], mine = weights(kEach * t, a.vocab, x), all, up = scan(mine, wave_s, all);
+        if (left && !(all > 0.0))
+        {
+            left = false;
+            mine = weights(kEach * t, a.vocab, x);
+            up = scan(mine, wave_s, all);
+        }
+        const Found in = search(kEach * t, x, up - mine, share * all);
+        if (t == 0) a.out_token[b] = (float)(in.first < a.vocab ? in.first : in.last);
+        return;
+    }
     auto of_segment = [&](unsigned i) -> double {
         if (i >= (left ? a.n_left : a.n_seg)) return 0.0;
-        if (DECIDE && left) return one;
         return left ? a.left[(size_t)b * a.n_left + i] : a.part_s[at + i] * term(a, powers, a.part_m[at + i], d.mt);
     };
     double whole = 0.0;
@@ -413,8 +445,7 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
         if (whole > 0.0 || !left) break;
         left = false;
     }
-    const float w = a.pick[b];
-    const double want = (w >= 1.0f ? 1.0 - 0x1p-53 : w > 0.0f ? (double)w : 0.0) * whole;
+    const double want = share * whole;
     // The first segment whose cumulative sum is above that, the last one with anything where rounding leaves none.
     const unsigned segs = left ? a.n_left : a.n_seg, size = left ? a.left_seg : a.seg;
     Found in{segs, 0};
@@ -433,36 +464,15 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     }
     const bool some = in.first < segs;
     const unsigned seg = some ? in.first : in.last;
-    // The token, alike: a thread takes kEach neighbouring ones.
-    constexpr int kEach = 8;
+    // The token, alike.
     const unsigned end = min((seg + 1) * size, a.vocab);
     in = {a.vocab, 0};
     sum = some ? base : -__builtin_inf();
     for (unsigned v0 = seg * size; v0 < end && in.first == a.vocab; v0 += kThreads * kEach)
     {
-        double x[kEach], mine = 0.0, all;
-        const unsigned v = v0 + kEach * t;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-        {
-            const unsigned at = min(v + i, end - 1);
-            x[i] = left ? left_of(a, powers, d, at) : term(a, powers, a.target[(size_t)d.row * a.t_row + (size_t)at * a.t_col], d.mt);
-            if (v + i >= end) x[i] = 0.0;
-            mine += x[i];
-        }
-        double up = sum + (scan(mine, wave_s, all) - mine);
-        unsigned first = a.vocab, last = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-        {
-            up += x[i];
-            if (x[i] > 0.0)
-            {
-                last = v + i;
-                if (up > want) first = min(first, v + i);
-            }
-        }
-        const Found here = found(first, last, first_w, last_w);
+        double x[kEach], all;
+        const double mine = weights(v0 + kEach * t, end, x);
+        const Found here = search(v0 + kEach * t, x, sum + (scan(mine, wave_s, all) - mine), want);
         in.first = min(in.first, here.first);
         in.last = max(in.last, here.last);
         sum += all;
