@@ -186,6 +186,7 @@ struct DecideShared
 {
     float m[2 * kRowsAtOnce];
     double s[2 * kRowsAtOnce];   // or the index of m
+    int x[kRowsAtOnce];          // the drafted tokens behind the rows
     int first;
 };
 // A workgroup: what becomes of sequence b.
@@ -199,6 +200,21 @@ template <bool GREEDY> __device__ __forceinline__ Decision decide(const VerifyAr
     d.mt = d.md = -__builtin_inff();
     for (int i0 = 0; i0 < n; i0 += kRowsAtOnce)
     {
+        // A row a lane: its drafted token and what belongs to that, on their way while the sums are joined.
+        const bool there = t < kRowsAtOnce && i0 + t < n, has_token = there && i0 + t < n - 1;
+        int x = -1;
+        float accept = 0.0f, zt = 0.0f, zd = 0.0f;
+        if (has_token)
+        {
+            const size_t row = lo + i0 + t;
+            x = drafted(a, row);
+            if (!GREEDY && x >= 0)
+            {
+                accept = a.accept[row];
+                zt = a.target[row * a.t_row + (size_t)x * a.t_col];
+                if (a.draft) zd = a.draft[row * a.d_row + (size_t)x * a.d_col];
+            }
+        }
         const int i = i0 + (group >> 1);
         if (i < n && (model == 0 || (a.draft && i < n - 1)))
         {
@@ -228,24 +244,20 @@ template <bool GREEDY> __device__ __forceinline__ Decision decide(const VerifyAr
         }
         if (t == 0) sh.first = n;
         __syncthreads();
-        if (t < 64)   // a row a lane
+        if (t < 64)
         {
-            const bool there = t < kRowsAtOnce && i0 + t < n;
             bool stands = false;
-            if (there && i0 + t < n - 1)
+            if (has_token)
             {
-                const unsigned row = lo + i0 + t;
-                const int x = drafted(a, row);
                 if constexpr (GREEDY) stands = (int)sh.s[2 * t] == x;
-                else
+                else if (x >= 0)   // no token stands with 0 of p, as one that is none
                 {
-                    auto p_of = [&](const float* z, size_t r, size_t c, int k) {
-                        return x < 0 || sh.s[k] == 0.0 ? 0.0 : term(a, powers, z[row * r + (size_t)x * c], sh.m[k]) * (1.0 / sh.s[k]);
-                    };
-                    const double px = p_of(a.target, a.t_row, a.t_col, 2 * t), qx = a.draft ? p_of(a.draft, a.d_row, a.d_col, 2 * t + 1) : 1.0;
-                    stands = (double)a.accept[row] * qx < px;
+                    auto p_of = [&](float z, int k) { return sh.s[k] == 0.0 ? 0.0 : term(a, powers, z, sh.m[k]) * (1.0 / sh.s[k]); };
+                    const double px = p_of(zt, 2 * t), qx = a.draft ? p_of(zd, 2 * t + 1) : 1.0;
+                    stands = (double)accept * qx < px;
                 }
             }
+            if (there) sh.x[t] = x;
             const unsigned long long ends = __builtin_amdgcn_ballot_w64(there && !stands);
             if (t == 0 && ends) sh.first = i0 + __builtin_ctzll(ends);
         }
@@ -259,7 +271,7 @@ template <bool GREEDY> __device__ __forceinline__ Decision decide(const VerifyAr
             if constexpr (GREEDY) d.token = (int)sh.s[k];
             else
             {
-                d.token = d.drafted ? drafted(a, lo + f) : -1;
+                d.token = sh.x[f - i0];
                 d.mt = sh.m[k];
                 d.pt = sh.s[k] == 0.0 ? 0.0 : 1.0 / sh.s[k];
                 if (d.drafted && a.draft)
