@@ -28,6 +28,8 @@ struct ChunkArgs
     char* images;                    // its keys' and values' parts: `tiles` a piece, of the pieces (slot and key head)
     unsigned tiles, first_piece, pieces;   // that the launch is for
     int slots_by_batch;              // a slot a sequence
+    FastDiv by_block_rows;           // its blocks of rows are numbered from first row / these on, plus, if block_seqs, the
+    int block_seqs;                  // sequence's number
     FastDiv by_per, by_heads, by_q_heads, by_row_blocks, by_ranges;   // by_row_blocks: of k_attn_chunk_wide
     int q_rows;                      // queries lie a token a row, 16-byte aligned
     int vec;                         // the cache's rows can be read in pieces of 4 values

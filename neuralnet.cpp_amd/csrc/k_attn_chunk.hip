@@ -159,6 +159,7 @@ struct ChunkPlan
     int wide_from;
     unsigned narrow, wide;   // ranges of the two kernels' rows, 0: it is not launched
     size_t blocks, wide_row_blocks, wide_blocks;
+    bool wide_by_seqs;
     size_t image_slots, image_tiles, image_pieces;   // of the parts; pieces that are formed at a time
     unsigned slots() const { return std::max(narrow, wide); }
 };
@@ -185,8 +186,11 @@ ChunkPlan chunk_plan(const ChunkCall& c)
     p.blocks = (batch * p.narrow + 7) / 8 * 8 * heads;
     if (c.most * per > kNarrowRows)
     {
-        p.wide_row_blocks = c.tokens * per / kWideRows + batch;
-        const size_t others = heads * std::max<size_t>(c.tokens * per / kWideRows, 1), most_wide = (positions + 255) / 256;
+        // Numbers of blocks of rows: fewer by the sequences' numbers where these are few, else by rows alone.
+        const size_t by_seqs = c.tokens * per / kWideRows + batch, by_rows = c.tokens * per / (kNarrowRows + 1) + 1;
+        p.wide_by_seqs = by_seqs <= by_rows || batch == 1;
+        p.wide_row_blocks = p.wide_by_seqs ? by_seqs : by_rows;
+        const size_t others = heads * ((c.tokens * per + kWideRows - 1) / kWideRows), most_wide = (positions + 255) / 256;
         p.wide = static_cast<unsigned>(std::min<size_t>(std::min(std::max<size_t>(2 * cus / others, 1), most_wide), kMostRanges));
         p.wide_blocks = (p.wide_row_blocks * heads * p.wide + 7) / 8 * 8;
         if (batch == 1) p.narrow = 0, p.wide_from = 0;   // one launch, however few tokens the sequence has
@@ -309,13 +313,16 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
         w.ranges = p.wide;
         w.by_ranges = FastDiv(p.wide);
         w.by_row_blocks = FastDiv(static_cast<unsigned>(p.wide_row_blocks));
+        w.by_block_rows = FastDiv(p.wide_by_seqs ? kWideRows : kNarrowRows + 1);
+        w.block_seqs = p.wide_by_seqs;
         w.images = static_cast<char*>(workspace) + chunk_results(call, p);
         w.tiles = static_cast<unsigned>(p.image_tiles);
         w.slots_by_batch = p.image_slots == call.c.t.batch;
-        const size_t all = p.image_slots * call.c.t.heads;
+        // Workgroups: of several slots most may have nothing to do.
+        const size_t all = p.image_slots * call.c.t.heads, heads_of_one = call.c.t.heads;
         for (size_t at = 0; at < all; at += p.image_pieces)
         {
-            const size_t pieces = std::min(p.image_pieces, all - at), each = std::min(p.image_tiles, (8 * device_cus() + pieces - 1) / pieces);
+            const size_t pieces = std::min(p.image_pieces, all - at), each = std::min(p.image_tiles, ((all == heads_of_one ? 8 : 32) * device_cus() + pieces - 1) / pieces);
             w.first_piece = static_cast<unsigned>(at);
             w.pieces = static_cast<unsigned>(pieces);
             chunk_parts(w, call.bits, w.pieces, static_cast<unsigned>(each), s);

@@ -400,8 +400,9 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         part.h = a.by_ranges.div(piece);
         part.slot = piece - part.h * a.ranges;
         if (part.h >= a.c.t.heads) return;
-        // Sequence b's blocks of rows are numbered from first row / 128 + b on: at least as many as it has.
-        auto base = [&](unsigned b) { return (unsigned)((size_t)length_of(a.start[b], a.tokens) * a.by_per.d / kWideRows) + b; };
+        // At least as many numbers as a sequence of more than kNarrowRows rows has blocks: first row / 128 + its own number,
+        // or first row / (kNarrowRows + 1).
+        auto base = [&](unsigned b) { return a.by_block_rows.div(length_of(a.start[b], a.tokens) * a.by_per.d) + (a.block_seqs ? b : 0); };
         const int b = last_of(a.c.t.batch, [&](unsigned i) { return base(i) <= x; });
         if (b < 0) return;
         part.b = b;
