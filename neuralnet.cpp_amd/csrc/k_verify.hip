@@ -14,7 +14,7 @@
 // The first launch is bound by its exponentials (144 rows of 100003 of either
 // model: 32 us, 3.5 TB/s; 144 of 32000 by columns 17), the others by latency:
 // a sequence's decision, a scan of its row's sums and a search by one
-// workgroup, 10 to 18 us each.
+// workgroup, 9 to 17 us each.
 #include "kv_pages.hpp"
 
 namespace nnhip
@@ -297,8 +297,11 @@ __device__ __forceinline__ double left_of(const VerifyArgs& a, const Table& powe
     return fmax(p - q, 0.0);
 }
 
-// Sums of what is left of p over kLeft tokens, blockIdx.x = sequence * n_left + piece.
-constexpr unsigned kLeft = 8 * kThreads;
+// Sums of what is left of p over kLeft tokens, blockIdx.x = sequence * n_left + piece. A call of 24 sequences of up to 5 drafted
+// tokens of 32000 with pieces of 2048 tokens 45 us, of 1024 41, of 512 48; of one sequence 23.5, 21, 20.
+constexpr unsigned kLeft = 4 * kThreads;
+constexpr int kEach = 8;                       // neighbouring tokens of a thread that looks for one
+constexpr unsigned kWhole = kEach * kThreads;   // a vocabulary of which that thread's workgroup holds all
 __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
 {
     __shared__ DecideShared sh;
@@ -315,11 +318,11 @@ __global__ __launch_bounds__(kThreads) void k_verify_left(VerifyArgs a)
     double s = 0.0;
     for (unsigned v = v0 + t; v < end; v += kLeft)
     {
-        double x[8];
+        double x[kLeft / kThreads];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = left_of(a, powers, d, min(v + i * kThreads, end - 1));
+        for (unsigned i = 0; i < kLeft / kThreads; ++i) x[i] = left_of(a, powers, d, min(v + i * kThreads, end - 1));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += v + i * kThreads < end ? x[i] : 0.0;
+        for (unsigned i = 0; i < kLeft / kThreads; ++i) s += v + i * kThreads < end ? x[i] : 0.0;
     }
     s = wave_sum64(s);
     if ((t & 63) == 0) s_s[t >> 6] = s;
@@ -372,7 +375,7 @@ __device__ __forceinline__ Found found(unsigned first, unsigned last, unsigned (
 }
 
 // The next token of sequence blockIdx.x. DECIDE: without the second launch, which has nothing to do for single rows, and for
-// a vocabulary of one piece no more than this one does on its way: its threads hold all of it, so that it is read once
+// a vocabulary of kWhole no more than this one does on its way: its threads hold all of it, so that it is read once
 // (4 drafted tokens of 1024: 22 us a call with three launches, 15 with two that read it twice, 13 so).
 template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a)
 {
@@ -396,7 +399,6 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     }
     const size_t at = (size_t)d.row * a.n_seg;
     bool left = d.drafted;   // whether p is lessened by q
-    constexpr int kEach = 8;   // neighbouring tokens of a thread
     // The weights of tokens from v on, and their sum.
     auto weights = [&](unsigned v, unsigned end, double (&x)[kEach]) -> double {
         double sum = 0.0;
@@ -427,7 +429,7 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     };
     const float w = a.pick[b];
     const double share = w >= 1.0f ? 1.0 - 0x1p-53 : w > 0.0f ? (double)w : 0.0;
-    if (DECIDE && a.vocab <= kEach * kThreads)
+    if (DECIDE && a.vocab <= kWhole)
     {
         double x[kEach], mine = weights(kEach * t, a.vocab, x), all, up = scan(mine, wave_s, all);
         if (left && !(all > 0.0))
@@ -444,14 +446,15 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
         if (i >= (left ? a.n_left : a.n_seg)) return 0.0;
         return left ? a.left[(size_t)b * a.n_left + i] : a.part_s[at + i] * term(a, powers, a.part_m[at + i], d.mt);
     };
-    double whole = 0.0;
+    double whole = 0.0, own = 0.0, own_up = 0.0;
     for (int again = 0; again < 2; ++again)
     {
         whole = 0.0;
         for (unsigned i = 0; i < (left ? a.n_left : a.n_seg); i += kThreads)
         {
             double all;
-            scan(of_segment(i + t), wave_s, all);
+            own = of_segment(i + t);
+            own_up = scan(own, wave_s, all);
             whole += all;
         }
         if (whole > 0.0 || !left) break;
@@ -464,8 +467,9 @@ template <bool GREEDY, bool DECIDE> __global__ __launch_bounds__(kThreads) void 
     double sum = 0.0, base = 0.0;
     for (unsigned i = 0; i < segs && in.first == segs; i += kThreads)
     {
-        double all;
-        const double x = of_segment(i + t), up = sum + scan(x, wave_s, all);
+        double all = 0.0;
+        const bool once = segs <= kThreads;   // all of them are in the threads already
+        const double x = once ? own : of_segment(i + t), up = sum + (once ? own_up : scan(x, wave_s, all));
         const Found here = found(x > 0.0 && up > want ? i + t : segs, x > 0.0 ? i + t : 0, first_w, last_w);
         in.first = min(in.first, here.first);
         in.last = max(in.last, here.last);
@@ -618,7 +622,7 @@ extern "C" int nnhip_draft_verify(const float* target, size_t t_ld, const float*
     }
     sums(k_verify_sums<false, 4, kThreads>, k_verify_sums<false, 16, kThreads>, k_verify_sums<false, 4, 1024>, k_verify_sums<false, 16, 1024>);
     if (int rc = launch_status()) return rc;
-    if (most == 1 || plan.n_left == 1)
+    if (most == 1 || vocab <= kWhole)
     {
         hipLaunchKernelGGL((k_verify_pick<false, true>), all, dim3(kThreads), 0, s, a);
         return launch_status();
