@@ -36,6 +36,8 @@
 #include "attn_chunk.hpp"
 #include "f16_parts.hpp"
 
+#include <type_traits>
+
 namespace nnhip
 {
 namespace
@@ -48,13 +50,14 @@ __device__ __forceinline__ floatx16 mfma32(const half8& x, const half8& y, const
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
 }
 
-// A tile's parts, of one key head.
+// A tile's parts, of one key head of up to 16 KS dims.
 template <int BITS, int KS> struct alignas(16) Image
 {
     static constexpr int P = BITS == 32 ? 2 : 1;   // parts
+    static constexpr int NB = (KS + 1) / 2;        // blocks of 32 value dims
     // Operands by lane: [step or block of 32 dims and k step][part][lane's place]
     half8 k[KS][P][64];
-    half8 v[KS / 2][2][P][64];
+    half8 v[NB][2][P][64];
     float k_scale[kPos];           // of the scores
     float v_scale[kPos];           // of the weights: the values' scales; BITS 32: a quarter of 2^(exponent of the position's values)
     int v_top[4];                  // exponents of the values: of each group of 8 positions; BITS 8: all [0]
@@ -76,7 +79,7 @@ template <int BITS, int KS> struct Wide
 {
     using R = Raw<BITS, KS>;
     using S = Image<BITS, KS>;
-    static constexpr int P = S::P, NB = KS / 2;
+    static constexpr int P = S::P, NB = S::NB;
 
     const ChunkArgs& a;
     const Part& part;
@@ -190,7 +193,7 @@ template <int BITS, int KS> struct Wide
     __device__ __forceinline__ void stage(const R& r, S& sh, unsigned there)
     {
         const int dim = a.c.t.dim;
-        const bool whole = there == 0xffffffffu && dim == 16 * KS;
+        const bool whole = there == 0xffffffffu && dim == 32 * NB;
 #pragma unroll
         for (int i = 0; i < R::KI; ++i)
         {
@@ -286,7 +289,7 @@ template <int BITS, int KS> struct Wide
             for (int y = 0; y < R::VD; ++y)
             {
                 const int d = d0 + y;
-                if (d >= 16 * KS) continue;
+                if (d >= 32 * NB) continue;
                 const int slot = d % 32 + 32 * (group & 1), place = slot ^ (slot >> 3 & 7);
                 half8(&to)[P][64] = sh.v[d / 32][group >> 1];
                 if constexpr (BITS == 32)
@@ -384,7 +387,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256) void k_attn_chunk_
 template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chunk_wide(ChunkArgs a)
 {
     using S = Image<BITS, KS>;
-    constexpr int NB = KS / 2, P = S::P;
+    constexpr int NB = S::NB, P = S::P;
     constexpr size_t kLds = BITS == 32 && sizeof(WalkShared<KS>) > 2 * sizeof(S) ? sizeof(WalkShared<KS>) : 2 * sizeof(S);
     __shared__ __attribute__((aligned(16))) char lds[kLds];
     S* const sh = reinterpret_cast<S*>(lds);
@@ -431,24 +434,27 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 
     const int tiles = (end - begin + kPos - 1) / kPos;
     // A thread's 16-byte pieces of a tile's keys and then of its values, and of what is behind them.
-    constexpr int kHalf = sizeof(S::k) / 16, kPieces = (kHalf + 255) / 256, kTail = sizeof(S) / 16 - 2 * kHalf;
-    static_assert(sizeof(S::v) == sizeof(S::k) && kHalf % 64 == 0);
+    constexpr int kKeys = sizeof(S::k) / 16, kValues = sizeof(S::v) / 16, kTail = sizeof(S) / 16 - kKeys - kValues;
+    constexpr int kPieces = (kValues + 255) / 256;
+    static_assert(kValues >= kKeys && kKeys % 64 == 0 && kValues % 64 == 0 && kTail <= 64);
     const f32x4* image = reinterpret_cast<const f32x4*>(images + begin / kPos);
     f32x4 piece[kPieces], tail;
     auto fetch = [&](int i, int half) __attribute__((always_inline)) {
         // (a sequence whose length is 0 has no tile: the first one's place is read for it)
-        const f32x4* from = image + (size_t)max(min(i, tiles - 1), 0) * (sizeof(S) / 16) + half * kHalf;
+        const f32x4* from = image + (size_t)max(min(i, tiles - 1), 0) * (sizeof(S) / 16) + half * kKeys;
+        const int count = half ? kValues : kKeys;
 #pragma unroll
         for (int x = 0; x < kPieces; ++x)
-            if (256 * x + 256 <= kHalf || 256 * x + 64 * wave < kHalf) piece[x] = from[256 * x + t];
-        if (half == 1) tail = from[kHalf + min(lane, kTail - 1)];
+            if (256 * x + 256 <= count || 256 * x + 64 * wave < count) piece[x] = from[256 * x + t];
+        if (half == 1) tail = from[kValues + min(lane, kTail - 1)];
     };
     auto place = [&](S& to, int half) __attribute__((always_inline)) {
-        f32x4* at = reinterpret_cast<f32x4*>(&to) + half * kHalf;
+        f32x4* at = reinterpret_cast<f32x4*>(&to) + half * kKeys;
+        const int count = half ? kValues : kKeys;
 #pragma unroll
         for (int x = 0; x < kPieces; ++x)
-            if (256 * x + 256 <= kHalf || 256 * x + 64 * wave < kHalf) at[256 * x + t] = piece[x];
-        if (half == 1 && wave == 0 && lane < kTail) at[kHalf + lane] = tail;
+            if (256 * x + 256 <= count || 256 * x + 64 * wave < count) at[256 * x + t] = piece[x];
+        if (half == 1 && wave == 0 && lane < kTail) at[kValues + lane] = tail;
     };
     fetch(0, 0);
 
@@ -692,26 +698,41 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 
 } // namespace
 
+namespace
+{
+// f of the number of 16-dim groups, as a constant: at least 2.
+template <class F> void of_groups(unsigned dim, F&& f)
+{
+    switch ((dim + 15) / 16)
+    {
+    case 3: f(std::integral_constant<int, 3>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 5: f(std::integral_constant<int, 5>()); break;
+    case 6: f(std::integral_constant<int, 6>()); break;
+    case 7: f(std::integral_constant<int, 7>()); break;
+    case 8: f(std::integral_constant<int, 8>()); break;
+    default: f(std::integral_constant<int, 2>()); break;
+    }
+}
+} // namespace
+
 size_t chunk_image_bytes(int bits, unsigned dim)
 {
-    const size_t groups = (dim + 31) / 32;
-    return groups * (bits == 32 ? 8192 : 4096) + sizeof(float) * 2 * kPos + sizeof(int) * 8;
+    size_t bytes = 0;
+    of_groups(dim, [&](auto n) { bytes = bits == 32 ? sizeof(Image<32, n()>) : sizeof(Image<8, n()>); });
+    return bytes;
 }
 
 void chunk_parts(const ChunkArgs& a, int bits, unsigned pieces, unsigned blocks, hipStream_t s)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(pieces * blocks), dim3(256), 0, s, a, FastDiv(blocks)); };
-    const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
-    if (bits == 32) groups == 1 ? go(k_attn_chunk_parts<32, 2>) : groups == 2 ? go(k_attn_chunk_parts<32, 4>) : groups == 3 ? go(k_attn_chunk_parts<32, 6>) : go(k_attn_chunk_parts<32, 8>);
-    else groups == 1 ? go(k_attn_chunk_parts<8, 2>) : groups == 2 ? go(k_attn_chunk_parts<8, 4>) : groups == 3 ? go(k_attn_chunk_parts<8, 6>) : go(k_attn_chunk_parts<8, 8>);
+    of_groups(a.c.t.dim, [&](auto n) { bits == 32 ? go(k_attn_chunk_parts<32, n()>) : go(k_attn_chunk_parts<8, n()>); });
 }
 
 void chunk_wide(const ChunkArgs& a, int bits, unsigned blocks, hipStream_t s)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, s, a); };
-    const int groups = (static_cast<int>(a.c.t.dim) + 31) / 32;
-    if (bits == 32) groups == 1 ? go(k_attn_chunk_wide<32, 2>) : groups == 2 ? go(k_attn_chunk_wide<32, 4>) : groups == 3 ? go(k_attn_chunk_wide<32, 6>) : go(k_attn_chunk_wide<32, 8>);
-    else groups == 1 ? go(k_attn_chunk_wide<8, 2>) : groups == 2 ? go(k_attn_chunk_wide<8, 4>) : groups == 3 ? go(k_attn_chunk_wide<8, 6>) : go(k_attn_chunk_wide<8, 8>);
+    of_groups(a.c.t.dim, [&](auto n) { bits == 32 ? go(k_attn_chunk_wide<32, n()>) : go(k_attn_chunk_wide<8, n()>); });
 }
 
 } // namespace nnhip
