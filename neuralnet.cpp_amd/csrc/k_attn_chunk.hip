@@ -53,23 +53,43 @@ __device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigne
     return {ranges == 1 ? 0 : ranges, is_wide || a.c.K};
 }
 
+// Row i of a join's grid: its place among the results, token and head. Where rows of the wide kernel are whole already (wide 1)
+// the grid is of the others alone, kNarrowRows for each sequence and key head; i is past them where it has fewer.
+__device__ __forceinline__ bool row_of_join(const ChunkArgs& a, unsigned i, unsigned narrow, unsigned wide, unsigned& at, unsigned& n,
+                                            unsigned& h, Joined& r)
+{
+    if (wide != 1)
+    {
+        at = i;
+        n = a.by_q_heads.div(at);
+        h = at - n * a.q_heads;
+        if (n >= a.tokens) return false;
+        if (wide) r = joined(a, n, narrow, wide);
+        return !wide || r.ranges > 0;
+    }
+    const unsigned piece = i / kNarrowRows, row = i - piece * kNarrowRows, b = a.by_heads.div(piece), kh = piece - b * a.c.t.heads;
+    if (b >= a.c.t.batch) return false;
+    const Chunk c = chunk_of(a, b);
+    const int rows = c.n * (int)a.by_per.d;
+    if (rows > a.wide_from || (int)row >= rows) return false;
+    const unsigned t = a.by_per.div(row);
+    n = c.first + t;
+    h = kh * a.by_per.d + (row - t * a.by_per.d);
+    at = n * a.q_heads + h;
+    r = {narrow, a.c.K != nullptr};
+    return true;
+}
+
 // Up to kFewParts ranges: a wave a row, everything it needs on its way at once, the search for the token's sequence too. With
 // rows of both kernels the search comes first: most rows may have nothing to join, or few ranges (seven prompts' chunks of
-// 3900 tokens, 16 heads of 80, none of whose rows are cut: 67 us of reads that are not needed).
+// 3900 tokens, 16 heads of 80, none of whose rows are cut: 67 us of reads that are not needed, 12 of searches alone, 3 by narrow rows).
 constexpr unsigned kFewParts = 16;
 __global__ __launch_bounds__(256) void k_attn_chunk_join_few(ChunkArgs a, unsigned narrow, unsigned wide)
 {
-    const unsigned at = (blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64;
-    const unsigned n = a.by_q_heads.div(at), h = at - n * a.q_heads;
-    if (n >= a.tokens) return;
+    unsigned at, n, h;
     Joined r{};
-    unsigned last = a.slots - 1;
-    if (wide)
-    {
-        r = joined(a, n, narrow, wide);
-        if (r.ranges == 0) return;
-        last = r.ranges - 1;
-    }
+    if (!row_of_join(a, (blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64, narrow, wide, at, n, h, r)) return;
+    const unsigned last = wide ? r.ranges - 1 : a.slots - 1;
     const int lane = threadIdx.x & 63, dim = a.c.t.dim;
     const float2 own = reinterpret_cast<const float2*>(a.part_ml)[(size_t)at * a.slots + min((unsigned)lane, last)];
     const float* po = a.part_o + (size_t)at * a.slots * dim;
@@ -107,9 +127,10 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
 {
     static_assert(kMostRanges <= 256);
     __shared__ float w_s[256], red[2][4], o_s[256];
-    const unsigned at = blockIdx.y * gridDim.x + blockIdx.x, n = a.by_q_heads.div(at), h = at - n * a.q_heads;
-    if (n >= a.tokens) return;
-    const Joined r = joined(a, n, narrow, wide);
+    unsigned at, n, h;
+    Joined r{};
+    if (!row_of_join(a, blockIdx.y * gridDim.x + blockIdx.x, narrow, wide, at, n, h, r)) return;
+    if (!wide) r = joined(a, n, narrow, wide);
     if (r.ranges == 0) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, dim = a.c.t.dim;
     const int cols = dim <= 64 ? 64 : 128, groups = 256 / cols, d = t % cols, g = t / cols;
@@ -333,7 +354,8 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     }
     if (p.slots() == 1) return 0;
     const bool few = p.slots() <= kFewParts;
-    const size_t blocks = few ? (tokens * q_heads + 3) / 4 : tokens * q_heads, x = std::min(blocks, (size_t)1 << 20);
+    const size_t rows = p.wide == 1 ? call.c.t.batch * (size_t)call.c.t.heads * kNarrowRows : tokens * q_heads;
+    const size_t blocks = few ? (rows + 3) / 4 : rows, x = std::min(blocks, (size_t)1 << 20);
     const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>((blocks + x - 1) / x));
     hipLaunchKernelGGL(few ? k_attn_chunk_join_few : k_attn_chunk_join, grid, dim3(256), 0, s, a, p.narrow, p.wide);
     return launch_status();

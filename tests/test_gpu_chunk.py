@@ -431,6 +431,26 @@ def test_many_rows(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_few_rows_to_join(bits):
+    """Prompts whose rows are whole, beside single tokens and a few whose ranges are joined."""
+    rng = np.random.default_rng(bits)
+    page, heads, dim, qh = 16, 8, 8, 64
+    new, past = [900, 1, 0, 1000, 2, 4] + [1] * 14, [5, 700, 9, 40, 90, 0] + list(range(100, 800, 50))
+    lens, start = [n + p for n, p in zip(new, past)], np.concatenate([[0], np.cumsum(new)])
+    x, table, pages = cache_for(rng, lens, page, heads, dim, bits, holes=True)
+    q = rng.normal(size=(int(start[-1]), qh, dim)).astype(np.float32)
+    O, m, l = run_chunk(x, dict(pages=pages, page=page, heads=heads, dim=dim), table, q, start, max(new), lens, None, 0.5)
+    for b, (lo, hi) in enumerate(zip(start[:-1], start[1:])):
+        for n in range(lo, hi) if hi - lo < 5 else (lo, hi - 1):
+            seen = lens[b] - new[b] + n - int(lo) + 1
+            for h in range(0, qh, 7):
+                w = ch.attend(q[n:n + 1, h:h + 1], x["K64"][:, h // 8:h // 8 + 1], x["V64"][:, h // 8:h // 8 + 1], table[b:b + 1], page, pages, 1,
+                              [0, 1], 1, [seen], 0.5)
+                assert np.all(np.abs(O[n, h] - w[0][0, 0]) <= w[3][0, 0]) and abs(m[n, h] - w[1][0, 0]) <= w[4][0, 0]
+                assert abs(l[n, h] - w[2][0, 0]) <= w[2][0, 0] * (4 * w[4][0, 0] + (2 * 8192 + 8) * U)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_table_of_many_positions(bits):
     """Tables that reach 2^24 positions: the keys' and values' parts are formed a sequence and key head at a time."""
     rng = np.random.default_rng(bits)
