@@ -211,7 +211,10 @@ ChunkPlan chunk_plan(const ChunkCall& c)
         const size_t by_seqs = c.tokens * per / kWideRows + batch, by_rows = c.tokens * per / (kNarrowRows + 1) + 1;
         p.wide_by_seqs = by_seqs <= by_rows || batch == 1;
         p.wide_row_blocks = p.wide_by_seqs ? by_seqs : by_rows;
-        const size_t others = heads * ((c.tokens * per + kWideRows - 1) / kWideRows), most_wide = (positions + 255) / 256;
+        // Ranges for two workgroups a CU, of 128 positions at least (200 tokens behind 300, 12 heads: 32 us with 256, 27 with 128,
+        // 25 with 64; chunks of up to 60 of four sequences over bytes 32, 28, 29; 40 tokens behind 6000 87, 83, 83; 16 sequences of
+        // 12 behind 2000 213, 224, 226).
+        const size_t others = heads * ((c.tokens * per + kWideRows - 1) / kWideRows), most_wide = (positions + 127) / 128;
         p.wide = static_cast<unsigned>(std::min<size_t>(std::min(std::max<size_t>(2 * cus / others, 1), most_wide), kMostRanges));
         p.wide_blocks = (p.wide_row_blocks * heads * p.wide + 7) / 8 * 8;
         if (batch == 1) p.narrow = 0, p.wide_from = 0;   // one launch, however few tokens the sequence has
