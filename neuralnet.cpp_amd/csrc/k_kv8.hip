@@ -352,7 +352,8 @@ extern "C" int nnhip_kv8_append(const nnhip_kv8_pages* c, const float* k, long k
     const size_t pieces = turned + (rest + 7) / 8 > all_v ? turned + (rest + 7) / 8 : all_v;
     while (((size_t)1 << a.log2_group) < pieces) ++a.log2_group;
     const size_t threads = tokens * y << a.log2_group;
-    if (a.words && rope_dim % 8 == 0 && rows_of_4(k, k_t, k_f) && rows_of_4(v, v_t, v_f) && rows_of_4(q, q_t, q_f) &&
+    // Heads of tokens are divided by their slots: those of the last workgroup's threads, too, are below 2^31 (FastDiv).
+    if (tokens * y + 255 < 0x80000000u && a.words && rope_dim % 8 == 0 && rows_of_4(k, k_t, k_f) && rows_of_4(v, v_t, v_f) && rows_of_4(q, q_t, q_f) &&
         rows_of_4(q_out, o_t, o_f) && (!cos || (aligned16(cos) && aligned16(sin))) && threads / 256 < kGridMost && a.log2_group <= 5)
     {
         a.by_slots = FastDiv(static_cast<unsigned>(y));
