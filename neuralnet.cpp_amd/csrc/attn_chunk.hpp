@@ -115,7 +115,7 @@ __device__ __forceinline__ void load(const ChunkArgs& a, bool keys, int row, uns
     else
     {
         const signed char* p = (keys ? a.c.K : a.c.V) + at;
-        const float scale = (keys ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
+        const float scale = scale_or_nan((keys ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h]);
         if constexpr (VEC)
         {
             typedef signed char vec __attribute__((ext_vector_type(N)));

@@ -106,7 +106,7 @@ template <int KS, int W> __device__ __forceinline__ void load_keys8(const ChunkA
         }
     }
     const float z = (lane < 32 ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
-    x.scale = row >= 0 ? z : 0.0f;
+    x.scale = row >= 0 ? scale_or_nan(z) : 0.0f;
 }
 template <int KS, int W> __device__ __forceinline__ void load_values8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS, W>& x)
 {
@@ -266,6 +266,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
             int new_top = tile_top;
+            f32x4 own[2] = {vs[0], vs[1]};   // the values' scales of what the row sees
             if (odd)
             {
                 float size = 0.0f;
@@ -278,6 +279,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
                         const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q)), v = fabsf(vs[u][e]);
                         const bool sees = (now >> q & 1) && p + q < w.seen;
                         s[i][u][e] = sees ? z : -__builtin_inff();
+                        own[u][e] = sees ? own[u][e] : 0.0f;   // 0 times a NaN would be one
                         size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
                     }
                 if (part_seen)
@@ -307,7 +309,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
                 {
                     const float y = __builtin_amdgcn_exp2f(s[i][u][e] - mn);
                     sum += y;
-                    z[4 * u + e] = y == 0.0f ? 0.0f : y * vs[u][e] * to;   // a weight of 0 stays 0, whatever the scale is
+                    z[4 * u + e] = y * own[u][e] * to;
                 }
             w.l = w.l * f + sum;
             f = __builtin_ldexpf(f, w.top - new_top);

@@ -319,7 +319,7 @@ template <int BITS, int KS> struct Wide
             if (wave == 0)
             {
                 const bool ok = there >> (lane & 31) & 1;
-                const float s = ok ? r.scale : 0.0f;
+                const float s = ok ? scale_or_nan(r.scale) : 0.0f;
                 const float top = max_of<32>(fabsf(s) <= kMaxF ? fabsf(s) : 0.0f);
                 const int e = top > 0.0f ? exponent_of(top) : kNone;   // of the keys' scales, of the values'
                 if (lane < 32) sh.k_scale[lane] = s * 0x1p-5f;
@@ -586,6 +586,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
                     s[r] = sees ? s[r] : -__builtin_inff();
                     const float v = fabsf(vs[r / 4][r % 4]);
                     size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
+                    if constexpr (BITS == 8) vs[r / 4][r % 4] = sees ? vs[r / 4][r % 4] : 0.0f;   // 0 times a NaN would be one
                 }
                 size = across(size, [](float x, float y) { return fmaxf(x, y); });
                 new_top = size > 0.0f ? exponent_of(size) + (BITS == 32 ? 1 : 0) : kNone;
@@ -622,7 +623,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 #pragma unroll
                 for (int b = 0; b < NB; ++b) o[b] *= f;
             }
-            // The values' scales, into the weights. Weights that are 0 stay so, whatever their position's scale is.
+            // The values' scales, into the weights.
             const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - top);
             const int place1 = lane ^ (lane >> 3 & 7);
             half8 vh[NB], vl[NB];
@@ -646,8 +647,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
-                    const float x = s[8 * st + e], y = x * vs[2 * st + e / 4][e % 4] * to;
-                    z[e] = BITS == 8 && x == 0.0f ? 0.0f : y;
+                    z[e] = s[8 * st + e] * vs[2 * st + e / 4][e % 4] * to;
                 }
                 split2(z, pp[st][0], pp[st][1]);
             }

@@ -94,6 +94,9 @@ struct Pages8
     float *K_scale, *V_scale;
 };
 
+// A scale as attention takes it: one that is not finite is NaN, so that no byte of 0 and no weight of 0 hides it.
+__device__ __forceinline__ float scale_or_nan(float s) { return fabsf(s) <= kMaxF ? s : __builtin_nanf(""); }
+
 inline bool pages8_ok(const nnhip_kv8_pages* c, size_t max_dim)
 {
     if (!c || !c->K || !c->V || !c->K_scale || !c->V_scale) return false;

@@ -130,6 +130,7 @@ class CpuEngine final : public ComputeEngine
                 {
                     s.assign(rows.size(), 0.0);
                     double m = none, l = 0.0;
+                    bool some = false;
                     for (std::size_t x = 0; x < rows.size(); ++x)
                     {
                         double dot = 0.0;
@@ -137,9 +138,10 @@ class CpuEngine final : public ComputeEngine
                             dot += static_cast<double>(P(q)[(h * d + e) * N + first + i]) * at(K, K_scale, rows[x], h / per, e);
                         s[x] = alpha * dot - (slopes ? static_cast<double>(P(*slopes)[h]) * static_cast<double>(p - pos[x]) : 0.0);
                         m = std::max(m, s[x]);
+                        some = some || !(s[x] == none);   // NaN too
                     }
                     std::fill(o.begin(), o.end(), 0.0);
-                    if (m != none)
+                    if (some)
                         for (std::size_t x = 0; x < rows.size(); ++x)
                         {
                             const double w = std::exp(s[x] - m);
@@ -451,7 +453,10 @@ public:
         NN_TRY(H, paged::check_chunk("attn_chunk8", paged::dim_of8(c), c.heads, c.table.rows(), q, start, most, len, slopes));
         return chunk_(c.table, c.page, c.K.rows() / c.page, c.heads, c.dim, H, q, start, most, len, slopes, alpha,
                       [&](const Tensor& x, const Tensor* scale, std::size_t row, std::size_t h, std::size_t e) -> double {
-                          return static_cast<double>(byte_(c, x, row, h, e)) * P(*scale)[row * c.heads + h];
+                          // A scale that is not finite makes every row NaN that sees it.
+                          const float z = P(*scale)[row * c.heads + h];
+                          return std::isfinite(z) ? static_cast<double>(byte_(c, x, row, h, e)) * z
+                                                  : std::numeric_limits<double>::quiet_NaN();
                       },
                       c.K, &c.K_scale, c.V, &c.V_scale);
     }
