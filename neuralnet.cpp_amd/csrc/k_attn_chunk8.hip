@@ -105,8 +105,7 @@ template <int KS, int W> __device__ __forceinline__ void load_keys8(const ChunkA
             }
         }
     }
-    const float z = (lane < 32 ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
-    x.scale = row >= 0 ? scale_or_nan(z) : 0.0f;
+    x.scale = (lane < 32 ? a.c.K_scale : a.c.V_scale)[(size_t)max(row, 0) * a.c.t.heads + h];
 }
 template <int KS, int W> __device__ __forceinline__ void load_values8(const ChunkArgs& a, int row, unsigned h, int lane, Tile8<KS, W>& x)
 {
@@ -229,8 +228,9 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
 #pragma unroll
         for (int i = 0; i < RT; ++i) s[i][0] = s[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         // The scales, from a lane a position to a lane's positions, through LDS: the wave's own part of it.
-        (&sh.scales[wave][0][0])[lane] = lane < 32 ? x.scale * 0x1p-5f : x.scale;
-        const float vs_top = max_of<64>(lane >= 32 && fabsf(x.scale) <= kMaxF ? fabsf(x.scale) : 0.0f);
+        const float scale = there >> (lane & 31) & 1 ? scale_or_nan(x.scale) : 0.0f;
+        (&sh.scales[wave][0][0])[lane] = lane < 32 ? scale * 0x1p-5f : scale;
+        const float vs_top = max_of<64>(lane >= 32 && fabsf(scale) <= kMaxF ? fabsf(scale) : 0.0f);
 #pragma unroll
         for (int k = 0; k < B::steps; ++k)
 #pragma unroll
