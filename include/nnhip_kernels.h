@@ -589,17 +589,18 @@ int nnhip_kv8_read(const nnhip_kv8_pages* c, float* k, long k_t, long k_f, float
  * q_heads) may be NULL. Tokens that no sequence has, behind the last one's or past `most`, are left as they are. A start
  * that is negative or NaN counts as 0, one past `tokens` as that, a len as nnhip_attn_paged's. 1 <= most <= tokens; dim <=
  * 128; tokens * q_heads below 2^31. O, m and l overlap no input. Sums are float32. Sequences of more than 32 rows of a
- * key head (tokens times q_heads / heads) have their products formed from two float16 parts of each factor, exact to 2^-22
- * of the product and 2^-39 of the largest of a key's, query's or position's values; weights times values below 2^-39 of
- * the largest value that the row sees are lost. The workspace is nnhip_attn_chunk_workspace_bytes (0 where none is needed;
- * with many rows room for those parts, up to 2 GiB or what one key head's `width * page` positions take, the larger),
- * 16-byte aligned; calls that may overlap in time need one each. Results are the same bits every time. */
+ * key head (tokens times q_heads / heads; a call's only sequence where `most` tokens have more) have their products formed
+ * from two float16 parts of each factor, exact to 2^-22 of the product and 2^-39 of the largest of a key's, query's or
+ * position's values; of a position's weight times its largest value what is below 2^-37 of the row's largest such product
+ * is lost. The workspace is nnhip_attn_chunk_workspace_bytes (0 where none is needed; with many rows room for those parts,
+ * up to 2 GiB or what one key head's `width * page` positions take, the larger), 16-byte aligned; calls that may overlap
+ * in time need one each. Results are the same bits every time. */
 size_t nnhip_attn_chunk_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t tokens, size_t most);
 int nnhip_attn_chunk(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, size_t tokens,
                      const float* start, size_t most, const float* len, const float* slopes, float alpha, float* O,
                      long o_t, long o_f, float* m, float* l, void* workspace, size_t workspace_bytes, void* stream);
-/* The same over an 8-bit cache, by parts for any number of rows: weights times values below 2^-39 of the largest scale (its
- * byte taken to be 127) that the row sees are lost. A row whose query is not finite, or that sees a scale that is not, is NaN. */
+/* The same over an 8-bit cache, by parts for any number of rows: of a weight times a scale what is below 2^-37 of the row's
+ * largest such product is lost. A row whose query is not finite, or that sees a scale that is not, is NaN. */
 size_t nnhip_attn_chunk8_workspace_bytes(const nnhip_kv8_pages* c, size_t q_heads, size_t tokens, size_t most);
 int nnhip_attn_chunk8(const nnhip_kv8_pages* c, const float* q, long q_t, long q_f, size_t q_heads, size_t tokens,
                       const float* start, size_t most, const float* len, const float* slopes, float alpha, float* O,

@@ -86,6 +86,24 @@ template <class F> __device__ __forceinline__ float across(float x, F&& f)
     const unsigned lo = z[0], hi = z[1];
     return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
+// What weights times values are held against: 2^top, above the largest of these products that the row has met, as they
+// shrink with a growing score. past: bits that the products have shrunk by and top has not.
+struct Held
+{
+    int top;
+    float past;
+};
+constexpr Held kNothingHeld{kLeastTop, 0.0f};
+// Scores grow by `up` bits (0 and above), and the tile's products lie below 2^tile. What the outputs are multiplied by; the
+// sum of the weights by 2^-up.
+__device__ __forceinline__ float hold(Held& h, float up, int tile)
+{
+    const float past = h.past + up, whole = floorf(past);
+    const int was = h.top;
+    h.past = past - whole;
+    h.top = max(max(was - (int)fminf(whole, 2048.0f), tile), kLeastTop);
+    return __builtin_amdgcn_exp2f((float)(was - h.top) - up);
+}
 // The largest over the wave of each of 8 numbers a lane, none negative: lane l has the number l % 8's.
 __device__ __forceinline__ float max_of_8(const float (&x)[8], int lane)
 {

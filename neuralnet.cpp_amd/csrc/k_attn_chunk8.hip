@@ -47,7 +47,7 @@ template <int KS, int W> struct Row8
 {
     half8 q[KS / 2][2];
     int seen;
-    int top;                    // exponent that the values' scales are held against: of those that the row sees
+    Held held;                  // of weights times values' scales
     float slope, scale, m, l;   // slope, scale and m: times log2(e)
     f32x4 o[Bytes<KS, W>::VB];
 };
@@ -214,7 +214,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         }
         w.slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
         w.scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);
-        w.top = kNone;
+        w.held = kNothingHeld;
         w.m = kLowest;
         w.l = 0.0f;
 #pragma unroll
@@ -230,7 +230,6 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         // The scales, from a lane a position to a lane's positions, through LDS: the wave's own part of it.
         const float scale = there >> (lane & 31) & 1 ? scale_or_nan(x.scale) : 0.0f;
         (&sh.scales[wave][0][0])[lane] = lane < 32 ? scale * 0x1p-5f : scale;
-        const float vs_top = max_of<64>(lane >= 32 && fabsf(scale) <= kMaxF ? fabsf(scale) : 0.0f);
 #pragma unroll
         for (int k = 0; k < B::steps; ++k)
 #pragma unroll
@@ -257,7 +256,6 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         __builtin_amdgcn_sched_barrier(0);
 
         const bool part_seen = now != 0xffffffffu || p + kPos > all, odd = a.slopes || part_seen;
-        const int tile_top = vs_top > 0.0f ? exponent_of(vs_top) : kNone;
         half8 pp[RT][2];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -265,60 +263,60 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
             Row8<KS, W>& w = rows[i];
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
-            int new_top = tile_top;
             f32x4 own[2] = {vs[0], vs[1]};   // the values' scales of what the row sees
             if (odd)
             {
-                float size = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                     {
                         const int q = 16 * u + 4 * g + e;
-                        const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q)), v = fabsf(vs[u][e]);
+                        const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q));
                         const bool sees = (now >> q & 1) && p + q < w.seen;
                         s[i][u][e] = sees ? z : -__builtin_inff();
                         own[u][e] = sees ? own[u][e] : 0.0f;   // 0 times a NaN would be one
-                        size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
                     }
-                if (part_seen)
-                {
-                    size = fmaxf(size, __shfl_xor(size, 16, 64));
-                    size = fmaxf(size, __shfl_xor(size, 32, 64));
-                    new_top = size > 0.0f ? exponent_of(size) : kNone;
-                }
             }
-            new_top = max(max(w.top, new_top), kLeastTop);
-            const float to = __builtin_ldexpf(1.0f, 15 - new_top);
             float high = kLowest;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) high = fmaxf(high, s[i][u][e]);
-            high = fmaxf(high, __shfl_xor(high, 16, 64));
-            high = fmaxf(high, __shfl_xor(high, 32, 64));
-            const float mn = fmaxf(w.m, high);
-            float f = __builtin_amdgcn_exp2f(w.m - mn), sum = 0.0f;
-            w.m = mn;
+            float up = 0.0f;
+            if (__builtin_amdgcn_ballot_w64(high > w.m))   // seldom past the first tiles
+            {
+                high = fmaxf(high, __shfl_xor(high, 16, 64));
+                high = fmaxf(high, __shfl_xor(high, 32, 64));
+                const float mn = fmaxf(w.m, high);
+                up = mn - w.m;
+                w.m = mn;
+            }
+            float sum = 0.0f, size = 0.0f;
             floatx8 z;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                 {
-                    const float y = __builtin_amdgcn_exp2f(s[i][u][e] - mn);
+                    const float y = __builtin_amdgcn_exp2f(s[i][u][e] - w.m);
                     sum += y;
-                    z[4 * u + e] = y * own[u][e] * to;
+                    z[4 * u + e] = y * own[u][e];
+                    size = fmaxf(size, fabsf(z[4 * u + e]));
                 }
-            w.l = w.l * f + sum;
-            f = __builtin_ldexpf(f, w.top - new_top);
-            w.top = new_top;
-            if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
+            if (__builtin_amdgcn_ballot_w64(up != 0.0f || exponent_of(size) > w.held.top))   // seldom, too
             {
+                size = fmaxf(size, __shfl_xor(size, 16, 64));
+                size = fmaxf(size, __shfl_xor(size, 32, 64));
+                const float f = hold(w.held, up, exponent_of(size));
+                w.l *= __builtin_amdgcn_exp2f(-up);
 #pragma unroll
                 for (int b = 0; b < B::VB; ++b) w.o[b] *= f;
             }
+            w.l += sum;
+            const float to = __builtin_ldexpf(1.0f, 15 - w.held.top);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] *= to;
             split2(z, pp[i][0], pp[i][1]);
         }
 #pragma unroll
@@ -358,7 +356,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
 #pragma unroll
         for (int b = 0; b < B::VB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], w.top - 15);
+            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], w.held.top - 15);
         __syncthreads();
         const int jr = t >> 4, r = part.first + i * kTile + jr;
         if (r >= part.n_rows) continue;

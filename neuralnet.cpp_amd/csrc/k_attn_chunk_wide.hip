@@ -11,9 +11,10 @@
 // rows a key head behind 2000 positions 200 and 181.
 //
 // Scales are exact: a key's goes into its scores, a value's into its position's
-// weights, relative to the largest that the row has seen (a row's outputs are
-// rescaled when that grows, as they are when its largest score does). Both are a
-// position's own, so that what a row does not see takes no accuracy from what it does.
+// weights, relative to the largest such product that the row has met (a row's
+// outputs are rescaled when that grows, and as it shrinks with a growing score).
+// So what a row does not see, and what has next to no weight, takes no accuracy
+// from the rest.
 //
 // A workgroup of k_attn_chunk_wide takes 128 rows, 32 to a wave, and 32 positions at
 // a time, copied to LDS a tile ahead. Both products are formed transposed (S^T = K
@@ -60,7 +61,6 @@ template <int BITS, int KS> struct alignas(16) Image
     half8 v[NB][2][P][64];
     float k_scale[kPos];           // of the scores
     float v_scale[kPos];           // of the weights: the values' scales; BITS 32: a quarter of 2^(exponent of the position's values)
-    int v_top[4];                  // exponents of the values: of each group of 8 positions; BITS 8: all [0]
     unsigned there[4];             // [0]: which positions exist
 };
 
@@ -280,10 +280,6 @@ template <int BITS, int KS> struct Wide
                     ve[e] = x > 0.0f ? exponent_of(x) : kNone;
                 }
                 if (lane < 8) sh.v_scale[value_pos(lane)] = mine > 0.0f ? __builtin_ldexpf(0.25f, exponent_of(mine)) : 0.0f;
-                int highest = ve[0];
-#pragma unroll
-                for (int e = 1; e < 8; ++e) highest = max(highest, ve[e]);
-                if (lane == 0) sh.v_top[group] = highest;
             }
 #pragma unroll
             for (int y = 0; y < R::VD; ++y)
@@ -320,14 +316,8 @@ template <int BITS, int KS> struct Wide
             {
                 const bool ok = there >> (lane & 31) & 1;
                 const float s = ok ? scale_or_nan(r.scale) : 0.0f;
-                const float top = max_of<32>(fabsf(s) <= kMaxF ? fabsf(s) : 0.0f);
-                const int e = top > 0.0f ? exponent_of(top) : kNone;   // of the keys' scales, of the values'
                 if (lane < 32) sh.k_scale[lane] = s * 0x1p-5f;
-                else
-                {
-                    sh.v_scale[lane - 32] = s;
-                    if (lane == 32) sh.v_top[0] = e;
-                }
+                else sh.v_scale[lane - 32] = s;
             }
     }
 };
@@ -508,7 +498,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     const float by_alpha = __builtin_ldexpf(fabsf(a.alpha) * kLog2e, qe - 10), scale = by_alpha == 0.0f ? 0x1p-149f : by_alpha;
     const float by = a.slopes ? 1.0f : scale;   // of the scores as the softmax sees them
     float m = kLowest, l = 0.0f;
-    int top = kNone;                // exponent that the row's values are held against
+    Held held = kNothingHeld;
     floatx16 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -572,59 +562,57 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             f32x4 vs[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) vs[q] = *reinterpret_cast<const f32x4*>(&in.v_scale[8 * q + 4 * g]);
-            int new_top = in.v_top[0];
-            if constexpr (BITS == 32) new_top = max(max(new_top, in.v_top[1]), max(in.v_top[2], in.v_top[3]));
             if (now != 0xffffffffu || p0 + kPos > all)
             {
-                // Of the values, too, only those that the row sees count.
-                float size = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                 {
                     const int p = 8 * (r / 4) + 4 * g + r % 4;
                     const bool sees = (now >> p & 1) && p0 + p < seen;
                     s[r] = sees ? s[r] : -__builtin_inff();
-                    const float v = fabsf(vs[r / 4][r % 4]);
-                    size = fmaxf(size, sees && v <= kMaxF ? v : 0.0f);
                     if constexpr (BITS == 8) vs[r / 4][r % 4] = sees ? vs[r / 4][r % 4] : 0.0f;   // 0 times a NaN would be one
                 }
-                size = across(size, [](float x, float y) { return fmaxf(x, y); });
-                new_top = size > 0.0f ? exponent_of(size) + (BITS == 32 ? 1 : 0) : kNone;
             }
             float high = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
-            high = across(high, [](float x, float y) { return fmaxf(x, y); });
-            const float mn = fmaxf(m, high * by);
-            float f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+            high *= by;
+            float up = 0.0f;
+            if (__builtin_amdgcn_ballot_w64(high > m))   // seldom past the first tiles
+            {
+                const float mn = fmaxf(m, across(high, [](float x, float y) { return fmaxf(x, y); }));
+                up = mn - m;
+                m = mn;
+            }
             // What rounding the largest score took away is added to the weights' exponents: of scores past 2^20 it may be
             // more than an exponent holds, and these are rounded first.
             float once = by;
-            if (__builtin_amdgcn_ballot_w64(fabsf(mn) > 0x1p20f && mn != kLowest))
+            if (__builtin_amdgcn_ballot_w64(fabsf(m) > 0x1p20f && m != kLowest))
             {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= by;
                 once = 1.0f;
             }
-            float sum = 0.0f;
+            float sum = 0.0f, size = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
             {
-                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], once, -mn));
+                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], once, -m));
                 sum += s[r];
+                s[r] *= vs[r / 4][r % 4];
+                size = fmaxf(size, fabsf(s[r]));
             }
-            l = l * f + sum;
-            new_top = max(max(top, new_top), kLeastTop);
-            f = __builtin_ldexpf(f, top - new_top);
-            top = new_top;
-            if (__builtin_amdgcn_ballot_w64(f != 1.0f))   // seldom past the first tiles
+            constexpr int kQuarter = BITS == 32 ? 2 : 0;   // weights are held with the scales' quarters
+            if (__builtin_amdgcn_ballot_w64(up != 0.0f || exponent_of(size) + kQuarter > held.top))   // seldom, too
             {
+                size = across(size, [](float x, float y) { return fmaxf(x, y); });
+                const float f = hold(held, up, exponent_of(size) + kQuarter);
+                l *= __builtin_amdgcn_exp2f(-up);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) o[b] *= f;
             }
-            // The values' scales, into the weights.
-            const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - top);
+            l += sum;
+            const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - held.top);
             const int place1 = lane ^ (lane >> 3 & 7);
             half8 vh[NB], vl[NB];
             auto values = [&](int st, int x, half8(&to)[NB]) __attribute__((always_inline)) {
@@ -645,10 +633,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             {
                 floatx8 z;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    z[e] = s[8 * st + e] * vs[2 * st + e / 4][e % 4] * to;
-                }
+                for (int e = 0; e < 8; ++e) z[e] = s[8 * st + e] * to;
                 split2(z, pp[st][0], pp[st][1]);
             }
             product(vh, pp[0][1]);
@@ -668,7 +653,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     }
 
     l = across(l, [](float x, float y) { return x + y; });
-    const int unscale = top - (BITS == 32 ? 30 : 15);
+    const int unscale = held.top - (BITS == 32 ? 30 : 15);
     bool bad = false;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
