@@ -86,6 +86,13 @@ template <class F> __device__ __forceinline__ float across(float x, F&& f)
     const unsigned lo = z[0], hi = z[1];
     return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
+// Scores. alpha log2(e) is by_m 2^by_e: the query's parts take by_m, and a score, times log2(e), is s f 2^e with s the sum of
+// the parts' products, f the key's scale and e the row's exponent. A tile's scales are multiplied by 2^-shift_of them and e is
+// raised by it, so that neither s f leaves float32's range where the score does not, nor f has bits below that range: of
+// scales above 2^80, of which s f might pass 2^128, it is 64, of nothing but scales below 2^-75 -64, else 0.
+constexpr float kFar = 0x1p80f, kNear = 0x1p-75f;
+__device__ __forceinline__ int shift_of(unsigned long long far, bool all_near) { return far ? 64 : all_near ? -64 : 0; }
+
 // What weights times values are held against: 2^top, above the largest of these products that the row has met, as they
 // shrink with a growing score. past: bits that the products have shrunk by and top has not.
 struct Held

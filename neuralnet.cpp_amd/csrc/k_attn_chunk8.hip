@@ -48,7 +48,8 @@ template <int KS, int W> struct Row8
     half8 q[KS / 2][2];
     int seen;
     Held held;                  // of weights times values' scales
-    float slope, scale, m, l;   // slope, scale and m: times log2(e)
+    int e;                      // the scores' exponent
+    float slope, m, l;          // slope and m: times log2(e)
     f32x4 o[Bytes<KS, W>::VB];
 };
 
@@ -162,6 +163,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
     const int dim = a.c.t.dim, begin = part.begin, end = part.end, step = 4 * kPos;
     Row8<KS, W> rows[RT];
     int all = 0x7fffffff;
+    const float by = a.alpha * kLog2e, by_m = __builtin_amdgcn_frexp_mantf(by);
     const int p1 = begin + wave * kPos;
     // Lane p and lane 32 + p: the table's entry and the row of position p of a tile.
     auto entry = [&](int p) { return a.c.t.entry_of(part.b, p + (lane & 31)); };
@@ -204,16 +206,16 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
             }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const int qe = exponent_of(top);
+        const int qe = exponent_of(by_m == 0.0f ? top : top * by_m);
 #pragma unroll
         for (int s = 0; s < B::steps; ++s)
         {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[s][e] = __builtin_ldexpf(z[s][e], 15 - qe);
+            for (int e = 0; e < 8; ++e) z[s][e] = __builtin_ldexpf(z[s][e], 15 - qe) * by_m;
             split2(z[s], w.q[s][0], w.q[s][1]);
         }
         w.slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
-        w.scale = __builtin_ldexpf(a.alpha * kLog2e, qe - 10);
+        w.e = qe - 15 + __builtin_amdgcn_frexp_expf(by);
         w.held = kNothingHeld;
         w.m = kLowest;
         w.l = 0.0f;
@@ -229,7 +231,9 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         for (int i = 0; i < RT; ++i) s[i][0] = s[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         // The scales, from a lane a position to a lane's positions, through LDS: the wave's own part of it.
         const float scale = there >> (lane & 31) & 1 ? scale_or_nan(x.scale) : 0.0f;
-        (&sh.scales[wave][0][0])[lane] = lane < 32 ? scale * 0x1p-5f : scale;
+        const float size = fabsf(scale);
+        const int shift = shift_of(__builtin_amdgcn_ballot_w64(lane < 32 && size > kFar), !__builtin_amdgcn_ballot_w64(lane < 32 && size >= kNear));
+        (&sh.scales[wave][0][0])[lane] = lane < 32 ? __builtin_ldexpf(scale, -shift) : scale;
 #pragma unroll
         for (int k = 0; k < B::steps; ++k)
 #pragma unroll
@@ -262,7 +266,9 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         {
             Row8<KS, W>& w = rows[i];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) s[i][u] = s[i][u] * ks[u] * w.scale;
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][u][e] = __builtin_ldexpf(s[i][u][e] * ks[u][e], w.e + shift);
             f32x4 own[2] = {vs[0], vs[1]};   // the values' scales of what the row sees
             if (odd)
             {

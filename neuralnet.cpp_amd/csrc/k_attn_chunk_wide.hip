@@ -37,6 +37,7 @@
 #include "attn_chunk.hpp"
 #include "f16_parts.hpp"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace nnhip
@@ -59,9 +60,9 @@ template <int BITS, int KS> struct alignas(16) Image
     // Operands by lane: [step or block of 32 dims and k step][part][lane's place]
     half8 k[KS][P][64];
     half8 v[NB][2][P][64];
-    float k_scale[kPos];           // of the scores
+    float k_scale[kPos];           // of the scores, times 2^-shift
     float v_scale[kPos];           // of the weights: the values' scales; BITS 32: a quarter of 2^(exponent of the position's values)
-    unsigned there[4];             // [0]: which positions exist
+    int there[4];                  // [0]: which positions exist; [1]: the keys' shift (shift_of)
 };
 
 // What a thread of k_attn_chunk_parts holds of a tile. Keys: 8 dims of one position each; values: VD dims of the 8 positions of
@@ -316,7 +317,7 @@ template <int BITS, int KS> struct Wide
             {
                 const bool ok = there >> (lane & 31) & 1;
                 const float s = ok ? scale_or_nan(r.scale) : 0.0f;
-                if (lane < 32) sh.k_scale[lane] = s * 0x1p-5f;
+                if (lane < 32) sh.k_scale[lane] = s;
                 else sh.v_scale[lane - 32] = s;
             }
     }
@@ -367,9 +368,21 @@ template <int BITS, int KS> __global__ __launch_bounds__(256) void k_attn_chunk_
         w.stage(raw, sh, there);
         if (t < 4) sh.there[t] = there;
         __syncthreads();
+        const float size = fabsf(sh.k_scale[j]);
+        const int shift = shift_of(__builtin_amdgcn_ballot_w64(size > kFar),
+                                   !__builtin_amdgcn_ballot_w64(size >= kNear) && __builtin_amdgcn_ballot_w64(size > 0.0f));
         const f32x4* from = reinterpret_cast<const f32x4*>(&sh);
         f32x4* out = reinterpret_cast<f32x4*>(to + i);
-        for (int x = t; x < (int)(sizeof(S) / 16); x += 256) out[x] = from[x];
+        constexpr int kScales = offsetof(S, k_scale) / 16, kThere = offsetof(S, there) / 16;
+        for (int x = t; x < (int)(sizeof(S) / 16); x += 256)
+        {
+            f32x4 z = from[x];
+            if (x == kThere) z[1] = __builtin_bit_cast(float, shift);
+            if (shift != 0 && x >= kScales && x < kScales + kPos / 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = __builtin_ldexpf(z[e], -shift);
+            out[x] = z;
+        }
         __syncthreads();
     }
 }
@@ -450,7 +463,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 
     // The queries' parts: row l % 32, dims 16 k + 8 (l / 32) + e.
     half8 qp[KS][2];
-    int qe;
+    int se;   // the scores' exponent
     {
         floatx8 z[KS];
         const float* qp0 = a.q + (long)(part.chunk.first + n) * a.q_t + (long)qh * dim * a.q_f;   // rows that are none are formed and dropped
@@ -476,13 +489,15 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
                 top = fmaxf(top, fabsf(z[k][e]));
             }
         }
-        qe = exponent_of(across(top, [](float x, float y) { return fmaxf(x, y); }));
-        const float sign = a.alpha < 0.0f ? -1.0f : a.alpha == 0.0f ? 0.0f : 1.0f;
+        const float by = a.alpha * kLog2e, by_m = __builtin_amdgcn_frexp_mantf(by);
+        top = across(top, [](float x, float y) { return fmaxf(x, y); });
+        const int qe = exponent_of(by_m == 0.0f ? top : top * by_m);
+        se = qe - (BITS == 32 ? 10 : 15) + __builtin_amdgcn_frexp_expf(by);   // a float32 key's scale has the other 5
 #pragma unroll
         for (int k = 0; k < KS; ++k)
         {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[k][e] = __builtin_ldexpf(z[k][e] * sign, 15 - qe);
+            for (int x = 0; x < 8; ++x) z[k][x] = __builtin_ldexpf(z[k][x], 15 - qe) * by_m;
             split2(z[k], qp[k][0], qp[k][1]);
         }
     }
@@ -493,10 +508,9 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     fetch(1, 0);
     __syncthreads();
     const float slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
-    // Scores times log2(e), of queries that have alpha's sign (0 of an alpha of 0); not 0, which would make a masked score's
-    // product NaN.
-    const float by_alpha = __builtin_ldexpf(fabsf(a.alpha) * kLog2e, qe - 10), scale = by_alpha == 0.0f ? 0x1p-149f : by_alpha;
-    const float by = a.slopes ? 1.0f : scale;   // of the scores as the softmax sees them
+    // Of the scores, which the softmax takes as products with it. Not 0, which would make a masked score's product NaN.
+    const float scale = fmaxf(__builtin_ldexpf(1.0f, se), 0x1p-149f);
+    const bool whole = a.slopes || __builtin_amdgcn_ballot_w64(!(scale <= kMaxF));   // scores that are formed themselves
     float m = kLowest, l = 0.0f;
     Held held = kNothingHeld;
     floatx16 o[NB];
@@ -518,6 +532,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             fetch(i + 1 + half, half ^ 1);
         };
         const bool work = p0 < most;   // some row of the wave sees some of it
+        const int shift = __builtin_amdgcn_readfirstlane(in.there[1]);
         floatx16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
@@ -554,10 +569,12 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         turn(0);
         if (work)
         {
-            if (a.slopes)
+            float by = scale;   // of the scores as the softmax sees them
+            if (whole || shift != 0)
             {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = s[r] * scale - slope * (float)(seen - 1 - (p0 + 8 * (r / 4) + 4 * g + r % 4));
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_ldexpf(s[r], se + shift) - slope * (float)(seen - 1 - (p0 + 8 * (r / 4) + 4 * g + r % 4));
+                by = 1.0f;
             }
             f32x4 vs[4];
 #pragma unroll
