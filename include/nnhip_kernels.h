@@ -592,9 +592,10 @@ int nnhip_kv8_read(const nnhip_kv8_pages* c, float* k, long k_t, long k_f, float
  * key head (tokens times q_heads / heads; a call's only sequence where `most` tokens have more) have their products formed
  * from two float16 parts of each factor, exact to 2^-22 of the product and 2^-39 of the largest of a key's, query's or
  * position's values; of a position's weight times its largest value what is below 2^-37 of the row's largest such product
- * is lost. The workspace is nnhip_attn_chunk_workspace_bytes (0 where none is needed; with many rows room for those parts,
- * up to 2 GiB or what one key head's `width * page` positions take, the larger), 16-byte aligned; calls that may overlap
- * in time need one each. Results are the same bits every time. */
+ * is lost. The workspace is nnhip_attn_chunk_workspace_bytes (0 where none is needed; room for the results of ranges of
+ * positions, below 128 MiB with 256 CUs, and with many rows for those parts, up to 2 GiB or what one key head's
+ * `width * page` positions take, the larger), 16-byte aligned; calls that may overlap in time need one each. Results are
+ * the same bits every time. */
 size_t nnhip_attn_chunk_workspace_bytes(const nnhip_kv_pages* c, size_t q_heads, size_t tokens, size_t most);
 int nnhip_attn_chunk(const nnhip_kv_pages* c, const float* q, long q_t, long q_f, size_t q_heads, size_t tokens,
                      const float* start, size_t most, const float* len, const float* slopes, float alpha, float* O,

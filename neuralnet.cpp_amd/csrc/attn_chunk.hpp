@@ -12,6 +12,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kTile = 16;          // positions and rows of a product
 constexpr int kChunkMaxDim = 128;
+constexpr int kNarrowRows = 32;   // of a sequence and key head that the kernels of few rows take at most
 
 struct ChunkArgs
 {
@@ -21,9 +22,11 @@ struct ChunkArgs
     float* O;
     long o_t, o_f;
     float *m, *l;
-    float *part_ml, *part_o;         // per (token, head, range): m and l; O unnormalised
+    float *part_ml, *part_o;         // per (row, range): m and l; O unnormalised (result_of)
+    float *wide_ml, *wide_o;         // in the joins: those of k_attn_chunk_wide's rows
     unsigned q_heads, tokens, most;
-    unsigned ranges, slots;          // that the kernel cuts positions into; and results of a row
+    unsigned ranges;                 // that the kernel cuts positions into
+    int few_rows;                    // results are of kNarrowRows for each sequence and key head, not of every token and head
     int wide_from;                   // sequences of more rows are k_attn_chunk_wide's
     char* images;                    // its keys' and values' parts: `tiles` a piece, of the pieces (slot and key head)
     unsigned tiles, first_piece, pieces;   // that the launch is for
@@ -307,6 +310,18 @@ template <int KS> struct WalkShared
     float ml[4][kTile][2];
 };
 
+// The place of a row's results of ranges.
+__device__ __forceinline__ size_t few_result_of(const ChunkArgs& a, unsigned b, unsigned h, unsigned row)
+{
+    return ((size_t)b * a.c.t.heads + h) * kNarrowRows + row;
+}
+__device__ __forceinline__ size_t result_of(const ChunkArgs& a, const Part& part, unsigned row)
+{
+    if (a.few_rows) return few_result_of(a, part.b, part.h, row);
+    const unsigned i = a.by_per.div(row);
+    return (size_t)(part.chunk.first + i) * a.q_heads + part.h * a.by_per.d + (row - i * a.by_per.d);
+}
+
 // Where a row's results go: m, l and values d .. d + 3 of O, unnormalised. LOG2: m is a score times log2(e). The results of
 // ranges that others form so (WIDE) are joined so: a score's product with log2(e) is rounded once, before the ranges part.
 template <bool WIDE, bool LOG2>
@@ -328,7 +343,7 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int ro
         if (stats && a.l) a.l[at] = l;
         return;
     }
-    const size_t p = at * a.slots + part.slot;
+    const size_t p = (a.few_rows ? few_result_of(a, part.b, part.h, row) : at) * a.ranges + part.slot;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (d + e < dim) a.part_o[p * dim + d + e] = o[e];
@@ -491,10 +506,9 @@ __device__ __forceinline__ bool cut_range(const ChunkArgs& a, Part& part, int ro
     if (part.begin < part.end || a.ranges == 1) return true;
     for (int row = part.first + threadIdx.x; row <= last; row += blockDim.x)
     {
-        const unsigned i = a.by_per.div(row);
-        const size_t at = (size_t)(part.chunk.first + i) * a.q_heads + part.h * a.by_per.d + (row - i * a.by_per.d);
-        a.part_ml[2 * (at * a.slots + part.slot)] = kLowest;
-        a.part_ml[2 * (at * a.slots + part.slot) + 1] = 0.0f;
+        const size_t p = result_of(a, part, row) * a.ranges + part.slot;
+        a.part_ml[2 * p] = kLowest;
+        a.part_ml[2 * p + 1] = 0.0f;
     }
     return false;
 }
@@ -521,7 +535,6 @@ __device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int 
 // of a workgroup.
 void chunk8(const ChunkArgs& a, int bytes, unsigned blocks, hipStream_t s);
 constexpr int kWideRows = 128;
-constexpr int kNarrowRows = 32;   // of a sequence and key head that the kernels of few rows take at most
 size_t chunk_image_bytes(int bits, unsigned dim);
 void chunk_parts(const ChunkArgs& a, int bits, unsigned pieces, unsigned blocks, hipStream_t s);
 void chunk_wide(const ChunkArgs& a, int bits, unsigned blocks, hipStream_t s);

@@ -36,35 +36,40 @@ constexpr float kNoRange = -1.0f;
 constexpr size_t kMostRanges = 256;
 
 // The joins: narrow, wide: the ranges of the rows of either kernel. A row's ranges, 0 where it has nothing to join: written
-// already, or no sequence's token.
+// already, or no sequence's token; and the place of their results.
 struct Joined
 {
     unsigned ranges;
     bool log2;   // m is a score times log2(e)
+    bool is_wide;
+    size_t at;
 };
-__device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigned narrow, unsigned wide)
+__device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigned h, unsigned narrow, unsigned wide)
 {
     const int b = last_of(a.c.t.batch, [&](unsigned i) { return length_of(a.start[i], a.tokens) <= (int)n; });
-    if (b < 0) return {0, false};
+    if (b < 0) return {};
     const Chunk c = chunk_of(a, b);
-    if (n >= c.first + c.n) return {0, false};
+    if (n >= c.first + c.n) return {};
     const bool is_wide = c.n * (int)a.by_per.d > a.wide_from;
-    const unsigned ranges = is_wide ? wide : narrow;
-    return {ranges == 1 ? 0 : ranges, is_wide || a.c.K};
+    const unsigned ranges = is_wide ? wide : narrow, kh = a.by_per.div(h);
+    const size_t own = (size_t)n * a.q_heads + h;
+    return {ranges == 1 ? 0 : ranges, is_wide || a.c.K, is_wide,
+            is_wide || !a.few_rows ? own : few_result_of(a, b, kh, (n - c.first) * a.by_per.d + (h - kh * a.by_per.d))};
 }
 
-// Row i of a join's grid: its place among the results, token and head. Where rows of the wide kernel are whole already (wide 1)
-// the grid is of the others alone, kNarrowRows for each sequence and key head; i is past them where it has fewer.
-__device__ __forceinline__ bool row_of_join(const ChunkArgs& a, unsigned i, unsigned narrow, unsigned wide, unsigned& at, unsigned& n,
-                                            unsigned& h, Joined& r)
+// Row i of a join's grid: token and head, and, where the grid's order does not say it (wide), what is joined. Where rows of the
+// wide kernel are whole already, or there are none (wide 1), the grid is of the others alone, kNarrowRows for each sequence and key head; i is past
+// them where it has fewer.
+__device__ __forceinline__ bool row_of_join(const ChunkArgs& a, unsigned i, unsigned narrow, unsigned wide, unsigned& n, unsigned& h,
+                                            Joined& r)
 {
     if (wide != 1)
     {
-        at = i;
-        n = a.by_q_heads.div(at);
-        h = at - n * a.q_heads;
+        n = a.by_q_heads.div(i);
+        h = i - n * a.q_heads;
         if (n >= a.tokens) return false;
-        if (wide) r = joined(a, n, narrow, wide);
+        if (wide) r = joined(a, n, h, narrow, wide);
+        else r.at = i;
         return !wide || r.ranges > 0;
     }
     const unsigned piece = i / kNarrowRows, row = i - piece * kNarrowRows, b = a.by_heads.div(piece), kh = piece - b * a.c.t.heads;
@@ -75,8 +80,7 @@ __device__ __forceinline__ bool row_of_join(const ChunkArgs& a, unsigned i, unsi
     const unsigned t = a.by_per.div(row);
     n = c.first + t;
     h = kh * a.by_per.d + (row - t * a.by_per.d);
-    at = n * a.q_heads + h;
-    r = {narrow, a.c.K != nullptr};
+    r = {narrow, a.c.K != nullptr, false, i};
     return true;
 }
 
@@ -86,19 +90,19 @@ __device__ __forceinline__ bool row_of_join(const ChunkArgs& a, unsigned i, unsi
 constexpr unsigned kFewParts = 16;
 __global__ __launch_bounds__(256) void k_attn_chunk_join_few(ChunkArgs a, unsigned narrow, unsigned wide)
 {
-    unsigned at, n, h;
+    unsigned n, h;
     Joined r{};
-    if (!row_of_join(a, (blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64, narrow, wide, at, n, h, r)) return;
-    const unsigned last = wide ? r.ranges - 1 : a.slots - 1;
+    if (!row_of_join(a, (blockIdx.y * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64, narrow, wide, n, h, r)) return;
+    const unsigned slots = wide ? r.ranges : narrow, last = slots - 1;
     const int lane = threadIdx.x & 63, dim = a.c.t.dim;
-    const float2 own = reinterpret_cast<const float2*>(a.part_ml)[(size_t)at * a.slots + min((unsigned)lane, last)];
-    const float* po = a.part_o + (size_t)at * a.slots * dim;
+    const float2 own = reinterpret_cast<const float2*>(r.is_wide ? a.wide_ml : a.part_ml)[r.at * slots + min((unsigned)lane, last)];
+    const float* po = (r.is_wide ? a.wide_o : a.part_o) + r.at * slots * dim;
     float x[kFewParts][2];
 #pragma unroll
     for (unsigned i = 0; i < kFewParts; ++i)
 #pragma unroll
         for (int y = 0; y < 2; ++y) x[i][y] = po[(size_t)min(i, last) * dim + min(lane + 64 * y, dim - 1)];
-    if (!wide) r = joined(a, n, narrow, wide);
+    if (!wide) r = joined(a, n, h, narrow, wide);
     if (r.ranges == 0) return;
     const bool any = lane < (int)r.ranges && own.y != 0.0f;
     const float m = wave_max(any ? own.x : kLowest);
@@ -118,8 +122,9 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join_few(ChunkArgs a, unsign
         const int d = lane + 64 * y;
         if (d < dim) a.O[(long)n * a.o_t + ((long)h * dim + d) * a.o_f] = l == 0.0f ? 0.0f : o[y] / l;
     }
-    if (lane == 0 && a.m) a.m[at] = r.log2 && m != kLowest ? m * kLn2 : m;
-    if (lane == 0 && a.l) a.l[at] = l;
+    const size_t to = (size_t)n * a.q_heads + h;
+    if (lane == 0 && a.m) a.m[to] = r.log2 && m != kLowest ? m * kLn2 : m;
+    if (lane == 0 && a.l) a.l[to] = l;
 }
 
 // More: a workgroup a row. The ranges' factors go to LDS, then 2 or 4 groups of threads sum every 2nd or 4th range.
@@ -127,15 +132,15 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
 {
     static_assert(kMostRanges <= 256);
     __shared__ float w_s[256], red[2][4], o_s[256];
-    unsigned at, n, h;
+    unsigned n, h;
     Joined r{};
-    if (!row_of_join(a, blockIdx.y * gridDim.x + blockIdx.x, narrow, wide, at, n, h, r)) return;
-    if (!wide) r = joined(a, n, narrow, wide);
+    if (!row_of_join(a, blockIdx.y * gridDim.x + blockIdx.x, narrow, wide, n, h, r)) return;
+    if (!wide) r = joined(a, n, h, narrow, wide);
     if (r.ranges == 0) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, dim = a.c.t.dim;
     const int cols = dim <= 64 ? 64 : 128, groups = 256 / cols, d = t % cols, g = t / cols;
-    const float2 own = reinterpret_cast<const float2*>(a.part_ml)[(size_t)at * a.slots + min((unsigned)t, r.ranges - 1)];
-    const float* po = a.part_o + (size_t)at * a.slots * dim + (d < dim ? d : 0);
+    const float2 own = reinterpret_cast<const float2*>(r.is_wide ? a.wide_ml : a.part_ml)[r.at * r.ranges + min((unsigned)t, r.ranges - 1)];
+    const float* po = (r.is_wide ? a.wide_o : a.part_o) + r.at * r.ranges * dim + (d < dim ? d : 0);
     const bool any = t < (int)r.ranges && own.y != 0.0f;
     float m = wave_max(any ? own.x : kLowest);
     if (lane == 0) red[0][wave] = m;
@@ -161,8 +166,9 @@ __global__ __launch_bounds__(256) void k_attn_chunk_join(ChunkArgs a, unsigned n
         for (int i = 0; i < groups; ++i) o += o_s[i * cols + t];
         a.O[(long)n * a.o_t + ((long)h * dim + t) * a.o_f] = l == 0.0f ? 0.0f : o / l;
     }
-    if (t == 0 && a.m) a.m[at] = r.log2 && m != kLowest ? m * kLn2 : m;
-    if (t == 0 && a.l) a.l[at] = l;
+    const size_t to = (size_t)n * a.q_heads + h;
+    if (t == 0 && a.m) a.m[to] = r.log2 && m != kLowest ? m * kLn2 : m;
+    if (t == 0 && a.l) a.l[to] = l;
 }
 
 // A call's sizes, whichever cache it is over.
@@ -182,7 +188,7 @@ struct ChunkPlan
     size_t blocks, wide_row_blocks, wide_blocks;
     bool wide_by_seqs;
     size_t image_slots, image_tiles, image_pieces;   // of the parts; pieces that are formed at a time
-    unsigned slots() const { return std::max(narrow, wide); }
+    unsigned most_ranges() const { return std::max(narrow, wide); }
 };
 
 // Parts of keys and values that are formed at a time, or those of one piece: past this a call takes several launches. They are
@@ -225,16 +231,30 @@ ChunkPlan chunk_plan(const ChunkCall& c)
     return p;
 }
 
-// m and l of every row and range, in whole 16 bytes.
-size_t ml_floats(const ChunkCall& c, const ChunkPlan& p) { return (2 * c.tokens * c.q_heads * p.slots() + 3) / 4 * 4; }
-// The ranges' results, in whole 16 bytes, and behind them the parts.
-size_t chunk_results(const ChunkCall& c, const ChunkPlan& p)
+// The workspace: the ranges' results of the rows of either kernel (m and l, then O), and the parts; floats, each in whole 16
+// bytes. Beside prompts, and where most tokens are padding, the narrow kernel's are those of kNarrowRows for each sequence and
+// key head: its ranges are chosen for that many, and of every token they would be gigabytes that nothing writes (two prompts
+// of 8192 tokens, 32 heads on 8 of 128: 12 GiB, and 12 MiB so).
+struct ChunkSpace
 {
-    return p.slots() == 1 ? 0 : (ml_floats(c, p) + (c.tokens * c.q_heads * p.slots() * c.c.t.dim + 3) / 4 * 4) * sizeof(float);
-}
-size_t chunk_workspace(const ChunkCall& c, const ChunkPlan& p)
+    size_t narrow_o, wide_ml, wide_o, images;
+    size_t bytes;
+    bool few_rows;
+};
+ChunkSpace chunk_space(const ChunkCall& c, const ChunkPlan& p)
 {
-    return chunk_results(c, p) + p.image_pieces * p.image_tiles * chunk_image_bytes(c.bits, c.c.t.dim);
+    const size_t all = c.tokens * c.q_heads, few = (size_t)c.c.t.batch * c.c.t.heads * kNarrowRows;
+    const bool few_rows = p.wide || all > few;
+    const size_t narrow = p.narrow > 1 ? (few_rows ? few : all) * p.narrow : 0, wide = p.wide > 1 ? all * p.wide : 0, dim = c.c.t.dim;
+    auto whole = [](size_t n) { return (n + 3) / 4 * 4; };
+    ChunkSpace s{};
+    s.few_rows = few_rows;
+    s.narrow_o = whole(2 * narrow);
+    s.wide_ml = s.narrow_o + whole(narrow * dim);
+    s.wide_o = s.wide_ml + whole(2 * wide);
+    s.images = s.wide_o + whole(wide * dim);
+    s.bytes = s.images * sizeof(float) + p.image_pieces * p.image_tiles * chunk_image_bytes(c.bits, c.c.t.dim);
+    return s;
 }
 
 bool chunk_ok(const ChunkCall& c, size_t heads)
@@ -279,7 +299,7 @@ template <int BITS, bool VEC> void chunk_launch(const ChunkArgs& a, const ChunkP
 template <class C> size_t chunk_bytes(const C* c, size_t q_heads, size_t tokens, size_t most)
 {
     ChunkCall call;
-    return chunk_call(c, q_heads, tokens, most, call) ? chunk_workspace(call, chunk_plan(call)) : 0;
+    return chunk_call(c, q_heads, tokens, most, call) ? chunk_space(call, chunk_plan(call)).bytes : 0;
 }
 
 template <class C>
@@ -290,8 +310,8 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     ChunkCall call;
     if (!chunk_call(c, q_heads, tokens, most, call) || !q || !start || !len || !O || q_t < 0 || q_f < 0 || o_t < 0 || o_f < 0) return -1;
     const ChunkPlan p = chunk_plan(call);
-    const size_t need = chunk_workspace(call, p);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return -1;
+    const ChunkSpace space = chunk_space(call, p);
+    if (space.bytes > 0 && (!workspace || workspace_bytes < space.bytes || !aligned16(workspace))) return -1;
     if (p.blocks > kGridMost || p.wide_blocks > kGridMost) return -1;
     auto* ws = static_cast<float*>(workspace);
     ChunkArgs a{};
@@ -308,12 +328,14 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     a.m = m;
     a.l = l;
     a.part_ml = ws;
-    if (p.slots() > 1) a.part_o = ws + ml_floats(call, p);
+    a.part_o = ws + space.narrow_o;
+    a.wide_ml = ws + space.wide_ml;
+    a.wide_o = ws + space.wide_o;
+    a.few_rows = space.few_rows;
     a.q_heads = static_cast<unsigned>(q_heads);
     a.tokens = static_cast<unsigned>(tokens);
     a.most = static_cast<unsigned>(most);
     a.ranges = p.narrow;
-    a.slots = p.slots();
     a.wide_from = p.wide_from;
     a.by_per = FastDiv(static_cast<unsigned>(q_heads / c->heads));
     a.by_heads = FastDiv(call.c.t.heads);
@@ -335,11 +357,14 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     {
         ChunkArgs w = a;
         w.ranges = p.wide;
+        w.part_ml = a.wide_ml;
+        w.part_o = a.wide_o;
+        w.few_rows = 0;
         w.by_ranges = FastDiv(p.wide);
         w.by_row_blocks = FastDiv(static_cast<unsigned>(p.wide_row_blocks));
         w.by_block_rows = FastDiv(p.wide_by_seqs ? kWideRows : kNarrowRows + 1);
         w.block_seqs = p.wide_by_seqs;
-        w.images = static_cast<char*>(workspace) + chunk_results(call, p);
+        w.images = reinterpret_cast<char*>(ws + space.images);
         w.tiles = static_cast<unsigned>(p.image_tiles);
         w.slots_by_batch = p.image_slots == call.c.t.batch;
         // Workgroups: of several slots most may have nothing to do.
@@ -355,12 +380,13 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
             if (int rc = launch_status()) return rc;
         }
     }
-    if (p.slots() == 1) return 0;
-    const bool few = p.slots() <= kFewParts;
-    const size_t rows = p.wide == 1 ? call.c.t.batch * (size_t)call.c.t.heads * kNarrowRows : tokens * q_heads;
+    if (p.most_ranges() == 1) return 0;
+    const bool few = p.most_ranges() <= kFewParts;
+    const unsigned wide = p.wide == 0 && space.few_rows ? 1 : p.wide;   // no wide rows, or whole ones: the others' grid
+    const size_t rows = wide == 1 ? call.c.t.batch * (size_t)call.c.t.heads * kNarrowRows : tokens * q_heads;
     const size_t blocks = few ? (rows + 3) / 4 : rows, x = std::min(blocks, (size_t)1 << 20);
     const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>((blocks + x - 1) / x));
-    hipLaunchKernelGGL(few ? k_attn_chunk_join_few : k_attn_chunk_join, grid, dim3(256), 0, s, a, p.narrow, p.wide);
+    hipLaunchKernelGGL(few ? k_attn_chunk_join_few : k_attn_chunk_join, grid, dim3(256), 0, s, a, p.narrow, wide);
     return launch_status();
 }
 
