@@ -27,6 +27,7 @@ struct ChunkArgs
     unsigned q_heads, tokens, most;
     unsigned ranges;                 // that the kernel cuts positions into
     int few_rows;                    // results are of kNarrowRows for each sequence and key head, not of every token and head
+    unsigned result_step;            // from a token's results to the next one's
     int wide_from;                   // sequences of more rows are k_attn_chunk_wide's
     char* images;                    // its keys' and values' parts: `tiles` a piece, of the pieces (slot and key head)
     unsigned tiles, first_piece, pieces;   // that the launch is for
@@ -303,6 +304,7 @@ struct Part
     int n_rows;             // of the sequence
     unsigned slot;          // range
     int begin, end;
+    size_t results;         // the place of the first row's results of ranges
 };
 template <int KS> struct WalkShared
 {
@@ -310,16 +312,14 @@ template <int KS> struct WalkShared
     float ml[4][kTile][2];
 };
 
-// The place of a row's results of ranges.
-__device__ __forceinline__ size_t few_result_of(const ChunkArgs& a, unsigned b, unsigned h, unsigned row)
+// The place of the results of a sequence's first row of a key head, and of token i's head qh of them.
+__device__ __forceinline__ size_t results_of(const ChunkArgs& a, unsigned b, unsigned h, unsigned first)
 {
-    return ((size_t)b * a.c.t.heads + h) * kNarrowRows + row;
+    return a.few_rows ? ((size_t)b * a.c.t.heads + h) * kNarrowRows : (size_t)first * a.q_heads + h * a.by_per.d;
 }
-__device__ __forceinline__ size_t result_of(const ChunkArgs& a, const Part& part, unsigned row)
+__device__ __forceinline__ size_t result_of(const ChunkArgs& a, size_t results, unsigned i, unsigned qh)
 {
-    if (a.few_rows) return few_result_of(a, part.b, part.h, row);
-    const unsigned i = a.by_per.div(row);
-    return (size_t)(part.chunk.first + i) * a.q_heads + part.h * a.by_per.d + (row - i * a.by_per.d);
+    return results + (size_t)i * a.result_step + qh;
 }
 
 // Where a row's results go: m, l and values d .. d + 3 of O, unnormalised. LOG2: m is a score times log2(e). The results of
@@ -329,8 +329,8 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int ro
 {
     if (LOG2 && a.ranges == 1 && m != kLowest) m *= kLn2;
     if (WIDE && !LOG2 && a.ranges > 1 && m != kLowest) m *= kLog2e;
-    const unsigned i = a.by_per.div(row), qh = part.h * a.by_per.d + (row - i * a.by_per.d);
-    const size_t n = part.chunk.first + i, at = n * a.q_heads + qh;
+    const unsigned i = a.by_per.div(row), own = row - i * a.by_per.d, qh = part.h * a.by_per.d + own;
+    const size_t n = part.chunk.first + i;
     const int dim = a.c.t.dim;
     if (a.ranges == 1)
     {
@@ -339,11 +339,11 @@ __device__ __forceinline__ void put(const ChunkArgs& a, const Part& part, int ro
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (d + e < dim) to[(long)(d + e) * a.o_f] = l == 0.0f ? 0.0f : o[e] * inv;
-        if (stats && a.m) a.m[at] = m;
-        if (stats && a.l) a.l[at] = l;
+        if (stats && a.m) a.m[n * a.q_heads + qh] = m;
+        if (stats && a.l) a.l[n * a.q_heads + qh] = l;
         return;
     }
-    const size_t p = (a.few_rows ? few_result_of(a, part.b, part.h, row) : at) * a.ranges + part.slot;
+    const size_t p = result_of(a, part.results, i, own) * a.ranges + part.slot;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (d + e < dim) a.part_o[p * dim + d + e] = o[e];
@@ -506,7 +506,8 @@ __device__ __forceinline__ bool cut_range(const ChunkArgs& a, Part& part, int ro
     if (part.begin < part.end || a.ranges == 1) return true;
     for (int row = part.first + threadIdx.x; row <= last; row += blockDim.x)
     {
-        const size_t p = result_of(a, part, row) * a.ranges + part.slot;
+        const unsigned i = a.by_per.div(row);
+        const size_t p = result_of(a, part.results, i, row - i * a.by_per.d) * a.ranges + part.slot;
         a.part_ml[2 * p] = kLowest;
         a.part_ml[2 * p + 1] = 0.0f;
     }
@@ -528,6 +529,7 @@ __device__ __forceinline__ bool narrow_part(const ChunkArgs& a, Part& part, int 
     part.chunk = chunk_of(a, part.b);
     part.n_rows = part.chunk.n * a.by_per.d;
     part.first = 0;
+    part.results = results_of(a, part.b, part.h, part.chunk.first);
     return part.n_rows > 0 && part.n_rows <= a.wide_from && cut_range(a, part, part.n_rows, step);
 }
 

@@ -86,6 +86,17 @@ template <class F> __device__ __forceinline__ float across(float x, F&& f)
     const unsigned lo = z[0], hi = z[1];
     return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
+// The wave's four rows of 16 lanes: f of the values of lanes l, l ^ 16, l ^ 32 and l ^ 48.
+template <class F> __device__ __forceinline__ float across4(float x, F&& f)
+{
+    unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+    asm("" : "+v"(b));
+    const auto z = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    const unsigned lo = z[0], hi = z[1];
+    return across(f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)), f);
+}
+__device__ __forceinline__ float larger_of(float a, float b) { return fmaxf(a, b); }
+
 // Scores. alpha log2(e) is by_m 2^by_e: the query's parts take by_m, and a score, times log2(e), is s f 2^e with s the sum of
 // the parts' products, f the key's scale and e the row's exponent. A tile's scales are multiplied by 2^-shift_of them and e is
 // raised by it, so that neither s f leaves float32's range where the score does not, nor f has bits below that range: of
@@ -93,23 +104,26 @@ template <class F> __device__ __forceinline__ float across(float x, F&& f)
 constexpr float kFar = 0x1p80f, kNear = 0x1p-75f;
 __device__ __forceinline__ int shift_of(unsigned long long far, bool all_near) { return far ? 64 : all_near ? -64 : 0; }
 
-// What weights times values are held against: 2^top, above the largest of these products that the row has met, as they
-// shrink with a growing score. past: bits that the products have shrunk by and top has not.
+// What weights times values are held against: 2^top, above the largest of these products that the row has met, which shrink
+// with a growing score. size: that exponent before it is rounded up, so that no small step is lost.
 struct Held
 {
-    int top;
-    float past;
+    float size = kLeastTop;
+    __device__ __forceinline__ int top() const { return (int)ceilf(size); }
 };
-constexpr Held kNothingHeld{kLeastTop, 0.0f};
-// Scores grow by `up` bits (0 and above), and the tile's products lie below 2^tile. What the outputs are multiplied by; the
-// sum of the weights by 2^-up.
-__device__ __forceinline__ float hold(Held& h, float up, int tile)
+// Scores grow by `up` bits: what the outputs are multiplied by. The sum of the weights is by 2^-up.
+__device__ __forceinline__ float shrink(Held& h, float up)
 {
-    const float past = h.past + up, whole = floorf(past);
-    const int was = h.top;
-    h.past = past - whole;
-    h.top = max(max(was - (int)fminf(whole, 2048.0f), tile), kLeastTop);
-    return __builtin_amdgcn_exp2f((float)(was - h.top) - up);
+    const int was = h.top();
+    h.size = fmaxf(h.size - up, kLeastTop);
+    return __builtin_amdgcn_exp2f((float)(was - h.top()) - up);
+}
+// Products below 2^e have come: what the outputs are multiplied by.
+__device__ __forceinline__ float raise(Held& h, int e)
+{
+    const int was = h.top();
+    h.size = fmaxf(h.size, (float)e);
+    return __builtin_ldexpf(1.0f, was - h.top());
 }
 // The largest over the wave of each of 8 numbers a lane, none negative: lane l has the number l % 8's.
 __device__ __forceinline__ float max_of_8(const float (&x)[8], int lane)
@@ -121,12 +135,7 @@ __device__ __forceinline__ float max_of_8(const float (&x)[8], int lane)
     for (int i = 0; i < 2; ++i) b[i] = fmaxf(lane & 2 ? a[2 + i] : a[i], swap_dpp<0x4e>(lane & 2 ? a[i] : a[2 + i]));
     float r = fmaxf(lane & 1 ? b[1] : b[0], swap_dpp<0xb1>(lane & 1 ? b[0] : b[1]));
     r = max_dpp<0x128>(r);   // each 16 turned by 8
-    unsigned u = __builtin_bit_cast(unsigned, r), v = u;
-    asm("" : "+v"(v));
-    const auto z = __builtin_amdgcn_permlane16_swap(u, v, false, false);
-    const unsigned lo = z[0], hi = z[1];
-    r = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
-    return across(r, [](float y, float w) { return fmaxf(y, w); });
+    return across4(r, larger_of);
 }
 
 } // namespace nnhip

@@ -52,9 +52,8 @@ __device__ __forceinline__ Joined joined(const ChunkArgs& a, unsigned n, unsigne
     if (n >= c.first + c.n) return {};
     const bool is_wide = c.n * (int)a.by_per.d > a.wide_from;
     const unsigned ranges = is_wide ? wide : narrow, kh = a.by_per.div(h);
-    const size_t own = (size_t)n * a.q_heads + h;
     return {ranges == 1 ? 0 : ranges, is_wide || a.c.K, is_wide,
-            is_wide || !a.few_rows ? own : few_result_of(a, b, kh, (n - c.first) * a.by_per.d + (h - kh * a.by_per.d))};
+            is_wide ? (size_t)n * a.q_heads + h : result_of(a, results_of(a, b, kh, c.first), n - c.first, h - kh * a.by_per.d)};
 }
 
 // Row i of a join's grid: token and head, and, where the grid's order does not say it (wide), what is joined. Where rows of the
@@ -332,6 +331,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
     a.wide_ml = ws + space.wide_ml;
     a.wide_o = ws + space.wide_o;
     a.few_rows = space.few_rows;
+    a.result_step = static_cast<unsigned>(space.few_rows ? q_heads / c->heads : q_heads);
     a.q_heads = static_cast<unsigned>(q_heads);
     a.tokens = static_cast<unsigned>(tokens);
     a.most = static_cast<unsigned>(most);
@@ -360,6 +360,7 @@ int attn_chunk(const C* c, const float* q, long q_t, long q_f, size_t q_heads, s
         w.part_ml = a.wide_ml;
         w.part_o = a.wide_o;
         w.few_rows = 0;
+        w.result_step = a.q_heads;
         w.by_ranges = FastDiv(p.wide);
         w.by_row_blocks = FastDiv(static_cast<unsigned>(p.wide_row_blocks));
         w.by_block_rows = FastDiv(p.wide_by_seqs ? kWideRows : kNarrowRows + 1);

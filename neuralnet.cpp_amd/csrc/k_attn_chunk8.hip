@@ -204,8 +204,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
                 z[s][e] = B::dim_of(s, g) + e < dim ? z[s][e] : 0.0f;   // dims past the last one
                 top = fmaxf(top, fabsf(z[s][e]));
             }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = across4(top, larger_of);
         const int qe = exponent_of(by_m == 0.0f ? top : top * by_m);
 #pragma unroll
         for (int s = 0; s < B::steps; ++s)
@@ -216,7 +215,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
         }
         w.slope = a.slopes && live ? a.slopes[qh] * kLog2e : 0.0f;
         w.e = qe - 15 + __builtin_amdgcn_frexp_expf(by);
-        w.held = kNothingHeld;
+        w.held = Held();
         w.m = kLowest;
         w.l = 0.0f;
 #pragma unroll
@@ -269,7 +268,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][u][e] = __builtin_ldexpf(s[i][u][e] * ks[u][e], w.e + shift);
-            f32x4 own[2] = {vs[0], vs[1]};   // the values' scales of what the row sees
+            unsigned mine = 0;   // which of the lane's positions its row sees, where it does not see all
             if (odd)
             {
 #pragma unroll
@@ -281,7 +280,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
                         const float z = s[i][u][e] - w.slope * (float)(w.seen - 1 - (p + q));
                         const bool sees = (now >> q & 1) && p + q < w.seen;
                         s[i][u][e] = sees ? z : -__builtin_inff();
-                        own[u][e] = sees ? own[u][e] : 0.0f;   // 0 times a NaN would be one
+                        mine |= (sees ? 1u : 0u) << (4 * u + e);
                     }
             }
             float high = kLowest;
@@ -289,14 +288,13 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) high = fmaxf(high, s[i][u][e]);
-            float up = 0.0f;
             if (__builtin_amdgcn_ballot_w64(high > w.m))   // seldom past the first tiles
             {
-                high = fmaxf(high, __shfl_xor(high, 16, 64));
-                high = fmaxf(high, __shfl_xor(high, 32, 64));
-                const float mn = fmaxf(w.m, high);
-                up = mn - w.m;
+                const float mn = fmaxf(w.m, across4(high, larger_of)), up = mn - w.m, f = shrink(w.held, up);
                 w.m = mn;
+                w.l *= __builtin_amdgcn_exp2f(-up);
+#pragma unroll
+                for (int b = 0; b < B::VB; ++b) w.o[b] *= f;
             }
             float sum = 0.0f, size = 0.0f;
             floatx8 z;
@@ -307,20 +305,24 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
                 {
                     const float y = __builtin_amdgcn_exp2f(s[i][u][e] - w.m);
                     sum += y;
-                    z[4 * u + e] = y * own[u][e];
-                    size = fmaxf(size, fabsf(z[4 * u + e]));
+                    z[4 * u + e] = y * vs[u][e];
                 }
-            if (__builtin_amdgcn_ballot_w64(up != 0.0f || exponent_of(size) > w.held.top))   // seldom, too
+            if (part_seen)   // 0 times a NaN would be one
             {
-                size = fmaxf(size, __shfl_xor(size, 16, 64));
-                size = fmaxf(size, __shfl_xor(size, 32, 64));
-                const float f = hold(w.held, up, exponent_of(size));
-                w.l *= __builtin_amdgcn_exp2f(-up);
+                asm volatile("");   // stays a branch
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = mine >> e & 1 ? z[e] : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) size = fmaxf(size, fabsf(z[e]));
+            if (__builtin_amdgcn_ballot_w64(exponent_of(size) > w.held.top()))   // seldom, too
+            {
+                const float f = raise(w.held, exponent_of(across4(size, larger_of)));
 #pragma unroll
                 for (int b = 0; b < B::VB; ++b) w.o[b] *= f;
             }
             w.l += sum;
-            const float to = __builtin_ldexpf(1.0f, 15 - w.held.top);
+            const float to = __builtin_ldexpf(1.0f, 15 - w.held.top());
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] *= to;
             split2(z, pp[i][0], pp[i][1]);
@@ -351,8 +353,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
     for (int i = 0; i < RT; ++i)
     {
         Row8<KS, W>& w = rows[i];
-        w.l += __shfl_xor(w.l, 16, 64);
-        w.l += __shfl_xor(w.l, 32, 64);
+        w.l = across4(w.l, [](float x, float y) { return x + y; });
         __syncthreads();
         if (g == 0)
         {
@@ -362,7 +363,7 @@ template <int KS, int W, int RT> __device__ __forceinline__ void walk8(const Chu
 #pragma unroll
         for (int b = 0; b < B::VB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], w.held.top - 15);
+            for (int r = 0; r < 4; ++r) sh.o[wave][j][B::VB * (4 * g + r) + b] = __builtin_ldexpf(w.o[b][r], w.held.top() - 15);
         __syncthreads();
         const int jr = t >> 4, r = part.first + i * kTile + jr;
         if (r >= part.n_rows) continue;

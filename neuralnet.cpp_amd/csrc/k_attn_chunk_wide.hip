@@ -419,6 +419,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
         if (part.n_rows <= a.wide_from || at_piece >= a.pieces || block >= (unsigned)(part.n_rows + kWideRows - 1) / kWideRows) return;
         images = reinterpret_cast<const S*>(a.images) + (size_t)at_piece * a.tiles;
         part.first = block * kWideRows;
+        part.results = results_of(a, part.b, part.h, part.chunk.first);
         if (!cut_range(a, part, kWideRows, 64)) return;
     }
     const int dim = a.c.t.dim, begin = part.begin, end = part.end;
@@ -490,7 +491,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
             }
         }
         const float by = a.alpha * kLog2e, by_m = __builtin_amdgcn_frexp_mantf(by);
-        top = across(top, [](float x, float y) { return fmaxf(x, y); });
+        top = across(top, larger_of);
         const int qe = exponent_of(by_m == 0.0f ? top : top * by_m);
         se = qe - (BITS == 32 ? 10 : 15) + __builtin_amdgcn_frexp_expf(by);   // a float32 key's scale has the other 5
 #pragma unroll
@@ -512,7 +513,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     const float scale = fmaxf(__builtin_ldexpf(1.0f, se), 0x1p-149f);
     const bool whole = a.slopes || __builtin_amdgcn_ballot_w64(!(scale <= kMaxF));   // scores that are formed themselves
     float m = kLowest, l = 0.0f;
-    Held held = kNothingHeld;
+    Held held;
     floatx16 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -594,12 +595,14 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
 #pragma unroll
             for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
             high *= by;
-            float up = 0.0f;
             if (__builtin_amdgcn_ballot_w64(high > m))   // seldom past the first tiles
             {
-                const float mn = fmaxf(m, across(high, [](float x, float y) { return fmaxf(x, y); }));
-                up = mn - m;
+                const float mn = fmaxf(m, across(high, larger_of));
+                const float up = mn - m, f = shrink(held, up);
                 m = mn;
+                l *= __builtin_amdgcn_exp2f(-up);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[b] *= f;
             }
             // What rounding the largest score took away is added to the weights' exponents: of scores past 2^20 it may be
             // more than an exponent holds, and these are rounded first.
@@ -620,16 +623,14 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
                 size = fmaxf(size, fabsf(s[r]));
             }
             constexpr int kQuarter = BITS == 32 ? 2 : 0;   // weights are held with the scales' quarters
-            if (__builtin_amdgcn_ballot_w64(up != 0.0f || exponent_of(size) + kQuarter > held.top))   // seldom, too
+            if (__builtin_amdgcn_ballot_w64(exponent_of(size) + kQuarter > held.top()))   // seldom, too
             {
-                size = across(size, [](float x, float y) { return fmaxf(x, y); });
-                const float f = hold(held, up, exponent_of(size) + kQuarter);
-                l *= __builtin_amdgcn_exp2f(-up);
+                const float f = raise(held, exponent_of(across(size, larger_of)) + kQuarter);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) o[b] *= f;
             }
             l += sum;
-            const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - held.top);
+            const float to = __builtin_ldexpf(BITS == 32 ? 4.0f : 1.0f, 15 - held.top());
             const int place1 = lane ^ (lane >> 3 & 7);
             half8 vh[NB], vl[NB];
             auto values = [&](int st, int x, half8(&to)[NB]) __attribute__((always_inline)) {
@@ -670,7 +671,7 @@ template <int BITS, int KS> __global__ __launch_bounds__(256, 2) void k_attn_chu
     }
 
     l = across(l, [](float x, float y) { return x + y; });
-    const int unscale = held.top - (BITS == 32 ? 30 : 15);
+    const int unscale = held.top() - (BITS == 32 ? 30 : 15);
     bool bad = false;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
