@@ -225,14 +225,14 @@ int nnhip_gpt_beam_search(nnhip_gpt* g, const uint64_t* prompt, size_t n_prompt,
                           uint64_t eos, uint64_t* out, size_t* out_len, float* out_scores);
 /* Speculative decoding with a draft session of the same engine and vocabulary (no reference counterpart): continues n
  * prompts (one after another in prompts, prompt_len tokens each, 1 to seq_len) by up to max_new tokens, distributed as if
- * each were drawn from this session's softmax(logits / temperature); temperature 0 takes the largest logit, as
- * _generate does. The draft proposes draft_len tokens (1 to 1023) at a time, which this model verifies in one pass. A
- * sequence ends at eos (an id past the vocabulary: none does), after max_new tokens or where the context is full
- * (seq_len - prompt_len + 1 tokens); the draft's context has to hold it too. cache_bits 32: float32 caches; 8: a byte a
- * value (nnhip_kv8_append), for both models. seed: of the random numbers. out (n * max_new places, sequence i's tokens
- * from i * max_new on, eos not among them), out_len (n), stats (or NULL): passes of the target model, drafted tokens
- * and those of them that stood. 1 to 1024 prompts; heads at most 128 wide. Caches (_forward_step) and backward passes,
- * of both sessions, as with _beam_search. */
+ * each were drawn from this session's softmax(logits / temperature), to the 2^-24 that its random numbers are apart;
+ * temperature 0 takes the largest logit, as _generate does. The draft proposes draft_len tokens (1 to 1023) at a time,
+ * which this model verifies in one pass. A sequence ends at eos (an id past the vocabulary: none does), after max_new
+ * tokens or where the context is full (seq_len - prompt_len + 1 tokens); the draft's context has to hold it too.
+ * cache_bits 32: float32 caches; 8: a byte a value (nnhip_kv8_append), for both models. seed: of the random numbers. out
+ * (n * max_new places, sequence i's tokens from i * max_new on, eos not among them), out_len (n), stats (or NULL): passes
+ * of the target model, drafted tokens and those of them that stood. 1 to 1024 prompts; heads at most 128 wide. Caches
+ * (_forward_step) and backward passes, of both sessions, as with _beam_search. */
 int nnhip_gpt_speculate(nnhip_gpt* g, nnhip_gpt* draft, const uint64_t* prompts, const size_t* prompt_len, size_t n,
                         size_t max_new, size_t draft_len, float temperature, uint64_t eos, uint64_t seed,
                         size_t cache_bits, uint64_t* out, size_t* out_len, uint64_t* stats);

@@ -612,11 +612,13 @@ int nnhip_attn_chunk8(const nnhip_kv8_pages* c, const float* q, long q_t, long q
  * from a row to the next; the draft's alike with d_ld. Sequence b was fed the tokens fed[start[b] .. start[b + 1)), at most
  * `most`, of which all but the first were drafted: row n's distributions are those of the token after it, so that
  * fed[n + 1] was drawn from the draft's row n. With p = softmax(target / temperature) and q = softmax(draft /
- * temperature), both in float64, the token x after row n stands if accept[n] * q(x) < p(x) (of NaN it does not). At the first row whose token
- * does not stand, the next token is drawn from max(p - q, 0) (from p where that is 0 throughout), behind the last row
- * from p: the smallest v whose cumulative sum exceeds pick[b] times the whole sum. out_accepted[b] is the number of tokens
- * that stand, out_token[b] the token drawn: these many drafted tokens and that one continue the sequence, distributed as
- * if drawn from the target. Without drafted tokens (one row a sequence) this is sampling.
+ * temperature), held and summed in float64 of exponentials good to 2^-37, the token x after row n stands if accept[n] * q(x)
+ * < p(x) (of NaN it does not). At the first row whose token does not stand, the next token is drawn from max(p - q, 0)
+ * (from p where that is 0 throughout), behind the last row from p: the smallest v whose cumulative sum exceeds pick[b]
+ * times the whole sum. (A number nearer to a border than 2^-36 of the probabilities on its sides may fall to either.)
+ * out_accepted[b] is the number of tokens that stand, out_token[b] the token drawn: these many drafted tokens and that one
+ * continue the sequence, distributed as if drawn from the target, as finely as accept and pick are: of multiples of 2^-24 a
+ * token's probability is met to 2^-24. Without drafted tokens (one row a sequence) this is sampling.
  * draft NULL: the tokens were chosen without probabilities; q is 1 at the drafted token. temperature 0: a token stands if
  * it is the target's largest logit (the lowest index of equal ones), and that of the first row whose token is another
  * comes next; draft, accept and pick are not used and may be NULL. A logit that is NaN counts as -inf; of rows with +inf

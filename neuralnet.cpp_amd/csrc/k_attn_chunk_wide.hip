@@ -23,13 +23,17 @@
 // the second product's operand as they lie, if its k index 8 (l / 32) + e of step t
 // stands for position 8 (2 t + e / 4) + 4 (l / 32) + e % 4.
 //
-// What bounds it: the matrix cores are busy for 55 % of the cycles, the vector
-// instructions of the softmax and of the weights' parts (some 160 a tile and wave,
-// the exponentials at a quarter of the rate) for 40 %, and as the clock falls under
-// both (1.8 GHz) two waves a SIMD hardly hide one behind the other: time is 190 us
-// and 4.1 us a dim for 2048 tokens behind 6000 of 32 heads (dims 32, 64, 128: 291,
-// 411, 712 us). No order of reads, products and priorities changed it by 2 %; four
-// waves of 64 rows each, with half the reads from LDS, ran 1503 us.
+// What bounds it, 2048 tokens behind 6000 of 32 heads: with 128 dims the matrix
+// cores are busy for 53 % of the cycles and the vector instructions of the softmax
+// and of the weights' parts (some 200 a tile and wave, 16 of them exponentials, at a
+// quarter of the rate) for 41 %, and as the clock falls under both (1.8 GHz) two
+// waves a SIMD hardly hide one behind the other. There no order of reads, products
+// and priorities changed it by 2 %; four waves of 64 rows each, with half the reads
+// from LDS, ran 1503 us. Heads of 32, 64 and 128 take 301, 426 and 732 us (and up to
+// 10 % more on other cards); up to 64 it is the float32 walk below that takes the
+// registers of a third wave (245 to 256, 163 to 167 without it). Over 8 bits, 16
+// heads of 80, the matrix cores are busy for 33 % and the vector instructions, as
+// many beside 22 products a tile instead of 48, for 49 %.
 //
 // Of a float32 cache, results that are not finite are formed again by the float32
 // walk: infinities and NaN among keys, queries and values, also at positions

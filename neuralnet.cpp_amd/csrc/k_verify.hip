@@ -8,8 +8,9 @@
 // the first whose token does not stand, and leaves that row's sums of
 // max(p - q, 0) by segment. The third finds the segment that the random number
 // falls into, and the token within it. Sums, probabilities and comparisons are
-// in float64: float32's would move the border between two tokens by 2^-24 of
-// the whole, far more than most tokens' probability.
+// in float64, of exponentials good to 2^-37: float32's would move the border
+// between two tokens by 2^-24 of the whole, far more than most tokens'
+// probability.
 //
 // The first launch is bound by its exponentials (144 rows of 100003 of either
 // model: 32 us, 3.5 TB/s; 144 of 32000 by columns 17), the others by latency:

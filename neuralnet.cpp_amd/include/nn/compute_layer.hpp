@@ -1592,8 +1592,8 @@ public:
     }
 
     // Speculative decoding (no reference counterpart): continues every prompt by up to max_new tokens, distributed as
-    // if each were drawn from this model's softmax(logits / temperature) (temperature 0: its largest logit). The draft
-    // model, cheaper to run and of the same vocabulary, proposes draft_len tokens one by one; this model then runs over
+    // if each were drawn from this model's softmax(logits / temperature), to the 2^-24 that the random numbers are apart
+    // (temperature 0: its largest logit). The draft model, cheaper to run and of the same vocabulary, proposes draft_len tokens one by one; this model then runs over
     // all of them at once, and draft_verify keeps those that stand and draws the next one. A sequence ends at eos (an id
     // past the vocabulary: none does), after max_new tokens or where the context is full.
     //
